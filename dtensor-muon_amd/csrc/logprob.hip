@@ -1,0 +1,572 @@
+// Log probabilities of tokens under rows of logits, and the clipped policy loss on them, with the
+// gradients to the logits (muon_token_logprobs, muon_policy_loss and their backward passes).
+//
+// For a row x of V logits, its token t and the temperature tau:
+//   m = max x,  s = sum exp((x - m) / tau),  logp = (x_t - m) / tau - log s.
+// With r = exp(logp - old), advantage A, weight w and the reference's log probability ref:
+//   term = -min(r A, clip(r, 1 - lo, 1 + hi) A) + beta (exp(ref - logp) - (ref - logp) - 1)
+//   loss = sum over rows of w term,  g = w d term / d logp.
+// The gradient of g logp: dx_v = g / tau ([v = t] - exp((x_v - m) / tau) / s).
+//
+// A row with weight 0, or a negative token, is left out: nothing of it is read, logp is 0 and its
+// gradient 0. A token of V or more gives NaN.
+#include <algorithm>
+
+#include "rowops.h"
+
+namespace {
+
+constexpr double LOG2E_D = 1.4426950408889634074;
+
+struct Rows {
+  const void* x;
+  int64_t stride;  // between rows, in elements
+  int64_t N, V;
+  const int64_t* tokens;
+  float k;     // log2(e) / tau
+  double tau_inv;
+  float* logp;
+  float* stats;  // per row m, then per row 1 / s (null: not kept)
+};
+
+// The policy loss's per-row inputs; weights null: plain log probabilities.
+struct Policy {
+  const float* old;
+  const float* adv;
+  const float* weights;
+  const float* ref;  // or null
+  float lo, hi, beta;
+  float* terms;  // w term per row
+  float* coef;   // g per row (two-pass form)
+};
+
+MUON_DEVICE bool left_out(const Rows& a, const Policy& p, int64_t row) {
+  return a.tokens[row] < 0 || (p.weights && p.weights[row] == 0.0f);
+}
+
+// A running maximum and the sum of exp((x - m) / tau) under it.
+struct Sum {
+  float m, s;
+};
+// exp2 of -inf - -inf would be NaN: against a maximum of -inf the sum is 0 whatever is added.
+MUON_DEVICE float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
+MUON_DEVICE Sum join(Sum a, Sum b, float k) {
+  Sum r;
+  r.m = fmaxf(a.m, b.m);
+  const float base = base_of(r.m);
+  r.s = a.s * __builtin_amdgcn_exp2f((a.m - base) * k) + b.s * __builtin_amdgcn_exp2f((b.m - base) * k);
+  return r;
+}
+template <int N>
+MUON_DEVICE void add_values(Sum& a, const float (&v)[N], float k) {
+  float m = a.m;
+#pragma unroll
+  for (int e = 0; e < N; ++e) m = fmaxf(m, v[e]);
+  const float base = base_of(m);
+  float s = 0.0f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) s += __builtin_amdgcn_exp2f((v[e] - base) * k);
+  a.s = a.s * __builtin_amdgcn_exp2f((a.m - base) * k) + s;
+  a.m = m;
+}
+
+// Joined over a workgroup of NT threads in a fixed order; the result in every thread.
+template <int NT>
+MUON_DEVICE Sum block_join(Sum v, float k, Sum* lds) {
+  v = group_reduce<64>(v, [k](Sum a, Sum b) { return join(a, b, k); });
+  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
+  __syncthreads();
+  Sum r = lds[0];
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) r = join(r, lds[w], k);
+  return r;
+}
+
+// Values [i0, i0 + N) of a row that ends at V; -inf behind it.
+template <int DT>
+MUON_DEVICE muon_u4 load_tail(const void* x, int64_t at, int64_t i0, int64_t V) {
+  constexpr int N = Vec16<DT>::N;
+  float v[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = i0 + e < V ? Elem<DT>::load(x, at + i0 + e) : -INFINITY;
+  return Vec16<DT>::pack(v);
+}
+template <int DT>
+MUON_DEVICE void store_tail(void* x, int64_t at, int64_t i0, int64_t V, const float* v) {
+#pragma unroll
+  for (int e = 0; e < Vec16<DT>::N; ++e)
+    if (i0 + e < V) Elem<DT>::store(x, at + i0 + e, v[e]);
+}
+
+// What a row's sum gives: logp, and for the policy loss its term and slope g. One thread; in
+// double, since logp is the small difference of larger numbers and the loss a sum of terms of
+// both signs (one row's worth of it costs nothing beside the row).
+template <int DT>
+MUON_DEVICE float finish_row(const Rows& a, const Policy& p, int64_t row, Sum t) {
+  const int64_t tok = a.tokens[row];
+  double logp = __builtin_nan("");
+  if (tok < a.V) {
+    const double xt = Elem<DT>::load(a.x, row * a.stride + tok);
+    logp = (xt - (double)t.m) * a.tau_inv - log((double)t.s);
+  }
+  a.logp[row] = (float)logp;
+  if (a.stats) {
+    a.stats[row] = t.m;
+    a.stats[a.N + row] = tok < a.V ? 1.0f / t.s : __int_as_float(0x7fc00000);
+  }
+  if (!p.weights) return 0.0f;
+  const double w = p.weights[row], A = p.adv[row], r = exp(logp - (double)p.old[row]);
+  const double low = 1.0 - (double)p.lo, high = 1.0 + (double)p.hi;
+  // NaN ratios stay NaN: comparisons below leave r in place
+  const double clipped = r < low ? low : r > high ? high : r;
+  const double plain = r * A, other = clipped * A;
+  double term = -(other < plain ? other : plain);
+  // the smaller one is r A where r is inside, or outside on the side that A pulls it back from
+  const bool cut = A >= 0.0 ? r > high : r < low;
+  double slope = cut ? 0.0 : -plain;
+  if (p.ref) {
+    const double ahead = (double)p.ref[row] - logp, e = exp(ahead);
+    term += (double)p.beta * (e - ahead - 1.0);
+    slope += (double)p.beta * (1.0 - e);
+  }
+  p.terms[row] = (float)(w * term);
+  const float g = (float)(w * slope);
+  if (p.coef) p.coef[row] = g;
+  return g;
+}
+
+MUON_DEVICE void skip_row(const Rows& a, const Policy& p, int64_t row) {
+  a.logp[row] = 0.0f;
+  if (a.stats) a.stats[row] = a.stats[a.N + row] = 0.0f;
+  if (p.weights) {
+    p.terms[row] = 0.0f;
+    if (p.coef) p.coef[row] = 0.0f;
+  }
+}
+
+constexpr int SUM_THREADS = 512;
+constexpr int SUM_UNROLL = 4;  // 16-byte loads in flight per thread
+
+// One pass over (a slice of) a row with a running maximum and sum. Grid: slices x rows; with
+// one slice a row the workgroup finishes its row, else it leaves (m, s) for logp_join_kernel.
+template <int DT>
+__global__ __launch_bounds__(SUM_THREADS) void logp_kernel(Rows a, Policy p, Sum* part) {
+  constexpr int N = Vec16<DT>::N;
+  __shared__ Sum lds[SUM_THREADS / 64];
+  const int slices = gridDim.x;
+  for (int64_t row = blockIdx.y; row < a.N; row += gridDim.y) {
+    if (left_out(a, p, row)) {
+      if (threadIdx.x == 0 && slices == 1) skip_row(a, p, row);
+      continue;
+    }
+    const int64_t at = row * a.stride;
+    const int64_t vecs = a.V / N;
+    const int64_t begin = vecs * blockIdx.x / slices, end = vecs * (blockIdx.x + 1) / slices;
+    Sum t = {-INFINITY, 0.0f};
+    int64_t i = begin + threadIdx.x;
+    for (; i + (SUM_UNROLL - 1) * SUM_THREADS < end; i += SUM_UNROLL * SUM_THREADS) {
+      muon_u4 w[SUM_UNROLL];
+#pragma unroll
+      for (int u = 0; u < SUM_UNROLL; ++u) w[u] = load_u4(elem_at<DT>(a.x, at + (i + u * SUM_THREADS) * N));
+      float v[SUM_UNROLL * N];
+#pragma unroll
+      for (int u = 0; u < SUM_UNROLL; ++u) {
+        float h[N];
+        Vec16<DT>::unpack(w[u], h);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[u * N + e] = h[e];
+      }
+      add_values(t, v, a.k);
+    }
+    for (; i < end; i += SUM_THREADS) {
+      float v[N];
+      Vec16<DT>::unpack(load_u4(elem_at<DT>(a.x, at + i * N)), v);
+      add_values(t, v, a.k);
+    }
+    if (blockIdx.x == slices - 1 && threadIdx.x < a.V - vecs * N) {
+      const float v[1] = {Elem<DT>::load(a.x, at + vecs * N + threadIdx.x)};
+      add_values(t, v, a.k);
+    }
+    t = block_join<SUM_THREADS>(t, a.k, lds);
+    if (threadIdx.x == 0) {
+      if (slices == 1) finish_row<DT>(a, p, row, t);
+      else part[row * slices + blockIdx.x] = t;
+    }
+    __syncthreads();  // lds is written again for the next row
+  }
+}
+
+// A wave a row: the slices' sums joined in a fixed order.
+template <int DT>
+__global__ __launch_bounds__(256) void logp_join_kernel(Rows a, Policy p, const Sum* part, int slices) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  if (row >= a.N) return;
+  const int lane = threadIdx.x % 64;
+  if (left_out(a, p, row)) {
+    if (lane == 0) skip_row(a, p, row);
+    return;
+  }
+  Sum t = {-INFINITY, 0.0f};
+  for (int i = lane; i < slices; i += 64) t = join(t, part[row * slices + i], a.k);
+  t = group_reduce<64>(t, [&](Sum x, Sum y) { return join(x, y, a.k); });
+  if (lane == 0) finish_row<DT>(a, p, row, t);
+}
+
+struct Back {
+  const void* x;
+  int64_t stride, N, V;
+  const int64_t* tokens;
+  const float* stats;
+  const float* coef;   // per row: the gradient of logp
+  const float* scale;  // one value, or null
+  float k, tau_inv;
+  void* dx;  // contiguous
+};
+
+// dx of one run of values of a row; tok - i0 is the token's place in it, if any.
+template <int DT>
+MUON_DEVICE void slopes(const float (&x)[Vec16<DT>::N], float m, float k, float pc, float g,
+                        int64_t tok, float (&d)[Vec16<DT>::N]) {
+#pragma unroll
+  for (int e = 0; e < Vec16<DT>::N; ++e) {
+    const float q = pc * __builtin_amdgcn_exp2f((x[e] - m) * k);
+    d[e] = tok == e ? g - q : -q;
+  }
+}
+
+constexpr int BACK_THREADS = 256;
+constexpr int BACK_VECS = 4;  // 16-byte pieces per thread
+
+// The gradient from the logits again and the kept m and 1 / s. Grid: pieces of a row x rows.
+template <int DT>
+__global__ __launch_bounds__(BACK_THREADS) void logp_backward_kernel(Back a) {
+  constexpr int N = Vec16<DT>::N;
+  const float scale = a.scale ? a.scale[0] : 1.0f;
+  for (int64_t row = blockIdx.y; row < a.N; row += gridDim.y) {
+    const int64_t tok = a.tokens[row];
+    const float g = tok < 0 ? 0.0f : a.coef[row] * scale * a.tau_inv;
+    const int64_t at = row * a.stride, to = row * a.V;
+    const int64_t i0 = ((int64_t)blockIdx.x * BACK_VECS * BACK_THREADS + threadIdx.x) * N;
+    if (g == 0.0f) {
+#pragma unroll
+      for (int u = 0; u < BACK_VECS; ++u) {
+        const int64_t i = i0 + (int64_t)u * BACK_THREADS * N;
+        if (i + N <= a.V) store_u4((void*)elem_at<DT>(a.dx, to + i), muon_u4{0, 0, 0, 0});
+        else if (i < a.V) {
+          const float z[N] = {};
+          store_tail<DT>(a.dx, to, i, a.V, z);
+        }
+      }
+      continue;
+    }
+    const float m = a.stats[row], pc = g * a.stats[a.N + row];
+    muon_u4 w[BACK_VECS];
+#pragma unroll
+    for (int u = 0; u < BACK_VECS; ++u) {
+      const int64_t i = i0 + (int64_t)u * BACK_THREADS * N;
+      if (i + N <= a.V) w[u] = load_u4(elem_at<DT>(a.x, at + i));
+      else if (i < a.V) w[u] = load_tail<DT>(a.x, at, i, a.V);
+    }
+#pragma unroll
+    for (int u = 0; u < BACK_VECS; ++u) {
+      const int64_t i = i0 + (int64_t)u * BACK_THREADS * N;
+      if (i >= a.V) break;
+      float x[N], d[N];
+      Vec16<DT>::unpack(w[u], x);
+      slopes<DT>(x, m, a.k, pc, g, tok - i, d);
+      if (i + N <= a.V) store_u4((void*)elem_at<DT>(a.dx, to + i), Vec16<DT>::pack(d));
+      else store_tail<DT>(a.dx, to, i, a.V, d);
+    }
+  }
+}
+
+// The policy loss with its gradient in one pass over the logits: a workgroup holds its whole row
+// in registers (NV 16-byte pieces a thread), sums it, makes the slope g, and writes the gradient
+// from the same registers.
+template <int DT, int NT, int NV>
+__global__ __launch_bounds__(NT) void policy_row_kernel(Rows a, Policy p, void* dx, int64_t row0) {
+  constexpr int N = Vec16<DT>::N;
+  __shared__ Sum lds[NT / 64];
+  __shared__ float slope;
+  const int64_t row = row0 + blockIdx.x;
+  const int64_t at = row * a.stride, to = row * a.V;
+  const int V = (int)a.V, vecs = V / N;
+  // one address register a thread: the pieces' places are added to the scalar base
+  const char* xr = elem_at<DT>(a.x, at);
+  char* dr = (char*)elem_at<DT>(dx, to);
+  const uint32_t off = threadIdx.x * 16;
+  const int tid = threadIdx.x;
+  if (left_out(a, p, row)) {
+    if (tid == 0) skip_row(a, p, row);
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int i = u * NT + tid;
+      if (i < vecs) store_u4(dr + (int64_t)u * NT * 16 + off, muon_u4{0, 0, 0, 0});
+      else if (i == vecs) {
+        const float z[N] = {};
+        store_tail<DT>(dx, to, (int64_t)i * N, V, z);
+      }
+    }
+    return;
+  }
+  muon_u4 w[NV];
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    if ((u + 1) * NT <= vecs) {
+      w[u] = load_u4(xr + (int64_t)u * NT * 16 + off);
+    } else {  // the piece that the row's end cuts, and pieces behind it
+      const int i = u * NT + tid;
+      const uint32_t none = DT == MUON_DT_F32 ? 0xff800000u : 0xff80ff80u;  // -inf
+      w[u] = muon_u4{none, none, none, none};
+      if (i < vecs) w[u] = load_u4(xr + (int64_t)u * NT * 16 + off);
+      else if (i == vecs) w[u] = load_tail<DT>(a.x, at, (int64_t)i * N, V);
+    }
+  }
+  Sum t = {-INFINITY, 0.0f};
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    float v[N];
+    Vec16<DT>::unpack(w[u], v);
+    add_values(t, v, a.k);
+    // one piece unpacked at a time: the row itself takes most of the registers
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  t = block_join<NT>(t, a.k, lds);
+  if (tid == 0) slope = finish_row<DT>(a, p, row, t);
+  __syncthreads();
+  const bool known = a.tokens[row] < a.V;
+  const int tok = known ? (int)a.tokens[row] : -1;
+  const float g = slope * (float)a.tau_inv;
+  const float pc = known ? g * (1.0f / t.s) : __int_as_float(0x7fc00000);
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int i = u * NT + tid;
+    if (u * NT > vecs) break;
+    float v[N], d[N];
+    // unpacked again: the compiler would else keep the first pass's floats beside the row
+    asm("" : "+v"(w[u]));
+    Vec16<DT>::unpack(w[u], v);
+    slopes<DT>(v, t.m, a.k, pc, g, tok - i * N, d);
+    if (i < vecs) store_u4(dr + (int64_t)u * NT * 16 + off, Vec16<DT>::pack(d));
+    else if (i == vecs) store_tail<DT>(dx, to, (int64_t)i * N, V, d);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// loss = the rows' terms summed in a fixed order, in double.
+__global__ __launch_bounds__(1024) void loss_kernel(const float* terms, int64_t n, float* loss) {
+  __shared__ double red[16];
+  double s = 0.0;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += terms[i];
+  for (int off = 32; off; off >>= 1) s += __shfl_xor(s, off, 64);
+  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = s;
+  __syncthreads();
+  if (threadIdx.x) return;
+  s = 0.0;
+  for (int w = 0; w < 16; ++w) s += red[w];
+  loss[0] = (float)s;
+}
+
+// x *= scale in place; nothing to do where the scale is one.
+template <int DT>
+__global__ __launch_bounds__(256) void scale_kernel(void* x, int64_t n, const float* scale) {
+  constexpr int N = Vec16<DT>::N;
+  const float g = scale[0];
+  if (g == 1.0f) return;
+  const int64_t vecs = n / N, step = (int64_t)gridDim.x * 256;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (int64_t i = id; i < vecs; i += step) {
+    float v[N];
+    Vec16<DT>::unpack(load_u4(elem_at<DT>(x, i * N)), v);
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] *= g;
+    store_u4((void*)elem_at<DT>(x, i * N), Vec16<DT>::pack(v));
+  }
+  for (int64_t i = vecs * N + id; i < n; i += step) Elem<DT>::store(x, i, Elem<DT>::load(x, i) * g);
+}
+
+bool io_ok(int dt) { return dt == MUON_DT_F32 || dt == MUON_DT_BF16 || dt == MUON_DT_F16; }
+
+int check(const char* what, int dtype, int64_t N, int64_t V, int64_t stride, float tau) {
+  if (!io_ok(dtype)) {
+    muon_set_error("%s: unsupported dtype %d", what, dtype);
+    return MUON_ERR_DTYPE;
+  }
+  if (N < 0 || N >= (1LL << 31) || V < 1 || V >= (1LL << 31) || stride < 0) {
+    muon_set_error("%s: bad extents (rows %lld, vocabulary %lld, row stride %lld)", what,
+                   (long long)N, (long long)V, (long long)stride);
+    return MUON_ERR_SHAPE;
+  }
+  // 1 / tau and log2(e) / tau stay in fp32's range
+  if (!(tau >= 1e-30f && tau <= 1e30f)) {
+    muon_set_error("%s: temperature %g is not within 1e-30 and 1e30", what, (double)tau);
+    return MUON_ERR_ARG;
+  }
+  return MUON_OK;
+}
+
+constexpr int64_t MAX_GRID_Y = 65535;
+
+// Slices of a row: until a launch has four workgroups per CU, but none of less than 16 KB (one
+// round of a workgroup's loads is 32 KB).
+int slices_for(int dtype, int64_t N, int64_t V) {
+  const int64_t bytes = V * (dtype == MUON_DT_F32 ? 4 : 2);
+  const int64_t want = N ? (1024 + N - 1) / N : 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, bytes / 16384), 64));
+}
+
+int launch_sums(const Rows& a, const Policy& p, int dtype, void* ws, hipStream_t s) {
+  const int slices = slices_for(dtype, a.N, a.V);
+  const dim3 grid(slices, (unsigned)std::min(a.N, MAX_GRID_Y));
+  Sum* part = (Sum*)ws;
+  if (dtype == MUON_DT_F32) logp_kernel<MUON_DT_F32><<<grid, SUM_THREADS, 0, s>>>(a, p, part);
+  else if (dtype == MUON_DT_BF16) logp_kernel<MUON_DT_BF16><<<grid, SUM_THREADS, 0, s>>>(a, p, part);
+  else logp_kernel<MUON_DT_F16><<<grid, SUM_THREADS, 0, s>>>(a, p, part);
+  MUON_CHECK_LAUNCH("token_logprobs");
+  if (slices == 1) return MUON_OK;
+  const unsigned blocks = (unsigned)((a.N + 3) / 4);
+  if (dtype == MUON_DT_F32) logp_join_kernel<MUON_DT_F32><<<blocks, 256, 0, s>>>(a, p, part, slices);
+  else if (dtype == MUON_DT_BF16) logp_join_kernel<MUON_DT_BF16><<<blocks, 256, 0, s>>>(a, p, part, slices);
+  else logp_join_kernel<MUON_DT_F16><<<blocks, 256, 0, s>>>(a, p, part, slices);
+  MUON_CHECK_LAUNCH("token_logprobs join");
+  return MUON_OK;
+}
+
+template <int DT>
+int launch_policy_rows(const Rows& a, const Policy& p, void* dx, hipStream_t s) {
+  const int64_t vecs = (a.V + Vec16<DT>::N - 1) / Vec16<DT>::N;
+#define MUON_POLICY_ROWS(NT, NV)                                      \
+  if (vecs <= (int64_t)NT * NV) {                                     \
+    /* a launch holds fewer than 2^32 threads */                      \
+    for (int64_t r = 0; r < a.N; r += 1 << 20) {                      \
+      const unsigned rows = (unsigned)std::min<int64_t>(a.N - r, 1 << 20); \
+      policy_row_kernel<DT, NT, NV><<<rows, NT, 0, s>>>(a, p, dx, r); \
+      MUON_CHECK_LAUNCH("policy_loss");                               \
+    }                                                                 \
+    return MUON_OK;                                                   \
+  }
+  MUON_POLICY_ROWS(256, 2)
+  MUON_POLICY_ROWS(256, 4)
+  MUON_POLICY_ROWS(512, 4)
+  MUON_POLICY_ROWS(512, 8)
+  MUON_POLICY_ROWS(1024, 8)
+  MUON_POLICY_ROWS(1024, 12)
+  MUON_POLICY_ROWS(1024, 16)
+  MUON_POLICY_ROWS(1024, 20)
+#undef MUON_POLICY_ROWS
+  muon_set_error("policy_loss: a row of %lld values does not fit the registers", (long long)a.V);
+  return MUON_ERR_SHAPE;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t muon_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab) {
+  if (!io_ok(dtype) || rows < 0 || vocab < 1) return -1;
+  const int slices = slices_for(dtype, rows, vocab);
+  return slices == 1 ? 0 : rows * slices * (int64_t)sizeof(Sum);
+}
+
+int muon_token_logprobs(const void* logits, int dtype, int64_t row_stride, int64_t rows,
+                        int64_t vocab, const int64_t* tokens, float temperature, float* logprobs,
+                        float* stats, void* ws, void* stream) {
+  const int rc = check("token_logprobs", dtype, rows, vocab, row_stride, temperature);
+  if (rc || rows == 0) return rc;
+  if (!logits || !tokens || !logprobs || (!ws && slices_for(dtype, rows, vocab) > 1)) {
+    muon_set_error("token_logprobs: null tensor");
+    return MUON_ERR_ARG;
+  }
+  const double inv = 1.0 / (double)temperature;
+  const Rows a = {logits, row_stride, rows, vocab, tokens, (float)(LOG2E_D * inv), inv, logprobs, stats};
+  const Policy none = {};
+  return launch_sums(a, none, dtype, ws, (hipStream_t)stream);
+}
+
+int muon_token_logprobs_backward(const void* logits, int dtype, int64_t row_stride, int64_t rows,
+                                 int64_t vocab, const int64_t* tokens, float temperature,
+                                 const float* stats, const float* dlogprobs, const float* scale,
+                                 void* dlogits, void* stream) {
+  const int rc = check("token_logprobs_backward", dtype, rows, vocab, row_stride, temperature);
+  if (rc || rows == 0) return rc;
+  if (!logits || !tokens || !stats || !dlogprobs || !dlogits) {
+    muon_set_error("token_logprobs_backward: null tensor");
+    return MUON_ERR_ARG;
+  }
+  const double inv = 1.0 / (double)temperature;
+  const Back a = {logits, row_stride, rows, vocab, tokens, stats, dlogprobs, scale,
+                  (float)(LOG2E_D * inv), (float)inv, dlogits};
+  const int64_t per = (int64_t)BACK_THREADS * BACK_VECS * (dtype == MUON_DT_F32 ? 4 : 8);
+  const dim3 grid((unsigned)((vocab + per - 1) / per), (unsigned)std::min(rows, MAX_GRID_Y));
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == MUON_DT_F32) logp_backward_kernel<MUON_DT_F32><<<grid, BACK_THREADS, 0, s>>>(a);
+  else if (dtype == MUON_DT_BF16) logp_backward_kernel<MUON_DT_BF16><<<grid, BACK_THREADS, 0, s>>>(a);
+  else logp_backward_kernel<MUON_DT_F16><<<grid, BACK_THREADS, 0, s>>>(a);
+  MUON_CHECK_LAUNCH("token_logprobs_backward");
+  return MUON_OK;
+}
+
+int muon_policy_loss_one_pass(int dtype, int64_t vocab) {
+  if (dtype == MUON_DT_BF16) return vocab >= 1 && vocab <= 1024 * 20 * 8;
+  return dtype == MUON_DT_F32 && vocab >= 1 && vocab <= 1024 * 20 * 4;
+}
+
+int muon_policy_loss(const void* logits, int dtype, int64_t row_stride, int64_t rows,
+                     int64_t vocab, const int64_t* tokens, const float* old_logprobs,
+                     const float* advantages, const float* weights, const float* ref_logprobs,
+                     float clip_low, float clip_high, float kl_coef, float temperature,
+                     float* loss, float* logprobs, float* terms, float* stats, float* coef,
+                     void* dlogits, void* ws, void* stream) {
+  const int rc = check("policy_loss", dtype, rows, vocab, row_stride, temperature);
+  if (rc) return rc;
+  if (!loss || (rows && (!logits || !tokens || !old_logprobs || !advantages || !weights ||
+                         !logprobs || !terms || (!ws && !dlogits && slices_for(dtype, rows, vocab) > 1)))) {
+    muon_set_error("policy_loss: null tensor");
+    return MUON_ERR_ARG;
+  }
+  if (!(clip_low >= 0.0f) || !(clip_high >= 0.0f)) {
+    muon_set_error("policy_loss: negative clip range");
+    return MUON_ERR_ARG;
+  }
+  if (dlogits && !muon_policy_loss_one_pass(dtype, vocab)) {
+    muon_set_error("policy_loss: no gradient in the forward pass for dtype %d, vocabulary %lld",
+                   dtype, (long long)vocab);
+    return MUON_ERR_ARG;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  const double inv = 1.0 / (double)temperature;
+  const Rows a = {logits, row_stride, rows, vocab, tokens, (float)(LOG2E_D * inv), inv, logprobs, stats};
+  const Policy p = {old_logprobs, advantages, weights, ref_logprobs, clip_low, clip_high, kl_coef,
+                    terms, coef};
+  if (rows) {
+    const int r = !dlogits ? launch_sums(a, p, dtype, ws, s)
+                  : dtype == MUON_DT_BF16 ? launch_policy_rows<MUON_DT_BF16>(a, p, dlogits, s)
+                                          : launch_policy_rows<MUON_DT_F32>(a, p, dlogits, s);
+    if (r) return r;
+  }
+  loss_kernel<<<1, 1024, 0, s>>>(terms, rows, loss);
+  MUON_CHECK_LAUNCH("policy_loss sum");
+  return MUON_OK;
+}
+
+int muon_scale_gradient(void* x, int dtype, int64_t n, const float* scale, void* stream) {
+  if (!io_ok(dtype)) {
+    muon_set_error("scale_gradient: unsupported dtype %d", dtype);
+    return MUON_ERR_DTYPE;
+  }
+  if (n < 0 || (n && (!x || !scale))) {
+    muon_set_error("scale_gradient: bad arguments");
+    return MUON_ERR_ARG;
+  }
+  if (n == 0) return MUON_OK;
+  const int grid = (int)std::min<int64_t>((n / 2048) + 1, 2048);
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == MUON_DT_F32) scale_kernel<MUON_DT_F32><<<grid, 256, 0, s>>>(x, n, scale);
+  else if (dtype == MUON_DT_BF16) scale_kernel<MUON_DT_BF16><<<grid, 256, 0, s>>>(x, n, scale);
+  else scale_kernel<MUON_DT_F16><<<grid, 256, 0, s>>>(x, n, scale);
+  MUON_CHECK_LAUNCH("scale_gradient");
+  return MUON_OK;
+}
+
+}  // extern "C"

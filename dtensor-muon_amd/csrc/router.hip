@@ -1,0 +1,565 @@
+// Expert routing: the top-k choice of a token's experts with their gates, the tokens each expert
+// gets, the balance loss and the z loss, with the gradient to the logits (muon_route,
+// muon_route_backward).
+//
+// For a token's logits z over E experts: p = softmax(z), lse = log sum exp z; the k largest are
+// chosen (ties: the lowest index; a NaN counts as the largest; an expert at -inf is never chosen,
+// and a slot that finds none holds -1 and gate 0). Gates are p, or p over the chosen ones' sum.
+// Over the N tokens that count (not masked, and not all -inf), with c_e tokens at expert e:
+//   balance = E sum_e (c_e / (k N)) (1 / N) sum_t p_te,   z = (1 / N) sum_t lse_t^2.
+// Backward, with a_e = db E c_e / (k N^2), G the gates' gradient:
+//   dz_e = p_e (a_e - sum p a) + 2 lse dzl / N p_e + [e chosen] g_e (G_e - sum g G)  (normalized)
+//   or, with the gates as they are, the last term p_e ([e chosen] G_e - sum over chosen p G).
+#include <algorithm>
+#include <type_traits>
+
+#include "rowops.h"
+
+namespace {
+
+constexpr int KMAX = 64;
+constexpr int EMAX = 1024;
+constexpr int FWD_THREADS = 512;
+constexpr int BWD_THREADS = 256;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+struct Args {
+  const void* z;
+  int64_t row;  // stride of a token's logits in elements
+  int64_t T;
+  int E, k, normalize;
+  const uint8_t* mask;  // or null: every token counts
+  float* gates;
+  int64_t* experts;
+  int64_t* counts;
+  float* balance;  // one value each: the losses, and the number of tokens that count
+  float* zloss;
+  float* kept;
+  // one partial a workgroup, of E or of one value
+  float* part_p;
+  int* part_c;
+  float* part_z;
+  int* part_n;
+};
+
+struct BackArgs {
+  const void* z;
+  int64_t row, T;
+  int E, k, normalize;
+  const uint8_t* mask;
+  const int64_t* experts;
+  const int64_t* counts;
+  const float* kept;
+  const float* dgates;    // or null
+  const float* dbalance;  // one value each, or null
+  const float* dzloss;
+  void* dz;  // contiguous
+};
+
+// The logits of one token that a lane owns: VPT experts in a row; -inf behind the last one.
+template <int DT, int VPT>
+MUON_DEVICE void load_logits(const void* z, int64_t at, int e0, int E, float (&v)[VPT]) {
+  constexpr int N = Vec16<DT>::N;
+#pragma unroll
+  for (int c = 0; c < VPT; c += N) {
+    const int e = e0 + c;
+    float x[N];
+    if (e + N <= E) {
+      Vec16<DT>::unpack(load_u4(elem_at<DT>(z, at + e)), x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = e + j < E ? Elem<DT>::load(z, at + e + j) : -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[c + j] = x[j];
+  }
+}
+
+// An order-preserving integer of a value: NaNs (as one) over +inf over ... over -inf, and -0 as 0.
+MUON_DEVICE uint32_t ordered(float v) {
+  const uint32_t u = v != v ? 0x7fc00000u : __float_as_uint(v + 0.0f);
+  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+MUON_DEVICE float unordered(uint32_t o) {
+  return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+// A value and its index as one number, larger for a larger value and, among equal ones, for a
+// lower index; 0 for what cannot be chosen (-inf). All keys of a token are distinct, so the next
+// choice is the largest key below the last one: nothing has to be taken out of the registers.
+// Values of two bytes have at most 19 significant bits in fp32: 32 bits hold both. fp32 takes
+// 63 bits, compared as a positive double (one maximum instruction; no key reaches the exponent of
+// infinities, since the largest ordered value, the NaN's, is 0xffc00000).
+template <int DT>
+struct Key {
+  typedef uint32_t T;
+  static MUON_DEVICE T make(float v, int e) {
+    return v == -INFINITY ? 0u : (ordered(v) & 0xffffe000u) | (uint32_t)(0x1fff - e);
+  }
+  static MUON_DEVICE bool none(T k) { return k == 0; }
+  static MUON_DEVICE int index(T k) { return 0x1fff - (int)(k & 0x1fffu); }
+  static MUON_DEVICE float value(T k) {
+    // a negative value's ordered form has ones in the masked bits
+    const uint32_t o = k & 0xffffe000u;
+    return unordered((o >> 31) ? o : o | 0x1fffu);
+  }
+  // The largest key below `last`: key - last wraps to the top of the range exactly for the keys
+  // below it, in their order, so one subtraction and one maximum serve a key.
+  template <int VPT, int G>
+  static MUON_DEVICE T next(const T (&key)[VPT], T last) {
+    T best = 0;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) best = max(best, key[j] - last);
+    best = group_reduce<G>(best, [](T a, T b) { return max(a, b); });
+    const T found = best + last;
+    return found < last ? found : 0;
+  }
+  template <int VPT, int G>
+  static MUON_DEVICE T first(const T (&key)[VPT]) {
+    T best = 0;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) best = max(best, key[j]);
+    return group_reduce<G>(best, [](T a, T b) { return max(a, b); });
+  }
+};
+template <>
+struct Key<MUON_DT_F32> {
+  typedef double T;
+  static MUON_DEVICE T make(float v, int e) {
+    const uint64_t b = v == -INFINITY ? 0 : ((uint64_t)ordered(v) << 31) | (uint64_t)(0x7fffffff - e);
+    return __builtin_bit_cast(double, b);
+  }
+  static MUON_DEVICE bool none(T k) { return __builtin_bit_cast(uint64_t, k) == 0; }
+  static MUON_DEVICE int index(T k) {
+    return 0x7fffffff - (int)(__builtin_bit_cast(uint64_t, k) & 0x7fffffffu);
+  }
+  static MUON_DEVICE float value(T k) {
+    return unordered((uint32_t)(__builtin_bit_cast(uint64_t, k) >> 31));
+  }
+  template <int VPT, int G>
+  static MUON_DEVICE T next(const T (&key)[VPT], T last) {
+    T best = 0.0;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) best = __builtin_fmax(best, key[j] < last ? key[j] : 0.0);
+    return group_reduce<G>(best, [](T a, T b) { return __builtin_fmax(a, b); });
+  }
+  template <int VPT, int G>
+  static MUON_DEVICE T first(const T (&key)[VPT]) {
+    T best = 0.0;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) best = __builtin_fmax(best, key[j]);
+    return group_reduce<G>(best, [](T a, T b) { return __builtin_fmax(a, b); });
+  }
+};
+
+// What one wave writes to LDS and reads back itself needs no barrier of the workgroup: LDS
+// operations of a wave are done in order, and this keeps the compiler from reordering them.
+MUON_DEVICE void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The losses from sum_e c_e sum_t p_te, sum lse^2 and the number of tokens that count.
+MUON_DEVICE void write_losses(const Args& a, double balance, double z, int64_t n) {
+  const double d = (double)n;
+  a.balance[0] = n ? (float)(balance * (double)a.E / ((double)a.k * d * d)) : 0.0f;
+  a.zloss[0] = n ? (float)(z / d) : 0.0f;
+  a.kept[0] = (float)n;
+}
+
+// Groups of G lanes take a token each, VPT experts a lane, and walk over the tokens; each lane
+// sums its experts' p in registers over all its tokens, the chosen ones are counted in LDS
+// (integers: any order gives the same), and the workgroup writes one partial of E sums and
+// counts. A single workgroup writes the results itself.
+template <int DT, int G, int VPT>
+__global__ __launch_bounds__(FWD_THREADS) void route_kernel(Args a) {
+  constexpr int GROUPS = FWD_THREADS / G;
+  constexpr int ECAP = G * VPT;
+  constexpr int KCAP = ECAP < KMAX ? ECAP : KMAX;
+  typedef Key<DT> K;
+  struct Pick { float v; int e; };
+  __shared__ Pick picks[GROUPS][KCAP];
+  __shared__ float cols[GROUPS][ECAP + 1];
+  __shared__ int cnt[ECAP];
+  __shared__ float zs[GROUPS];
+  __shared__ int ns[GROUPS];
+  const int lane = threadIdx.x % G, group = threadIdx.x / G;
+  const int e0 = lane * VPT;
+  for (int e = threadIdx.x; e < ECAP; e += FWD_THREADS) cnt[e] = 0;
+  __syncthreads();
+  float acc[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) acc[j] = 0.0f;
+  float zsum = 0.0f;
+  int n = 0;
+  for (int64_t t = (int64_t)blockIdx.x * GROUPS + group; t < a.T; t += (int64_t)gridDim.x * GROUPS) {
+    float v[VPT], p[VPT];
+    load_logits<DT, VPT>(a.z, t * a.row, e0, a.E, v);
+    float m = v[0];
+#pragma unroll
+    for (int j = 1; j < VPT; ++j) m = fmaxf(m, v[j]);
+    m = group_max<G>(m);
+    bool on = !a.mask || a.mask[t];
+    // all -inf (a NaN, which fmaxf passes over, is no such row): counts nowhere
+    float bad = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) bad = v[j] != v[j] ? 1.0f : bad;
+    if (m == -INFINITY && group_max<G>(bad) == 0.0f) on = false;
+    float total = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      p[j] = __builtin_amdgcn_exp2f((v[j] - m) * LOG2E);
+      total += p[j];
+    }
+    total = group_sum<G>(total);
+    const float inv = 1.0f / total;
+    if (on) {
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) acc[j] += e0 + j < a.E ? p[j] * inv : 0.0f;
+      const float lse = m + __builtin_amdgcn_logf(total) * LN2;
+      zsum += lse * lse;
+      n += 1;
+    }
+    typename K::T key[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+      key[j] = e0 + j < a.E ? K::make(v[j], e0 + j) : (typename K::T)0;
+    if (on) {
+      typename K::T best = K::template first<VPT, G>(key);
+      for (int i = 0; i < a.k; ++i) {
+        if (lane == 0) picks[group][i] = {K::value(best), K::none(best) ? -1 : K::index(best)};
+        if (i + 1 < a.k && !K::none(best)) best = K::template next<VPT, G>(key, best);
+      }
+    }
+    wave_lds_fence();
+    float held = 0.0f;
+    if (on) {
+      for (int i = lane; i < a.k; i += G)
+        if (picks[group][i].e >= 0) held += __builtin_amdgcn_exp2f((picks[group][i].v - m) * LOG2E);
+    }
+    held = group_sum<G>(held);
+    for (int i = lane; i < a.k; i += G) {
+      Pick q = {0.0f, -1};
+      if (on) q = picks[group][i];
+      const float e2 = __builtin_amdgcn_exp2f((q.v - m) * LOG2E);
+      a.experts[t * a.k + i] = q.e;
+      a.gates[t * a.k + i] = q.e < 0 ? 0.0f : a.normalize ? e2 / held : e2 * inv;
+      if (q.e >= 0) atomicAdd(&cnt[q.e], 1);
+    }
+    wave_lds_fence();
+  }
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) cols[group][e0 + j] = acc[j];
+  if (lane == 0) {
+    zs[group] = zsum;
+    ns[group] = n;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += FWD_THREADS) {
+    float sum = 0.0f;
+    for (int g = 0; g < GROUPS; ++g) sum += cols[g][e];
+    if (gridDim.x == 1) {
+      a.counts[e] = cnt[e];
+      cols[0][e] = sum;
+    } else {
+      a.part_p[(int64_t)blockIdx.x * a.E + e] = sum;
+      a.part_c[(int64_t)blockIdx.x * a.E + e] = cnt[e];
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  double z = 0.0, b = 0.0;
+  int c = 0;
+  for (int g = threadIdx.x; g < GROUPS; g += 64) {
+    z += zs[g];
+    c += ns[g];
+  }
+  if (gridDim.x == 1)
+    for (int e = threadIdx.x; e < a.E; e += 64) b += (double)cnt[e] * (double)cols[0][e];
+  for (int off = 32; off; off >>= 1) {
+    z += __shfl_xor(z, off, 64);
+    b += __shfl_xor(b, off, 64);
+    c += __shfl_xor(c, off, 64);
+  }
+  if (threadIdx.x) return;
+  if (gridDim.x == 1) {
+    write_losses(a, b, z, c);
+  } else {
+    a.part_z[blockIdx.x] = (float)z;
+    a.part_n[blockIdx.x] = c;
+  }
+}
+
+// The workgroups' partials summed in a fixed order by one workgroup: C columns (a power of two)
+// times 1024 / C rows of threads, joined through LDS.
+__global__ __launch_bounds__(1024) void route_finish_kernel(Args a, int blocks, int C) {
+  __shared__ float ps[1024];
+  __shared__ int cs[1024];
+  __shared__ double red[3][16];
+  const int col = threadIdx.x & (C - 1), row = threadIdx.x / C, rows = 1024 / C;
+  double bal = 0.0;
+  for (int e0 = 0; e0 < a.E; e0 += C) {
+    const int e = e0 + col;
+    float p = 0.0f;
+    int c = 0;
+    if (e < a.E) {
+#pragma unroll 8
+      for (int b = row; b < blocks; b += rows) {
+        p += a.part_p[(int64_t)b * a.E + e];
+        c += a.part_c[(int64_t)b * a.E + e];
+      }
+    }
+    ps[threadIdx.x] = p;
+    cs[threadIdx.x] = c;
+    __syncthreads();
+    if (row == 0 && e < a.E) {
+      double sum = 0.0;
+      int64_t count = 0;
+      for (int r = 0; r < rows; ++r) {
+        sum += ps[r * C + col];
+        count += cs[r * C + col];
+      }
+      a.counts[e] = count;
+      bal += sum * (double)count;
+    }
+    __syncthreads();
+  }
+  double z = 0.0, n = 0.0;  // token counts below 2^53 are exact
+  for (int b = threadIdx.x; b < blocks; b += 1024) {
+    z += a.part_z[b];
+    n += a.part_n[b];
+  }
+  for (int off = 32; off; off >>= 1) {
+    bal += __shfl_xor(bal, off, 64);
+    z += __shfl_xor(z, off, 64);
+    n += __shfl_xor(n, off, 64);
+  }
+  if (threadIdx.x % 64 == 0) {
+    red[0][threadIdx.x / 64] = bal;
+    red[1][threadIdx.x / 64] = z;
+    red[2][threadIdx.x / 64] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+  bal = z = n = 0.0;
+  for (int w = 0; w < 16; ++w) {
+    bal += red[0][w];
+    z += red[1][w];
+    n += red[2][w];
+  }
+  write_losses(a, bal, z, (int64_t)n);
+}
+
+// One group a token again: p from the logits, the dense part of the gradient in registers, and
+// the chosen experts' part through the group's row in LDS (where it is added at their indices).
+template <int DT, int G, int VPT>
+__global__ __launch_bounds__(BWD_THREADS) void route_backward_kernel(BackArgs a) {
+  constexpr int GROUPS = BWD_THREADS / G;
+  constexpr int ECAP = G * VPT;
+  constexpr int SLOTS = (ECAP < KMAX ? ECAP : KMAX) / G;
+  // rows 16 bytes aligned for the vector accesses, 4 words apart in their banks
+  __shared__ __attribute__((aligned(16))) float rows[GROUPS][ECAP + 4];
+  const int lane = threadIdx.x % G, group = threadIdx.x / G;
+  const int e0 = lane * VPT;
+  const float n = a.kept[0];
+  const float db = a.dbalance && n > 0.0f ? a.dbalance[0] : 0.0f;
+  const float zc = a.dzloss && n > 0.0f ? 2.0f * a.dzloss[0] / n : 0.0f;
+  const float bc = n > 0.0f ? db * (float)a.E / ((float)a.k * n) : 0.0f;
+  float coef[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j)
+    coef[j] = e0 + j < a.E && n > 0.0f ? bc * ((float)a.counts[e0 + j] / n) : 0.0f;
+  float* mine = rows[group];
+  for (int64_t t = (int64_t)blockIdx.x * GROUPS + group; t < a.T; t += (int64_t)gridDim.x * GROUPS) {
+    float v[VPT];
+    load_logits<DT, VPT>(a.z, t * a.row, e0, a.E, v);
+    const bool masked = a.mask && !a.mask[t];
+    float m = v[0], bad = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      m = fmaxf(m, v[j]);
+      bad = v[j] != v[j] ? 1.0f : bad;
+    }
+    m = group_max<G>(m);
+    const bool on = !masked && !(m == -INFINITY && group_max<G>(bad) == 0.0f);
+    float total = 0.0f, dot = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      v[j] = e0 + j < a.E ? __builtin_amdgcn_exp2f((v[j] - m) * LOG2E) : 0.0f;
+      total += v[j];
+    }
+    total = group_sum<G>(total);
+    const float inv = 1.0f / total;
+    const float lse = m + __builtin_amdgcn_logf(total) * LN2;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      v[j] *= inv;
+      dot += v[j] * coef[j];
+      mine[e0 + j] = v[j];
+    }
+    dot = group_sum<G>(dot);
+    wave_lds_fence();
+    // slot lane + q G of the token is this lane's: the chosen expert, its p, its gate's gradient
+    int at[SLOTS];
+    float part[SLOTS], up[SLOTS];
+    float held = 0.0f, inner = 0.0f;  // sums of p and of p G over the chosen
+#pragma unroll
+    for (int q = 0; q < SLOTS; ++q) {
+      const int i = lane + q * G;
+      at[q] = -1;
+      if (!a.dgates || !on || i >= a.k) continue;
+      const int64_t e = a.experts[t * a.k + i];
+      if (e < 0 || e >= a.E) continue;
+      at[q] = (int)e;
+      part[q] = mine[e];
+      up[q] = a.dgates[t * a.k + i];
+      held += part[q];
+      inner += part[q] * up[q];
+    }
+    held = group_sum<G>(held);
+    inner = group_sum<G>(inner);
+    wave_lds_fence();
+    const float shift = zc * lse - dot - (a.normalize ? 0.0f : inner);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) mine[e0 + j] = v[j] * (coef[j] + shift);
+    wave_lds_fence();
+    const float scale = a.normalize ? 1.0f / held : 1.0f;
+    const float mean = a.normalize ? inner * scale : 0.0f;
+#pragma unroll
+    for (int q = 0; q < SLOTS; ++q)  // a token's experts are distinct: no two lanes meet
+      if (at[q] >= 0) mine[at[q]] += part[q] * scale * (up[q] - mean);
+    wave_lds_fence();
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) v[j] = on ? mine[e0 + j] : 0.0f;
+    wave_lds_fence();
+    constexpr int N = Vec16<DT>::N;
+#pragma unroll
+    for (int c = 0; c < VPT; c += N) {
+      float x[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = v[c + j];
+      const int e = e0 + c;
+      if (e + N <= a.E) {
+        store_u4((void*)elem_at<DT>(a.dz, t * a.E + e), Vec16<DT>::pack(x));
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (e + j < a.E) Elem<DT>::store(a.dz, t * a.E + e + j, x[j]);
+      }
+    }
+  }
+}
+
+// Lanes and experts per lane for E experts: 8 experts a lane up to 16 lanes, then 16. More
+// lanes cost more exchange steps per choice, more experts a lane more registers.
+template <typename F>
+int by_experts(int64_t E, F f) {
+  if (E <= 8) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
+  if (E <= 16) return f(std::integral_constant<int, 2>(), std::integral_constant<int, 8>());
+  if (E <= 32) return f(std::integral_constant<int, 4>(), std::integral_constant<int, 8>());
+  if (E <= 64) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 8>());
+  if (E <= 128) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 8>());
+  if (E <= 256) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 16>());
+  if (E <= 512) return f(std::integral_constant<int, 32>(), std::integral_constant<int, 16>());
+  return f(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
+}
+
+int lanes_of(int64_t E) {
+  return by_experts(E, [](auto G, auto) { return (int)decltype(G)::value; });
+}
+
+// Forward workgroups: enough to hold two per CU, each at least one round of tokens; their partials
+// (E sums and counts each) are what the finishing workgroup reads.
+constexpr int MAX_BLOCKS = 512;
+int forward_blocks(int64_t T, int64_t E) {
+  const int64_t groups = FWD_THREADS / lanes_of(E);
+  return (int)std::max<int64_t>(1, std::min<int64_t>((T + groups - 1) / groups, MAX_BLOCKS));
+}
+
+bool io_ok(int dt) { return dt == MUON_DT_F32 || dt == MUON_DT_BF16 || dt == MUON_DT_F16; }
+
+int check(const char* what, int dtype, int64_t T, int64_t E, int64_t k, int64_t row) {
+  if (!io_ok(dtype)) {
+    muon_set_error("%s: unsupported dtype %d", what, dtype);
+    return MUON_ERR_DTYPE;
+  }
+  if (T < 0 || E < 1 || E > EMAX || k < 1 || k > E || k > KMAX || (T > 1 && row < 0)) {
+    muon_set_error("%s: bad extents (tokens %lld, experts %lld in 1..%d, top %lld in 1..%d and at "
+                   "most the experts)", what, (long long)T, (long long)E, EMAX, (long long)k, KMAX);
+    return MUON_ERR_SHAPE;
+  }
+  return MUON_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t muon_route_workspace_bytes(int64_t tokens, int64_t experts) {
+  if (tokens < 0 || experts < 1 || experts > EMAX) return -1;
+  return (int64_t)forward_blocks(tokens, experts) * (experts * 8 + 8);
+}
+
+int muon_route(const void* logits, int dtype, int64_t row_stride, int64_t tokens, int64_t experts,
+               int64_t top, int normalize, const void* token_mask, float* gates,
+               int64_t* chosen, int64_t* counts, float* balance, float* zloss, float* kept, void* ws,
+               void* stream) {
+  const int rc = check("route", dtype, tokens, experts, top, row_stride);
+  if (rc) return rc;
+  if (!counts || !balance || !zloss || !kept || !ws || (tokens && (!logits || !gates || !chosen))) {
+    muon_set_error("route: null tensor");
+    return MUON_ERR_ARG;
+  }
+  const int blocks = forward_blocks(tokens, experts);
+  Args a = {logits, row_stride, tokens, (int)experts, (int)top, normalize,
+            (const uint8_t*)token_mask, gates, chosen, counts, balance,
+            zloss, kept, (float*)ws, nullptr, nullptr, nullptr};
+  a.part_c = (int*)(a.part_p + (int64_t)blocks * experts);
+  a.part_z = (float*)(a.part_c + (int64_t)blocks * experts);
+  a.part_n = (int*)(a.part_z + blocks);
+  hipStream_t s = (hipStream_t)stream;
+  const int r = by_experts(experts, [&](auto G, auto V) {
+    constexpr int g = decltype(G)::value, v = decltype(V)::value;
+    if (dtype == MUON_DT_F32) route_kernel<MUON_DT_F32, g, v><<<blocks, FWD_THREADS, 0, s>>>(a);
+    else if (dtype == MUON_DT_BF16) route_kernel<MUON_DT_BF16, g, v><<<blocks, FWD_THREADS, 0, s>>>(a);
+    else route_kernel<MUON_DT_F16, g, v><<<blocks, FWD_THREADS, 0, s>>>(a);
+    MUON_CHECK_LAUNCH("route");
+    return MUON_OK;
+  });
+  if (r || blocks == 1) return r;
+  int C = 8;
+  while (C < experts && C < 1024) C *= 2;
+  route_finish_kernel<<<1, 1024, 0, s>>>(a, blocks, C);
+  MUON_CHECK_LAUNCH("route totals");
+  return MUON_OK;
+}
+
+int muon_route_backward(const void* logits, int dtype, int64_t row_stride, int64_t tokens,
+                        int64_t experts, int64_t top, int normalize, const void* token_mask,
+                        const int64_t* chosen, const int64_t* counts, const float* kept,
+                        const float* dgates, const float* dbalance, const float* dzloss,
+                        void* dlogits, void* stream) {
+  const int rc = check("route_backward", dtype, tokens, experts, top, row_stride);
+  if (rc || tokens == 0) return rc;
+  if (!logits || !chosen || !counts || !kept || !dlogits) {
+    muon_set_error("route_backward: null tensor");
+    return MUON_ERR_ARG;
+  }
+  const BackArgs a = {logits, row_stride, tokens, (int)experts, (int)top, normalize,
+                      (const uint8_t*)token_mask, chosen, counts, kept, dgates, dbalance, dzloss,
+                      dlogits};
+  hipStream_t s = (hipStream_t)stream;
+  return by_experts(experts, [&](auto G, auto V) {
+    constexpr int g = decltype(G)::value, v = decltype(V)::value;
+    const int64_t groups = BWD_THREADS / g;
+    const int grid = (int)std::min<int64_t>((tokens + groups - 1) / groups, 2048);
+    if (dtype == MUON_DT_F32) route_backward_kernel<MUON_DT_F32, g, v><<<grid, BWD_THREADS, 0, s>>>(a);
+    else if (dtype == MUON_DT_BF16) route_backward_kernel<MUON_DT_BF16, g, v><<<grid, BWD_THREADS, 0, s>>>(a);
+    else route_backward_kernel<MUON_DT_F16, g, v><<<grid, BWD_THREADS, 0, s>>>(a);
+    MUON_CHECK_LAUNCH("route_backward");
+    return MUON_OK;
+  });
+}
+
+}  // extern "C"

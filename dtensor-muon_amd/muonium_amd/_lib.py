@@ -102,6 +102,43 @@ _SIGNATURES = {
         [_c_int, _pp, _c_int, _pp, _pp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_f32,
          _c_int, _c_int, _vp, _c_int, _c_i64, _vp],
     ),
+    "muon_qk_norm_rope": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_i64, _vp, _c_int, _c_i64, _vp, _vp, _c_int,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_f32, _vp],
+    ),
+    "muon_qk_norm_rope_workspace_bytes": (_c_i64, [_c_i64]),
+    "muon_qk_norm_rope_backward": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_i64, _vp, _c_int, _c_i64, _vp,
+         _vp, _vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int,
+         _c_f32, _vp],
+    ),
+    "muon_route_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "muon_route": (
+        _c_int,
+        [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+         _vp, _vp],
+    ),
+    "muon_route_backward": (
+        _c_int,
+        [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+         _vp, _vp],
+    ),
+    "muon_token_logprobs_workspace_bytes": (_c_i64, [_c_int, _c_i64, _c_i64]),
+    "muon_token_logprobs": (
+        _c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_f32, _vp, _vp, _vp, _vp]
+    ),
+    "muon_token_logprobs_backward": (
+        _c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_f32, _vp, _vp, _vp, _vp, _vp]
+    ),
+    "muon_policy_loss_one_pass": (_c_int, [_c_int, _c_i64]),
+    "muon_policy_loss": (
+        _c_int,
+        [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_f32, _c_f32, _c_f32,
+         _c_f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "muon_scale_gradient": (_c_int, [_vp, _c_int, _c_i64, _vp, _vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -1,0 +1,95 @@
+"""Norm of queries and keys per head with the position rotation (libmuon_amd
+``muon_qk_norm_rope``). No counterpart in the reference."""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from .. import _row_ops
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _check_on(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+
+
+def qk_norm_rope(
+    q: Tensor,
+    k: Tensor,
+    q_weight: Tensor | None = None,
+    k_weight: Tensor | None = None,
+    cos: Tensor | None = None,
+    sin: Tensor | None = None,
+    positions: Tensor | None = None,
+    *,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+) -> tuple[Tensor, Tensor]:
+    """The RMS norm of every query and key head, then the rotation by the token's position, in
+    one pass: ``n = x / sqrt(mean(x^2) + eps) * weight`` over the last dimension, and
+    ``(a, b) -> (a cos - b sin, b cos + a sin)`` for the pairs of its first ``rotary`` values.
+
+    Args:
+        q, k: ``(batch, tokens, heads, dim)`` or ``(tokens, heads, dim)``, fp32, bf16 or fp16,
+            ``dim`` at most 1024; any strides (slices of a fused projection are read in
+            place) with a contiguous last dimension (others are copied first). k may have fewer
+            heads.
+        q_weight, k_weight: ``(dim,)`` gains of one floating type, or None for ones.
+        cos, sin: ``(length, rotary / 2)`` fp32 tables, or None for no rotation. ``rotary`` may be
+            less than ``dim``: the rest passes unturned.
+        positions: int32 or int64 rows of the tables, ``(tokens,)`` or ``(batch, tokens)``;
+            None: token t is at position t. A position outside the table makes its token NaN.
+        interleaved: pairs are (2i, 2i + 1) instead of (i, i + rotary / 2).
+
+    Returns the new queries and keys, contiguous, in their input's type. Differentiable in q, k
+    and the weights; computed in fp32 and rounded once."""
+    if q.dim() not in (3, 4) or k.dim() != q.dim():
+        raise ValueError(f"q and k are (batch, tokens, heads, dim) or (tokens, heads, dim); got "
+                         f"{tuple(q.shape)} and {tuple(k.shape)}")
+    if q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
+        raise ValueError(f"q and k differ in batch, tokens or dim: {tuple(q.shape)} and "
+                         f"{tuple(k.shape)}")
+    dim, device = q.shape[-1], q.device
+    if q.dtype not in _FLOATS or k.dtype != q.dtype:
+        raise TypeError(f"q and k are both fp32, bf16 or fp16; got {q.dtype} and {k.dtype}")
+    if not 1 <= dim <= 1024:
+        raise ValueError(f"dim is 1 to 1024; got {dim}")
+    _check_on(device, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin,
+              positions=positions)
+    for w in (q_weight, k_weight):
+        if w is not None:
+            if w.shape != (dim,):
+                raise ValueError(f"weights are ({dim},); got {tuple(w.shape)}")
+            if w.dtype not in _FLOATS:
+                raise TypeError(f"weights are fp32, bf16 or fp16; got {w.dtype}")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise TypeError(f"weights of two types: {q_weight.dtype} and {k_weight.dtype}")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] > dim:
+            raise ValueError(f"cos and sin are (length, rotary / 2) with rotary at most {dim}; got "
+                             f"{tuple(cos.shape)} and {tuple(sin.shape)}")
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            raise TypeError(f"cos and sin are fp32; got {cos.dtype} and {sin.dtype}")
+        if cos.requires_grad or sin.requires_grad:
+            raise ValueError("cos and sin are tables: no gradient is made for them")
+        cos, sin = cos.contiguous(), sin.contiguous()
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"positions are int32 or int64; got {positions.dtype}")
+        if positions.shape not in ((q.shape[-3],), tuple(q.shape[:-2])):
+            raise ValueError(f"positions are ({q.shape[-3]},) or {tuple(q.shape[:-2])}; got "
+                             f"{tuple(positions.shape)}")
+        positions = _row_ops._unit_last(positions)
+    elif cos is not None and q.shape[-3] > cos.shape[0]:
+        raise ValueError(f"{q.shape[-3]} tokens, but the tables have {cos.shape[0]} positions")
+    return _row_ops.qk_norm_rope(
+        _row_ops._unit_last(q), _row_ops._unit_last(k),
+        None if q_weight is None else q_weight.contiguous(),
+        None if k_weight is None else k_weight.contiguous(), cos, sin, positions, float(eps),
+        bool(interleaved))

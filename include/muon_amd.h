@@ -250,6 +250,90 @@ int muon_lp_prepass(int ntensors, void* const* grads, int g_dtype, void* const* 
                     int64_t nb, int64_t rows, int64_t cols, float momentum, int nesterov,
                     int maximize, void* ws, int ws_dtype, int64_t ws_batch, void* stream);
 
+/* ---- Row operators of the training step -----------------------------------------------
+ * No counterpart in the reference: what a model's forward and backward pass computes beside
+ * its matrix products and attention, where this optimizer's parameters are trained. Inputs of
+ * fp32, bf16 or fp16, every sum and exponential in fp32 or more, one rounding at the output.
+ * Strides are in elements; the last dimension is contiguous. Nothing is allocated; a call is
+ * one to three launches on the given stream, with the same bits on every run.
+ *
+ * Queries and keys: per head of `dim` values (at most 1024) the RMS norm
+ * n = x / sqrt(mean(x^2) + eps) * weight, and the rotation of its first `rotary` values (even)
+ * by the angles of the token's position: (a c - b s, b c + a s) for the pairs (i, i + rotary/2),
+ * or (2i, 2i+1) when interleaved. strides: batch, token, head of q, then of k (backward: then of
+ * dq_out and dk_out); outputs and dq, dk are contiguous (batch, tokens, heads, dim). Weights
+ * (w_dtype, dim values) may be NULL. cos and sin are (table_len, rotary/2) fp32; positions
+ * (pos_bits 32 or 64; NULL: token t is at t) may be shared by the batches
+ * (pos_batch_stride 0). A position outside the table gives NaN, and nothing is read there.
+ * The backward pass needs ws of muon_qk_norm_rope_workspace_bytes(dim) for weight gradients. */
+int muon_qk_norm_rope(const void* q, const void* k, const int64_t* strides, const void* q_weight,
+                      const void* k_weight, int w_dtype, const float* cosv, const float* sinv,
+                      int64_t table_len, const void* positions, int pos_bits,
+                      int64_t pos_batch_stride, void* q_out, void* k_out, int dtype, int64_t batch,
+                      int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t dim,
+                      int64_t rotary, int interleaved, float eps, void* stream);
+int64_t muon_qk_norm_rope_workspace_bytes(int64_t dim);
+int muon_qk_norm_rope_backward(const void* q, const void* k, const void* dq_out,
+                               const void* dk_out, const int64_t* strides, const void* q_weight,
+                               const void* k_weight, int w_dtype, const float* cosv,
+                               const float* sinv, int64_t table_len, const void* positions,
+                               int pos_bits, int64_t pos_batch_stride, void* dq, void* dk,
+                               void* dq_weight, void* dk_weight, void* ws, int dtype,
+                               int64_t batch, int64_t tokens, int64_t q_heads, int64_t k_heads,
+                               int64_t dim, int64_t rotary, int interleaved, float eps,
+                               void* stream);
+
+/* Expert routing of (tokens, experts) logits (at most 1024 experts): the `top` (at most 64)
+ * largest logits of each token in descending order, ties by the lower index, a NaN as the
+ * largest; an expert at -inf is never chosen, and a slot that finds none holds -1 with gate 0.
+ * gates (tokens, top) fp32: the softmax values, or (normalize) these over their sum. Tokens
+ * whose token_mask byte is 0 (NULL: none) and tokens with all logits -inf choose nothing and
+ * count nowhere. Over the N others (*kept): counts[e] = tokens that chose e;
+ * balance = experts * sum_e counts[e] / (top N) * mean_t softmax_te; zloss = mean_t lse_t^2
+ * (both 0 for N = 0). Any of dgates, dbalance, dzloss may be NULL (no gradient from there). */
+int64_t muon_route_workspace_bytes(int64_t tokens, int64_t experts);
+int muon_route(const void* logits, int dtype, int64_t row_stride, int64_t tokens, int64_t experts,
+               int64_t top, int normalize, const void* token_mask, float* gates,
+               int64_t* chosen, int64_t* counts, float* balance, float* zloss, float* kept,
+               void* ws, void* stream);
+int muon_route_backward(const void* logits, int dtype, int64_t row_stride, int64_t tokens,
+                        int64_t experts, int64_t top, int normalize, const void* token_mask,
+                        const int64_t* chosen, const int64_t* counts, const float* kept,
+                        const float* dgates, const float* dbalance, const float* dzloss,
+                        void* dlogits, void* stream);
+
+/* logprobs[n] = log softmax(logits[n] / temperature)[tokens[n]] in fp32. A negative token leaves
+ * its row out (0, and no gradient; the row is not read); one of `vocab` or more gives NaN. stats
+ * (2 * rows floats, NULL: not kept) is what the backward pass needs beside the logits, ws holds
+ * muon_token_logprobs_workspace_bytes (0: may be NULL). Backward: dlogits (rows, vocab), contiguous, from
+ * dlogprobs (rows) times *scale (NULL: 1); a row whose gradient is 0 is not read. */
+int64_t muon_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab);
+int muon_token_logprobs(const void* logits, int dtype, int64_t row_stride, int64_t rows,
+                        int64_t vocab, const int64_t* tokens, float temperature, float* logprobs,
+                        float* stats, void* ws, void* stream);
+int muon_token_logprobs_backward(const void* logits, int dtype, int64_t row_stride, int64_t rows,
+                                 int64_t vocab, const int64_t* tokens, float temperature,
+                                 const float* stats, const float* dlogprobs, const float* scale,
+                                 void* dlogits, void* stream);
+
+/* The clipped policy loss: with r = exp(logprob - old), per row
+ *   term = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *          + kl_coef (exp(ref - logprob) - (ref - logprob) - 1)      (ref_logprobs NULL: without)
+ * and *loss = sum weights * term. Rows of weight 0 are left out like negative tokens. terms holds
+ * one float a row. The gradient either in the same pass (dlogits, for a loss gradient of 1; where
+ * muon_policy_loss_one_pass says the row fits a workgroup's registers), or later by
+ * muon_token_logprobs_backward with dlogprobs = coef and the kept stats (both may be NULL
+ * when not needed). muon_scale_gradient multiplies n values by *scale in place (a scale of 1
+ * touches nothing). */
+int muon_policy_loss_one_pass(int dtype, int64_t vocab);
+int muon_policy_loss(const void* logits, int dtype, int64_t row_stride, int64_t rows,
+                     int64_t vocab, const int64_t* tokens, const float* old_logprobs,
+                     const float* advantages, const float* weights, const float* ref_logprobs,
+                     float clip_low, float clip_high, float kl_coef, float temperature,
+                     float* loss, float* logprobs, float* terms, float* stats, float* coef,
+                     void* dlogits, void* ws, void* stream);
+int muon_scale_gradient(void* x, int dtype, int64_t n, const float* scale, void* stream);
+
 /* ---- Kernel timing (measurement support) ------------------------------------------
  * No counterpart in the reference. While enabled, every kernel the step entry points
  * launch is bracketed by hipEvents on its own stream; muon_timing_read() waits for
