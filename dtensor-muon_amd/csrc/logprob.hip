@@ -70,16 +70,21 @@ MUON_DEVICE void add_values(Sum& a, const float (&v)[N], float k) {
   a.m = m;
 }
 
+MUON_DEVICE Sum first_lane(Sum v) {
+  return {__int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v.m))),
+          __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v.s)))};
+}
+
 // Joined over a workgroup of NT threads in a fixed order; the result in every thread.
 template <int NT>
 MUON_DEVICE Sum block_join(Sum v, float k, Sum* lds) {
-  v = group_reduce<64>(v, [k](Sum a, Sum b) { return join(a, b, k); });
+  auto op = [k](Sum a, Sum b) { return join(a, b, k); };
+  v = group_reduce<64>(v, op);
+  // the two operands' order decides the last bit: every lane takes the first one's
+  if constexpr (NT == 64) return first_lane(v);
   if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
   __syncthreads();
-  Sum r = lds[0];
-#pragma unroll
-  for (int w = 1; w < NT / 64; ++w) r = join(r, lds[w], k);
-  return r;
+  return first_lane(group_reduce<NT / 64>(lds[threadIdx.x % (NT / 64)], op));
 }
 
 // Values [i0, i0 + N) of a row that ends at V; -inf behind it.
@@ -98,16 +103,33 @@ MUON_DEVICE void store_tail(void* x, int64_t at, int64_t i0, int64_t V, const fl
     if (i0 + e < V) Elem<DT>::store(x, at + i0 + e, v[e]);
 }
 
-// What a row's sum gives: logp, and for the policy loss its term and slope g. One thread; in
-// double, since logp is the small difference of larger numbers and the loss a sum of terms of
-// both signs (one row's worth of it costs nothing beside the row).
+template <bool STREAM>
+MUON_DEVICE void put(void* p, muon_u4 w) {
+  if constexpr (STREAM) store_u4_nt(p, w);
+  else store_u4(p, w);
+}
+
+// log s for s in 1..2^31 (s is 0, infinite or NaN where a row has no sum), to 2^-24 of one: the
+// hardware's logarithm of the fraction beside the whole exponent, which a single fp32 result
+// would round away.
+MUON_DEVICE double log_of(float s) {
+  constexpr double LN2_D = 0.69314718055994530942;
+  if (!(s > 0.0f && s < INFINITY)) return s == 0.0f ? -INFINITY : s;
+  return LN2_D * ((double)__builtin_amdgcn_frexp_expf(s) +
+                  (double)__builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(s)));
+}
+MUON_DEVICE float exp_of(double x) { return __builtin_amdgcn_exp2f((float)(x * LOG2E_D)); }
+
+// What a row's sum gives: logp, and for the policy loss its term and slope g. One thread, while
+// its workgroup waits: differences, which cancel, in double, and exponentials of what is left in
+// fp32 (with double ones the loss on 128000 values a row took 8% longer).
 template <int DT>
 MUON_DEVICE float finish_row(const Rows& a, const Policy& p, int64_t row, Sum t) {
   const int64_t tok = a.tokens[row];
   double logp = __builtin_nan("");
   if (tok < a.V) {
-    const double xt = Elem<DT>::load(a.x, row * a.stride + tok);
-    logp = (xt - (double)t.m) * a.tau_inv - log((double)t.s);
+    const float xt = Elem<DT>::load(a.x, row * a.stride + tok);
+    logp = ((double)xt - (double)t.m) * a.tau_inv - log_of(t.s);
   }
   a.logp[row] = (float)logp;
   if (a.stats) {
@@ -115,22 +137,23 @@ MUON_DEVICE float finish_row(const Rows& a, const Policy& p, int64_t row, Sum t)
     a.stats[a.N + row] = tok < a.V ? 1.0f / t.s : __int_as_float(0x7fc00000);
   }
   if (!p.weights) return 0.0f;
-  const double w = p.weights[row], A = p.adv[row], r = exp(logp - (double)p.old[row]);
-  const double low = 1.0 - (double)p.lo, high = 1.0 + (double)p.hi;
+  const float w = p.weights[row], A = p.adv[row], r = exp_of(logp - (double)p.old[row]);
+  const float low = 1.0f - p.lo, high = 1.0f + p.hi;
   // NaN ratios stay NaN: comparisons below leave r in place
-  const double clipped = r < low ? low : r > high ? high : r;
-  const double plain = r * A, other = clipped * A;
-  double term = -(other < plain ? other : plain);
+  const float clipped = r < low ? low : r > high ? high : r;
+  const float plain = r * A, other = clipped * A;
+  float term = -(other < plain ? other : plain);
   // the smaller one is r A where r is inside, or outside on the side that A pulls it back from
-  const bool cut = A >= 0.0 ? r > high : r < low;
-  double slope = cut ? 0.0 : -plain;
+  const bool cut = A >= 0.0f ? r > high : r < low;
+  float slope = cut ? 0.0f : -plain;
   if (p.ref) {
-    const double ahead = (double)p.ref[row] - logp, e = exp(ahead);
-    term += (double)p.beta * (e - ahead - 1.0);
-    slope += (double)p.beta * (1.0 - e);
+    const double ahead = (double)p.ref[row] - logp;
+    const double e = exp_of(ahead);
+    term += p.beta * (float)(e - ahead - 1.0);
+    slope += p.beta * (float)(1.0 - e);
   }
-  p.terms[row] = (float)(w * term);
-  const float g = (float)(w * slope);
+  p.terms[row] = w * term;
+  const float g = w * slope;
   if (p.coef) p.coef[row] = g;
   return g;
 }
@@ -144,15 +167,14 @@ MUON_DEVICE void skip_row(const Rows& a, const Policy& p, int64_t row) {
   }
 }
 
-constexpr int SUM_THREADS = 512;
 constexpr int SUM_UNROLL = 4;  // 16-byte loads in flight per thread
 
 // One pass over (a slice of) a row with a running maximum and sum. Grid: slices x rows; with
 // one slice a row the workgroup finishes its row, else it leaves (m, s) for logp_join_kernel.
-template <int DT>
-__global__ __launch_bounds__(SUM_THREADS) void logp_kernel(Rows a, Policy p, Sum* part) {
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void logp_kernel(Rows a, Policy p, Sum* part) {
   constexpr int N = Vec16<DT>::N;
-  __shared__ Sum lds[SUM_THREADS / 64];
+  __shared__ Sum lds[NT / 64];
   const int slices = gridDim.x;
   for (int64_t row = blockIdx.y; row < a.N; row += gridDim.y) {
     if (left_out(a, p, row)) {
@@ -164,10 +186,10 @@ __global__ __launch_bounds__(SUM_THREADS) void logp_kernel(Rows a, Policy p, Sum
     const int64_t begin = vecs * blockIdx.x / slices, end = vecs * (blockIdx.x + 1) / slices;
     Sum t = {-INFINITY, 0.0f};
     int64_t i = begin + threadIdx.x;
-    for (; i + (SUM_UNROLL - 1) * SUM_THREADS < end; i += SUM_UNROLL * SUM_THREADS) {
+    for (; i + (SUM_UNROLL - 1) * NT < end; i += SUM_UNROLL * NT) {
       muon_u4 w[SUM_UNROLL];
 #pragma unroll
-      for (int u = 0; u < SUM_UNROLL; ++u) w[u] = load_u4(elem_at<DT>(a.x, at + (i + u * SUM_THREADS) * N));
+      for (int u = 0; u < SUM_UNROLL; ++u) w[u] = load_u4(elem_at<DT>(a.x, at + (i + u * NT) * N));
       float v[SUM_UNROLL * N];
 #pragma unroll
       for (int u = 0; u < SUM_UNROLL; ++u) {
@@ -178,7 +200,7 @@ __global__ __launch_bounds__(SUM_THREADS) void logp_kernel(Rows a, Policy p, Sum
       }
       add_values(t, v, a.k);
     }
-    for (; i < end; i += SUM_THREADS) {
+    for (; i < end; i += NT) {
       float v[N];
       Vec16<DT>::unpack(load_u4(elem_at<DT>(a.x, at + i * N)), v);
       add_values(t, v, a.k);
@@ -187,7 +209,7 @@ __global__ __launch_bounds__(SUM_THREADS) void logp_kernel(Rows a, Policy p, Sum
       const float v[1] = {Elem<DT>::load(a.x, at + vecs * N + threadIdx.x)};
       add_values(t, v, a.k);
     }
-    t = block_join<SUM_THREADS>(t, a.k, lds);
+    t = block_join<NT>(t, a.k, lds);
     if (threadIdx.x == 0) {
       if (slices == 1) finish_row<DT>(a, p, row, t);
       else part[row * slices + blockIdx.x] = t;
@@ -223,14 +245,16 @@ struct Back {
   void* dx;  // contiguous
 };
 
-// dx of one run of values of a row; tok - i0 is the token's place in it, if any.
+// dx of one run of values of a row; tok is the token's place in it, if it is there at all.
 template <int DT>
 MUON_DEVICE void slopes(const float (&x)[Vec16<DT>::N], float m, float k, float pc, float g,
                         int64_t tok, float (&d)[Vec16<DT>::N]) {
+  constexpr int N = Vec16<DT>::N;
 #pragma unroll
-  for (int e = 0; e < Vec16<DT>::N; ++e) {
-    const float q = pc * __builtin_amdgcn_exp2f((x[e] - m) * k);
-    d[e] = tok == e ? g - q : -q;
+  for (int e = 0; e < N; ++e) d[e] = -pc * __builtin_amdgcn_exp2f((x[e] - m) * k);
+  if ((uint64_t)tok < (uint64_t)N) {  // one run of the row
+#pragma unroll
+    for (int e = 0; e < N; ++e) d[e] += tok == e ? g : 0.0f;
   }
 }
 
@@ -238,7 +262,7 @@ constexpr int BACK_THREADS = 256;
 constexpr int BACK_VECS = 4;  // 16-byte pieces per thread
 
 // The gradient from the logits again and the kept m and 1 / s. Grid: pieces of a row x rows.
-template <int DT>
+template <int DT, bool STREAM>
 __global__ __launch_bounds__(BACK_THREADS) void logp_backward_kernel(Back a) {
   constexpr int N = Vec16<DT>::N;
   const float scale = a.scale ? a.scale[0] : 1.0f;
@@ -251,7 +275,7 @@ __global__ __launch_bounds__(BACK_THREADS) void logp_backward_kernel(Back a) {
 #pragma unroll
       for (int u = 0; u < BACK_VECS; ++u) {
         const int64_t i = i0 + (int64_t)u * BACK_THREADS * N;
-        if (i + N <= a.V) store_u4((void*)elem_at<DT>(a.dx, to + i), muon_u4{0, 0, 0, 0});
+        if (i + N <= a.V) put<STREAM>((void*)elem_at<DT>(a.dx, to + i), muon_u4{0, 0, 0, 0});
         else if (i < a.V) {
           const float z[N] = {};
           store_tail<DT>(a.dx, to, i, a.V, z);
@@ -274,7 +298,7 @@ __global__ __launch_bounds__(BACK_THREADS) void logp_backward_kernel(Back a) {
       float x[N], d[N];
       Vec16<DT>::unpack(w[u], x);
       slopes<DT>(x, m, a.k, pc, g, tok - i, d);
-      if (i + N <= a.V) store_u4((void*)elem_at<DT>(a.dx, to + i), Vec16<DT>::pack(d));
+      if (i + N <= a.V) put<STREAM>((void*)elem_at<DT>(a.dx, to + i), Vec16<DT>::pack(d));
       else store_tail<DT>(a.dx, to, i, a.V, d);
     }
   }
@@ -283,7 +307,7 @@ __global__ __launch_bounds__(BACK_THREADS) void logp_backward_kernel(Back a) {
 // The policy loss with its gradient in one pass over the logits: a workgroup holds its whole row
 // in registers (NV 16-byte pieces a thread), sums it, makes the slope g, and writes the gradient
 // from the same registers.
-template <int DT, int NT, int NV>
+template <int DT, int NT, int NV, bool STREAM>
 __global__ __launch_bounds__(NT) void policy_row_kernel(Rows a, Policy p, void* dx, int64_t row0) {
   constexpr int N = Vec16<DT>::N;
   __shared__ Sum lds[NT / 64];
@@ -301,7 +325,7 @@ __global__ __launch_bounds__(NT) void policy_row_kernel(Rows a, Policy p, void* 
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int i = u * NT + tid;
-      if (i < vecs) store_u4(dr + (int64_t)u * NT * 16 + off, muon_u4{0, 0, 0, 0});
+      if (i < vecs) put<STREAM>(dr + (int64_t)u * NT * 16 + off, muon_u4{0, 0, 0, 0});
       else if (i == vecs) {
         const float z[N] = {};
         store_tail<DT>(dx, to, (int64_t)i * N, V, z);
@@ -323,12 +347,19 @@ __global__ __launch_bounds__(NT) void policy_row_kernel(Rows a, Policy p, void* 
     }
   }
   Sum t = {-INFINITY, 0.0f};
+  // few pieces unpacked at a time: the row itself takes most of the registers
+  constexpr int STEP = NV <= 16 ? 2 : 1;
 #pragma unroll
-  for (int u = 0; u < NV; ++u) {
-    float v[N];
-    Vec16<DT>::unpack(w[u], v);
+  for (int u = 0; u < NV; u += STEP) {
+    float v[STEP * N];
+#pragma unroll
+    for (int i = 0; i < STEP; ++i) {
+      float h[N];
+      Vec16<DT>::unpack(w[u + i], h);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[i * N + e] = h[e];
+    }
     add_values(t, v, a.k);
-    // one piece unpacked at a time: the row itself takes most of the registers
     __builtin_amdgcn_sched_barrier(0);
   }
   t = block_join<NT>(t, a.k, lds);
@@ -347,7 +378,7 @@ __global__ __launch_bounds__(NT) void policy_row_kernel(Rows a, Policy p, void* 
     asm("" : "+v"(w[u]));
     Vec16<DT>::unpack(w[u], v);
     slopes<DT>(v, t.m, a.k, pc, g, tok - i * N, d);
-    if (i < vecs) store_u4(dr + (int64_t)u * NT * 16 + off, Vec16<DT>::pack(d));
+    if (i < vecs) put<STREAM>(dr + (int64_t)u * NT * 16 + off, Vec16<DT>::pack(d));
     else if (i == vecs) store_tail<DT>(dx, to, (int64_t)i * N, V, d);
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -407,6 +438,18 @@ int check(const char* what, int dtype, int64_t N, int64_t V, int64_t stride, flo
 }
 
 constexpr int64_t MAX_GRID_Y = 65535;
+// Gradients of this many bytes are stored past the caches (half of the 256 MB last-level one).
+constexpr int64_t STREAM_FROM = 128 << 20;
+
+template <int DT>
+void launch_backward(const Back& a, hipStream_t s) {
+  const int64_t per = (int64_t)BACK_THREADS * BACK_VECS * Vec16<DT>::N;
+  const dim3 grid((unsigned)((a.V + per - 1) / per), (unsigned)std::min(a.N, MAX_GRID_Y));
+  if (a.N * a.V * (DT == MUON_DT_F32 ? 4 : 2) >= STREAM_FROM)
+    logp_backward_kernel<DT, true><<<grid, BACK_THREADS, 0, s>>>(a);
+  else
+    logp_backward_kernel<DT, false><<<grid, BACK_THREADS, 0, s>>>(a);
+}
 
 // Slices of a row: until a launch has four workgroups per CU, but none of less than 16 KB (one
 // round of a workgroup's loads is 32 KB).
@@ -416,13 +459,28 @@ int slices_for(int dtype, int64_t N, int64_t V) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, bytes / 16384), 64));
 }
 
+// Threads a row: the fewest that give 2^18 in all (four waves per SIMD), with at most 64
+// 16-byte pieces each (32 above a wave). 8192 rows of bf16 with 64, 128, 256 and 512 threads:
+// 2000 values 12, 14, 20, 40 us, 16000 values 45, 44, 47, 77 us; 4096 rows of 32000 values 42, 46,
+// 44, 52 us; 8192 rows of 128000 values with 256 and 512: 348 and 334 us.
+template <int DT>
+void launch_sums_dt(const Rows& a, const Policy& p, int slices, Sum* part, hipStream_t s) {
+  const dim3 grid(slices, (unsigned)std::min(a.N, MAX_GRID_Y));
+  const int64_t vecs = a.V / Vec16<DT>::N;
+  int threads = vecs <= 64 * 64 ? 64 : vecs <= 32 * 128 ? 128 : vecs <= 32 * 256 ? 256 : 512;
+  while (threads < 512 && a.N * threads < (1 << 18)) threads *= 2;
+  if (threads == 64) logp_kernel<DT, 64><<<grid, 64, 0, s>>>(a, p, part);
+  else if (threads == 128) logp_kernel<DT, 128><<<grid, 128, 0, s>>>(a, p, part);
+  else if (threads == 256) logp_kernel<DT, 256><<<grid, 256, 0, s>>>(a, p, part);
+  else logp_kernel<DT, 512><<<grid, 512, 0, s>>>(a, p, part);
+}
+
 int launch_sums(const Rows& a, const Policy& p, int dtype, void* ws, hipStream_t s) {
   const int slices = slices_for(dtype, a.N, a.V);
-  const dim3 grid(slices, (unsigned)std::min(a.N, MAX_GRID_Y));
   Sum* part = (Sum*)ws;
-  if (dtype == MUON_DT_F32) logp_kernel<MUON_DT_F32><<<grid, SUM_THREADS, 0, s>>>(a, p, part);
-  else if (dtype == MUON_DT_BF16) logp_kernel<MUON_DT_BF16><<<grid, SUM_THREADS, 0, s>>>(a, p, part);
-  else logp_kernel<MUON_DT_F16><<<grid, SUM_THREADS, 0, s>>>(a, p, part);
+  if (dtype == MUON_DT_F32) launch_sums_dt<MUON_DT_F32>(a, p, slices, part, s);
+  else if (dtype == MUON_DT_BF16) launch_sums_dt<MUON_DT_BF16>(a, p, slices, part, s);
+  else launch_sums_dt<MUON_DT_F16>(a, p, slices, part, s);
   MUON_CHECK_LAUNCH("token_logprobs");
   if (slices == 1) return MUON_OK;
   const unsigned blocks = (unsigned)((a.N + 3) / 4);
@@ -436,12 +494,14 @@ int launch_sums(const Rows& a, const Policy& p, int dtype, void* ws, hipStream_t
 template <int DT>
 int launch_policy_rows(const Rows& a, const Policy& p, void* dx, hipStream_t s) {
   const int64_t vecs = (a.V + Vec16<DT>::N - 1) / Vec16<DT>::N;
+  const bool stream = a.N * a.V * (DT == MUON_DT_F32 ? 4 : 2) >= STREAM_FROM;
 #define MUON_POLICY_ROWS(NT, NV)                                      \
   if (vecs <= (int64_t)NT * NV) {                                     \
     /* a launch holds fewer than 2^32 threads */                      \
     for (int64_t r = 0; r < a.N; r += 1 << 20) {                      \
       const unsigned rows = (unsigned)std::min<int64_t>(a.N - r, 1 << 20); \
-      policy_row_kernel<DT, NT, NV><<<rows, NT, 0, s>>>(a, p, dx, r); \
+      if (stream) policy_row_kernel<DT, NT, NV, true><<<rows, NT, 0, s>>>(a, p, dx, r); \
+      else policy_row_kernel<DT, NT, NV, false><<<rows, NT, 0, s>>>(a, p, dx, r); \
       MUON_CHECK_LAUNCH("policy_loss");                               \
     }                                                                 \
     return MUON_OK;                                                   \
@@ -497,12 +557,10 @@ int muon_token_logprobs_backward(const void* logits, int dtype, int64_t row_stri
   const double inv = 1.0 / (double)temperature;
   const Back a = {logits, row_stride, rows, vocab, tokens, stats, dlogprobs, scale,
                   (float)(LOG2E_D * inv), (float)inv, dlogits};
-  const int64_t per = (int64_t)BACK_THREADS * BACK_VECS * (dtype == MUON_DT_F32 ? 4 : 8);
-  const dim3 grid((unsigned)((vocab + per - 1) / per), (unsigned)std::min(rows, MAX_GRID_Y));
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == MUON_DT_F32) logp_backward_kernel<MUON_DT_F32><<<grid, BACK_THREADS, 0, s>>>(a);
-  else if (dtype == MUON_DT_BF16) logp_backward_kernel<MUON_DT_BF16><<<grid, BACK_THREADS, 0, s>>>(a);
-  else logp_backward_kernel<MUON_DT_F16><<<grid, BACK_THREADS, 0, s>>>(a);
+  if (dtype == MUON_DT_F32) launch_backward<MUON_DT_F32>(a, s);
+  else if (dtype == MUON_DT_BF16) launch_backward<MUON_DT_BF16>(a, s);
+  else launch_backward<MUON_DT_F16>(a, s);
   MUON_CHECK_LAUNCH("token_logprobs_backward");
   return MUON_OK;
 }
@@ -560,7 +618,7 @@ int muon_scale_gradient(void* x, int dtype, int64_t n, const float* scale, void*
     return MUON_ERR_ARG;
   }
   if (n == 0) return MUON_OK;
-  const int grid = (int)std::min<int64_t>((n / 2048) + 1, 2048);
+  const int grid = (int)std::min<int64_t>((n / 2048) + 1, 1024);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == MUON_DT_F32) scale_kernel<MUON_DT_F32><<<grid, 256, 0, s>>>(x, n, scale);
   else if (dtype == MUON_DT_BF16) scale_kernel<MUON_DT_BF16><<<grid, 256, 0, s>>>(x, n, scale);

@@ -47,7 +47,11 @@ struct Args {
 // token's angles and the weights are read once for all of them.
 constexpr int HC = 4;
 constexpr int NTHREADS = 256;
-constexpr int MAX_BWD_BLOCKS = 1024;
+constexpr int MAX_PAIRS = 9;  // SINGLE: up to 2 * 9 * 64 values a row
+constexpr int MAX_BWD_BLOCKS = 1024;  // of SINGLE; the others take half
+// Outputs of this many bytes (half of the 256 MB last-level cache) whose runs make whole 64-byte
+// pieces are stored past the caches.
+constexpr int64_t NT_FROM = 128 << 20;
 constexpr int64_t MAX_FWD_BLOCKS = 1 << 22;
 
 MUON_DEVICE void store_w(void* w, int wdt, int64_t i, float v) {
@@ -67,39 +71,79 @@ MUON_DEVICE int64_t position(const Args& a, int64_t b, int64_t t) {
   return p >= 0 && p < a.table_len ? p : -1;
 }
 
-// A lane's share of a row. Vec: 16 values in two runs of 8, which hold both partners of each
-// rotated pair, so the rotation needs no exchange: the runs at 8u and R/2 + 8u (halves) or one
-// run of 16 (interleaved, and behind R, where nothing turns). Needs D and R in 16s.
-// Otherwise NP pairs of single values, G apart: for any D and any even R.
-template <int DT, int G, int NP, bool VEC>
+// How a row's values are shared out over its lanes.
+//  WHOLE: two runs of W values (16 bytes) a lane, which hold both partners of each rotated pair, so
+//    the rotation needs no exchange between lanes: the runs at W u and R/2 + W u (halves), or
+//    2 W u and 2 W u + W (interleaved, and behind R, where nothing turns). D and R in multiples of
+//    2 W.
+//  RAGGED: the same runs for any other D and R of at least a run a part: a part's last run is moved
+//    back to end where the part ends, so that it too is one access; the values it shares with
+//    the run before are computed twice, alike, and counted once in sums (the first `skip` of a run
+//    are left out).
+//  SINGLE: NP pairs of single values a lane, G apart, for what is too small for a run.
+enum Form { WHOLE, RAGGED, SINGLE };
+
+template <int DT, int G, int NP, Form F, bool NT>
 struct Lane {
-  static constexpr int N = VEC ? 16 : 2 * NP;
-  int lo, hi;             // VEC: the first elements of the two runs
-  int at[VEC ? 1 : N];    // otherwise the element of each value, -1: none
-  int ang[VEC ? 1 : NP];  // index of a pair's angle, -1: not turned
-  bool on;    // VEC: this lane has values
+  static constexpr bool RUNS = F != SINGLE;
+  static constexpr int W = DT == MUON_DT_F32 ? 4 : 8;
+  static constexpr int N = RUNS ? 2 * W : 2 * NP;
+  int lo, hi;              // RUNS: the first elements of the two runs
+  int skip_lo, skip_hi;    // RAGGED: values at their start that belong to another lane
+  int at[RUNS ? 1 : N];    // SINGLE: the element of each value, -1: none
+  int ang[RUNS ? 1 : NP];  // index of a pair's angle, -1: not turned
+  bool on;                 // RUNS: this lane has values
 
   MUON_DEVICE void init(const Args& a, int lane) {
-    const int R = a.R, D = a.D;
-    if constexpr (VEC) {
-      on = lane < D / 16;
-      const bool turned = lane < R / 16;
-      ang[0] = turned ? 8 * lane : -1;
-      lo = turned && !a.inter ? 8 * lane : 16 * lane;
-      hi = turned && !a.inter ? R / 2 + 8 * lane : 16 * lane + 8;
+    const int R = a.R, D = a.D, half = R / 2;
+    if constexpr (F == WHOLE) {
+      on = lane < D / (2 * W);
+      const bool turned = lane < R / (2 * W);
+      ang[0] = turned ? W * lane : -1;
+      lo = turned && !a.inter ? W * lane : 2 * W * lane;
+      hi = turned && !a.inter ? half + W * lane : 2 * W * lane + W;
       if (!on) lo = hi = 0;
+      skip_lo = skip_hi = 0;
+    } else if constexpr (F == RAGGED) {
+      const int turning = (half + W - 1) / W;        // lanes of the rotated part
+      const int runs = (D - R + W - 1) / W;          // runs behind it, two a lane
+      on = lane < turning + (runs + 1) / 2;
+      skip_lo = skip_hi = 0;
+      if (!on) {
+        lo = hi = 0;
+        ang[0] = -1;
+      } else if (lane < turning) {
+        const int first = min(W * lane, half - W);   // first pair
+        ang[0] = first;
+        lo = a.inter ? 2 * first : first;
+        hi = a.inter ? 2 * first + W : first + half;
+        const int twice = W * lane - first;          // pairs that the lane before has
+        if (a.inter) {
+          skip_lo = min(2 * twice, W);
+          skip_hi = max(2 * twice - W, 0);
+        } else {
+          skip_lo = skip_hi = twice;
+        }
+      } else {
+        const int v = 2 * (lane - turning);
+        ang[0] = -1;
+        lo = min(R + W * v, D - W);
+        hi = min(R + W * (v + 1), D - W);
+        skip_lo = R + W * v - lo;
+        skip_hi = min(R + W * (v + 1) - hi, W);      // W: no second run, all of it another's
+      }
     } else {
       on = true;
-      const int turned = R / 2, rest = D - R;
+      const int rest = D - R;
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
         const int u = lane + j * G;
-        if (u < turned) {
+        if (u < half) {
           ang[j] = u;
           at[2 * j] = a.inter ? 2 * u : u;
-          at[2 * j + 1] = a.inter ? 2 * u + 1 : u + turned;
+          at[2 * j + 1] = a.inter ? 2 * u + 1 : u + half;
         } else {
-          const int v = 2 * (u - turned);
+          const int v = 2 * (u - half);
           ang[j] = -1;
           at[2 * j] = v < rest ? R + v : -1;
           at[2 * j + 1] = v + 1 < rest ? R + v + 1 : -1;
@@ -109,19 +153,38 @@ struct Lane {
   }
 
   MUON_DEVICE int element(int j) const {
-    if constexpr (VEC) return j < 8 ? lo + j : hi + j - 8;
+    if constexpr (RUNS) return j < W ? lo + j : hi + j - W;
     else return at[j];
+  }
+  // Whether value j is this lane's to count (where the lane is on).
+  MUON_DEVICE bool counts(int j) const {
+    if constexpr (F == WHOLE) return true;
+    else if constexpr (F == RAGGED) return j < W ? j >= skip_lo : j - W >= skip_hi;
+    else return at[j] >= 0;
+  }
+
+  template <int T>
+  static MUON_DEVICE void load_run(const void* p, int64_t i, float* v) {
+    constexpr int M = Vec16<T>::N;
+    float h[M];
+#pragma unroll
+    for (int c = 0; c < W; c += M) {
+      if constexpr (W < M) {  // 4 values of two bytes beside runs of fp32
+        muon_u4 w = {0, 0, 0, 0};
+        __builtin_memcpy(&w, elem_at<T>(p, i), W * 2);
+        Vec16<T>::unpack(w, h);
+      } else {
+        Vec16<T>::unpack(load_u4(elem_at<T>(p, i + c)), h);
+      }
+#pragma unroll
+      for (int e = 0; e < M && e < W; ++e) v[c + e] = h[e];
+    }
   }
 
   MUON_DEVICE void load(const void* p, int64_t base, float (&v)[N]) const {
-    if constexpr (VEC) {
-      float h[8];
-      Vec8<DT>::load(p, base + lo, h);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = h[e];
-      Vec8<DT>::load(p, base + hi, h);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[8 + e] = h[e];
+    if constexpr (RUNS) {
+      load_run<DT>(p, base + lo, v);
+      load_run<DT>(p, base + hi, v + W);
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j) v[j] = at[j] >= 0 ? Elem<DT>::load(p, base + at[j]) : 0.0f;
@@ -129,20 +192,24 @@ struct Lane {
   }
 
   MUON_DEVICE void store(void* p, int64_t base, const float (&v)[N]) const {
-    if constexpr (VEC) {
+    if constexpr (RUNS) {
       if (!on) return;
-      float h[8];
+      float h[W];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = v[e];
-      Vec8<DT>::store(p, base + lo, h);
+      for (int e = 0; e < W; ++e) h[e] = v[e];
+      put((void*)elem_at<DT>(p, base + lo), Vec16<DT>::pack(h));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = v[8 + e];
-      Vec8<DT>::store(p, base + hi, h);
+      for (int e = 0; e < W; ++e) h[e] = v[W + e];
+      put((void*)elem_at<DT>(p, base + hi), Vec16<DT>::pack(h));
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j)
         if (at[j] >= 0) Elem<DT>::store(p, base + at[j], v[j]);
     }
+  }
+  static MUON_DEVICE void put(void* p, muon_u4 w) {
+    if constexpr (NT) store_u4_nt(p, w);
+    else store_u4(p, w);
   }
 
   MUON_DEVICE void weights(const void* w, int wdt, float (&v)[N]) const {
@@ -155,14 +222,9 @@ struct Lane {
   }
   template <int WT>
   MUON_DEVICE void weights_of(const void* w, float (&v)[N]) const {
-    if constexpr (VEC) {
-      float h[8];
-      Vec8<WT>::load(w, lo, h);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = h[e];
-      Vec8<WT>::load(w, hi, h);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[8 + e] = h[e];
+    if constexpr (RUNS) {
+      load_run<WT>(w, lo, v);
+      load_run<WT>(w, hi, v + W);
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j) v[j] = at[j] >= 0 ? Elem<WT>::load(w, at[j]) : 0.0f;
@@ -175,14 +237,14 @@ struct Lane {
     const int half = a.R / 2;
     const bool gone = a.R && p < 0;
     const int64_t row = p < 0 ? 0 : p * half;  // read only where the table holds something
-    if constexpr (VEC) {
+    if constexpr (RUNS) {
       if (a.R && a.table_len) {
         const int i = ang[0] < 0 ? 0 : ang[0];
-        Vec8<MUON_DT_F32>::load(a.cosv, row + i, c);
-        Vec8<MUON_DT_F32>::load(a.sinv, row + i, s);
+        load_run<MUON_DT_F32>(a.cosv, row + i, c);
+        load_run<MUON_DT_F32>(a.sinv, row + i, s);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < W; ++e) {
         c[e] = gone ? nan : ang[0] < 0 ? 1.0f : c[e];
         s[e] = gone ? nan : ang[0] < 0 ? 0.0f : s[e];
       }
@@ -200,7 +262,7 @@ struct Lane {
   template <bool BACK>
   MUON_DEVICE void turn(const Args& a, const float (&c)[N / 2], const float (&s)[N / 2],
                         float (&v)[N]) const {
-    if constexpr (VEC) {
+    if constexpr (RUNS) {
       if (ang[0] < 0) {  // nothing turns here: an infinity stays out of its neighbours
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] *= c[e / 2];
@@ -209,7 +271,7 @@ struct Lane {
         for (int e = 0; e < N / 2; ++e) pair<BACK>(c[e], s[e], v[2 * e], v[2 * e + 1]);
       } else {
 #pragma unroll
-        for (int e = 0; e < N / 2; ++e) pair<BACK>(c[e], s[e], v[e], v[8 + e]);
+        for (int e = 0; e < N / 2; ++e) pair<BACK>(c[e], s[e], v[e], v[W + e]);
       }
     } else {
 #pragma unroll
@@ -238,9 +300,9 @@ MUON_DEVICE int side_of(const Args& a, int& block) {
   return 1;
 }
 
-template <int DT, int G, int NP, bool VEC>
+template <int DT, int G, int NP, Form F, bool NT>
 __global__ __launch_bounds__(NTHREADS) void qk_forward_kernel(Args a) {
-  typedef Lane<DT, G, NP, VEC> L;
+  typedef Lane<DT, G, NP, F, NT> L;
   int block;
   const int which = side_of(a, block);
   const Side& sd = a.s[which];
@@ -266,11 +328,9 @@ __global__ __launch_bounds__(NTHREADS) void qk_forward_kernel(Args a) {
 #pragma unroll
     for (int i = 0; i < HC; ++i) {
       float q = 0.0f;
-      if (l.on) {
 #pragma unroll
-        for (int e = 0; e < L::N; ++e) q += x[i][e] * x[i][e];
-      }
-      const float r = 1.0f / sqrtf(group_sum<G>(q) / (float)a.D + a.eps);
+      for (int e = 0; e < L::N; ++e) q += l.counts(e) ? x[i][e] * x[i][e] : 0.0f;
+      const float r = 1.0f / sqrtf(group_sum<G>(l.on ? q : 0.0f) / (float)a.D + a.eps);
 #pragma unroll
       for (int e = 0; e < L::N; ++e) x[i][e] = x[i][e] * r * w[e];
       l.template turn<false>(a, c, s, x[i]);
@@ -282,9 +342,9 @@ __global__ __launch_bounds__(NTHREADS) void qk_forward_kernel(Args a) {
 // Workgroups walk over a side's (token, head group) units; each lane keeps the weight gradient
 // of its own values in registers, the groups of a workgroup are joined through LDS in a fixed
 // order, and the workgroup writes one partial of D values.
-template <int DT, int G, int NP, bool VEC>
+template <int DT, int G, int NP, Form F, bool NT>
 __global__ __launch_bounds__(NTHREADS) void qk_backward_kernel(Args a) {
-  typedef Lane<DT, G, NP, VEC> L;
+  typedef Lane<DT, G, NP, F, NT> L;
   constexpr int GROUPS = NTHREADS / G;
   __shared__ float part[GROUPS][G * L::N + 1];
   int block;
@@ -317,13 +377,12 @@ __global__ __launch_bounds__(NTHREADS) void qk_backward_kernel(Args a) {
     for (int i = 0; i < HC; ++i) {
       l.template turn<true>(a, c, s, u[i]);
       float q = 0.0f, dot = 0.0f;
-      if (l.on) {
 #pragma unroll
-        for (int e = 0; e < L::N; ++e) {
-          q += x[i][e] * x[i][e];
-          dot += u[i][e] * w[e] * x[i][e];
-        }
+      for (int e = 0; e < L::N; ++e) {
+        q += l.counts(e) ? x[i][e] * x[i][e] : 0.0f;
+        dot += l.counts(e) ? u[i][e] * w[e] * x[i][e] : 0.0f;
       }
+      if (!l.on) q = dot = 0.0f;
       const float r = 1.0f / sqrtf(group_sum<G>(q) / (float)a.D + a.eps);
       // r^3 alone leaves the range for rows of very small or large values: r dot stays in it
       const float k = group_sum<G>(dot) * r / (float)a.D * r;
@@ -349,7 +408,7 @@ __global__ __launch_bounds__(NTHREADS) void qk_backward_kernel(Args a) {
     own.init(a, v / L::N);
     int i = -1;
 #pragma unroll
-    for (int j = 0; j < L::N; ++j) i = j == v % L::N && own.on ? own.element(j) : i;
+    for (int j = 0; j < L::N; ++j) i = j == v % L::N && own.on && own.counts(j) ? own.element(j) : i;
     if (i >= 0)
       a.part[((int64_t)(which ? a.blocks[0] : 0) + block) * a.D + i] = sum;
   }
@@ -376,42 +435,40 @@ __global__ __launch_bounds__(1024) void qk_weight_grad_kernel(Args a) {
   }
 }
 
-// Lanes of a row in the vector form: D / 16, rounded up to a power of two.
-int vec_lanes(int64_t D) {
-  int g = 4;
-  while (g * 16 < D) g *= 2;
-  return g;
-}
-
-template <int DT, int G, int NP, bool VEC>
-int launch(const Args& a, bool backward, hipStream_t s) {
+template <int DT, int G, int NP, Form F>
+int launch(const Args& a, bool backward, bool nt, hipStream_t s) {
   const int grid = a.blocks[0] + a.blocks[1];
-  if (backward) qk_backward_kernel<DT, G, NP, VEC><<<grid, NTHREADS, 0, s>>>(a);
-  else qk_forward_kernel<DT, G, NP, VEC><<<grid, NTHREADS, 0, s>>>(a);
+  constexpr bool RUNS = F != SINGLE;  // single values are stored the ordinary way
+  if (backward) {
+    if (RUNS && nt) qk_backward_kernel<DT, G, NP, F, RUNS><<<grid, NTHREADS, 0, s>>>(a);
+    else qk_backward_kernel<DT, G, NP, F, false><<<grid, NTHREADS, 0, s>>>(a);
+  } else {
+    if (RUNS && nt) qk_forward_kernel<DT, G, NP, F, RUNS><<<grid, NTHREADS, 0, s>>>(a);
+    else qk_forward_kernel<DT, G, NP, F, false><<<grid, NTHREADS, 0, s>>>(a);
+  }
   MUON_CHECK_LAUNCH("qk_norm_rope");
   return MUON_OK;
 }
 
-template <int DT>
-int launch_dt(const Args& a, bool vec, int lanes, bool backward, hipStream_t s) {
-  if (vec) {
-    switch (lanes) {
-      case 4: return launch<DT, 4, 8, true>(a, backward, s);
-      case 8: return launch<DT, 8, 8, true>(a, backward, s);
-      case 16: return launch<DT, 16, 8, true>(a, backward, s);
-      case 32: return launch<DT, 32, 8, true>(a, backward, s);
-      default: return launch<DT, 64, 8, true>(a, backward, s);
-    }
-  }
-  switch (lanes) {
-    case 1: return launch<DT, 64, 1, false>(a, backward, s);
-    case 2: return launch<DT, 64, 2, false>(a, backward, s);
-    case 4: return launch<DT, 64, 4, false>(a, backward, s);
-    default: return launch<DT, 64, 9, false>(a, backward, s);
-  }
+template <int DT, Form F>
+int launch_runs(const Args& a, int lanes, bool backward, bool nt, hipStream_t s) {
+  if (lanes <= 4) return launch<DT, 4, 1, F>(a, backward, nt, s);
+  if (lanes <= 8) return launch<DT, 8, 1, F>(a, backward, nt, s);
+  if (lanes <= 16) return launch<DT, 16, 1, F>(a, backward, nt, s);
+  if (lanes <= 32) return launch<DT, 32, 1, F>(a, backward, nt, s);
+  if (lanes <= 64) return launch<DT, 64, 1, F>(a, backward, nt, s);
+  muon_set_error("qk_norm_rope: %d lanes a row", lanes);  // form_for gives at most 64
+  return MUON_ERR_SHAPE;
 }
 
-bool aligned16(const void* p) { return !((uintptr_t)p & 15); }
+template <int DT>
+int launch_dt(const Args& a, Form form, int lanes, bool backward, bool nt, hipStream_t s) {
+  if (form == WHOLE) return launch_runs<DT, WHOLE>(a, lanes, backward, nt, s);
+  if (form == RAGGED) return launch_runs<DT, RAGGED>(a, lanes, backward, nt, s);
+  if (lanes == 1) return launch<DT, 64, 1, SINGLE>(a, backward, false, s);
+  return launch<DT, 64, MAX_PAIRS, SINGLE>(a, backward, false, s);
+}
+
 bool io_ok(int dt) { return dt == MUON_DT_F32 || dt == MUON_DT_BF16 || dt == MUON_DT_F16; }
 
 constexpr int64_t MAX_DIM = 1024;
@@ -455,41 +512,52 @@ int check(const char* what, Args& a, int dtype, int64_t batch, int64_t T, int64_
   return MUON_OK;
 }
 
-// Whether rows can be moved in 16-byte pieces: D and R in 16s and every row 16-byte aligned.
-bool vectors(const Args& a, int dtype, bool backward) {
-  const int64_t es = dtype == MUON_DT_F32 ? 4 : 2;
-  if (a.D % 16 || a.R % 16) return false;
-  if (a.R && (!aligned16(a.cosv) || !aligned16(a.sinv))) return false;
-  for (int i = 0; i < 2; ++i) {
-    const Side& s = a.s[i];
-    if (!s.heads) continue;
-    if (!aligned16(s.x) || !aligned16(s.out) || !aligned16(s.w) || (s.sb | s.st | s.sh) * es % 16) return false;
-    if (backward && (!aligned16(s.dy) || (s.gb | s.gt | s.gh) * es % 16)) return false;
+// The form of a row's sharing-out and its lanes (SINGLE: pairs a lane of the wave, 1 or MAX_PAIRS).
+// Rows need no alignment: the hardware takes 16 bytes at any element's address.
+Form form_for(const Args& a, int dtype, int* lanes) {
+  const int W = dtype == MUON_DT_F32 ? 4 : 8;
+  const int half = a.R / 2, rest = a.D - a.R;
+  Form form = SINGLE;
+  if (a.D % (2 * W) == 0 && a.R % (2 * W) == 0) {
+    form = WHOLE;
+    *lanes = a.D / (2 * W);
+  } else if ((a.R == 0 || half >= W) && (rest == 0 || rest >= W)) {
+    form = RAGGED;
+    *lanes = (half + W - 1) / W + ((rest + W - 1) / W + 1) / 2;
   }
-  return true;
+  if (form == SINGLE || *lanes > 64) {
+    form = SINGLE;
+    *lanes = half + (rest + 1) / 2 <= 64 ? 1 : MAX_PAIRS;
+  }
+  return form;
 }
 
-// Lanes per row (vector form) or pairs per lane of a wave (otherwise).
-int lanes_for(const Args& a, bool vec) {
-  if (vec) return vec_lanes(a.D);
-  const int pairs = a.R / 2 + (a.D - a.R + 1) / 2;  // at most D / 2 + 1
-  return pairs <= 64 ? 1 : pairs <= 128 ? 2 : pairs <= 256 ? 4 : 9;
+int group_lanes(Form form, int lanes) {
+  int g = form == SINGLE ? 64 : 4;
+  while (g < lanes && form != SINGLE) g *= 2;
+  return g;
 }
 
-int run(const Args& a, int dtype, bool backward, bool vec, hipStream_t s) {
-  const int lanes = lanes_for(a, vec);
-  if (dtype == MUON_DT_F32) return launch_dt<MUON_DT_F32>(a, vec, lanes, backward, s);
-  if (dtype == MUON_DT_BF16) return launch_dt<MUON_DT_BF16>(a, vec, lanes, backward, s);
-  return launch_dt<MUON_DT_F16>(a, vec, lanes, backward, s);
+bool streams(const Args& a, int dtype) {
+  const int64_t es = dtype == MUON_DT_F32 ? 4 : 2;
+  // a store instruction writes each half of a row in one piece
+  if (a.inter || a.R != a.D || a.R / 2 * es % 16 || a.R / 2 * es < 64) return false;
+  return a.tokens * (a.s[0].heads + a.s[1].heads) * a.D * es >= NT_FROM;
 }
 
-// Workgroups of the backward pass for both sides: at most MAX_BWD_BLOCKS in all (four of 256
-// threads per CU), by their units.
-void backward_blocks(const int64_t (&units)[2], int groups, int (&blocks)[2]) {
+int run(const Args& a, int dtype, bool backward, Form form, int lanes, hipStream_t s) {
+  const bool nt = streams(a, dtype);
+  if (dtype == MUON_DT_F32) return launch_dt<MUON_DT_F32>(a, form, lanes, backward, nt, s);
+  if (dtype == MUON_DT_BF16) return launch_dt<MUON_DT_BF16>(a, form, lanes, backward, nt, s);
+  return launch_dt<MUON_DT_F16>(a, form, lanes, backward, nt, s);
+}
+
+// Workgroups of the backward pass for both sides: at most `most` (and one) in all, by their units.
+void backward_blocks(const int64_t (&units)[2], int groups, int most, int (&blocks)[2]) {
   const double total = (double)units[0] + (double)units[1];
   for (int i = 0; i < 2; ++i) {
     const int64_t need = (units[i] + groups - 1) / groups;
-    const int64_t share = std::max<int64_t>(1, (int64_t)(MAX_BWD_BLOCKS * (units[i] / total)));
+    const int64_t share = std::max<int64_t>(1, (int64_t)(most * (units[i] / total)));
     blocks[i] = (int)std::min(need, share);
   }
 }
@@ -517,13 +585,14 @@ int muon_qk_norm_rope(const void* q, const void* k, const int64_t* strides, cons
   bool empty = false;
   const int rc = check("qk_norm_rope", a, dtype, batch, tokens, q_heads, k_heads, dim, rotary, &empty);
   if (rc || empty) return rc;
-  const bool vec = vectors(a, dtype, false);
-  const int64_t groups = NTHREADS / (vec ? lanes_for(a, true) : 64);
+  int lanes = 0;
+  const Form form = form_for(a, dtype, &lanes);
+  const int64_t groups = NTHREADS / group_lanes(form, lanes);
   const int64_t b0 = (a.units[0] + groups - 1) / groups, b1 = (a.units[1] + groups - 1) / groups;
   // a launch holds fewer than 2^32 threads: beyond MAX_FWD_BLOCKS the workgroups walk on
   a.blocks[0] = (int)std::min<int64_t>(b0, MAX_FWD_BLOCKS);
   a.blocks[1] = (int)std::min<int64_t>(b1, MAX_FWD_BLOCKS);
-  return run(a, dtype, false, vec, (hipStream_t)stream);
+  return run(a, dtype, false, form, lanes, (hipStream_t)stream);
 }
 
 int64_t muon_qk_norm_rope_workspace_bytes(int64_t dim) {
@@ -564,9 +633,11 @@ int muon_qk_norm_rope_backward(const void* q, const void* k, const void* dq_out,
   hipStream_t s = (hipStream_t)stream;
   if (empty) a.D = (int)dim;  // no rows: the weights' gradients are sums over nothing
   if (!empty) {
-    const bool vec = vectors(a, dtype, true);
-    backward_blocks(a.units, NTHREADS / (vec ? lanes_for(a, true) : 64), a.blocks);
-    const int rb = run(a, dtype, true, vec, s);
+    int lanes = 0;
+    const Form form = form_for(a, dtype, &lanes);
+    backward_blocks(a.units, NTHREADS / group_lanes(form, lanes),
+                    form == SINGLE ? MAX_BWD_BLOCKS : MAX_BWD_BLOCKS / 2, a.blocks);
+    const int rb = run(a, dtype, true, form, lanes, s);
     if (rb) return rb;
   }
   if (!dw) return MUON_OK;

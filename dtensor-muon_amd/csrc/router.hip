@@ -36,7 +36,9 @@ struct Args {
   float* balance;  // one value each: the losses, and the number of tokens that count
   float* zloss;
   float* kept;
-  // one partial a workgroup, of E or of one value
+  // one partial a workgroup, of E or of one value; of the finishing workgroups (part_b, ticket)
+  double* part_b;
+  int* ticket;
   float* part_p;
   int* part_c;
   float* part_z;
@@ -59,97 +61,116 @@ struct BackArgs {
 
 // The logits of one token that a lane owns: VPT experts in a row; -inf behind the last one.
 template <int DT, int VPT>
-MUON_DEVICE void load_logits(const void* z, int64_t at, int e0, int E, float (&v)[VPT]) {
+MUON_DEVICE void load_logits(const void* z, int64_t at, int e0, int E,
+                             muon_u4 (&w)[VPT / Vec16<DT>::N]) {
   constexpr int N = Vec16<DT>::N;
 #pragma unroll
-  for (int c = 0; c < VPT; c += N) {
-    const int e = e0 + c;
-    float x[N];
+  for (int c = 0; c < VPT / N; ++c) {
+    const int e = e0 + c * N;
     if (e + N <= E) {
-      Vec16<DT>::unpack(load_u4(elem_at<DT>(z, at + e)), x);
+      w[c] = load_u4(elem_at<DT>(z, at + e));
     } else {
+      float x[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) x[j] = e + j < E ? Elem<DT>::load(z, at + e + j) : -INFINITY;
+      w[c] = Vec16<DT>::pack(x);
     }
+  }
+}
+template <int DT, int VPT>
+MUON_DEVICE void unpack_logits(const muon_u4 (&w)[VPT / Vec16<DT>::N], float (&v)[VPT]) {
+  constexpr int N = Vec16<DT>::N;
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[c + j] = x[j];
+  for (int c = 0; c < VPT / N; ++c) {
+    float x[N];
+    Vec16<DT>::unpack(w[c], x);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[c * N + j] = x[j];
   }
 }
 
-// An order-preserving integer of a value: NaNs (as one) over +inf over ... over -inf, and -0 as 0.
+// An order-preserving integer of a value that is no NaN, -0 as 0; +inf gives 0xff800000, the
+// lowest finite value 0x00800000, -inf less. The NaN 0x7fc00000 comes above them all.
 MUON_DEVICE uint32_t ordered(float v) {
-  const uint32_t u = v != v ? 0x7fc00000u : __float_as_uint(v + 0.0f);
-  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 MUON_DEVICE float unordered(uint32_t o) {
   return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
 }
+constexpr uint32_t ORDERED_LOWEST = 0x00800000u;
 
 // A value and its index as one number, larger for a larger value and, among equal ones, for a
-// lower index; 0 for what cannot be chosen (-inf). All keys of a token are distinct, so the next
-// choice is the largest key below the last one: nothing has to be taken out of the registers.
+// lower index; -inf, also behind the last expert, gives a number below all that can be chosen.
+// All keys of a token are distinct, so the next choice is the largest key below the last one:
+// nothing has to be taken out of the registers.
 // Values of two bytes have at most 19 significant bits in fp32: 32 bits hold both. fp32 takes
-// 63 bits, compared as a positive double (one maximum instruction; no key reaches the exponent of
-// infinities, since the largest ordered value, the NaN's, is 0xffc00000).
+// 63 bits, compared as a positive double (no key reaches the exponent of infinities, since the
+// largest ordered value, the NaN's, is 0xffc00000).
 template <int DT>
 struct Key {
   typedef uint32_t T;
   static MUON_DEVICE T make(float v, int e) {
-    return v == -INFINITY ? 0u : (ordered(v) & 0xffffe000u) | (uint32_t)(0x1fff - e);
+    return (ordered(v) & 0xffffe000u) | (uint32_t)(0x1fff - e);
   }
-  static MUON_DEVICE bool none(T k) { return k == 0; }
+  static MUON_DEVICE bool none(T k) { return k < ORDERED_LOWEST; }
   static MUON_DEVICE int index(T k) { return 0x1fff - (int)(k & 0x1fffu); }
   static MUON_DEVICE float value(T k) {
     // a negative value's ordered form has ones in the masked bits
     const uint32_t o = k & 0xffffe000u;
     return unordered((o >> 31) ? o : o | 0x1fffu);
   }
+  static MUON_DEVICE T larger(T a, T b) { return max(a, b); }
+  template <int G>
+  static MUON_DEVICE T largest(T v) {
+    return group_reduce<G>(v, [](T a, T b) { return max(a, b); });
+  }
   // The largest key below `last`: key - last wraps to the top of the range exactly for the keys
-  // below it, in their order, so one subtraction and one maximum serve a key.
+  // below it, in their order, so one subtraction and one maximum serve a key. Past the last key
+  // the result is 0.
   template <int VPT, int G>
   static MUON_DEVICE T next(const T (&key)[VPT], T last) {
     T best = 0;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) best = max(best, key[j] - last);
-    best = group_reduce<G>(best, [](T a, T b) { return max(a, b); });
+    best = largest<G>(best);
     const T found = best + last;
     return found < last ? found : 0;
-  }
-  template <int VPT, int G>
-  static MUON_DEVICE T first(const T (&key)[VPT]) {
-    T best = 0;
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) best = max(best, key[j]);
-    return group_reduce<G>(best, [](T a, T b) { return max(a, b); });
   }
 };
 template <>
 struct Key<MUON_DT_F32> {
   typedef double T;
   static MUON_DEVICE T make(float v, int e) {
-    const uint64_t b = v == -INFINITY ? 0 : ((uint64_t)ordered(v) << 31) | (uint64_t)(0x7fffffff - e);
-    return __builtin_bit_cast(double, b);
+    const uint32_t o = ordered(v);
+    return __hiloint2double((int)(o >> 1), (int)((o << 31) | (uint32_t)(0x7fffffff - e)));
   }
-  static MUON_DEVICE bool none(T k) { return __builtin_bit_cast(uint64_t, k) == 0; }
-  static MUON_DEVICE int index(T k) {
-    return 0x7fffffff - (int)(__builtin_bit_cast(uint64_t, k) & 0x7fffffffu);
-  }
+  static MUON_DEVICE bool none(T k) { return (uint32_t)__double2hiint(k) < ORDERED_LOWEST >> 1; }
+  static MUON_DEVICE int index(T k) { return 0x7fffffff - (__double2loint(k) & 0x7fffffff); }
   static MUON_DEVICE float value(T k) {
-    return unordered((uint32_t)(__builtin_bit_cast(uint64_t, k) >> 31));
+    return unordered(((uint32_t)__double2hiint(k) << 1) | ((uint32_t)__double2loint(k) >> 31));
   }
+  // No operand is a NaN: fmax's extra step that quiets them is left out. The compiler sees no
+  // vector instruction in it and so no need for the wait states before a DPP read of the result:
+  // largest() passes it through an instruction of the compiler's own first.
+  static MUON_DEVICE T larger(T a, T b) {
+    T r;
+    asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+  }
+  template <int G>
+  static MUON_DEVICE T largest(T v) {
+    return group_reduce<G>(__builtin_fmax(v, 0.0), [](T a, T b) { return __builtin_fmax(a, b); });
+  }
+  // A key at or above `last` loses its upper half, which leaves it below every key that counts.
   template <int VPT, int G>
   static MUON_DEVICE T next(const T (&key)[VPT], T last) {
     T best = 0.0;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) best = __builtin_fmax(best, key[j] < last ? key[j] : 0.0);
-    return group_reduce<G>(best, [](T a, T b) { return __builtin_fmax(a, b); });
-  }
-  template <int VPT, int G>
-  static MUON_DEVICE T first(const T (&key)[VPT]) {
-    T best = 0.0;
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) best = __builtin_fmax(best, key[j]);
-    return group_reduce<G>(best, [](T a, T b) { return __builtin_fmax(a, b); });
+    for (int j = 0; j < VPT; ++j)
+      best = larger(best, __hiloint2double(key[j] < last ? __double2hiint(key[j]) : 0,
+                                           __double2loint(key[j])));
+    return largest<G>(best);
   }
 };
 
@@ -178,8 +199,8 @@ __global__ __launch_bounds__(FWD_THREADS) void route_kernel(Args a) {
   constexpr int ECAP = G * VPT;
   constexpr int KCAP = ECAP < KMAX ? ECAP : KMAX;
   typedef Key<DT> K;
-  struct Pick { float v; int e; };
-  __shared__ Pick picks[GROUPS][KCAP];
+  constexpr int RAW = VPT / Vec16<DT>::N;
+  __shared__ typename K::T picks[GROUPS][KCAP];
   __shared__ float cols[GROUPS][ECAP + 1];
   __shared__ int cnt[ECAP];
   __shared__ float zs[GROUPS];
@@ -193,59 +214,77 @@ __global__ __launch_bounds__(FWD_THREADS) void route_kernel(Args a) {
   for (int j = 0; j < VPT; ++j) acc[j] = 0.0f;
   float zsum = 0.0f;
   int n = 0;
-  for (int64_t t = (int64_t)blockIdx.x * GROUPS + group; t < a.T; t += (int64_t)gridDim.x * GROUPS) {
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  int64_t t = (int64_t)blockIdx.x * GROUPS + group;
+  muon_u4 raw[RAW];
+  if (t < a.T) load_logits<DT, VPT>(a.z, t * a.row, e0, a.E, raw);
+  for (; t < a.T; t += step) {
     float v[VPT], p[VPT];
-    load_logits<DT, VPT>(a.z, t * a.row, e0, a.E, v);
+    unpack_logits<DT, VPT>(raw, v);
+    if (t + step < a.T) load_logits<DT, VPT>(a.z, (t + step) * a.row, e0, a.E, raw);
     float m = v[0];
 #pragma unroll
     for (int j = 1; j < VPT; ++j) m = fmaxf(m, v[j]);
     m = group_max<G>(m);
     bool on = !a.mask || a.mask[t];
-    // all -inf (a NaN, which fmaxf passes over, is no such row): counts nowhere
-    float bad = 0.0f;
+    if (m == -INFINITY) {  // all -inf counts nowhere (a NaN, which fmaxf passes over, makes no such row)
+      float bad = 0.0f;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) bad = v[j] != v[j] ? 1.0f : bad;
-    if (m == -INFINITY && group_max<G>(bad) == 0.0f) on = false;
+      for (int j = 0; j < VPT; ++j) bad = v[j] != v[j] ? 1.0f : bad;
+      on = on && group_max<G>(bad) != 0.0f;
+    }
     float total = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      p[j] = __builtin_amdgcn_exp2f((v[j] - m) * LOG2E);
+      p[j] = __builtin_amdgcn_exp2f((v[j] - m) * LOG2E);  // 0 behind the last expert
       total += p[j];
     }
     total = group_sum<G>(total);
-    const float inv = 1.0f / total;
+    const float inv = __builtin_amdgcn_rcpf(total);
+    float held = 0.0f;
     if (on) {
 #pragma unroll
-      for (int j = 0; j < VPT; ++j) acc[j] += e0 + j < a.E ? p[j] * inv : 0.0f;
+      for (int j = 0; j < VPT; ++j) acc[j] += p[j] * inv;
       const float lse = m + __builtin_amdgcn_logf(total) * LN2;
       zsum += lse * lse;
       n += 1;
-    }
-    typename K::T key[VPT];
+      if (total != total) {  // a NaN somewhere, of whatever sign and payload: as one
 #pragma unroll
-    for (int j = 0; j < VPT; ++j)
-      key[j] = e0 + j < a.E ? K::make(v[j], e0 + j) : (typename K::T)0;
-    if (on) {
-      typename K::T best = K::template first<VPT, G>(key);
-      for (int i = 0; i < a.k; ++i) {
-        if (lane == 0) picks[group][i] = {K::value(best), K::none(best) ? -1 : K::index(best)};
-        if (i + 1 < a.k && !K::none(best)) best = K::template next<VPT, G>(key, best);
+        for (int j = 0; j < VPT; ++j) v[j] = v[j] != v[j] ? __uint_as_float(0x7fc00000u) : v[j];
       }
+      typename K::T key[VPT], best = 0;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        key[j] = K::make(v[j], e0 + j);
+        best = K::larger(best, key[j]);
+      }
+      best = K::template largest<G>(best);
+      for (int i = 0;;) {
+        if (lane == 0) picks[group][i] = best;
+        if (++i == a.k) break;
+        best = K::template next<VPT, G>(key, best);
+      }
+      wave_lds_fence();
+      for (int i = lane; i < a.k; i += G) {
+        const typename K::T q = picks[group][i];
+        held += K::none(q) ? 0.0f : __builtin_amdgcn_exp2f((K::value(q) - m) * LOG2E);
+      }
+      held = group_sum<G>(held);
     }
-    wave_lds_fence();
-    float held = 0.0f;
-    if (on) {
-      for (int i = lane; i < a.k; i += G)
-        if (picks[group][i].e >= 0) held += __builtin_amdgcn_exp2f((picks[group][i].v - m) * LOG2E);
-    }
-    held = group_sum<G>(held);
+    const float share = a.normalize ? __builtin_amdgcn_rcpf(held) : inv;
     for (int i = lane; i < a.k; i += G) {
-      Pick q = {0.0f, -1};
-      if (on) q = picks[group][i];
-      const float e2 = __builtin_amdgcn_exp2f((q.v - m) * LOG2E);
-      a.experts[t * a.k + i] = q.e;
-      a.gates[t * a.k + i] = q.e < 0 ? 0.0f : a.normalize ? e2 / held : e2 * inv;
-      if (q.e >= 0) atomicAdd(&cnt[q.e], 1);
+      int64_t e = -1;
+      float gate = 0.0f;
+      if (on) {
+        const typename K::T q = picks[group][i];
+        if (!K::none(q)) {
+          e = K::index(q);
+          gate = __builtin_amdgcn_exp2f((K::value(q) - m) * LOG2E) * share;
+          atomicAdd(&cnt[e], 1);
+        }
+      }
+      a.experts[t * a.k + i] = e;
+      a.gates[t * a.k + i] = gate;
     }
     wave_lds_fence();
   }
@@ -286,67 +325,74 @@ __global__ __launch_bounds__(FWD_THREADS) void route_kernel(Args a) {
   if (gridDim.x == 1) {
     write_losses(a, b, z, c);
   } else {
+    if (blockIdx.x == 0) *a.ticket = 0;  // for the launch after this one
     a.part_z[blockIdx.x] = (float)z;
     a.part_n[blockIdx.x] = c;
   }
 }
 
-// The workgroups' partials summed in a fixed order by one workgroup: C columns (a power of two)
-// times 1024 / C rows of threads, joined through LDS.
-__global__ __launch_bounds__(1024) void route_finish_kernel(Args a, int blocks, int C) {
-  __shared__ float ps[1024];
-  __shared__ int cs[1024];
-  __shared__ double red[3][16];
-  const int col = threadIdx.x & (C - 1), row = threadIdx.x / C, rows = 1024 / C;
-  double bal = 0.0;
-  for (int e0 = 0; e0 < a.E; e0 += C) {
-    const int e = e0 + col;
-    float p = 0.0f;
-    int c = 0;
-    if (e < a.E) {
+// The workgroups' partials summed in a fixed order: 16 experts a workgroup, 64 rows of threads over
+// the partials, joined through LDS. The workgroup that ends last (a ticket counts them, zeroed by
+// route_kernel) adds their shares of the balance loss, again in order.
+__global__ __launch_bounds__(1024) void route_finish_kernel(Args a, int blocks) {
+  __shared__ float ps[64][17];
+  __shared__ int cs[64][17];
+  __shared__ double red[2][16];
+  const int col = threadIdx.x % 16, row = threadIdx.x / 16;
+  const int e = blockIdx.x * 16 + col;
+  float p = 0.0f;
+  int c = 0;
+  if (e < a.E) {
 #pragma unroll 8
-      for (int b = row; b < blocks; b += rows) {
-        p += a.part_p[(int64_t)b * a.E + e];
-        c += a.part_c[(int64_t)b * a.E + e];
-      }
+    for (int b = row; b < blocks; b += 64) {
+      p += a.part_p[(int64_t)b * a.E + e];
+      c += a.part_c[(int64_t)b * a.E + e];
     }
-    ps[threadIdx.x] = p;
-    cs[threadIdx.x] = c;
-    __syncthreads();
-    if (row == 0 && e < a.E) {
-      double sum = 0.0;
-      int64_t count = 0;
-      for (int r = 0; r < rows; ++r) {
-        sum += ps[r * C + col];
-        count += cs[r * C + col];
-      }
-      a.counts[e] = count;
-      bal += sum * (double)count;
-    }
-    __syncthreads();
   }
+  ps[row][col] = p;
+  cs[row][col] = c;
   double z = 0.0, n = 0.0;  // token counts below 2^53 are exact
   for (int b = threadIdx.x; b < blocks; b += 1024) {
     z += a.part_z[b];
     n += a.part_n[b];
   }
   for (int off = 32; off; off >>= 1) {
-    bal += __shfl_xor(bal, off, 64);
     z += __shfl_xor(z, off, 64);
     n += __shfl_xor(n, off, 64);
   }
   if (threadIdx.x % 64 == 0) {
-    red[0][threadIdx.x / 64] = bal;
-    red[1][threadIdx.x / 64] = z;
-    red[2][threadIdx.x / 64] = n;
+    red[0][threadIdx.x / 64] = z;
+    red[1][threadIdx.x / 64] = n;
   }
   __syncthreads();
-  if (threadIdx.x) return;
-  bal = z = n = 0.0;
+  if (threadIdx.x >= 64) return;
+  {  // a wave: 4 threads a column
+    double sum = 0.0;
+    int64_t count = 0;
+    for (int r = row; r < 64; r += 4) {
+      sum += ps[r][col];
+      count += cs[r][col];
+    }
+    for (int off = 16; off < 64; off *= 2) {
+      sum += __shfl_xor(sum, off, 64);
+      count += __shfl_xor((long long)count, off, 64);
+    }
+    if (row == 0 && e < a.E) a.counts[e] = count;
+    double bal = e < a.E ? sum * (double)count : 0.0;
+    for (int off = 1; off < 16; off *= 2) bal += __shfl_xor(bal, off, 64);
+    if (threadIdx.x) return;
+    __hip_atomic_store(&a.part_b[blockIdx.x], bal, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__hip_atomic_fetch_add(a.ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) !=
+        (int)gridDim.x - 1)
+      return;
+  }
+  double bal = 0.0;
+  for (int b = 0; b < (int)gridDim.x; ++b)
+    bal += __hip_atomic_load(&a.part_b[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  z = n = 0.0;
   for (int w = 0; w < 16; ++w) {
-    bal += red[0][w];
-    z += red[1][w];
-    n += red[2][w];
+    z += red[0][w];
+    n += red[1][w];
   }
   write_losses(a, bal, z, (int64_t)n);
 }
@@ -371,26 +417,34 @@ __global__ __launch_bounds__(BWD_THREADS) void route_backward_kernel(BackArgs a)
   for (int j = 0; j < VPT; ++j)
     coef[j] = e0 + j < a.E && n > 0.0f ? bc * ((float)a.counts[e0 + j] / n) : 0.0f;
   float* mine = rows[group];
-  for (int64_t t = (int64_t)blockIdx.x * GROUPS + group; t < a.T; t += (int64_t)gridDim.x * GROUPS) {
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  int64_t t = (int64_t)blockIdx.x * GROUPS + group;
+  muon_u4 raw[VPT / Vec16<DT>::N];
+  if (t < a.T) load_logits<DT, VPT>(a.z, t * a.row, e0, a.E, raw);
+  for (; t < a.T; t += step) {
     float v[VPT];
-    load_logits<DT, VPT>(a.z, t * a.row, e0, a.E, v);
+    unpack_logits<DT, VPT>(raw, v);
+    if (t + step < a.T) load_logits<DT, VPT>(a.z, (t + step) * a.row, e0, a.E, raw);
     const bool masked = a.mask && !a.mask[t];
-    float m = v[0], bad = 0.0f;
+    float m = v[0];
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      m = fmaxf(m, v[j]);
-      bad = v[j] != v[j] ? 1.0f : bad;
-    }
+    for (int j = 1; j < VPT; ++j) m = fmaxf(m, v[j]);
     m = group_max<G>(m);
-    const bool on = !masked && !(m == -INFINITY && group_max<G>(bad) == 0.0f);
+    bool on = !masked;
+    if (m == -INFINITY) {
+      float bad = 0.0f;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) bad = v[j] != v[j] ? 1.0f : bad;
+      on = on && group_max<G>(bad) != 0.0f;
+    }
     float total = 0.0f, dot = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      v[j] = e0 + j < a.E ? __builtin_amdgcn_exp2f((v[j] - m) * LOG2E) : 0.0f;
+      v[j] = __builtin_amdgcn_exp2f((v[j] - m) * LOG2E);  // 0 behind the last expert
       total += v[j];
     }
     total = group_sum<G>(total);
-    const float inv = 1.0f / total;
+    const float inv = __builtin_amdgcn_rcpf(total);
     const float lse = m + __builtin_amdgcn_logf(total) * LN2;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
@@ -424,7 +478,7 @@ __global__ __launch_bounds__(BWD_THREADS) void route_backward_kernel(BackArgs a)
 #pragma unroll
     for (int j = 0; j < VPT; ++j) mine[e0 + j] = v[j] * (coef[j] + shift);
     wave_lds_fence();
-    const float scale = a.normalize ? 1.0f / held : 1.0f;
+    const float scale = a.normalize ? __builtin_amdgcn_rcpf(held) : 1.0f;
     const float mean = a.normalize ? inner * scale : 0.0f;
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q)  // a token's experts are distinct: no two lanes meet
@@ -472,6 +526,7 @@ int lanes_of(int64_t E) {
 // Forward workgroups: enough to hold two per CU, each at least one round of tokens; their partials
 // (E sums and counts each) are what the finishing workgroup reads.
 constexpr int MAX_BLOCKS = 512;
+constexpr int64_t WS_HEAD = (EMAX / 16) * 8 + 8;  // part_b, ticket
 int forward_blocks(int64_t T, int64_t E) {
   const int64_t groups = FWD_THREADS / lanes_of(E);
   return (int)std::max<int64_t>(1, std::min<int64_t>((T + groups - 1) / groups, MAX_BLOCKS));
@@ -498,7 +553,7 @@ extern "C" {
 
 int64_t muon_route_workspace_bytes(int64_t tokens, int64_t experts) {
   if (tokens < 0 || experts < 1 || experts > EMAX) return -1;
-  return (int64_t)forward_blocks(tokens, experts) * (experts * 8 + 8);
+  return WS_HEAD + (int64_t)forward_blocks(tokens, experts) * (experts * 8 + 8);
 }
 
 int muon_route(const void* logits, int dtype, int64_t row_stride, int64_t tokens, int64_t experts,
@@ -514,7 +569,9 @@ int muon_route(const void* logits, int dtype, int64_t row_stride, int64_t tokens
   const int blocks = forward_blocks(tokens, experts);
   Args a = {logits, row_stride, tokens, (int)experts, (int)top, normalize,
             (const uint8_t*)token_mask, gates, chosen, counts, balance,
-            zloss, kept, (float*)ws, nullptr, nullptr, nullptr};
+            zloss, kept, (double*)ws, nullptr, nullptr, nullptr, nullptr, nullptr};
+  a.ticket = (int*)(a.part_b + EMAX / 16);
+  a.part_p = (float*)((char*)ws + WS_HEAD);
   a.part_c = (int*)(a.part_p + (int64_t)blocks * experts);
   a.part_z = (float*)(a.part_c + (int64_t)blocks * experts);
   a.part_n = (int*)(a.part_z + blocks);
@@ -528,9 +585,7 @@ int muon_route(const void* logits, int dtype, int64_t row_stride, int64_t tokens
     return MUON_OK;
   });
   if (r || blocks == 1) return r;
-  int C = 8;
-  while (C < experts && C < 1024) C *= 2;
-  route_finish_kernel<<<1, 1024, 0, s>>>(a, blocks, C);
+  route_finish_kernel<<<(unsigned)((experts + 15) / 16), 1024, 0, s>>>(a, blocks);
   MUON_CHECK_LAUNCH("route totals");
   return MUON_OK;
 }

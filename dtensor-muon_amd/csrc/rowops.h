@@ -88,6 +88,12 @@ MUON_DEVICE muon_u4 load_u4(const void* p) {
   return w;
 }
 MUON_DEVICE void store_u4(void* p, muon_u4 w) { __builtin_memcpy(p, &w, 16); }
+// The same past the caches: for results larger than the 256 MB cache, which no store should
+// fill with lines that are gone before they are read.
+MUON_DEVICE void store_u4_nt(void* p, muon_u4 w) {
+  typedef muon_u4 __attribute__((aligned(2))) any_u4;
+  __builtin_nontemporal_store(w, (any_u4*)p);
+}
 
 template <int DT>
 MUON_DEVICE const char* elem_at(const void* p, int64_t i) {
