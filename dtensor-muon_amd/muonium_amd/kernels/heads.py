@@ -17,6 +17,16 @@ def _check_on(device, **tensors) -> None:
             raise RuntimeError(f"{name} is on {t.device}, expected {device}")
 
 
+def _weight(w: Tensor | None, dim: int) -> Tensor | None:
+    if w is None:
+        return None
+    if w.shape != (dim,):
+        raise ValueError(f"weights are ({dim},); got {tuple(w.shape)}")
+    if w.dtype not in _FLOATS:
+        raise TypeError(f"weights are fp32, bf16 or fp16; got {w.dtype}")
+    return w.contiguous()
+
+
 def qk_norm_rope(
     q: Tensor,
     k: Tensor,
@@ -47,25 +57,20 @@ def qk_norm_rope(
 
     Returns the new queries and keys, contiguous, in their input's type. Differentiable in q, k
     and the weights; computed in fp32 and rounded once."""
+    shape, dim, device = q.shape, q.shape[-1], q.device
     if q.dim() not in (3, 4) or k.dim() != q.dim():
         raise ValueError(f"q and k are (batch, tokens, heads, dim) or (tokens, heads, dim); got "
-                         f"{tuple(q.shape)} and {tuple(k.shape)}")
-    if q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
-        raise ValueError(f"q and k differ in batch, tokens or dim: {tuple(q.shape)} and "
+                         f"{tuple(shape)} and {tuple(k.shape)}")
+    if shape[:-2] != k.shape[:-2] or dim != k.shape[-1]:
+        raise ValueError(f"q and k differ in batch, tokens or dim: {tuple(shape)} and "
                          f"{tuple(k.shape)}")
-    dim, device = q.shape[-1], q.device
     if q.dtype not in _FLOATS or k.dtype != q.dtype:
         raise TypeError(f"q and k are both fp32, bf16 or fp16; got {q.dtype} and {k.dtype}")
     if not 1 <= dim <= 1024:
         raise ValueError(f"dim is 1 to 1024; got {dim}")
     _check_on(device, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin,
               positions=positions)
-    for w in (q_weight, k_weight):
-        if w is not None:
-            if w.shape != (dim,):
-                raise ValueError(f"weights are ({dim},); got {tuple(w.shape)}")
-            if w.dtype not in _FLOATS:
-                raise TypeError(f"weights are fp32, bf16 or fp16; got {w.dtype}")
+    q_weight, k_weight = _weight(q_weight, dim), _weight(k_weight, dim)
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise TypeError(f"weights of two types: {q_weight.dtype} and {k_weight.dtype}")
     if (cos is None) != (sin is None):
@@ -82,14 +87,12 @@ def qk_norm_rope(
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"positions are int32 or int64; got {positions.dtype}")
-        if positions.shape not in ((q.shape[-3],), tuple(q.shape[:-2])):
-            raise ValueError(f"positions are ({q.shape[-3]},) or {tuple(q.shape[:-2])}; got "
+        if positions.shape != shape[:-2] and positions.shape != shape[-3:-2]:
+            raise ValueError(f"positions are ({shape[-3]},) or {tuple(shape[:-2])}; got "
                              f"{tuple(positions.shape)}")
-        positions = _row_ops._unit_last(positions)
-    elif cos is not None and q.shape[-3] > cos.shape[0]:
-        raise ValueError(f"{q.shape[-3]} tokens, but the tables have {cos.shape[0]} positions")
-    return _row_ops.qk_norm_rope(
-        _row_ops._unit_last(q), _row_ops._unit_last(k),
-        None if q_weight is None else q_weight.contiguous(),
-        None if k_weight is None else k_weight.contiguous(), cos, sin, positions, float(eps),
-        bool(interleaved))
+        positions = _row_ops.unit_last(positions)
+    elif cos is not None and shape[-3] > cos.shape[0]:
+        raise ValueError(f"{shape[-3]} tokens, but the tables have {cos.shape[0]} positions")
+    _row_ops.check_device(device)
+    return _row_ops.qk_norm_rope(_row_ops.unit_last(q), _row_ops.unit_last(k), q_weight, k_weight,
+                                 cos, sin, positions, eps, interleaved)

@@ -35,7 +35,7 @@ def _check(logits: Tensor, tokens: Tensor, temperature: float) -> None:
 
 def _rows(logits: Tensor) -> Tensor:
     flat = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
-    return _row_ops._unit_last(flat)
+    return _row_ops.unit_last(flat)
 
 
 def _flat(t: Tensor) -> Tensor:
@@ -54,7 +54,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor, *, temperature: float = 1.0) 
     logits; the backward pass reads them once more and keeps two floats a row besides. Positions
     whose incoming gradient is 0 get zeros, whatever their logits hold."""
     _check(logits, tokens, temperature)
-    out = _row_ops.token_logprobs(_rows(logits), _flat(tokens), float(temperature))
+    _row_ops.check_device(logits.device)
+    out = _row_ops.token_logprobs(_rows(logits), _flat(tokens), temperature, False)[0]
     return out if logits.dim() == 2 else out.view(tokens.shape)
 
 
@@ -106,8 +107,9 @@ def policy_loss(
                              "alone (detach it)")
     if not (clip_low >= 0 and clip_high >= 0):
         raise ValueError(f"the clip range is not negative; got {clip_low}, {clip_high}")
-    loss, logp = _row_ops.policy_loss(
+    _row_ops.check_device(logits.device)
+    loss, logp, _, _ = _row_ops.policy_loss(
         _rows(logits), _flat(tokens), _flat(old_logprobs), _flat(advantages), _flat(weights),
-        None if ref_logprobs is None else _flat(ref_logprobs), float(clip_low), float(clip_high),
-        float(kl_coef), float(temperature))
+        None if ref_logprobs is None else _flat(ref_logprobs), clip_low, clip_high, kl_coef,
+        temperature, False, False)
     return PolicyLoss(loss, logp if logits.dim() == 2 else logp.view(tokens.shape))

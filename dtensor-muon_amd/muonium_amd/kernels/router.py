@@ -56,8 +56,9 @@ def route(logits: Tensor, k: int, *, token_mask: Tensor | None = None, normalize
                              f"{tuple(token_mask.shape)}")
         token_mask = token_mask.reshape(-1).contiguous()
     flat = logits if logits.dim() == 2 else logits.reshape(-1, experts)
-    gates, chosen, counts, balance, zloss, _ = _row_ops.route(
-        _row_ops._unit_last(flat), int(k), token_mask, bool(normalize))
+    _row_ops.check_device(logits.device)
+    gates, chosen, counts, balance, zloss, _ = _row_ops.route(_row_ops.unit_last(flat), k,
+                                                              token_mask, normalize)
     if logits.dim() != 2:
         gates, chosen = (t.view(*logits.shape[:-1], k) for t in (gates, chosen))
     return Routing(gates, chosen, counts, balance, zloss)

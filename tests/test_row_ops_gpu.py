@@ -658,6 +658,14 @@ def test_row_operators_in_a_captured_graph():
             assert torch.equal(a, b), i
 
 
+def test_row_operators_have_no_second_derivative():
+    x = leaf(torch.randn(4, 50, generator=gen(1)))
+    y = token_logprobs(x, torch.zeros(4, dtype=torch.int64, device="cuda"))
+    d, = torch.autograd.grad((y.sum(),), (x,), create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        d.sum().backward()
+
+
 def test_row_operators_under_an_outer_compile():
     run = _all_calls(1)
     want = run()

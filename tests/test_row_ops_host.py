@@ -132,8 +132,9 @@ def test_registered_ops_run_on_fake_tensors():
         tok = torch.empty(5, device="cuda", dtype=torch.int64)
         lp, st = ops.token_logprobs(z, tok, 1.0, True)
         assert lp.shape == (5,) and st.shape == (10,)
-        assert ops.token_logprobs_backward(lp, None, z, tok, st, 1.0).shape == z.shape
-        loss, _, rows = ops.policy_loss(z, tok, lp, lp, lp, None, 0.2, 0.2, 0.0, 1.0, True)
+        assert ops.token_logprobs_backward(lp, z, tok, st, 1.0).shape == z.shape
+        loss, _, rows, d = ops.policy_loss(z, tok, lp, lp, lp, None, 0.2, 0.2, 0.0, 1.0, True, False)
+        assert d.numel() == 0
         assert loss.shape == () and ops.policy_loss_backward(loss, z, tok, rows, 1.0).shape == z.shape
 
 
