@@ -399,38 +399,91 @@ __global__ __launch_bounds__(1024) void route_finish_kernel(Args a, int blocks) 
 
 // One group a token again: p from the logits, the dense part of the gradient in registers, and
 // the chosen experts' part through the group's row in LDS (where it is added at their indices).
+// A row holds a lane's VPT values as 16-byte pieces G lanes apart: neighbouring lanes' pieces
+// are neighbours, and no two lanes of an access meet in a bank (value after value, 16 of them a
+// lane, four lanes met in each: 51 us instead of 38 on 131071 tokens of 256 experts).
+template <int G, int VPT>
+MUON_DEVICE int row_at(int e) {
+  return (((e % VPT) / 4) * G + e / VPT) * 4 + e % 4;
+}
+template <int G, int VPT>
+MUON_DEVICE void put_row(float* row, int lane, const float (&v)[VPT]) {
+#pragma unroll
+  for (int c = 0; c < VPT / 4; ++c)
+    *(f32x4*)(row + (c * G + lane) * 4) = f32x4{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
+}
+template <int G, int VPT>
+MUON_DEVICE void get_row(const float* row, int lane, float (&v)[VPT]) {
+#pragma unroll
+  for (int c = 0; c < VPT / 4; ++c) {
+    const f32x4 w = *(const f32x4*)(row + (c * G + lane) * 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[4 * c + i] = w[i];
+  }
+}
+
+// Slot lane + q G of a token is this lane's: the chosen expert and its gate's gradient.
+template <int G, int SLOTS>
+MUON_DEVICE void load_slots(const BackArgs& a, int64_t t, int lane, int (&at)[SLOTS], float (&up)[SLOTS]) {
+#pragma unroll
+  for (int q = 0; q < SLOTS; ++q) {
+    at[q] = -1;
+    up[q] = 0.0f;
+    if (q * G >= a.k) continue;  // the same for all
+    const int i = lane + q * G;
+    if (!a.dgates || i >= a.k) continue;
+    const int64_t e = a.experts[t * a.k + i];
+    up[q] = a.dgates[t * a.k + i];
+    at[q] = e >= 0 && e < a.E ? (int)e : -1;
+  }
+}
+
 template <int DT, int G, int VPT>
 __global__ __launch_bounds__(BWD_THREADS) void route_backward_kernel(BackArgs a) {
   constexpr int GROUPS = BWD_THREADS / G;
   constexpr int ECAP = G * VPT;
   constexpr int SLOTS = (ECAP < KMAX ? ECAP : KMAX) / G;
-  // rows 16 bytes aligned for the vector accesses, 4 words apart in their banks
-  __shared__ __attribute__((aligned(16))) float rows[GROUPS][ECAP + 4];
+  __shared__ __attribute__((aligned(16))) float rows[GROUPS][ECAP];
   const int lane = threadIdx.x % G, group = threadIdx.x / G;
   const int e0 = lane * VPT;
   const float n = a.kept[0];
   const float db = a.dbalance && n > 0.0f ? a.dbalance[0] : 0.0f;
   const float zc = a.dzloss && n > 0.0f ? 2.0f * a.dzloss[0] / n : 0.0f;
-  const float bc = n > 0.0f ? db * (float)a.E / ((float)a.k * n) : 0.0f;
+  // a count is at most the tokens, which fit 31 bits; 1 / n twice, since n^2 may leave the range
+  const float inv_n = n > 0.0f ? 1.0f / n : 0.0f;
+  const float bc = db * (float)a.E / (float)a.k * inv_n;
   float coef[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j)
-    coef[j] = e0 + j < a.E && n > 0.0f ? bc * ((float)a.counts[e0 + j] / n) : 0.0f;
+    coef[j] = e0 + j < a.E ? bc * ((float)((const uint32_t*)a.counts)[2 * (e0 + j)] * inv_n) : 0.0f;
   float* mine = rows[group];
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   int64_t t = (int64_t)blockIdx.x * GROUPS + group;
   muon_u4 raw[VPT / Vec16<DT>::N];
-  if (t < a.T) load_logits<DT, VPT>(a.z, t * a.row, e0, a.E, raw);
+  int next_at[SLOTS];
+  float next_up[SLOTS];
+  if (t < a.T) {
+    load_logits<DT, VPT>(a.z, t * a.row, e0, a.E, raw);
+    load_slots<G, SLOTS>(a, t, lane, next_at, next_up);
+  }
   for (; t < a.T; t += step) {
-    float v[VPT];
+    float v[VPT], part[SLOTS], up[SLOTS];
+    int at[SLOTS];
     unpack_logits<DT, VPT>(raw, v);
-    if (t + step < a.T) load_logits<DT, VPT>(a.z, (t + step) * a.row, e0, a.E, raw);
-    const bool masked = a.mask && !a.mask[t];
+#pragma unroll
+    for (int q = 0; q < SLOTS; ++q) {
+      at[q] = next_at[q];
+      up[q] = next_up[q];
+    }
+    if (t + step < a.T) {  // the next token's loads are in flight meanwhile
+      load_logits<DT, VPT>(a.z, (t + step) * a.row, e0, a.E, raw);
+      load_slots<G, SLOTS>(a, t + step, lane, next_at, next_up);
+    }
     float m = v[0];
 #pragma unroll
     for (int j = 1; j < VPT; ++j) m = fmaxf(m, v[j]);
     m = group_max<G>(m);
-    bool on = !masked;
+    bool on = !(a.mask && !a.mask[t]);
     if (m == -INFINITY) {
       float bad = 0.0f;
 #pragma unroll
@@ -450,24 +503,16 @@ __global__ __launch_bounds__(BWD_THREADS) void route_backward_kernel(BackArgs a)
     for (int j = 0; j < VPT; ++j) {
       v[j] *= inv;
       dot += v[j] * coef[j];
-      mine[e0 + j] = v[j];
     }
     dot = group_sum<G>(dot);
+    put_row<G, VPT>(mine, lane, v);
     wave_lds_fence();
-    // slot lane + q G of the token is this lane's: the chosen expert, its p, its gate's gradient
-    int at[SLOTS];
-    float part[SLOTS], up[SLOTS];
     float held = 0.0f, inner = 0.0f;  // sums of p and of p G over the chosen
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) {
-      const int i = lane + q * G;
-      at[q] = -1;
-      if (!a.dgates || !on || i >= a.k) continue;
-      const int64_t e = a.experts[t * a.k + i];
-      if (e < 0 || e >= a.E) continue;
-      at[q] = (int)e;
-      part[q] = mine[e];
-      up[q] = a.dgates[t * a.k + i];
+      part[q] = 0.0f;
+      if (q * G >= a.k) continue;
+      part[q] = on && at[q] >= 0 ? mine[row_at<G, VPT>(at[q])] : 0.0f;
       held += part[q];
       inner += part[q] * up[q];
     }
@@ -476,23 +521,23 @@ __global__ __launch_bounds__(BWD_THREADS) void route_backward_kernel(BackArgs a)
     wave_lds_fence();
     const float shift = zc * lse - dot - (a.normalize ? 0.0f : inner);
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) mine[e0 + j] = v[j] * (coef[j] + shift);
+    for (int j = 0; j < VPT; ++j) v[j] *= coef[j] + shift;
+    put_row<G, VPT>(mine, lane, v);
     wave_lds_fence();
     const float scale = a.normalize ? __builtin_amdgcn_rcpf(held) : 1.0f;
     const float mean = a.normalize ? inner * scale : 0.0f;
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q)  // a token's experts are distinct: no two lanes meet
-      if (at[q] >= 0) mine[at[q]] += part[q] * scale * (up[q] - mean);
+      if (q * G < a.k && on && at[q] >= 0) mine[row_at<G, VPT>(at[q])] += part[q] * scale * (up[q] - mean);
     wave_lds_fence();
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) v[j] = on ? mine[e0 + j] : 0.0f;
+    get_row<G, VPT>(mine, lane, v);
     wave_lds_fence();
     constexpr int N = Vec16<DT>::N;
 #pragma unroll
     for (int c = 0; c < VPT; c += N) {
       float x[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = v[c + j];
+      for (int j = 0; j < N; ++j) x[j] = on ? v[c + j] : 0.0f;
       const int e = e0 + c;
       if (e + N <= a.E) {
         store_u4((void*)elem_at<DT>(a.dz, t * a.E + e), Vec16<DT>::pack(x));
@@ -526,6 +571,10 @@ int lanes_of(int64_t E) {
 // Forward workgroups: enough to hold two per CU, each at least one round of tokens; their partials
 // (E sums and counts each) are what the finishing workgroup reads.
 constexpr int MAX_BLOCKS = 512;
+// Backward workgroups: four of 256 threads per CU. With 512, 1024 and 2048 of them the backward pass of
+// 131071 x 256 bf16 took 39, 34 and 41 us, of 65536 x 256 fp32 33, 36 and 45 (each has the experts'
+// coefficients to make first).
+constexpr int MAX_BWD_BLOCKS = 1024;
 constexpr int64_t WS_HEAD = (EMAX / 16) * 8 + 8;  // part_b, ticket
 int forward_blocks(int64_t T, int64_t E) {
   const int64_t groups = FWD_THREADS / lanes_of(E);
@@ -539,7 +588,7 @@ int check(const char* what, int dtype, int64_t T, int64_t E, int64_t k, int64_t 
     muon_set_error("%s: unsupported dtype %d", what, dtype);
     return MUON_ERR_DTYPE;
   }
-  if (T < 0 || E < 1 || E > EMAX || k < 1 || k > E || k > KMAX || (T > 1 && row < 0)) {
+  if (T < 0 || T >= (1LL << 31) || E < 1 || E > EMAX || k < 1 || k > E || k > KMAX || (T > 1 && row < 0)) {
     muon_set_error("%s: bad extents (tokens %lld, experts %lld in 1..%d, top %lld in 1..%d and at "
                    "most the experts)", what, (long long)T, (long long)E, EMAX, (long long)k, KMAX);
     return MUON_ERR_SHAPE;
@@ -608,7 +657,7 @@ int muon_route_backward(const void* logits, int dtype, int64_t row_stride, int64
   return by_experts(experts, [&](auto G, auto V) {
     constexpr int g = decltype(G)::value, v = decltype(V)::value;
     const int64_t groups = BWD_THREADS / g;
-    const int grid = (int)std::min<int64_t>((tokens + groups - 1) / groups, 2048);
+    const int grid = (int)std::min<int64_t>((tokens + groups - 1) / groups, MAX_BWD_BLOCKS);
     if (dtype == MUON_DT_F32) route_backward_kernel<MUON_DT_F32, g, v><<<grid, BWD_THREADS, 0, s>>>(a);
     else if (dtype == MUON_DT_BF16) route_backward_kernel<MUON_DT_BF16, g, v><<<grid, BWD_THREADS, 0, s>>>(a);
     else route_backward_kernel<MUON_DT_F16, g, v><<<grid, BWD_THREADS, 0, s>>>(a);
