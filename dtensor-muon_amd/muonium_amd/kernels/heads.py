@@ -11,16 +11,16 @@ from .. import _row_ops
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _check_on(device, **tensors) -> None:
-    for name, t in tensors.items():
+def _check_on(device: torch.device, *tensors: Tensor | None) -> None:
+    for t in tensors:
         if t is not None and t.device != device:
-            raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+            raise RuntimeError(f"tensors on two devices: {device} and {t.device}")
 
 
 def _weight(w: Tensor | None, dim: int) -> Tensor | None:
     if w is None:
         return None
-    if w.shape != (dim,):
+    if w.dim() != 1 or w.size(0) != dim:
         raise ValueError(f"weights are ({dim},); got {tuple(w.shape)}")
     if w.dtype not in _FLOATS:
         raise TypeError(f"weights are fp32, bf16 or fp16; got {w.dtype}")
@@ -57,26 +57,27 @@ def qk_norm_rope(
 
     Returns the new queries and keys, contiguous, in their input's type. Differentiable in q, k
     and the weights; computed in fp32 and rounded once."""
-    shape, dim, device = q.shape, q.shape[-1], q.device
-    if q.dim() not in (3, 4) or k.dim() != q.dim():
+    shape, other, device = q.shape, k.shape, q.device
+    dim = shape[-1]
+    if len(shape) not in (3, 4) or len(other) != len(shape):
         raise ValueError(f"q and k are (batch, tokens, heads, dim) or (tokens, heads, dim); got "
-                         f"{tuple(shape)} and {tuple(k.shape)}")
-    if shape[:-2] != k.shape[:-2] or dim != k.shape[-1]:
+                         f"{tuple(shape)} and {tuple(other)}")
+    lead = shape[:-2]
+    if lead != other[:-2] or dim != other[-1]:
         raise ValueError(f"q and k differ in batch, tokens or dim: {tuple(shape)} and "
-                         f"{tuple(k.shape)}")
+                         f"{tuple(other)}")
     if q.dtype not in _FLOATS or k.dtype != q.dtype:
         raise TypeError(f"q and k are both fp32, bf16 or fp16; got {q.dtype} and {k.dtype}")
     if not 1 <= dim <= 1024:
         raise ValueError(f"dim is 1 to 1024; got {dim}")
-    _check_on(device, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin,
-              positions=positions)
+    _check_on(device, k, q_weight, k_weight, cos, sin, positions)
     q_weight, k_weight = _weight(q_weight, dim), _weight(k_weight, dim)
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise TypeError(f"weights of two types: {q_weight.dtype} and {k_weight.dtype}")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
     if cos is not None:
-        if cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] > dim:
+        if cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.size(1) > dim:
             raise ValueError(f"cos and sin are (length, rotary / 2) with rotary at most {dim}; got "
                              f"{tuple(cos.shape)} and {tuple(sin.shape)}")
         if cos.dtype != torch.float32 or sin.dtype != torch.float32:
@@ -87,12 +88,12 @@ def qk_norm_rope(
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"positions are int32 or int64; got {positions.dtype}")
-        if positions.shape != shape[:-2] and positions.shape != shape[-3:-2]:
-            raise ValueError(f"positions are ({shape[-3]},) or {tuple(shape[:-2])}; got "
+        if positions.shape != lead and positions.shape != lead[-1:]:
+            raise ValueError(f"positions are ({lead[-1]},) or {tuple(lead)}; got "
                              f"{tuple(positions.shape)}")
         positions = _row_ops.unit_last(positions)
-    elif cos is not None and shape[-3] > cos.shape[0]:
-        raise ValueError(f"{shape[-3]} tokens, but the tables have {cos.shape[0]} positions")
+    elif cos is not None and lead[-1] > cos.size(0):
+        raise ValueError(f"{lead[-1]} tokens, but the tables have {cos.size(0)} positions")
     _row_ops.check_device(device)
     return _row_ops.qk_norm_rope(_row_ops.unit_last(q), _row_ops.unit_last(k), q_weight, k_weight,
                                  cos, sin, positions, eps, interleaved)

@@ -24,7 +24,7 @@ def _check(logits: Tensor, tokens: Tensor, temperature: float) -> None:
         raise ValueError(f"logits are (..., vocabulary); got {tuple(logits.shape)}")
     if logits.dtype not in _FLOATS:
         raise TypeError(f"logits are fp32, bf16 or fp16; got {logits.dtype}")
-    _check_on(logits.device, tokens=tokens)
+    _check_on(logits.device, tokens)
     if tokens.dtype != torch.int64:
         raise TypeError(f"tokens are int64; got {tokens.dtype}")
     if tokens.shape != logits.shape[:-1]:
@@ -93,15 +93,16 @@ def policy_loss(
     is another number (one more rounding in bf16, none for a power of two). fp16, whose
     unscaled gradient would underflow, and longer rows read the logits again in the backward pass."""
     _check(logits, tokens, temperature)
-    given = {"old_logprobs": old_logprobs, "advantages": advantages, "weights": weights}
-    if ref_logprobs is not None:
-        given["ref_logprobs"] = ref_logprobs
-    _check_on(logits.device, **given)
-    for name, t in given.items():
+    _check_on(logits.device, old_logprobs, advantages, weights, ref_logprobs)
+    shape = tokens.shape
+    for name, t in (("old_logprobs", old_logprobs), ("advantages", advantages),
+                    ("weights", weights), ("ref_logprobs", ref_logprobs)):
+        if t is None:
+            continue
         if t.dtype != torch.float32:
             raise TypeError(f"{name} is fp32; got {t.dtype}")
-        if t.shape != tokens.shape:
-            raise ValueError(f"{name} is {tuple(tokens.shape)}; got {tuple(t.shape)}")
+        if t.shape != shape:
+            raise ValueError(f"{name} is {tuple(shape)}; got {tuple(t.shape)}")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient: policy_loss makes one for the logits "
                              "alone (detach it)")

@@ -48,7 +48,7 @@ def route(logits: Tensor, k: int, *, token_mask: Tensor | None = None, normalize
     if not 1 <= k <= min(experts, 64):
         raise ValueError(f"k is 1 to {min(experts, 64)} for {experts} experts; got {k}")
     if token_mask is not None:
-        _check_on(logits.device, token_mask=token_mask)
+        _check_on(logits.device, token_mask)
         if token_mask.dtype != torch.bool:
             raise TypeError(f"token_mask is bool; got {token_mask.dtype}")
         if token_mask.shape != logits.shape[:-1]:
