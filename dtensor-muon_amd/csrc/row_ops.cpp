@@ -64,6 +64,26 @@ Tensor unit_last(const Tensor& t) {
   return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
+// What a kernel takes by a plain pointer, contiguous: of one type, so many values, beside `like`.
+Tensor plain(const Tensor& t, const Tensor& like, at::ScalarType type, int64_t numel,
+             const char* name) {
+  TORCH_CHECK(t.scalar_type() == type && t.numel() == numel && t.device() == like.device(),
+              "muonium_amd: ", name, " has to be ", numel, " values of ", type, " on ",
+              like.device(), "; got ", t.numel(), " of ", t.scalar_type(), " on ", t.device());
+  return t.contiguous();
+}
+optional<Tensor> plain(const optional<Tensor>& t, const Tensor& like, at::ScalarType type,
+                       int64_t numel, const char* name) {
+  if (!t || !t->defined()) return std::nullopt;
+  return plain(*t, like, type, numel, name);
+}
+// Rows of logits with a contiguous last dimension.
+Tensor rows_of(const Tensor& logits) {
+  TORCH_CHECK(logits.dim() == 2, "muonium_amd: logits have to be (rows, values); got ",
+              logits.sizes());
+  return unit_last(logits);
+}
+
 // ---- queries and keys -------------------------------------------------------------------
 
 struct QkArgs {
@@ -73,6 +93,12 @@ struct QkArgs {
 
   QkArgs(const Tensor& q, const Tensor& k, const optional<Tensor>& qw, const optional<Tensor>& kw,
          const optional<Tensor>& cos, const optional<Tensor>& pos) {
+    TORCH_CHECK((q.dim() == 3 || q.dim() == 4) && k.dim() == q.dim() && k.size(0) == q.size(0) &&
+                    k.size(-3) == q.size(-3) && k.size(-1) == q.size(-1) &&
+                    k.scalar_type() == q.scalar_type() && k.device() == q.device() &&
+                    (!qw || !kw || qw->scalar_type() == kw->scalar_type()),
+                "muonium_amd: q and k, or their weights, do not belong together: ", q.sizes(),
+                " and ", k.sizes());
     put(q, 0);
     put(k, 3);
     if (qw) w_dtype = dtype_code(*qw);
@@ -96,11 +122,38 @@ struct QkArgs {
   }
 };
 
-Tensor2 qk_forward(const Tensor& q, const Tensor& k, const optional<Tensor>& qw,
-                   const optional<Tensor>& kw, const optional<Tensor>& cos,
-                   const optional<Tensor>& sin, const optional<Tensor>& pos, double eps,
+// The weights, tables and positions of a call, as the kernels take them.
+struct QkRest {
+  optional<Tensor> qw, kw, cos, sin, pos;
+
+  QkRest(const Tensor& q, const optional<Tensor>& qw_, const optional<Tensor>& kw_,
+         const optional<Tensor>& cos_, const optional<Tensor>& sin_, const optional<Tensor>& pos_) {
+    if (qw_) qw = plain(qw_, q, qw_->scalar_type(), q.size(-1), "a weight");
+    if (kw_) kw = plain(kw_, q, kw_->scalar_type(), q.size(-1), "a weight");
+    if (cos_) {
+      TORCH_CHECK(sin_ && cos_->dim() == 2, "muonium_amd: cos and sin are two tables");
+      cos = plain(cos_, q, at::kFloat, cos_->numel(), "cos");
+      sin = plain(sin_, q, at::kFloat, cos_->numel(), "sin");
+    }
+    if (pos_) {
+      const bool each = pos_->dim() == 2;
+      const int64_t batch = q.dim() == 4 ? q.size(0) : 1;
+      TORCH_CHECK((pos_->scalar_type() == at::kLong || pos_->scalar_type() == at::kInt) &&
+                      pos_->dim() >= 1 && pos_->dim() <= 2 && pos_->device() == q.device() &&
+                      pos_->size(-1) == q.size(-3) && (!each || pos_->size(0) == batch),
+                  "muonium_amd: positions have to be int32 or int64, (tokens,) or (batch, tokens)");
+      pos = unit_last(*pos_);
+    }
+  }
+};
+
+Tensor2 qk_forward(const Tensor& q_, const Tensor& k_, const optional<Tensor>& qw_,
+                   const optional<Tensor>& kw_, const optional<Tensor>& cos_,
+                   const optional<Tensor>& sin_, const optional<Tensor>& pos_, double eps,
                    bool interleaved) {
-  const at::DeviceGuard guard(q.device());
+  const at::DeviceGuard guard(q_.device());
+  const Tensor q = unit_last(q_), k = unit_last(k_);
+  const auto [qw, kw, cos, sin, pos] = QkRest(q, qw_, kw_, cos_, sin_, pos_);
   Tensor q_out = fresh(q), k_out = fresh(k);
   const QkArgs a(q, k, qw, kw, cos, pos);
   check(muon_qk_norm_rope(ptr(q), ptr(k), a.strides, ptr(qw), ptr(kw), a.w_dtype, ptr<float>(cos),
@@ -111,11 +164,18 @@ Tensor2 qk_forward(const Tensor& q, const Tensor& k, const optional<Tensor>& qw,
   return {q_out, k_out};
 }
 
-Tensor4 qk_backward(const Tensor& dq_out, const Tensor& dk_out, const Tensor& q, const Tensor& k,
-                    const optional<Tensor>& qw, const optional<Tensor>& kw,
-                    const optional<Tensor>& cos, const optional<Tensor>& sin,
-                    const optional<Tensor>& pos, double eps, bool interleaved) {
-  const at::DeviceGuard guard(q.device());
+Tensor4 qk_backward(const Tensor& dq_out, const Tensor& dk_out, const Tensor& q_, const Tensor& k_,
+                    const optional<Tensor>& qw_, const optional<Tensor>& kw_,
+                    const optional<Tensor>& cos_, const optional<Tensor>& sin_,
+                    const optional<Tensor>& pos_, double eps, bool interleaved) {
+  const at::DeviceGuard guard(q_.device());
+  const Tensor q = unit_last(q_), k = unit_last(k_);
+  const auto [qw, kw, cos, sin, pos] = QkRest(q, qw_, kw_, cos_, sin_, pos_);
+  TORCH_CHECK(dq_out.sizes() == q.sizes() && dk_out.sizes() == k.sizes() &&
+                  dq_out.scalar_type() == q.scalar_type() &&
+                  dk_out.scalar_type() == q.scalar_type() && dq_out.device() == q.device() &&
+                  dk_out.device() == q.device(),
+              "muonium_amd: gradients of q and k are not like them");
   const Tensor gq = unit_last(dq_out), gk = unit_last(dk_out);
   Tensor dq = fresh(q), dk = fresh(k);
   Tensor dqw = qw ? fresh(*qw) : empty(q, {0}, q.scalar_type());
@@ -137,10 +197,12 @@ Tensor4 qk_backward(const Tensor& dq_out, const Tensor& dk_out, const Tensor& q,
 
 // ---- routing ----------------------------------------------------------------------------
 
-Tensor6 route_forward(const Tensor& logits, int64_t top, const optional<Tensor>& mask,
+Tensor6 route_forward(const Tensor& logits_, int64_t top, const optional<Tensor>& mask_,
                       bool normalize) {
-  const at::DeviceGuard guard(logits.device());
+  const at::DeviceGuard guard(logits_.device());
+  const Tensor logits = rows_of(logits_);
   const int64_t n = logits.size(0), e = logits.size(1);
+  const auto mask = plain(mask_, logits, at::kBool, n, "the mask");
   Tensor gates = empty(logits, {n, top}, at::kFloat), experts = empty(logits, {n, top}, at::kLong);
   Tensor counts = empty(logits, {e}, at::kLong);
   Tensor balance = empty(logits, {}, at::kFloat), zloss = empty(logits, {}, at::kFloat);
@@ -155,17 +217,23 @@ Tensor6 route_forward(const Tensor& logits, int64_t top, const optional<Tensor>&
 }
 
 Tensor route_backward(const optional<Tensor>& dgates, const optional<Tensor>& dbalance,
-                      const optional<Tensor>& dzloss, const Tensor& logits,
-                      const optional<Tensor>& mask, const Tensor& experts, const Tensor& counts,
-                      const Tensor& kept, bool normalize) {
-  const at::DeviceGuard guard(logits.device());
+                      const optional<Tensor>& dzloss, const Tensor& logits_,
+                      const optional<Tensor>& mask_, const Tensor& experts_, const Tensor& counts_,
+                      const Tensor& kept_, bool normalize) {
+  const at::DeviceGuard guard(logits_.device());
+  const Tensor logits = rows_of(logits_);
+  const int64_t n = logits.size(0), e = logits.size(1), top = experts_.size(-1);
+  const auto mask = plain(mask_, logits, at::kBool, n, "the mask");
+  const Tensor experts = plain(experts_, logits, at::kLong, n * top, "the experts");
+  const Tensor counts = plain(counts_, logits, at::kLong, e, "the counts");
+  const Tensor kept = plain(kept_, logits, at::kFloat, 1, "the token count");
+  const auto dg = plain(dgates, logits, at::kFloat, n * top, "the gates' gradient");
+  const auto db = plain(dbalance, logits, at::kFloat, 1, "the balance loss's gradient");
+  const auto dz = plain(dzloss, logits, at::kFloat, 1, "the z loss's gradient");
   Tensor dlogits = fresh(logits);
-  optional<Tensor> dg = dgates;
-  if (dg && dg->defined()) dg = dg->contiguous();
-  check(muon_route_backward(ptr(logits), dtype_code(logits), logits.stride(0), logits.size(0),
-                            logits.size(1), experts.size(1), normalize, ptr(mask),
-                            ptr<int64_t>(experts), ptr<int64_t>(counts), ptr<float>(kept),
-                            ptr<float>(dg), ptr<float>(dbalance), ptr<float>(dzloss),
+  check(muon_route_backward(ptr(logits), dtype_code(logits), logits.stride(0), n, e, top,
+                            normalize, ptr(mask), ptr<int64_t>(experts), ptr<int64_t>(counts),
+                            ptr<float>(kept), ptr<float>(dg), ptr<float>(db), ptr<float>(dz),
                             ptr(dlogits), stream_of(logits)),
         "muon_route_backward");
   return dlogits;
@@ -178,9 +246,11 @@ Tensor logp_scratch(const Tensor& logits) {
                                                              logits.size(1)));
 }
 
-Tensor2 logp_forward(const Tensor& logits, const Tensor& tokens, double temperature, bool keep) {
-  const at::DeviceGuard guard(logits.device());
+Tensor2 logp_forward(const Tensor& logits_, const Tensor& tokens_, double temperature, bool keep) {
+  const at::DeviceGuard guard(logits_.device());
+  const Tensor logits = rows_of(logits_);
   const int64_t n = logits.size(0);
+  const Tensor tokens = plain(tokens_, logits, at::kLong, n, "the tokens");
   Tensor logp = empty(logits, {n}, at::kFloat), stats = empty(logits, {keep ? 2 * n : 0}, at::kFloat);
   Tensor ws = logp_scratch(logits);
   check(muon_token_logprobs(ptr(logits), dtype_code(logits), logits.stride(0), n, logits.size(1),
@@ -191,9 +261,10 @@ Tensor2 logp_forward(const Tensor& logits, const Tensor& tokens, double temperat
 }
 
 Tensor logp_gradient(const Tensor& dlogp, const float* scale, const Tensor& logits,
-                     const Tensor& tokens, const float* stats, double temperature) {
+                     const Tensor& tokens_, const float* stats, double temperature) {
+  const Tensor tokens = plain(tokens_, logits, at::kLong, logits.size(0), "the tokens");
+  const Tensor g = plain(dlogp, logits, at::kFloat, logits.size(0), "the gradient");
   Tensor dlogits = fresh(logits);
-  const Tensor g = dlogp.contiguous();
   check(muon_token_logprobs_backward(ptr(logits), dtype_code(logits), logits.stride(0),
                                      logits.size(0), logits.size(1), ptr<int64_t>(tokens),
                                      (float)temperature, stats, ptr<float>(g), scale, ptr(dlogits),
@@ -205,17 +276,24 @@ Tensor logp_gradient(const Tensor& dlogp, const float* scale, const Tensor& logi
 Tensor logp_backward(const Tensor& dlogp, const Tensor& logits, const Tensor& tokens,
                      const Tensor& stats, double temperature) {
   const at::DeviceGuard guard(logits.device());
-  return logp_gradient(dlogp, nullptr, logits, tokens, ptr<float>(stats), temperature);
+  const Tensor kept = plain(stats, logits, at::kFloat, 2 * logits.size(0), "the statistics");
+  return logp_gradient(dlogp, nullptr, rows_of(logits), tokens, ptr<float>(kept), temperature);
 }
 
 // rows: per row the term, and (keep) the slope and the two statistics that a later gradient
 // needs; dlogits: the gradient for a loss gradient of 1 (one_pass), else empty.
-Tensor4 policy_forward(const Tensor& logits, const Tensor& tokens, const Tensor& old,
-                       const Tensor& advantages, const Tensor& weights, const optional<Tensor>& ref,
-                       double clip_low, double clip_high, double kl_coef, double temperature,
+Tensor4 policy_forward(const Tensor& logits_, const Tensor& tokens_, const Tensor& old_,
+                       const Tensor& advantages_, const Tensor& weights_,
+                       const optional<Tensor>& ref_, double clip_low, double clip_high, double kl_coef, double temperature,
                        bool keep, bool one_pass) {
-  const at::DeviceGuard guard(logits.device());
+  const at::DeviceGuard guard(logits_.device());
+  const Tensor logits = rows_of(logits_);
   const int64_t n = logits.size(0);
+  const Tensor tokens = plain(tokens_, logits, at::kLong, n, "the tokens");
+  const Tensor old = plain(old_, logits, at::kFloat, n, "the old log probabilities");
+  const Tensor advantages = plain(advantages_, logits, at::kFloat, n, "the advantages");
+  const Tensor weights = plain(weights_, logits, at::kFloat, n, "the weights");
+  const auto ref = plain(ref_, logits, at::kFloat, n, "the reference log probabilities");
   Tensor loss = empty(logits, {}, at::kFloat), logp = empty(logits, {n}, at::kFloat);
   Tensor rows = empty(logits, {keep ? 4 : 1, n}, at::kFloat);
   Tensor dlogits = one_pass ? fresh(logits) : empty(logits, {0}, logits.scalar_type());
@@ -237,8 +315,11 @@ Tensor4 policy_forward(const Tensor& logits, const Tensor& tokens, const Tensor&
 Tensor policy_backward(const Tensor& dloss, const Tensor& logits, const Tensor& tokens,
                        const Tensor& rows, double temperature) {
   const at::DeviceGuard guard(logits.device());
-  return logp_gradient(rows.select(0, 1), ptr<float>(dloss), logits, tokens,
-                       ptr<float>(rows) + 2 * logits.size(0), temperature);
+  const int64_t n = logits.size(0);
+  const Tensor kept = plain(rows, logits, at::kFloat, 4 * n, "the rows' values").view({4, n});
+  const Tensor scale = plain(dloss, logits, at::kFloat, 1, "the loss's gradient");
+  return logp_gradient(kept.select(0, 1), ptr<float>(scale), rows_of(logits), tokens,
+                       ptr<float>(kept) + 2 * n, temperature);
 }
 
 // ---- gradients --------------------------------------------------------------------------
@@ -427,8 +508,9 @@ struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
         none[0] = made->second.toTensor();
         ctx->saved_data.erase(made);
         const at::DeviceGuard guard(none[0].device());
+        const Tensor scale = plain(grads[0], none[0], at::kFloat, 1, "the loss's gradient");
         check(muon_scale_gradient(ptr(none[0]), dtype_code(none[0]), none[0].numel(),
-                                  ptr<float>(grads[0]), stream_of(none[0])),
+                                  ptr<float>(scale), stream_of(none[0])),
               "muon_scale_gradient");
       } else {
         none[0] = OP("policy_loss_backward", policy_backward)

@@ -658,6 +658,34 @@ def test_row_operators_in_a_captured_graph():
             assert torch.equal(a, b), i
 
 
+def test_registered_ops_refuse_what_their_kernels_could_not_read():
+    """The torch operators behind the entry points check what the kernels take by pointer."""
+    ops = torch.ops.muonium_amd
+    z = torch.randn(6, 8, device="cuda")
+    tok = torch.zeros(6, dtype=torch.int64, device="cuda")
+    f = torch.zeros(6, device="cuda")
+    q = torch.randn(1, 3, 2, 16, device="cuda")
+    for call in (lambda: ops.token_logprobs(z, tok.int(), 1.0, False),
+                 lambda: ops.token_logprobs(z, tok[:5], 1.0, False),
+                 lambda: ops.token_logprobs(z, tok.cpu(), 1.0, False),
+                 lambda: ops.token_logprobs(z.double(), tok, 1.0, False),
+                 lambda: ops.token_logprobs_backward(f, z, tok, f, 1.0),
+                 lambda: ops.route(z, 2, torch.ones(5, dtype=torch.bool, device="cuda"), True),
+                 lambda: ops.route(z, 9, None, True),
+                 lambda: ops.route(z[0], 2, None, True),
+                 lambda: ops.policy_loss(z, tok, f.double(), f, f, None, 0.2, 0.2, 0.0, 1.0, False, False),
+                 lambda: ops.policy_loss(z.half(), tok, f, f, f, None, 0.2, 0.2, 0.0, 1.0, True, True),
+                 lambda: ops.policy_loss_backward(f[0], z, tok, f, 1.0),
+                 lambda: ops.qk_norm_rope(q, q[:, :2], None, None, None, None, None, 1e-6, False),
+                 lambda: ops.qk_norm_rope(q, q, f, None, None, None, None, 1e-6, False),
+                 lambda: ops.qk_norm_rope(q, q, None, None, z[:, :5], z[:, :5], tok[:2], 1e-6, False),
+                 lambda: ops.qk_norm_rope(q, q, None, None, torch.ones(4, 9, device="cuda"),
+                                          torch.ones(4, 9, device="cuda"), None, 1e-6, False)):
+        with pytest.raises((RuntimeError, TypeError)):
+            call()
+    torch.cuda.synchronize()
+
+
 def test_row_operators_have_no_second_derivative():
     x = leaf(torch.randn(4, 50, generator=gen(1)))
     y = token_logprobs(x, torch.zeros(4, dtype=torch.int64, device="cuda"))
