@@ -451,32 +451,37 @@ void launch_backward(const Back& a, hipStream_t s) {
     logp_backward_kernel<DT, false><<<grid, BACK_THREADS, 0, s>>>(a);
 }
 
-// Slices of a row: until a launch has four workgroups per CU, but none of less than 16 KB (one
-// round of a workgroup's loads is 32 KB).
-int slices_for(int dtype, int64_t N, int64_t V) {
-  const int64_t bytes = V * (dtype == MUON_DT_F32 ? 4 : 2);
-  const int64_t want = N ? (1024 + N - 1) / N : 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, bytes / 16384), 64));
+// Slices of a row. One workgroup a row as a rule: joining slices takes a second launch. Longer
+// rows than SPLIT_FROM, of which fewer than 128 come together, are cut until there are four
+// workgroups per CU. One row, whole and cut (us a call): 32000 values 6.1 and 10.0, 128000 9.0 and
+// 10.4, 262144 14.6 and 9.2, 524288 26.1 and 9.7; 64 rows of 262144 values 17.3 and 15.3.
+constexpr int64_t SPLIT_FROM = 131072;
+int slices_for(int64_t N, int64_t V) {
+  if (V <= SPLIT_FROM || N >= 128 || N < 1) return 1;
+  return (int)std::min<int64_t>(std::min<int64_t>(1024 / N, V / 8192), 64);
 }
 
 // Threads a row: the fewest that give 2^18 in all (four waves per SIMD), with at most 64
 // 16-byte pieces each (32 above a wave). 8192 rows of bf16 with 64, 128, 256 and 512 threads:
 // 2000 values 12, 14, 20, 40 us, 16000 values 45, 44, 47, 77 us; 4096 rows of 32000 values 42, 46,
-// 44, 52 us; 8192 rows of 128000 values with 256 and 512: 348 and 334 us.
+// 44, 52 us; 8192 rows of 128000 values with 256 and 512: 348 and 334 us. Fewer rows than CUs take
+// 1024 (200 rows of 128000 values 12 us, with 512 15).
 template <int DT>
 void launch_sums_dt(const Rows& a, const Policy& p, int slices, Sum* part, hipStream_t s) {
   const dim3 grid(slices, (unsigned)std::min(a.N, MAX_GRID_Y));
   const int64_t vecs = a.V / Vec16<DT>::N;
   int threads = vecs <= 64 * 64 ? 64 : vecs <= 32 * 128 ? 128 : vecs <= 32 * 256 ? 256 : 512;
-  while (threads < 512 && a.N * threads < (1 << 18)) threads *= 2;
+  while (threads < 512 && a.N * threads < (1 << 18) && 2 * threads <= vecs) threads *= 2;
+  if (threads == 512 && slices == 1 && a.N <= 256 && vecs >= 2048) threads = 1024;
   if (threads == 64) logp_kernel<DT, 64><<<grid, 64, 0, s>>>(a, p, part);
   else if (threads == 128) logp_kernel<DT, 128><<<grid, 128, 0, s>>>(a, p, part);
   else if (threads == 256) logp_kernel<DT, 256><<<grid, 256, 0, s>>>(a, p, part);
-  else logp_kernel<DT, 512><<<grid, 512, 0, s>>>(a, p, part);
+  else if (threads == 512) logp_kernel<DT, 512><<<grid, 512, 0, s>>>(a, p, part);
+  else logp_kernel<DT, 1024><<<grid, 1024, 0, s>>>(a, p, part);
 }
 
 int launch_sums(const Rows& a, const Policy& p, int dtype, void* ws, hipStream_t s) {
-  const int slices = slices_for(dtype, a.N, a.V);
+  const int slices = slices_for(a.N, a.V);
   Sum* part = (Sum*)ws;
   if (dtype == MUON_DT_F32) launch_sums_dt<MUON_DT_F32>(a, p, slices, part, s);
   else if (dtype == MUON_DT_BF16) launch_sums_dt<MUON_DT_BF16>(a, p, slices, part, s);
@@ -525,7 +530,7 @@ extern "C" {
 
 int64_t muon_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab) {
   if (!io_ok(dtype) || rows < 0 || vocab < 1) return -1;
-  const int slices = slices_for(dtype, rows, vocab);
+  const int slices = slices_for(rows, vocab);
   return slices == 1 ? 0 : rows * slices * (int64_t)sizeof(Sum);
 }
 
@@ -534,7 +539,7 @@ int muon_token_logprobs(const void* logits, int dtype, int64_t row_stride, int64
                         float* stats, void* ws, void* stream) {
   const int rc = check("token_logprobs", dtype, rows, vocab, row_stride, temperature);
   if (rc || rows == 0) return rc;
-  if (!logits || !tokens || !logprobs || (!ws && slices_for(dtype, rows, vocab) > 1)) {
+  if (!logits || !tokens || !logprobs || (!ws && slices_for(rows, vocab) > 1)) {
     muon_set_error("token_logprobs: null tensor");
     return MUON_ERR_ARG;
   }
@@ -579,7 +584,7 @@ int muon_policy_loss(const void* logits, int dtype, int64_t row_stride, int64_t 
   const int rc = check("policy_loss", dtype, rows, vocab, row_stride, temperature);
   if (rc) return rc;
   if (!loss || (rows && (!logits || !tokens || !old_logprobs || !advantages || !weights ||
-                         !logprobs || !terms || (!ws && !dlogits && slices_for(dtype, rows, vocab) > 1)))) {
+                         !logprobs || !terms || (!ws && !dlogits && slices_for(rows, vocab) > 1)))) {
     muon_set_error("policy_loss: null tensor");
     return MUON_ERR_ARG;
   }

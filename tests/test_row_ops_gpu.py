@@ -391,7 +391,7 @@ def test_token_logprobs_and_its_gradient(case, dtype):
     assert abs((d.double().cpu() * step).sum() - slope) <= room
 
 
-@pytest.mark.parametrize("v", [50, 40000])
+@pytest.mark.parametrize("v", [50, 40000, 140000])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_logprobs_special_rows(dtype, v):
     """Left-out and impossible tokens, masked vocabularies, rows of the lowest value, of infinities
