@@ -10,6 +10,13 @@
 //
 // A row with weight 0, or a negative token, is left out: nothing of it is read, logp is 0 and its
 // gradient 0. A token of V or more gives NaN.
+//
+// Every pass is bound by memory, or nearly: 8192 rows of 128000 bf16 logits are read in 335 us,
+// 6.3 TB/s, and the gradient of 4096 such rows is made in 381 us, 5.5 TB/s. The policy loss reads its
+// logits once for loss and gradient: 6144 rows of 128000, a quarter of them left out, 510 us,
+// 5.4 TB/s, where a copy of 2 GiB moves 5.0 and a second reading would add 190 us.
+// Sums and exponentials are fp32 with the row's maximum taken off first, logp is formed in
+// double, gradients are rounded once at the store.
 #include <algorithm>
 
 #include "rowops.h"
@@ -305,8 +312,11 @@ __global__ __launch_bounds__(BACK_THREADS) void logp_backward_kernel(Back a) {
 }
 
 // The policy loss with its gradient in one pass over the logits: a workgroup holds its whole row
-// in registers (NV 16-byte pieces a thread), sums it, makes the slope g, and writes the gradient
-// from the same registers.
+// in registers (NV 16-byte pieces a thread; the 512 KB of a CU hold 163840 bf16 values beside
+// the working registers), sums it, makes the slope g, and writes the gradient from the same
+// registers. A CU works on one long row at a time, so what its waves compute between reading and
+// writing counts: with two thirds of the instructions the launch above went from 585 to
+// 505 us.
 template <int DT, int NT, int NV, bool STREAM>
 __global__ __launch_bounds__(NT) void policy_row_kernel(Rows a, Policy p, void* dx, int64_t row0) {
   constexpr int N = Vec16<DT>::N;
@@ -439,6 +449,7 @@ int check(const char* what, int dtype, int64_t N, int64_t V, int64_t stride, flo
 
 constexpr int64_t MAX_GRID_Y = 65535;
 // Gradients of this many bytes are stored past the caches (half of the 256 MB last-level one).
+// The gradient of 4096 rows of 128000 bf16 values 406 -> 381 us, of 2047 rows of 50257 73 -> 63.
 constexpr int64_t STREAM_FROM = 128 << 20;
 
 template <int DT>

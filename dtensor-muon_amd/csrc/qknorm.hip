@@ -7,6 +7,11 @@
 // Backward, with u the gradient turned back by the same angle (the rotation's transpose):
 //   dw_i = sum over rows of u_i x_i r,   dx_i = r u_i w_i - x_i r^3 / D * sum_j u_j w_j x_j.
 // r is recomputed from x, which the backward pass reads anyway: nothing is kept between them.
+//
+// Both passes are bound by memory: they read and write each row once (the angles and weights of a
+// token are 4 kB beside 20 kB of bf16 rows). 32768 tokens of 32 + 8 heads of 128 in bf16: forward
+// 123 us, 5.4 TB/s, backward with the weights' gradients 197 us, 5.1 TB/s, where a copy of
+// 2 GiB moves 5.0. Sums, square roots and rotations are fp32, rounded once at the store.
 #include <algorithm>
 
 #include "rowops.h"
@@ -44,13 +49,21 @@ struct Args {
 };
 
 // Heads of a token that one group of lanes takes: their loads are in flight together, and the
-// token's angles and the weights are read once for all of them.
+// token's angles and the weights are read once for all of them. Forward / backward of the size
+// above with 2, 4 and 8 heads: 134 / 223, 134 / 212 and 137 / 218 us (before the stores below).
 constexpr int HC = 4;
 constexpr int NTHREADS = 256;
 constexpr int MAX_PAIRS = 9;  // SINGLE: up to 2 * 9 * 64 values a row
-constexpr int MAX_BWD_BLOCKS = 1024;  // of SINGLE; the others take half
-// Outputs of this many bytes (half of the 256 MB last-level cache) whose runs make whole 64-byte
-// pieces are stored past the caches.
+// Workgroups of the backward pass (each leaves a partial of the weights' gradients): two per CU
+// hold as many loads as their registers allow; SINGLE, whose loads are small, takes twice as
+// many. 6000 tokens of the size above with 512 and 1024: 39.5 and 41.3 us; 8192 tokens of 162
+// values as single values 561 and 334.
+constexpr int MAX_BWD_BLOCKS = 1024;
+// Outputs of this many bytes (half of the 256 MB last-level cache, which else would lose its inputs to
+// lines nobody reads before they are gone) are stored past the caches, if each store instruction
+// writes whole pieces of at least 64 bytes. Forward / backward with and without: the size above
+// 123 / 198 and 130 / 207 us, 18000 tokens of it 59 / 112 and 76 / 120; heads of 48, whose
+// stores make pieces of 48 bytes, 44 / 55 and 26 / 46.
 constexpr int64_t NT_FROM = 128 << 20;
 constexpr int64_t MAX_FWD_BLOCKS = 1 << 22;
 
@@ -81,6 +94,8 @@ MUON_DEVICE int64_t position(const Args& a, int64_t b, int64_t t) {
 //    the run before are computed twice, alike, and counted once in sums (the first `skip` of a run
 //    are left out).
 //  SINGLE: NP pairs of single values a lane, G apart, for what is too small for a run.
+// 8192 tokens of 40 heads of 162 values as RAGGED and as SINGLE: forward 44 and 130, backward 92 and
+// 334 us.
 enum Form { WHOLE, RAGGED, SINGLE };
 
 template <int DT, int G, int NP, Form F, bool NT>

@@ -10,6 +10,12 @@
 // Backward, with a_e = db E c_e / (k N^2), G the gates' gradient:
 //   dz_e = p_e (a_e - sum p a) + 2 lse dzl / N p_e + [e chosen] g_e (G_e - sum g G)  (normalized)
 //   or, with the gates as they are, the last term p_e ([e chosen] G_e - sum over chosen p G).
+//
+// The counts of all tokens stand between the two passes, so both read the logits and make p.
+// Bound by vector instructions, not by memory: a wave's four tokens of 256 experts with 8 choices
+// take about 550 of them forward. 131071 tokens of 256 experts in bf16: forward 45 us (of it 8 for the
+// totals), backward 34 us, where reading the logits takes 13; 32768 tokens of 64 experts in fp32
+// 14 and 7 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -551,7 +557,9 @@ __global__ __launch_bounds__(BWD_THREADS) void route_backward_kernel(BackArgs a)
 }
 
 // Lanes and experts per lane for E experts: 8 experts a lane up to 16 lanes, then 16. More
-// lanes cost more exchange steps per choice, more experts a lane more registers.
+// lanes cost more exchange steps per choice, more experts a lane more registers. 65536 tokens of 256
+// fp32 experts on 16 lanes of 16 and 8 lanes of 32: forward 47 and 43, backward 36 and 57 us;
+// 131072 tokens of 64 on 8 lanes of 8 and 4 of 16: 27 and 27, 18 and 54 us.
 template <typename F>
 int by_experts(int64_t E, F f) {
   if (E <= 8) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
@@ -568,8 +576,9 @@ int lanes_of(int64_t E) {
   return by_experts(E, [](auto G, auto) { return (int)decltype(G)::value; });
 }
 
-// Forward workgroups: enough to hold two per CU, each at least one round of tokens; their partials
-// (E sums and counts each) are what the finishing workgroup reads.
+// Forward workgroups: two of 512 threads per CU; their partials (E sums and counts each) are what
+// the finishing workgroups read. 131071 tokens of 256 bf16 experts with 256, 512 and 1024 of
+// them: 52, 45 and 48 us.
 constexpr int MAX_BLOCKS = 512;
 // Backward workgroups: four of 256 threads per CU. With 512, 1024 and 2048 of them the backward pass of
 // 131071 x 256 bf16 took 39, 34 and 41 us, of 65536 x 256 fp32 33, 36 and 45 (each has the experts'
