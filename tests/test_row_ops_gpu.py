@@ -588,6 +588,66 @@ def test_policy_loss_strided_rows():
             assert torch.equal(a, b)
 
 
+# ---- tensors of more than 2^31 values ---------------------------------------------------------
+
+
+def test_rows_past_32_bit_offsets():
+    """The last rows of tensors of more than 2^31 values come out as they do alone, forward and
+    backward, in every operator."""
+    bf16, n = torch.bfloat16, 3
+    x = torch.randn(17000, 128000, device="cuda", dtype=bf16)
+    assert x.numel() > 2**31
+    tokens = torch.randint(0, 128000, (17000,), device="cuda")
+    f = torch.rand(17000, device="cuda")
+
+    def logits_calls(x, tokens, f):
+        x = x.detach().requires_grad_()
+        lp = token_logprobs(x, tokens)
+        d, = torch.autograd.grad((lp,), (x,), (f,))
+        keep = [lp[-n:].detach().clone(), d[-n:].clone()]
+        del d
+        out = policy_loss(x, tokens, lp.detach() - 0.1, f, f)
+        d, = torch.autograd.grad((out.loss,), (x,))
+        return keep + [out.logprobs[-n:].clone(), d[-n:].clone()]
+
+    big, small = logits_calls(x, tokens, f), logits_calls(x[-n:], tokens[-n:], f[-n:])
+    for a, b in zip(big, small):
+        # a few rows alone take another number of threads: sums in another order
+        torch.testing.assert_close(a, b, rtol=2.0**-7, atol=1e-5)
+    del x, big, small
+    torch.cuda.empty_cache()
+
+    z = torch.randn(9_000_000, 256, device="cuda", dtype=bf16).requires_grad_()
+    assert z.numel() > 2**31
+    r = route(z, 8)
+    few = route(z[-n:].detach(), 8)
+    assert torch.equal(r.experts[-n:], few.experts) and torch.equal(r.gates[-n:], few.gates)
+    assert int(r.counts.sum()) == 8 * 9_000_000
+    g = torch.zeros_like(r.gates)
+    g[-n:] = torch.rand(n, 8, device="cuda")
+    d, = torch.autograd.grad((r.gates,), (z,), (g,))
+    y = z[-n:].detach().requires_grad_()
+    e, = torch.autograd.grad((route(y, 8).gates,), (y,), (g[-n:],))
+    assert torch.equal(d[-n:], e) and torch.count_nonzero(d[:-n]) == 0
+    del z, r, d, g
+    torch.cuda.empty_cache()
+
+    q = torch.randn(560_000, 32, 128, device="cuda", dtype=bf16)
+    assert q.numel() > 2**31
+    angle = torch.rand(560_000, 64, device="cuda")
+    w = torch.rand(128, device="cuda")
+
+    def heads_calls(q, positions):
+        q = q.detach().requires_grad_()
+        a, b = qk_norm_rope(q, q[:, :1], w, w, angle, angle, positions)
+        d, = torch.autograd.grad((a,), (q,), (a.detach(),))
+        return a[-n:].detach().clone(), b[-n:].detach().clone(), d[-n:].clone()
+
+    positions = torch.arange(560_000, device="cuda")
+    for a, b in zip(heads_calls(q, positions), heads_calls(q[-n:], positions[-n:])):
+        assert torch.equal(a, b)
+
+
 # ---- streams, determinism, graphs, torch.compile ----------------------------------------------
 
 
