@@ -386,21 +386,27 @@ __global__ __launch_bounds__(1024) void route_finish_kernel(Args a, int blocks) 
     if (row == 0 && e < a.E) a.counts[e] = count;
     double bal = e < a.E ? sum * (double)count : 0.0;
     for (int off = 1; off < 16; off *= 2) bal += __shfl_xor(bal, off, 64);
-    if (threadIdx.x) return;
-    __hip_atomic_store(&a.part_b[blockIdx.x], bal, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (__hip_atomic_fetch_add(a.ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) !=
-        (int)gridDim.x - 1)
-      return;
+    int ticket = 0;
+    if (threadIdx.x == 0) {
+      __hip_atomic_store(&a.part_b[blockIdx.x], bal, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      ticket = __hip_atomic_fetch_add(a.ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (__shfl(ticket, 0, 64) != (int)gridDim.x - 1) return;
   }
+  // the wave of the last workgroup: at most 64 shares of the balance loss, 16 of the others
+  static_assert(EMAX / 16 <= 64, "a lane a workgroup");
+  const int lane = threadIdx.x;
   double bal = 0.0;
-  for (int b = 0; b < (int)gridDim.x; ++b)
-    bal += __hip_atomic_load(&a.part_b[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  z = n = 0.0;
-  for (int w = 0; w < 16; ++w) {
-    z += red[0][w];
-    n += red[1][w];
+  if (lane < (int)gridDim.x)
+    bal = __hip_atomic_load(&a.part_b[lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  z = lane < 16 ? red[0][lane] : 0.0;
+  n = lane < 16 ? red[1][lane] : 0.0;
+  for (int off = 32; off; off >>= 1) {
+    bal += __shfl_xor(bal, off, 64);
+    z += __shfl_xor(z, off, 64);
+    n += __shfl_xor(n, off, 64);
   }
-  write_losses(a, bal, z, (int64_t)n);
+  if (lane == 0) write_losses(a, bal, z, (int64_t)n);
 }
 
 // One group a token again: p from the logits, the dense part of the gradient in registers, and
