@@ -13,7 +13,7 @@
 //
 // The counts of all tokens stand between the two passes, so both read the logits and make p.
 // Bound by vector instructions, not by memory: a wave's four tokens of 256 experts with 8 choices
-// take about 550 of them forward. 131071 tokens of 256 experts in bf16: forward 45 us (of it 8 for the
+// take about 550 of them forward. 131071 tokens of 256 experts in bf16: forward 43 us (of it 7 for the
 // totals), backward 34 us, where reading the logits takes 13; 32768 tokens of 64 experts in fp32
 // 14 and 7 us.
 #include <algorithm>

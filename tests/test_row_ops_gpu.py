@@ -754,6 +754,20 @@ def test_row_operators_have_no_second_derivative():
         d.sum().backward()
 
 
+def test_row_operators_are_well_behaved_torch_operators():
+    """Schemas, autograd registration, fake implementations and ahead-of-time tracing."""
+    ops = torch.ops.muonium_amd
+    q, k = leaf(torch.randn(2, 3, 4, 32)), leaf(torch.randn(2, 3, 2, 32))
+    w, cos = leaf(torch.ones(32)), torch.rand(9, 16, device="cuda")
+    z = leaf(torch.randn(20, 16))
+    tokens, f = torch.randint(0, 16, (20,), device="cuda"), torch.rand(20, device="cuda")
+    torch.library.opcheck(ops.qk_norm_rope.default, (q, k, w, None, cos, cos, None, 1e-6, False))
+    torch.library.opcheck(ops.route.default, (z, 2, f > 0.2, True))
+    torch.library.opcheck(ops.token_logprobs.default, (z, tokens, 1.0, True))
+    torch.library.opcheck(ops.policy_loss.default,
+                          (z, tokens, f, f, f, None, 0.2, 0.2, 0.1, 1.0, True, False))
+
+
 def test_row_operators_under_an_outer_compile():
     run = _all_calls(1)
     want = run()
