@@ -341,6 +341,16 @@ bool any_needs(const T&... t) {
   return at::GradMode::is_enabled() && (needs(t) || ...);
 }
 
+// There is no forward-mode derivative. Below autograd a dual tensor's tangent would be dropped and
+// the result pass for a constant; torch itself refuses only where a gradient is asked for too.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const optional<Tensor>& t) { return t && has_tangent(*t); }
+template <typename... T>
+void refuse_tangents(const T&... t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(t) || ...),
+                              "muonium_amd's row operators have no forward-mode derivative");
+}
+
 Tensor or_undefined(const optional<Tensor>& t) { return t ? *t : Tensor(); }
 optional<Tensor> or_none(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
 
@@ -398,6 +408,7 @@ Tensor2 qk_autograd(const Tensor& q, const Tensor& k, const optional<Tensor>& qw
                     const optional<Tensor>& kw, const optional<Tensor>& cos,
                     const optional<Tensor>& sin, const optional<Tensor>& pos, double eps,
                     bool interleaved) {
+  refuse_tangents(q, k, qw, kw, cos, sin);
   if (any_needs(q, k, qw, kw)) {
     auto out = QkFunction::apply(q, k, qw, kw, cos, sin, pos, eps, interleaved);
     return {out[0], out[1]};
@@ -433,6 +444,7 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
 
 Tensor6 route_autograd(const Tensor& logits, int64_t top, const optional<Tensor>& mask,
                        bool normalize) {
+  refuse_tangents(logits);
   if (any_needs(logits)) {
     auto o = RouteFunction::apply(logits, top, mask, normalize);
     return {o[0], o[1], o[2], o[3], o[4], o[5]};
@@ -464,6 +476,7 @@ struct LogpFunction : torch::autograd::Function<LogpFunction> {
 };
 
 Tensor2 logp_autograd(const Tensor& logits, const Tensor& tokens, double temperature, bool keep) {
+  refuse_tangents(logits);
   if (any_needs(logits)) {
     auto o = LogpFunction::apply(logits, tokens, temperature);
     return {o[0], o[1]};
@@ -526,6 +539,7 @@ Tensor4 policy_autograd(const Tensor& logits, const Tensor& tokens, const Tensor
                         const Tensor& advantages, const Tensor& weights, const optional<Tensor>& ref,
                         double clip_low, double clip_high, double kl_coef, double temperature,
                         bool keep, bool one_pass) {
+  refuse_tangents(logits, old, advantages, weights, ref);
   if (any_needs(logits)) {
     auto o = PolicyFunction::apply(logits, tokens, old, advantages, weights, ref, clip_low,
                                    clip_high, kl_coef, temperature);

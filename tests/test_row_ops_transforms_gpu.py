@@ -1,0 +1,66 @@
+"""The row operators under torch's transforms of a program: forward mode, torch.func, tracing by a
+dispatch mode, saved-tensor hooks, captured graphs with a backward pass, an outer compile; and
+gradients that meet what was left out. Tolerances are those of test_row_ops_gpu.py."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwad
+
+from muonium_amd.kernels import policy_loss, qk_norm_rope, route, token_logprobs
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- forward mode -------------------------------------------------------------------------
+
+
+def _forward_mode_calls():
+    """(name, a call on one input, that input): every floating input of every operator."""
+    q, k = torch.randn(2, 3, 4, 16, device="cuda"), torch.randn(2, 3, 2, 16, device="cuda")
+    w, cos = torch.ones(16, device="cuda"), torch.rand(9, 8, device="cuda")
+    z = torch.randn(6, 8, device="cuda")
+    tok, f = torch.zeros(6, dtype=torch.int64, device="cuda"), torch.rand(6, device="cuda")
+    return [
+        ("q", lambda t: qk_norm_rope(t, k, w, w, cos, cos)[0], q),
+        ("k", lambda t: qk_norm_rope(q, t, w, w, cos, cos)[1], k),
+        ("q_weight", lambda t: qk_norm_rope(q, k, t, w, cos, cos)[0], w),
+        ("k_weight", lambda t: qk_norm_rope(q, k, None, t, cos, cos)[1], w),
+        ("cos", lambda t: qk_norm_rope(q, k, w, w, t, cos)[0], cos),
+        ("sin", lambda t: qk_norm_rope(q, k, w, w, cos, t)[0], cos),
+        ("route", lambda t: route(t, 2).gates, z),
+        ("logprobs", lambda t: token_logprobs(t, tok), z),
+        ("policy", lambda t: policy_loss(t, tok, f, f, f).loss, z),
+        ("old", lambda t: policy_loss(z, tok, t, f, f).loss, f),
+        ("advantages", lambda t: policy_loss(z, tok, f, t, f).loss, f),
+        ("weights", lambda t: policy_loss(z, tok, f, f, t).loss, f),
+        ("ref", lambda t: policy_loss(z, tok, f, f, f, t, kl_coef=0.1).loss, f),
+    ]
+
+
+@pytest.mark.parametrize("case", range(13))
+def test_forward_mode_raises(case):
+    """There is no forward-mode derivative: a tangent on any input is refused, never dropped."""
+    name, call, x = _forward_mode_calls()[case]
+    tangent = torch.ones_like(x)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(call, (x,), (tangent,))
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jacfwd(call)(x)
+    with fwad.dual_level():
+        dual = fwad.make_dual(x, tangent)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(dual)
+        call(x)  # without a tangent, as ever
+    call(x)
+
+
+# ---- torch.func, tracing by a dispatch mode ----------------------------------------------------
+
+
+def test_reverse_transforms_of_torch_func_are_refused():
+    """torch has no torch.func transforms over C++ autograd functions: they raise."""
+    for _, call, x in _forward_mode_calls()[6:9]:
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: call(t).sum())(x)
