@@ -434,7 +434,8 @@ MUON_DEVICE void get_row(const float* row, int lane, float (&v)[VPT]) {
   }
 }
 
-// Slot lane + q G of a token is this lane's: the chosen expert and its gate's gradient.
+// Slot lane + q G of a token is this lane's: the chosen expert and its gate's gradient. An empty slot's
+// gate is the constant 0: what comes back for it, infinities too, is none of the token's.
 template <int G, int SLOTS>
 MUON_DEVICE void load_slots(const BackArgs& a, int64_t t, int lane, int (&at)[SLOTS], float (&up)[SLOTS]) {
 #pragma unroll
@@ -445,8 +446,10 @@ MUON_DEVICE void load_slots(const BackArgs& a, int64_t t, int lane, int (&at)[SL
     const int i = lane + q * G;
     if (!a.dgates || i >= a.k) continue;
     const int64_t e = a.experts[t * a.k + i];
-    up[q] = a.dgates[t * a.k + i];
-    at[q] = e >= 0 && e < a.E ? (int)e : -1;
+    const float g = a.dgates[t * a.k + i];
+    const bool held = e >= 0 && e < a.E;
+    up[q] = held ? g : 0.0f;
+    at[q] = held ? (int)e : -1;
   }
 }
 

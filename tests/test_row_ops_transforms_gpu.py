@@ -2,11 +2,15 @@
 dispatch mode, saved-tensor hooks, captured graphs with a backward pass, an outer compile; and
 gradients that meet what was left out. Tolerances are those of test_row_ops_gpu.py."""
 
+import math
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
 
 from muonium_amd.kernels import policy_loss, qk_norm_rope, route, token_logprobs
+from oracle import row_ops_ref as ref
+from test_row_ops_gpu import TYPES, check, gen, leaf
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +68,36 @@ def test_reverse_transforms_of_torch_func_are_refused():
     for _, call, x in _forward_mode_calls()[6:9]:
         with pytest.raises(RuntimeError):
             torch.func.grad(lambda t: call(t).sum())(x)
+
+
+# ---- routing: gradients of empty slots -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("normalize", [False, True])
+@pytest.mark.parametrize("experts", [5, 12, 200])
+def test_route_empty_slots_take_no_gradient(dtype, normalize, experts):
+    """The gradient of a gate that is 0 because its slot is empty, or its token masked, reaches
+    nothing, whatever it is: the entropy of the gates has a slope of infinity there."""
+    z = torch.randn(9, experts, generator=gen(1)).to(dtype)
+    z[0] = -math.inf
+    z[1, 2:] = -math.inf
+    z[2, 1:] = -math.inf
+    mask = torch.ones(9, dtype=torch.bool)
+    mask[5] = mask[6] = False
+    want = ref.route(z, 4, mask, normalize)
+    empty = want["experts"] < 0
+    assert empty.sum() == 4 + 2 + 3 + 8
+    dg = torch.randn(9, 4, generator=gen(2))
+    scale = 256.0 if dtype == torch.float16 else 1.0
+    d, sd = ref.route_grad(want, dg * scale, torch.tensor(scale), torch.tensor(scale))
+    one = torch.tensor(scale, device="cuda")
+    for bad in (math.inf, -math.inf, math.nan):
+        x = leaf(z)
+        got = route(x, 4, token_mask=mask.cuda(), normalize=normalize)
+        up = torch.where(empty, bad, dg * scale).cuda()
+        dz, = torch.autograd.grad((got.gates, got.balance_loss, got.z_loss), (x,), (up, one, one))
+        check(dz, d, sd, 320, dtype, bad)
+    x = leaf(z)
+    torch.special.entr(route(x, 4, token_mask=mask.cuda(), normalize=normalize).gates).sum().backward()
+    assert x.grad.isfinite().all()
