@@ -19,11 +19,9 @@
 // double, gradients are rounded once at the store.
 #include <algorithm>
 
-#include "rowops.h"
+#include "logits.h"
 
 namespace {
-
-constexpr double LOG2E_D = 1.4426950408889634074;
 
 struct Rows {
   const void* x;
@@ -111,28 +109,6 @@ MUON_DEVICE Sum block_join(Sum v, float k, Sum* lds) {
   if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
   __syncthreads();
   return first_lane(group_reduce<NT / 64>(lds[threadIdx.x % (NT / 64)], op));
-}
-
-// Values [i0, i0 + N) of a row that ends at V; -inf behind it.
-template <int DT>
-MUON_DEVICE muon_u4 load_tail(const void* x, int64_t at, int64_t i0, int64_t V) {
-  constexpr int N = Vec16<DT>::N;
-  float v[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) v[e] = i0 + e < V ? Elem<DT>::load(x, at + i0 + e) : -INFINITY;
-  return Vec16<DT>::pack(v);
-}
-template <int DT>
-MUON_DEVICE void store_tail(void* x, int64_t at, int64_t i0, int64_t V, const float* v) {
-#pragma unroll
-  for (int e = 0; e < Vec16<DT>::N; ++e)
-    if (i0 + e < V) Elem<DT>::store(x, at + i0 + e, v[e]);
-}
-
-template <bool STREAM>
-MUON_DEVICE void put(void* p, muon_u4 w) {
-  if constexpr (STREAM) store_u4_nt(p, w);
-  else store_u4(p, w);
 }
 
 // log s for s in 1..2^31 (s is 0, infinite or NaN where a row has no sum), to 2^-24 of one: the
@@ -260,78 +236,6 @@ __global__ __launch_bounds__(256) void logp_join_kernel(Rows a, Policy p, const 
   if (lane == 0) finish_row(a, p, row, in, t);
 }
 
-struct Back {
-  const void* x;
-  int64_t stride, N, V;
-  const int64_t* tokens;
-  const float* stats;
-  const float* coef;   // per row: the gradient of logp
-  const float* scale;  // one value, or null
-  float k, tau_inv;
-  void* dx;  // contiguous
-  int last_first;  // rows from the last to the first
-};
-
-// dx of one run of values of a row; tok is the token's place in it, if it is there at all.
-template <int DT>
-MUON_DEVICE void slopes(const float (&x)[Vec16<DT>::N], float m, float k, float pc, float g,
-                        int64_t tok, float (&d)[Vec16<DT>::N]) {
-  constexpr int N = Vec16<DT>::N;
-#pragma unroll
-  for (int e = 0; e < N; ++e) d[e] = -pc * __builtin_amdgcn_exp2f((x[e] - m) * k);
-  if ((uint64_t)tok < (uint64_t)N) {  // one run of the row
-#pragma unroll
-    for (int e = 0; e < N; ++e) d[e] += tok == e ? g : 0.0f;
-  }
-}
-
-constexpr int BACK_THREADS = 256;
-constexpr int BACK_VECS = 4;  // 16-byte pieces per thread
-
-// The gradient from the logits again and the kept m and 1 / s. Grid: pieces of a row x rows.
-template <int DT, bool STREAM>
-__global__ __launch_bounds__(BACK_THREADS) void logp_backward_kernel(Back a) {
-  constexpr int N = Vec16<DT>::N;
-  const float scale = a.scale ? a.scale[0] : 1.0f;
-  for (int64_t y = blockIdx.y; y < a.N; y += gridDim.y) {
-    const int64_t row = a.last_first ? a.N - 1 - y : y;
-    const int64_t tok = a.tokens[row];
-    const float g = tok < 0 ? 0.0f : a.coef[row] * scale * a.tau_inv;
-    const int64_t at = row * a.stride, to = row * a.V;
-    const int64_t i0 = ((int64_t)blockIdx.x * BACK_VECS * BACK_THREADS + threadIdx.x) * N;
-    if (g == 0.0f) {
-#pragma unroll
-      for (int u = 0; u < BACK_VECS; ++u) {
-        const int64_t i = i0 + (int64_t)u * BACK_THREADS * N;
-        if (i + N <= a.V) put<STREAM>((void*)elem_at<DT>(a.dx, to + i), muon_u4{0, 0, 0, 0});
-        else if (i < a.V) {
-          const float z[N] = {};
-          store_tail<DT>(a.dx, to, i, a.V, z);
-        }
-      }
-      continue;
-    }
-    const float m = a.stats[row], pc = g * a.stats[a.N + row];
-    muon_u4 w[BACK_VECS];
-#pragma unroll
-    for (int u = 0; u < BACK_VECS; ++u) {
-      const int64_t i = i0 + (int64_t)u * BACK_THREADS * N;
-      if (i + N <= a.V) w[u] = load_u4(elem_at<DT>(a.x, at + i));
-      else if (i < a.V) w[u] = load_tail<DT>(a.x, at, i, a.V);
-    }
-#pragma unroll
-    for (int u = 0; u < BACK_VECS; ++u) {
-      const int64_t i = i0 + (int64_t)u * BACK_THREADS * N;
-      if (i >= a.V) break;
-      float x[N], d[N];
-      Vec16<DT>::unpack(w[u], x);
-      slopes<DT>(x, m, a.k, pc, g, tok - i, d);
-      if (i + N <= a.V) put<STREAM>((void*)elem_at<DT>(a.dx, to + i), Vec16<DT>::pack(d));
-      else store_tail<DT>(a.dx, to, i, a.V, d);
-    }
-  }
-}
-
 // The policy loss with its gradient in one pass over the logits: a workgroup holds its whole row
 // in registers (NV 16-byte pieces a thread; the 512 KB of a CU hold 163840 bf16 values beside
 // the working registers), sums it, makes the slope g, and writes the gradient from the same
@@ -450,49 +354,6 @@ __global__ __launch_bounds__(256) void scale_kernel(void* x, int64_t n, const fl
   for (int64_t i = vecs * N + id; i < n; i += step) Elem<DT>::store(x, i, Elem<DT>::load(x, i) * g);
 }
 
-bool io_ok(int dt) { return dt == MUON_DT_F32 || dt == MUON_DT_BF16 || dt == MUON_DT_F16; }
-
-int check(const char* what, int dtype, int64_t N, int64_t V, int64_t stride, float tau) {
-  if (!io_ok(dtype)) {
-    muon_set_error("%s: unsupported dtype %d", what, dtype);
-    return MUON_ERR_DTYPE;
-  }
-  if (N < 0 || N >= (1LL << 31) || V < 1 || V >= (1LL << 31) || stride < 0) {
-    muon_set_error("%s: bad extents (rows %lld, vocabulary %lld, row stride %lld)", what,
-                   (long long)N, (long long)V, (long long)stride);
-    return MUON_ERR_SHAPE;
-  }
-  // 1 / tau and log2(e) / tau stay in fp32's range
-  if (!(tau >= 1e-30f && tau <= 1e30f)) {
-    muon_set_error("%s: temperature %g is not within 1e-30 and 1e30", what, (double)tau);
-    return MUON_ERR_ARG;
-  }
-  return MUON_OK;
-}
-
-constexpr int64_t MAX_GRID_Y = 65535;
-// Gradients of this many bytes are stored past the caches (half of the 256 MB last-level one).
-// The gradient of 4096 rows of 128000 bf16 values 406 -> 381 us, of 2047 rows of 50257 73 -> 63.
-constexpr int64_t STREAM_FROM = 128 << 20;
-
-// The backward pass follows the forward pass that read the same logits. Where they are more than
-// the last-level cache holds, what is left of them there are the last rows, and it begins with
-// those: forward and backward of 4096 rows of 128000 bf16 logits 559 -> 547 us, of 4096 x 64000 in
-// fp16 288 -> 272; logits that fit go from first to last (2047 rows of 50257: 109 us, the other
-// way 111).
-constexpr int64_t CACHE_BYTES = 256 << 20;
-
-template <int DT>
-void launch_backward(Back a, hipStream_t s) {
-  a.last_first = a.N * a.V * (DT == MUON_DT_F32 ? 4 : 2) > CACHE_BYTES;
-  const int64_t per = (int64_t)BACK_THREADS * BACK_VECS * Vec16<DT>::N;
-  const dim3 grid((unsigned)((a.V + per - 1) / per), (unsigned)std::min(a.N, MAX_GRID_Y));
-  if (a.N * a.V * (DT == MUON_DT_F32 ? 4 : 2) >= STREAM_FROM)
-    logp_backward_kernel<DT, true><<<grid, BACK_THREADS, 0, s>>>(a);
-  else
-    logp_backward_kernel<DT, false><<<grid, BACK_THREADS, 0, s>>>(a);
-}
-
 // Slices of a row. One workgroup a row as a rule: joining slices takes a second launch. Longer
 // rows than SPLIT_FROM, of which fewer than 128 come together, are cut until there are four
 // workgroups per CU. One row, whole and cut (us a call): 32000 values 6.1 and 10.0, 128000 9.0 and
@@ -604,12 +465,7 @@ int muon_token_logprobs_backward(const void* logits, int dtype, int64_t row_stri
   const double inv = 1.0 / (double)temperature;
   const Back a = {logits, row_stride, rows, vocab, tokens, stats, dlogprobs, scale,
                   (float)(LOG2E_D * inv), (float)inv, dlogits, 0};
-  hipStream_t s = (hipStream_t)stream;
-  if (dtype == MUON_DT_F32) launch_backward<MUON_DT_F32>(a, s);
-  else if (dtype == MUON_DT_BF16) launch_backward<MUON_DT_BF16>(a, s);
-  else launch_backward<MUON_DT_F16>(a, s);
-  MUON_CHECK_LAUNCH("token_logprobs_backward");
-  return MUON_OK;
+  return launch_backward<false>("token_logprobs_backward", a, dtype, (hipStream_t)stream);
 }
 
 int muon_policy_loss_one_pass(int dtype, int64_t vocab) {

@@ -323,6 +323,27 @@ Tensor policy_backward(const Tensor& dloss, const Tensor& logits, const Tensor& 
                        ptr<float>(kept) + 2 * n, temperature);
 }
 
+// dlogits, as policy_forward's one pass made it of these logits, for a loss gradient of dloss.
+void policy_rescale(const Tensor& dlogits, const Tensor& dloss, const Tensor& logits_,
+                    const Tensor& tokens_, const Tensor& rows, double temperature) {
+  const at::DeviceGuard guard(logits_.device());
+  const Tensor logits = rows_of(logits_);
+  const int64_t n = logits.size(0);
+  TORCH_CHECK(dlogits.sizes() == logits.sizes() && dlogits.is_contiguous() &&
+                  dlogits.scalar_type() == logits.scalar_type() &&
+                  dlogits.device() == logits.device(),
+              "muonium_amd: the gradient is not like its logits");
+  const Tensor tokens = plain(tokens_, logits, at::kLong, n, "the tokens");
+  const Tensor kept = plain(rows, logits, at::kFloat, 4 * n, "the rows' values");
+  const Tensor scale = plain(dloss, logits, at::kFloat, 1, "the loss's gradient");
+  const float* r = ptr<float>(kept);
+  check(muon_policy_loss_rescale(ptr(logits), dtype_code(logits), logits.stride(0), n,
+                                 logits.size(1), ptr<int64_t>(tokens), (float)temperature,
+                                 r + 2 * n, r + n, ptr<float>(scale), ptr(dlogits),
+                                 stream_of(logits)),
+        "muon_policy_loss_rescale");
+}
+
 // ---- gradients --------------------------------------------------------------------------
 
 
@@ -521,11 +542,8 @@ struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
         // the same graph makes its own from the logits.
         none[0] = made->second.toTensor();
         ctx->saved_data.erase(made);
-        const at::DeviceGuard guard(none[0].device());
-        const Tensor scale = plain(grads[0], none[0], at::kFloat, 1, "the loss's gradient");
-        check(muon_scale_gradient(ptr(none[0]), dtype_code(none[0]), none[0].numel(),
-                                  ptr<float>(scale), stream_of(none[0])),
-              "muon_scale_gradient");
+        policy_rescale(none[0], grads[0], s[0], s[1], s[2],
+                       ctx->saved_data["temperature"].toDouble());
       } else {
         none[0] = OP("policy_loss_backward", policy_backward)
                       .call(grads[0], s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble());

@@ -138,6 +138,9 @@ _SIGNATURES = {
         [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_f32, _c_f32, _c_f32,
          _c_f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     ),
+    "muon_policy_loss_rescale": (
+        _c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_f32, _vp, _vp, _vp, _vp, _vp]
+    ),
     "muon_scale_gradient": (_c_int, [_vp, _c_int, _c_i64, _vp, _vp]),
 }
 

@@ -89,9 +89,9 @@ def policy_loss(
 
     Differentiable in the logits alone. In bf16 and fp32, for rows that fit a workgroup's registers
     (163840 and 81920 values), the gradient is made in the forward pass, from one reading of the
-    logits, for a loss gradient of 1, and the backward pass only multiplies it where that gradient
-    is another number (one more rounding in bf16, none for a power of two). fp16, whose
-    unscaled gradient would underflow, and longer rows read the logits again in the backward pass."""
+    logits, for a loss gradient of 1; for any other one the backward pass makes it again from
+    the logits, so that each value is rounded once. fp16, whose unscaled gradient would underflow,
+    and longer rows read the logits again in the backward pass."""
     _check(logits, tokens, temperature)
     _check_on(logits.device, old_logprobs, advantages, weights, ref_logprobs)
     shape = tokens.shape

@@ -323,8 +323,11 @@ int muon_token_logprobs_backward(const void* logits, int dtype, int64_t row_stri
  * one float a row. The gradient either in the same pass (dlogits, for a loss gradient of 1; where
  * muon_policy_loss_one_pass says the row fits a workgroup's registers), or later by
  * muon_token_logprobs_backward with dlogprobs = coef and the kept stats (both may be NULL
- * when not needed). muon_scale_gradient multiplies n values by *scale in place (a scale of 1
- * touches nothing). */
+ * when not needed). muon_policy_loss_rescale takes the dlogits of the same pass, with the coef
+ * and stats that it kept, to the loss gradient *scale: it makes the rows that have a gradient again
+ * from the logits, each value rounded once (a scale of 1 touches nothing).
+ * muon_scale_gradient multiplies any n values by *scale in place, the rounded ones (a
+ * scale of 1 touches nothing). */
 int muon_policy_loss_one_pass(int dtype, int64_t vocab);
 int muon_policy_loss(const void* logits, int dtype, int64_t row_stride, int64_t rows,
                      int64_t vocab, const int64_t* tokens, const float* old_logprobs,
@@ -332,6 +335,10 @@ int muon_policy_loss(const void* logits, int dtype, int64_t row_stride, int64_t 
                      float clip_low, float clip_high, float kl_coef, float temperature,
                      float* loss, float* logprobs, float* terms, float* stats, float* coef,
                      void* dlogits, void* ws, void* stream);
+int muon_policy_loss_rescale(const void* logits, int dtype, int64_t row_stride, int64_t rows,
+                             int64_t vocab, const int64_t* tokens, float temperature,
+                             const float* stats, const float* coef, const float* scale,
+                             void* dlogits, void* stream);
 int muon_scale_gradient(void* x, int dtype, int64_t n, const float* scale, void* stream);
 
 /* ---- Kernel timing (measurement support) ------------------------------------------

@@ -1,0 +1,47 @@
+"""The row operators' libraries without a device: what their entry points refuse before a launch, and
+what their kernels keep in registers."""
+
+import os
+import re
+import subprocess
+
+import pytest
+
+from muonium_amd import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HIPCC = "/opt/rocm/bin/hipcc"
+
+
+@pytest.mark.parametrize("call, code", [
+    (lambda L: L.muon_policy_loss_rescale(1, 7, 4, 3, 4, 1, 1.0, 1, 1, 1, 1, None), 2),
+    (lambda L: L.muon_policy_loss_rescale(1, 1, 4, 3, 0, 1, 1.0, 1, 1, 1, 1, None), 1),
+    (lambda L: L.muon_policy_loss_rescale(1, 1, 4, 3, 4, 1, 0.0, 1, 1, 1, 1, None), 5),
+    (lambda L: L.muon_policy_loss_rescale(1, 2, 4, 3, 4, 1, 1.0, 1, 1, 1, 1, None), 5),
+    (lambda L: L.muon_policy_loss_rescale(1, 0, 1 << 17, 3, 1 << 17, 1, 1.0, 1, 1, 1, 1, None), 5),
+    (lambda L: L.muon_policy_loss_rescale(1, 1, 4, 3, 4, 1, 1.0, None, 1, 1, 1, None), 5),
+    (lambda L: L.muon_policy_loss_rescale(1, 1, 4, 3, 4, 1, 1.0, 1, None, 1, 1, None), 5),
+    (lambda L: L.muon_policy_loss_rescale(1, 1, 4, 3, 4, 1, 1.0, 1, 1, None, 1, None), 5),
+    (lambda L: L.muon_policy_loss_rescale(1, 1, 4, 3, 4, 1, 1.0, 1, 1, 1, None, None), 5),
+])
+def test_rescale_refuses_without_launching(call, code):
+    assert call(_lib.load()) == code
+    assert "policy_loss_rescale" in _lib.last_error()
+
+
+def test_rescale_of_no_rows_returns_ok():
+    assert _lib.load().muon_policy_loss_rescale(None, 1, 4, 0, 4, None, 1.0, None, None, None, None, None) == 0
+
+
+@pytest.mark.skipif(not os.path.exists(HIPCC), reason="needs hipcc")
+def test_rescale_kernels_use_no_scratch(tmp_path):
+    asm = tmp_path / "kernels.s"
+    cmd = [HIPCC, "-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-w", "-mllvm",
+           "-pragma-unroll-threshold=1000000", "-Xclang", "-target-feature", "-Xclang",
+           "-packed-fp32-ops", "-I" + os.path.join(ROOT, "include"), "--cuda-device-only", "-S",
+           os.path.join(ROOT, "dtensor-muon_amd", "csrc", "rescale.hip"), "-o", str(asm)]
+    subprocess.run(cmd, check=True, capture_output=True, timeout=900)
+    text = asm.read_text()
+    found = re.findall(r"\.private_segment_fixed_size:\s+(\d+).*?\.vgpr_spill_count:\s+(\d+)", text, re.S)
+    assert len(found) == 4 and all(f == ("0", "0") for f in found)
+    assert not re.search(r"v_pk_(add|mul|fma)_f32", text)

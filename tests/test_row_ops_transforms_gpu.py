@@ -10,7 +10,7 @@ import torch.autograd.forward_ad as fwad
 
 from muonium_amd.kernels import policy_loss, qk_norm_rope, route, token_logprobs
 from oracle import row_ops_ref as ref
-from test_row_ops_gpu import TYPES, check, gen, leaf
+from test_row_ops_gpu import TYPES, check, gen, leaf, policy_case
 
 pytestmark = pytest.mark.gpu
 
@@ -68,6 +68,29 @@ def test_reverse_transforms_of_torch_func_are_refused():
     for _, call, x in _forward_mode_calls()[6:9]:
         with pytest.raises(RuntimeError):
             torch.func.grad(lambda t: call(t).sum())(x)
+
+
+# ---- the policy gradient under any loss gradient ------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [70, 1500, 50257])
+def test_policy_gradient_is_rounded_once(dtype, v):
+    """One rounding whatever the loss gradient, and however many backward passes a graph serves."""
+    x, tokens, old, adv, w, r, logp, p = policy_case(6, v, dtype, 3, True, 0.7)
+    args = [t.cuda() for t in (tokens, old, adv, w, r)]
+    _, slope, _, sizes = ref.policy(logp, old, adv, w, r, 0.2, 0.2, 0.1)
+    want, ds = ref.logprobs_grad(p, tokens, slope, 0.7)
+    _, room = ref.logprobs_grad(p, tokens, sizes, 0.7)
+    xl = leaf(x)
+    lift = 1024.0 if dtype == torch.float16 else 1.0
+    for scales in ((1 / 3,), (3.0, 0.7), (1.0, 0.1), (0.0, 1.3), (-2.6, 1.0)):
+        out = policy_loss(xl, *args, kl_coef=0.1, temperature=0.7)
+        for scale in scales:
+            s = torch.tensor(scale * lift, device="cuda")
+            d, = torch.autograd.grad((out.loss,), (xl,), (s,), retain_graph=True)
+            # the slope's product with the loss gradient is one more rounding in fp32
+            check(d, want * s.item(), (ds + 2 * room) * abs(s.item()), 257, dtype, scale)
 
 
 # ---- routing: gradients of empty slots -----------------------------------------------------------
