@@ -10,6 +10,7 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -372,6 +373,12 @@ void refuse_tangents(const T&... t) {
                               "muonium_amd's row operators have no forward-mode derivative");
 }
 
+// Whether somebody records or replaces the operators that run: a tracer or a checkpoint that keeps
+// results, by a dispatch mode (over plain tensors too), or a tensor subclass. What it sees has to be
+// all that happens.
+bool watched() { return c10::impl::TorchDispatchModeTLS::any_modes_set(); }
+bool watched(const Tensor& t) { return watched() || t.key_set().has(c10::DispatchKey::Python); }
+
 Tensor or_undefined(const optional<Tensor>& t) { return t ? *t : Tensor(); }
 optional<Tensor> or_none(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
 
@@ -512,10 +519,9 @@ struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
                                const optional<Tensor>& ref, double clip_low, double clip_high,
                                double kl_coef, double temperature) {
     at::AutoDispatchBelowADInplaceOrView below;
-    // A tensor subclass (a tracer's fake tensor) takes the form whose gradient is an operation
-    // of its own on what is saved.
-    const bool one_pass = !logits.key_set().has(c10::DispatchKey::Python) &&
-                          muon_policy_loss_one_pass(dtype_code(logits), logits.size(1));
+    // who watches sees the form whose gradient is an operation of its own on what is saved
+    const bool one_pass =
+        !watched(logits) && muon_policy_loss_one_pass(dtype_code(logits), logits.size(1));
     auto [loss, logp, rows, dlogits] =
         OP("policy_loss", policy_forward)
             .call(logits, tokens, old, advantages, weights, ref, clip_low, clip_high, kl_coef,
@@ -537,13 +543,13 @@ struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       auto made = ctx->saved_data.find("dlogits");
-      if (made != ctx->saved_data.end()) {
+      if (made != ctx->saved_data.end() && !watched()) {
         // The gradient of the forward pass is handed over once; a second backward pass through
-        // the same graph makes its own from the logits.
+        // the same graph makes its own from the logits, as does a recorded one, which may run again.
         none[0] = made->second.toTensor();
         ctx->saved_data.erase(made);
-        policy_rescale(none[0], grads[0], s[0], s[1], s[2],
-                       ctx->saved_data["temperature"].toDouble());
+        OP("policy_loss_rescale_", policy_rescale)
+            .call(none[0], grads[0], s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble());
       } else {
         none[0] = OP("policy_loss_backward", policy_backward)
                       .call(grads[0], s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble());
@@ -590,6 +596,8 @@ TORCH_LIBRARY_FRAGMENT(muonium_amd, m) {
         "float temperature, bool keep, bool one_pass) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("policy_loss_backward(Tensor dloss, Tensor logits, Tensor tokens, Tensor rows, "
         "float temperature) -> Tensor");
+  m.def("policy_loss_rescale_(Tensor(a!) dlogits, Tensor dloss, Tensor logits, Tensor tokens, "
+        "Tensor rows, float temperature) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(muonium_amd, CUDA, m) {
@@ -601,6 +609,7 @@ TORCH_LIBRARY_IMPL(muonium_amd, CUDA, m) {
   m.impl("token_logprobs_backward", logp_backward);
   m.impl("policy_loss", policy_forward);
   m.impl("policy_loss_backward", policy_backward);
+  m.impl("policy_loss_rescale_", policy_rescale);
 }
 
 TORCH_LIBRARY_IMPL(muonium_amd, AutogradCUDA, m) {

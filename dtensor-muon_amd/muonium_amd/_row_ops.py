@@ -111,3 +111,8 @@ def _(logits, tokens, old, advantages, weights, ref, clip_low, clip_high, kl_coe
 @_fake("policy_loss_backward")
 def _(dloss, logits, tokens, rows, temperature):
     return _like(logits)
+
+
+@_fake("policy_loss_rescale_")
+def _(dlogits, dloss, logits, tokens, rows, temperature):
+    return None

@@ -7,12 +7,19 @@ import math
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from muonium_amd.kernels import policy_loss, qk_norm_rope, route, token_logprobs
 from oracle import row_ops_ref as ref
 from test_row_ops_gpu import TYPES, check, gen, leaf, policy_case
 
 pytestmark = pytest.mark.gpu
+
+
+def policy_args(n, v, dtype, seed=3):
+    """Logits on the device and the other arguments of a policy loss with a reference."""
+    x, tokens, old, adv, w, r, _, _ = policy_case(n, v, dtype, seed, True, 1.0)
+    return x.cuda(), [t.cuda() for t in (tokens, old, adv, w, r)]
 
 
 # ---- forward mode -------------------------------------------------------------------------
@@ -68,6 +75,50 @@ def test_reverse_transforms_of_torch_func_are_refused():
     for _, call, x in _forward_mode_calls()[6:9]:
         with pytest.raises(RuntimeError):
             torch.func.grad(lambda t: call(t).sum())(x)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_traced_policy_gradient_keeps_its_scale(dtype):
+    """A trace over plain tensors, by a dispatch mode, computes what eager does, whatever the loss
+    gradient, also on other inputs than those it was recorded with; as does a trace of the
+    backward pass alone."""
+    x, args = policy_args(6, 500, dtype)
+
+    def grad_of(t):
+        t = t.detach().requires_grad_()
+        return torch.autograd.grad((3 * policy_loss(t, *args, kl_coef=0.1).loss,), (t,))[0]
+
+    graph = make_fx(grad_of)(x)
+    for t in (x, x.flip(1).contiguous(), x):
+        torch.testing.assert_close(graph(t), grad_of(t), rtol=2.0**-7, atol=1e-6)
+    a = x.clone().requires_grad_()
+    loss = policy_loss(a, *args, kl_coef=0.1).loss
+
+    def back(g):
+        return torch.autograd.grad((loss,), (a,), (g,), retain_graph=True)[0]
+
+    graph = make_fx(back)(torch.tensor(3.0, device="cuda"))
+    for scale in (3.0, 1.0, 0.5, 3.0):
+        got = graph(torch.tensor(scale, device="cuda"))
+        torch.testing.assert_close(got, grad_of(x) * (scale / 3), rtol=2.0**-6, atol=1e-6)
+
+
+def test_rescale_is_a_well_behaved_torch_operator():
+    """It says what it changes, and does so in eager and traced programs."""
+    ops = torch.ops.muonium_amd
+    x, args = policy_args(6, 300, torch.bfloat16)
+    _, _, rows, d = ops.policy_loss(x, *args, 0.2, 0.2, 0.1, 1.0, True, True)
+    scale = torch.tensor(3.0, device="cuda")
+    torch.library.opcheck(ops.policy_loss_rescale_.default, (d.clone(), scale, x, args[0], rows, 1.0))
+    want = ops.policy_loss_backward(scale, x, args[0], rows, 1.0)
+    got = d.clone()
+    ops.policy_loss_rescale_(got, scale, x, args[0], rows, 1.0)
+    assert torch.equal(got, want) and not torch.equal(got, d)
+    ops.policy_loss_rescale_(d, torch.ones((), device="cuda"), x, args[0], rows, 1.0)
+    assert torch.equal(d, ops.policy_loss_backward(scale / 3, x, args[0], rows, 1.0))
+    for bad in (d[:5], d.float(), d.t().contiguous().t(), d.cpu()):
+        with pytest.raises((RuntimeError, TypeError)):
+            ops.policy_loss_rescale_(bad, scale, x, args[0], rows, 1.0)
 
 
 # ---- the policy gradient under any loss gradient ------------------------------------------------
