@@ -483,11 +483,12 @@ Tensor6 route_autograd(const Tensor& logits, int64_t top, const optional<Tensor>
 
 struct LogpFunction : torch::autograd::Function<LogpFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens,
-                               double temperature) {
+                               double temperature, bool keep) {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [logp, stats] = OP("token_logprobs", logp_forward).call(logits, tokens, temperature, true);
     ctx->save_for_backward({logits, tokens, stats});
     ctx->saved_data["temperature"] = temperature;
+    if (!keep) stats = empty(logits, {0}, at::kFloat);  // kept for the backward pass alone
     ctx->mark_non_differentiable({stats});
     return {logp, stats};
   }
@@ -499,14 +500,14 @@ struct LogpFunction : torch::autograd::Function<LogpFunction> {
       d = OP("token_logprobs_backward", logp_backward)
               .call(grads[0], s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble());
     }
-    return once({d, Tensor(), Tensor()}, {s[0], grads[0]});
+    return once({d, Tensor(), Tensor(), Tensor()}, {s[0], grads[0]});
   }
 };
 
 Tensor2 logp_autograd(const Tensor& logits, const Tensor& tokens, double temperature, bool keep) {
   refuse_tangents(logits);
   if (any_needs(logits)) {
-    auto o = LogpFunction::apply(logits, tokens, temperature);
+    auto o = LogpFunction::apply(logits, tokens, temperature, keep);
     return {o[0], o[1]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
@@ -517,27 +518,29 @@ struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens,
                                const Tensor& old, const Tensor& advantages, const Tensor& weights,
                                const optional<Tensor>& ref, double clip_low, double clip_high,
-                               double kl_coef, double temperature) {
+                               double kl_coef, double temperature, bool keep, bool one_pass) {
     at::AutoDispatchBelowADInplaceOrView below;
-    // who watches sees the form whose gradient is an operation of its own on what is saved
-    const bool one_pass =
-        !watched(logits) && muon_policy_loss_one_pass(dtype_code(logits), logits.size(1));
+    // A gradient made here is the caller's (one_pass), or kept for the backward pass alone. Who
+    // watches sees the form whose gradient is an operation of its own on what is saved.
+    const bool ours = !one_pass && !watched(logits) &&
+                      muon_policy_loss_one_pass(dtype_code(logits), logits.size(1));
     auto [loss, logp, rows, dlogits] =
         OP("policy_loss", policy_forward)
             .call(logits, tokens, old, advantages, weights, ref, clip_low, clip_high, kl_coef,
-                  temperature, true, one_pass);
+                  temperature, true, one_pass || ours);
     ctx->save_for_backward({logits, tokens, rows});
     ctx->saved_data["temperature"] = temperature;
-    if (one_pass) {  // kept for the backward pass alone
+    if (ours) {
       ctx->saved_data["dlogits"] = dlogits;
       dlogits = empty(logits, {0}, logits.scalar_type());
     }
+    if (!keep) rows = rows.narrow(0, 0, 1);
     ctx->mark_non_differentiable({logp, rows, dlogits});
     ctx->set_materialize_grads(false);
     return {loss, logp, rows, dlogits};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    variable_list none(10);
+    variable_list none(12);
     if (!grads[0].defined()) return none;
     const auto s = ctx->get_saved_variables();
     {
@@ -566,7 +569,7 @@ Tensor4 policy_autograd(const Tensor& logits, const Tensor& tokens, const Tensor
   refuse_tangents(logits, old, advantages, weights, ref);
   if (any_needs(logits)) {
     auto o = PolicyFunction::apply(logits, tokens, old, advantages, weights, ref, clip_low,
-                                   clip_high, kl_coef, temperature);
+                                   clip_high, kl_coef, temperature, keep, one_pass);
     return {o[0], o[1], o[2], o[3]};
   }
   at::AutoDispatchBelowADInplaceOrView below;

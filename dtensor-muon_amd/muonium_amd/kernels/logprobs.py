@@ -42,6 +42,11 @@ def _flat(t: Tensor) -> Tensor:
     return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
 
+def _keeps(logits: Tensor) -> bool:
+    """Whether a backward pass may ask for what the forward pass knows of each row."""
+    return logits.requires_grad and torch.is_grad_enabled()
+
+
 def token_logprobs(logits: Tensor, tokens: Tensor, *, temperature: float = 1.0) -> Tensor:
     """``log softmax(logits / temperature)`` at each position's token, in fp32.
 
@@ -55,7 +60,7 @@ def token_logprobs(logits: Tensor, tokens: Tensor, *, temperature: float = 1.0) 
     whose incoming gradient is 0 get zeros, whatever their logits hold."""
     _check(logits, tokens, temperature)
     _row_ops.check_device(logits.device)
-    out = _row_ops.token_logprobs(_rows(logits), _flat(tokens), temperature, False)[0]
+    out = _row_ops.token_logprobs(_rows(logits), _flat(tokens), temperature, _keeps(logits))[0]
     return out if logits.dim() == 2 else out.view(tokens.shape)
 
 
@@ -112,5 +117,5 @@ def policy_loss(
     loss, logp, _, _ = _row_ops.policy_loss(
         _rows(logits), _flat(tokens), _flat(old_logprobs), _flat(advantages), _flat(weights),
         None if ref_logprobs is None else _flat(ref_logprobs), clip_low, clip_high, kl_coef,
-        temperature, False, False)
+        temperature, _keeps(logits), False)
     return PolicyLoss(loss, logp if logits.dim() == 2 else logp.view(tokens.shape))

@@ -121,6 +121,46 @@ def test_rescale_is_a_well_behaved_torch_operator():
             ops.policy_loss_rescale_(bad, scale, x, args[0], rows, 1.0)
 
 
+# ---- the registered operators keep their schemas -------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_registered_results_are_what_was_asked_for(dtype):
+    """keep and one_pass decide the shapes with and without a gradient, and a gradient that was asked
+    for as a result stays as it is when the backward pass runs."""
+    ops = torch.ops.muonium_amd
+    x, args = policy_args(6, 300, dtype)
+    rest = (0.2, 0.2, 0.1, 1.0)
+    for keep in (False, True):
+        for one_pass in (False, True):
+            a = x.clone().requires_grad_()
+            loss, logp, rows, d = ops.policy_loss(a, *args, *rest, keep, one_pass)
+            plain = ops.policy_loss(x, *args, *rest, keep, one_pass)
+            assert rows.shape == plain[2].shape == (4 if keep else 1, 6)
+            assert d.shape == plain[3].shape == (x.shape if one_pass else (0,))
+            held = d.clone()
+            g, = torch.autograd.grad((loss,), (a,), (torch.tensor(3.0, device="cuda"),))
+            assert torch.equal(d, held) and torch.equal(d, plain[3])
+            one, = torch.autograd.grad((ops.policy_loss(a, *args, *rest, True, False)[0],), (a,))
+            torch.testing.assert_close(g, 3 * one, rtol=2.0**-6, atol=1e-6)
+            if one_pass:
+                torch.testing.assert_close(d, one, rtol=2.0**-7, atol=1e-6)
+        b = x.clone().requires_grad_()
+        for t in (x, b):
+            assert ops.token_logprobs(t, args[0], 1.0, keep)[1].shape == (12 if keep else 0,)
+
+
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("one_pass", [False, True])
+def test_policy_operators_are_well_behaved_torch_operators(keep, one_pass):
+    ops = torch.ops.muonium_amd
+    z = leaf(torch.randn(20, 16))
+    tokens, f = torch.randint(0, 16, (20,), device="cuda"), torch.rand(20, device="cuda")
+    args = (z, tokens, f, f, f, None, 0.2, 0.2, 0.1, 1.0)
+    torch.library.opcheck(ops.policy_loss.default, (*args, keep, one_pass))
+    torch.library.opcheck(ops.token_logprobs.default, (z, tokens, 1.0, keep))
+
+
 # ---- the policy gradient under any loss gradient ------------------------------------------------
 
 
