@@ -528,12 +528,11 @@ struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
         OP("policy_loss", policy_forward)
             .call(logits, tokens, old, advantages, weights, ref, clip_low, clip_high, kl_coef,
                   temperature, true, one_pass || ours);
-    ctx->save_for_backward({logits, tokens, rows});
+    // the gradient too is a saved tensor: hooks move or drop it like the logits
+    ctx->save_for_backward({logits, tokens, rows, ours ? dlogits : Tensor()});
     ctx->saved_data["temperature"] = temperature;
-    if (ours) {
-      ctx->saved_data["dlogits"] = dlogits;
-      dlogits = empty(logits, {0}, logits.scalar_type());
-    }
+    ctx->saved_data["made"] = ours;
+    if (ours) dlogits = empty(logits, {0}, logits.scalar_type());
     if (!keep) rows = rows.narrow(0, 0, 1);
     ctx->mark_non_differentiable({logp, rows, dlogits});
     ctx->set_materialize_grads(false);
@@ -545,12 +544,13 @@ struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
     const auto s = ctx->get_saved_variables();
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      auto made = ctx->saved_data.find("dlogits");
-      if (made != ctx->saved_data.end() && !watched()) {
+      if (ctx->saved_data["made"].toBool() && !watched()) {
         // The gradient of the forward pass is handed over once; a second backward pass through
-        // the same graph makes its own from the logits, as does a recorded one, which may run again.
-        none[0] = made->second.toTensor();
-        ctx->saved_data.erase(made);
+        // the same graph makes its own from the logits, as does a recorded one, which may run
+        // again. What is handed over has a version of its own: what its taker does to it is no
+        // change of what this graph saved.
+        ctx->saved_data["made"] = false;
+        none[0] = s[3].variable_data();
         OP("policy_loss_rescale_", policy_rescale)
             .call(none[0], grads[0], s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble());
       } else {

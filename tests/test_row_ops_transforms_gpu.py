@@ -8,6 +8,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwad
 from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
 
 from muonium_amd.kernels import policy_loss, qk_norm_rope, route, token_logprobs
 from oracle import row_ops_ref as ref
@@ -159,6 +160,68 @@ def test_policy_operators_are_well_behaved_torch_operators(keep, one_pass):
     args = (z, tokens, f, f, f, None, 0.2, 0.2, 0.1, 1.0)
     torch.library.opcheck(ops.policy_loss.default, (*args, keep, one_pass))
     torch.library.opcheck(ops.token_logprobs.default, (z, tokens, 1.0, keep))
+
+
+# ---- saved-tensor hooks --------------------------------------------------------------------
+
+
+def test_saved_tensor_hooks_see_the_gradient_of_the_forward_pass():
+    """What the forward pass keeps of the logits' size is offered to saved-tensor hooks, which may
+    move it: to the host and back, or away until a checkpoint is computed again."""
+    x, args = policy_args(64, 32000, torch.bfloat16)
+    x.requires_grad_()
+    scale = torch.tensor(0.3, device="cuda")
+
+    def loss():
+        return policy_loss(x, *args, kl_coef=0.1).loss
+
+    want, = torch.autograd.grad((loss(),), (x,), (scale,))
+    seen = []
+
+    def pack(t):
+        seen.append(t.shape)
+        return t.to("cpu")
+
+    size = x.numel() * x.element_size()
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to("cuda")):
+        before = torch.cuda.memory_allocated()
+        out = loss()
+        assert torch.cuda.memory_allocated() - before < size
+    assert seen.count(x.shape) == 2  # the logits and the gradient made of them
+    assert torch.equal(torch.autograd.grad((out,), (x,), (scale,))[0], want)
+    before = torch.cuda.memory_allocated()
+    out = checkpoint(loss, use_reentrant=False)
+    assert torch.cuda.memory_allocated() - before < size
+    assert torch.equal(torch.autograd.grad((out,), (x,), (scale,))[0], want)
+    # one that keeps the operator's results, by a dispatch mode
+    op = torch.ops.muonium_amd.policy_loss.default
+
+    def keep(ctx, func, *args, **kwargs):
+        return CheckpointPolicy.MUST_SAVE if func == op else CheckpointPolicy.PREFER_RECOMPUTE
+
+    out = checkpoint(loss, use_reentrant=False,
+                     context_fn=lambda: create_selective_checkpoint_contexts(keep))
+    got, = torch.autograd.grad((out,), (x,), (scale,))
+    torch.testing.assert_close(got, want, rtol=2.0**-7, atol=1e-9)
+
+
+def test_a_handed_over_gradient_is_its_takers():
+    """What becomes of the first gradient of a graph changes no later one."""
+    x, args = policy_args(6, 1500, torch.bfloat16)
+    x.requires_grad_()
+    loss = policy_loss(x, *args, kl_coef=0.1).loss
+    scale = torch.tensor(3.0, device="cuda")
+    first, = torch.autograd.grad((loss,), (x,), (scale,), retain_graph=True)
+    want = first.clone()
+    first.zero_()
+    assert torch.equal(torch.autograd.grad((loss,), (x,), (scale,), retain_graph=True)[0], want)
+    loss.backward(scale)
+    loss = policy_loss(x, *args, kl_coef=0.1).loss
+    loss.backward(scale, retain_graph=True)
+    loss.backward(scale)
+    torch.testing.assert_close(x.grad, 3 * want, rtol=2.0**-6, atol=1e-9)
+    with pytest.raises(RuntimeError, match="second time"):
+        loss.backward(scale)
 
 
 # ---- the policy gradient under any loss gradient ------------------------------------------------
