@@ -93,7 +93,9 @@ __global__ __launch_bounds__(BACK_THREADS) void logp_backward_kernel(Back a) {
       if (own.tok < 0 || own.up == 0.0f) continue;
     }
     const int64_t tok = MADE ? own.tok : a.tokens[row];
-    const float g = tok < 0 ? 0.0f : (MADE ? own.up : a.coef[row]) * scale * a.tau_inv;
+    const float up = tok < 0 ? 0.0f : MADE ? own.up : a.coef[row];
+    // no gradient, whatever the scale: one that overflowed makes none of it
+    const float g = up == 0.0f ? 0.0f : up * scale * a.tau_inv;
     const int64_t at = row * a.stride, to = row * a.V;
     const int64_t i0 = ((int64_t)blockIdx.x * BACK_VECS * BACK_THREADS + threadIdx.x) * N;
     if (g == 0.0f) {

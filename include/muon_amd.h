@@ -306,7 +306,8 @@ int muon_route_backward(const void* logits, int dtype, int64_t row_stride, int64
  * its row out (0, and no gradient; the row is not read); one of `vocab` or more gives NaN. stats
  * (2 * rows floats, NULL: not kept) is what the backward pass needs beside the logits, ws holds
  * muon_token_logprobs_workspace_bytes (0: may be NULL). Backward: dlogits (rows, vocab), contiguous, from
- * dlogprobs (rows) times *scale (NULL: 1); a row whose gradient is 0 is not read. */
+ * dlogprobs (rows) times *scale (NULL: 1); a row whose gradient is 0 is not read, and gets 0
+ * whatever *scale is. */
 int64_t muon_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab);
 int muon_token_logprobs(const void* logits, int dtype, int64_t row_stride, int64_t rows,
                         int64_t vocab, const int64_t* tokens, float temperature, float* logprobs,

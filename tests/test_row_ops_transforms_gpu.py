@@ -247,6 +247,24 @@ def test_policy_gradient_is_rounded_once(dtype, v):
             check(d, want * s.item(), (ds + 2 * room) * abs(s.item()), 257, dtype, scale)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_left_out_rows_stay_out_of_a_gradient_that_is_not_finite(dtype):
+    """A loss gradient of infinity or NaN (a loss scale that overflowed) makes no gradient in rows of
+    weight 0 and of negative tokens."""
+    x, (tokens, old, adv, w, r) = policy_args(9, 700, dtype, 4)
+    tokens[2] = -100
+    on = (w != 0) & (tokens >= 0)
+    assert on.any() and not on.all()
+    for scale in (math.inf, math.nan):
+        a = x.clone().requires_grad_()
+        out = policy_loss(a, tokens, old, adv, w, r, kl_coef=0.1)
+        for _ in range(2):  # the gradient of the forward pass, then one made from the logits
+            d, = torch.autograd.grad((out.loss,), (a,), (torch.tensor(scale, device="cuda"),),
+                                     retain_graph=True)
+            assert torch.count_nonzero(d[~on]) == 0
+            assert not d[on].isfinite().all(1).any()
+
+
 # ---- routing: gradients of empty slots -----------------------------------------------------------
 
 
