@@ -12,7 +12,7 @@ from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selectiv
 
 from muonium_amd.kernels import policy_loss, qk_norm_rope, route, token_logprobs
 from oracle import row_ops_ref as ref
-from test_row_ops_gpu import TYPES, check, gen, leaf, policy_case
+from test_row_ops_gpu import E, TYPES, check, gen, leaf, policy_case
 
 pytestmark = pytest.mark.gpu
 
@@ -296,3 +296,57 @@ def test_route_empty_slots_take_no_gradient(dtype, normalize, experts):
     x = leaf(z)
     torch.special.entr(route(x, 4, token_mask=mask.cuda(), normalize=normalize).gates).sum().backward()
     assert x.grad.isfinite().all()
+
+
+# ---- the KL term of neighbouring policies -----------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [64, 5000, 170001])
+def test_policy_kl_term_of_neighbouring_policies(dtype, v):
+    """exp(d) - d - 1 and its slope follow their own size, not that of exp(d), where policy and
+    reference nearly agree: off by what logp is off by (256 2^-24, times the term's slope, and its
+    square) and by 16 roundings of the result; and the term is never negative."""
+    n = 24
+    x, tokens, old, _, _, _, logp, _ = policy_case(n, v, dtype, 5, False, 1.0)
+    ahead = torch.logspace(-6, 0.8, n, dtype=torch.float64) * torch.tensor([1.0, -1.0]).repeat(n // 2)
+    r = (logp + ahead).float()
+    ahead = r.double() - logp
+    em1 = torch.expm1(ahead)
+    # d^2 / 2 + d^3 / 6 + ...: the difference itself would cancel in float64 too
+    series = sum(ahead ** i / float(math.factorial(i)) for i in range(2, 30))
+    term = torch.where(ahead.abs() < 1, series, em1 - ahead)
+    off = 256 * E
+    zero, one = torch.zeros(n, device="cuda"), torch.ones(n, device="cuda")
+    a = x.cuda()
+    loss, _, rows, _ = torch.ops.muonium_amd.policy_loss(
+        a, tokens.cuda(), old.cuda(), zero, one, r.cuda(), 0.2, 0.2, 1.0, 1.0, True, False)
+    terms, slopes = rows[0].double().cpu(), rows[1].double().cpu()
+    assert (terms >= 0).all()
+    room = em1.abs() * off + (em1 + 1) * off**2 + 16 * E * term
+    assert ((terms - term).abs() <= room).all(), ((terms - term).abs() / room).max()
+    assert ((slopes + em1).abs() <= (em1 + 1) * off + 16 * E * em1.abs()).all()
+    got = policy_loss(a, tokens.cuda(), old.cuda(), zero, one, r.cuda(), kl_coef=1.0).loss
+    assert abs(got.item() - term.sum().item()) <= (room + E * term).sum().item() + E * term.sum().item()
+    # exactly the reference: nothing, or next to it
+    same = token_logprobs(a, tokens.cuda())
+    none = policy_loss(a, tokens.cuda(), old.cuda(), zero, one, same, kl_coef=1.0).loss
+    assert 0 <= none.item() <= n * (off + E * same.abs().max().item())**2
+
+
+def test_policy_kl_term_of_distant_policies():
+    """The same where the reference thinks a token far less, or far more, likely."""
+    n = 12
+    x, tokens, old, _, _, _, logp, _ = policy_case(n, 300, torch.float32, 5, False, 1.0)
+    ahead = torch.linspace(1.0, 60.0, n, dtype=torch.float64) * torch.tensor([1.0, -1.0]).repeat(n // 2)
+    r = (logp + ahead).float()
+    ahead = r.double() - logp
+    e = torch.exp(ahead)
+    zero, one = torch.zeros(n, device="cuda"), torch.ones(n, device="cuda")
+    _, _, rows, _ = torch.ops.muonium_amd.policy_loss(
+        x.cuda(), tokens.cuda(), old.cuda(), zero, one, r.cuda(), 0.2, 0.2, 1.0, 1.0, True, False)
+    terms, slopes = rows[0].double().cpu(), rows[1].double().cpu()
+    # logp's error and the argument's rounding move the exponential, then 16 roundings
+    off = (256 + 2 * ahead.abs()) * E
+    assert ((terms - (e - ahead - 1)).abs() <= (e - 1).abs() * off + 16 * E * (e + ahead.abs())).all()
+    assert ((slopes + e - 1).abs() <= e * off + 16 * E * (e - 1).abs()).all()
