@@ -1,9 +1,10 @@
-"""The row operators' libraries without a device: what their entry points refuse before a launch, and
-what their kernels keep in registers."""
+"""The row operators' libraries without a device: what their entry points refuse before a launch,
+what needs which library, and what the kernels keep in registers."""
 
 import os
 import re
 import subprocess
+import sys
 
 import pytest
 
@@ -31,6 +32,43 @@ def test_rescale_refuses_without_launching(call, code):
 
 def test_rescale_of_no_rows_returns_ok():
     assert _lib.load().muon_policy_loss_rescale(None, 1, 4, 0, 4, None, 1.0, None, None, None, None, None) == 0
+
+
+def run_python(code):
+    path = os.path.join(ROOT, "dtensor-muon_amd")
+    return subprocess.run([sys.executable, "-c", code, path], capture_output=True, text=True, timeout=300)
+
+
+def test_gram_needs_nothing_of_the_torch_operators():
+    """Its import neither loads nor misses their library; theirs says what is missing."""
+    done = run_python('''
+import sys
+sys.path.insert(0, sys.argv[1])
+import muonium_amd.kernels as kernels
+from muonium_amd.kernels import gram, gram_
+from muonium_amd import _lib
+assert "muonium_amd._row_ops" not in sys.modules
+assert "libmuon_amd_torch" not in open("/proc/self/maps").read()
+assert {"gram", "route", "policy_loss", "Routing"} <= set(dir(kernels))
+_lib._LIB_PATH = "/nowhere/libmuon_amd.so"
+try:
+    from muonium_amd.kernels import route
+except ImportError as e:
+    assert "libmuon_amd_torch.so is missing" in str(e), e
+else:
+    raise AssertionError("imported")
+assert not hasattr(kernels, "other")
+''')
+    assert done.returncode == 0, done.stderr
+    done = run_python('''
+import sys
+sys.path.insert(0, sys.argv[1])
+from muonium_amd.kernels import *
+import muonium_amd.kernels as kernels
+assert kernels.route is route and "libmuon_amd_torch" in open("/proc/self/maps").read()
+assert qk_norm_rope and token_logprobs and policy_loss and gram and gram_ and PolicyLoss and Routing
+''')
+    assert done.returncode == 0, done.stderr
 
 
 @pytest.mark.skipif(not os.path.exists(HIPCC), reason="needs hipcc")
