@@ -71,6 +71,36 @@ assert qk_norm_rope and token_logprobs and policy_loss and gram and gram_ and Po
     assert done.returncode == 0, done.stderr
 
 
+def planned(tmp_path, python):
+    """What make would run from nothing, with `python` as its python3."""
+    (tmp_path / "python3").write_text(f"#!/bin/sh\n{python}\n")
+    (tmp_path / "python3").chmod(0o755)
+    env = {**os.environ, "PATH": f"{tmp_path}:{os.environ['PATH']}"}
+    env.pop("TORCH_DIR", None)
+    done = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "dtensor-muon_amd", "csrc")],
+                          env=env, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr
+    assert "-shared -fPIC -o ../muonium_amd/_lib/libmuon_amd.so.tmp" in done.stdout
+    return done.stdout
+
+
+@pytest.mark.parametrize("missing", ["python", "torch", "rocm"])
+def test_make_builds_the_c_abi_without_torch(tmp_path, missing):
+    """Without a python3, without torch, and beside a torch of another device."""
+    (tmp_path / "torch").mkdir()
+    (tmp_path / "torch" / "__init__.py").write_text("")
+    python = {"python": "exit 127",
+              "torch": f'exec {sys.executable} -I -S "$@"',
+              "rocm": f'PYTHONPATH={tmp_path} exec {sys.executable} -S "$@"'}[missing]
+    plan = planned(tmp_path, python)
+    assert "row_ops.cpp" not in plan and "is not built" in plan
+
+
+def test_make_builds_the_torch_operators_with_torch(tmp_path):
+    plan = planned(tmp_path, f'exec {sys.executable} "$@"')
+    assert "row_ops.cpp" in plan and "is not built" not in plan
+
+
 @pytest.mark.skipif(not os.path.exists(HIPCC), reason="needs hipcc")
 def test_rescale_kernels_use_no_scratch(tmp_path):
     asm = tmp_path / "kernels.s"
