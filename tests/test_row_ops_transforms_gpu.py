@@ -12,7 +12,7 @@ from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selectiv
 
 from muonium_amd.kernels import policy_loss, qk_norm_rope, route, token_logprobs
 from oracle import row_ops_ref as ref
-from test_row_ops_gpu import E, TYPES, check, gen, leaf, policy_case
+from test_row_ops_gpu import E, TYPES, _all_calls, check, gen, leaf, policy_case
 
 pytestmark = pytest.mark.gpu
 
@@ -350,3 +350,110 @@ def test_policy_kl_term_of_distant_policies():
     off = (256 + 2 * ahead.abs()) * E
     assert ((terms - (e - ahead - 1)).abs() <= (e - 1).abs() * off + 16 * E * (e + ahead.abs())).all()
     assert ((slopes + e - 1).abs() <= e * off + 16 * E * (e - 1).abs()).all()
+
+
+# ---- rows past the grid's second dimension ------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_more_rows_than_a_grid_has(dtype):
+    """65536 rows and more, left-out ones on both sides of the line: kernels that walk over rows do
+    each of them once, in both directions."""
+    n, v = 70000, 40
+    x, tokens, old, adv, w, r, logp, p = policy_case(n, v, dtype, 6, True, 1.0)
+    out = torch.tensor([3, 65533, 65534, 65535, 65536, 65537, 69999])
+    tokens[out] = -100
+    w[:] = 0.5 + torch.rand(n, generator=gen(7))
+    w[out[::2]] = 0.0
+    w[65530], w[65540] = 0.0, 0.0
+    logp, p = ref.logprobs(x, tokens)
+    xl = leaf(x)
+    got = token_logprobs(xl, tokens.cuda())
+    check(got, logp, torch.ones(n, dtype=torch.float64), 256, torch.float32, "logp")
+    g = torch.randn(n, generator=gen(8))
+    d, = torch.autograd.grad((got,), (xl,), (g.cuda(),))
+    check(d, *ref.logprobs_grad(p, tokens, g), 256, dtype, "dlogits")
+    # fp16 reads the logits again for the gradient, bf16 makes it in the forward pass
+    on = (w != 0) & (tokens >= 0)
+    w = torch.where(on, w, 0.0)
+    loss, slope, size, sizes = ref.policy(logp, old, adv, w, r, 0.2, 0.2, 0.1)
+    args = [t.cuda() for t in (tokens, old, adv, w, r)]
+    for scale in (1.0, 3.0):
+        res = policy_loss(xl, *args, kl_coef=0.1)
+        # 70000 terms of both signs, each rounded to fp32 before the sum in double
+        check(res.loss, loss, size, 2 * 256 + 1, torch.float32, "loss")
+        check(res.logprobs, torch.where(on, logp, 0.0), torch.ones(n, dtype=torch.float64), 256, torch.float32)
+        d, = torch.autograd.grad((res.loss,), (xl,), (torch.tensor(scale, device="cuda"),))
+        want, ds = ref.logprobs_grad(p, tokens, slope)
+        _, room = ref.logprobs_grad(p, tokens, sizes)
+        check(d, want * scale, (ds + 2 * room) * scale, 257, dtype, "policy dlogits")
+        assert torch.count_nonzero(d[(~on).cuda()]) == 0
+    plain = policy_loss(x.cuda(), *args, kl_coef=0.1)
+    check(plain.loss, loss, size, 2 * 256 + 1, torch.float32, "loss without gradient")
+
+
+# ---- captured graphs with a backward pass ------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_forward_and_backward_in_a_captured_graph(dtype):
+    """Every replay gives the eager results and gradients of its inputs, for any loss gradient."""
+    g = gen(9)
+    q = torch.randn(3, 9, 8, 64, generator=g).to(dtype).cuda().requires_grad_()
+    w = torch.ones(64, device="cuda").requires_grad_()
+    z = torch.randn(3000, 64, generator=g).to(dtype).cuda().requires_grad_()
+    x, args = policy_args(12, 9000, dtype, 2)
+    x.requires_grad_()
+    ups = [torch.randn(3, 9, 8, 64, generator=g).to(dtype).cuda(), torch.randn(3000, 6, generator=g).cuda(),
+           torch.tensor(0.3, device="cuda"), torch.tensor(0.01, device="cuda"),
+           torch.randn(12, generator=g).cuda(), torch.tensor(1 / 3, device="cuda")]
+
+    def run():
+        a, b = qk_norm_rope(q, q, w, w)
+        rt = route(z, 6)
+        lp = token_logprobs(x, args[0])
+        out = policy_loss(x, *args, kl_coef=0.1)
+        grads = [*torch.autograd.grad((a, b), (q, w), (ups[0], ups[0])),
+                 *torch.autograd.grad((rt.gates, rt.balance_loss, rt.z_loss), (z,), ups[1:4]),
+                 *torch.autograd.grad((lp,), (x,), (ups[4],)),
+                 *torch.autograd.grad((out.loss,), (x,), (ups[5],))]
+        return [t.detach() for t in (a, b, *rt, lp, *out)] + grads
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run()
+    for i, scale in enumerate((1 / 3, 1.0, 0.0, 2.5, 1.0)):
+        with torch.no_grad():
+            for t in (q, z, x, *ups[:2]):
+                t.copy_(torch.randn(t.shape, generator=g))
+            ups[5].fill_(scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        for j, (a, b) in enumerate(zip(outs, run())):
+            assert torch.equal(a, b), (i, j)
+
+
+# ---- an outer compile ------------------------------------------------------------------------
+
+
+def test_outer_compile_gives_the_same_bits():
+    """Under an outer compile the same kernels run: the same bits, but for the policy loss, whose
+    gradient takes two readings there, and the sums of the logits' gradient with it."""
+    run = _all_calls(1)
+    want = run()
+    torch._dynamo.reset()
+    got = torch.compile(run, backend="aot_eager")()
+    torch._dynamo.reset()
+    names = ["q_out", "k_out", "gates", "experts", "counts", "logprobs", "loss", "q", "k", "w", "z", "x"]
+    assert len(got) == len(want) == len(names)
+    for name, a, b in zip(names, got, want):
+        if name in ("loss", "x"):
+            tol = 2.0**-7 if a.dtype == torch.bfloat16 else 1e-5
+            torch.testing.assert_close(a, b, rtol=tol, atol=1e-6, msg=lambda m: f"{name}: {m}")
+        else:
+            assert torch.equal(a, b), name
