@@ -11,6 +11,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -379,6 +380,12 @@ void refuse_tangents(const T&... t) {
 bool watched() { return c10::impl::TorchDispatchModeTLS::any_modes_set(); }
 bool watched(const Tensor& t) { return watched() || t.key_set().has(c10::DispatchKey::Python); }
 
+// Whether launches beside `t` are being recorded into a graph.
+bool captured(const Tensor& t) {
+  const at::DeviceGuard guard(t.device());
+  return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+
 Tensor or_undefined(const optional<Tensor>& t) { return t ? *t : Tensor(); }
 optional<Tensor> or_none(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
 
@@ -532,6 +539,7 @@ struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
     ctx->save_for_backward({logits, tokens, rows, ours ? dlogits : Tensor()});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["made"] = ours;
+    ctx->saved_data["captured"] = ours && captured(logits);
     if (ours) dlogits = empty(logits, {0}, logits.scalar_type());
     if (!keep) rows = rows.narrow(0, 0, 1);
     ctx->mark_non_differentiable({logp, rows, dlogits});
@@ -544,11 +552,12 @@ struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
     const auto s = ctx->get_saved_variables();
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      if (ctx->saved_data["made"].toBool() && !watched()) {
-        // The gradient of the forward pass is handed over once; a second backward pass through
-        // the same graph makes its own from the logits, as does a recorded one, which may run
-        // again. What is handed over has a version of its own: what its taker does to it is no
-        // change of what this graph saved.
+      // The gradient of the forward pass is handed over once; a second backward pass through the same
+      // graph makes its own from the logits, as does one that may run again without its forward
+      // pass: one that is watched, or captured alone. What is handed over has a version of its own:
+      // what its taker does to it is no change of what this graph saved.
+      if (ctx->saved_data["made"].toBool() && !watched() &&
+          (ctx->saved_data["captured"].toBool() || !captured(s[0]))) {
         ctx->saved_data["made"] = false;
         none[0] = s[3].variable_data();
         OP("policy_loss_rescale_", policy_rescale)

@@ -438,6 +438,38 @@ def test_forward_and_backward_in_a_captured_graph(dtype):
             assert torch.equal(a, b), (i, j)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_backward_alone_in_a_captured_graph(dtype):
+    """A graph of the backward pass of an eager forward pass gives the gradient of each replay's loss
+    gradient. (The engine runs a node on the stream of its forward pass: both are on the one that
+    is captured.)"""
+    x, args = policy_args(12, 3000, dtype, 2)
+    x.requires_grad_()
+    up = torch.tensor(3.0, device="cuda")
+
+    def loss():
+        return policy_loss(x, *args, kl_coef=0.1).loss
+
+    def back(value):
+        return torch.autograd.grad((value,), (x,), (up,), retain_graph=True)[0]
+
+    want = back(loss()).float() / 3
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        back(loss())
+        out = loss()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = back(out)
+    for scale in (3.0, 3.0, 1.0, 0.5, 3.0):
+        up.fill_(scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        torch.testing.assert_close(got.float(), want * scale, rtol=2.0**-6, atol=1e-6, msg=str(scale))
+
+
 # ---- an outer compile ------------------------------------------------------------------------
 
 
