@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256) void scale_kernel(void* x, int64_t n, const fl
 
 // Slices of a row. One workgroup a row as a rule: joining slices takes a second launch. Longer
 // rows than SPLIT_FROM, of which fewer than 128 come together, are cut until there are four
-// workgroups per CU. One row, whole and cut (us a call): 32000 values 6.1 and 10.0, 128000 9.0 and
+// workgroups per CU, into slices of at least 8192 values and at most 64 a row. One row, whole and cut (us a call): 32000 values 6.1 and 10.0, 128000 9.0 and
 // 10.4, 262144 14.6 and 9.2, 524288 26.1 and 9.7; 64 rows of 262144 values 17.3 and 15.3.
 constexpr int64_t SPLIT_FROM = 131072;
 int slices_for(int64_t N, int64_t V) {
