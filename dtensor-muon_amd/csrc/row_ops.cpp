@@ -11,7 +11,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -382,8 +382,9 @@ bool watched(const Tensor& t) { return watched() || t.key_set().has(c10::Dispatc
 
 // Whether launches beside `t` are being recorded into a graph.
 bool captured(const Tensor& t) {
-  const at::DeviceGuard guard(t.device());
-  return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  C10_HIP_CHECK(hipStreamIsCapturing((hipStream_t)stream_of(t), &status));
+  return status != hipStreamCaptureStatusNone;
 }
 
 Tensor or_undefined(const optional<Tensor>& t) { return t ? *t : Tensor(); }
@@ -522,6 +523,8 @@ Tensor2 logp_autograd(const Tensor& logits, const Tensor& tokens, double tempera
 }
 
 struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
+  // Whether a gradient of the forward pass waits for the backward pass, and where it was made.
+  enum Made { NO, EAGERLY, IN_GRAPH };
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens,
                                const Tensor& old, const Tensor& advantages, const Tensor& weights,
                                const optional<Tensor>& ref, double clip_low, double clip_high,
@@ -538,8 +541,7 @@ struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
     // the gradient too is a saved tensor: hooks move or drop it like the logits
     ctx->save_for_backward({logits, tokens, rows, ours ? dlogits : Tensor()});
     ctx->saved_data["temperature"] = temperature;
-    ctx->saved_data["made"] = ours;
-    ctx->saved_data["captured"] = ours && captured(logits);
+    ctx->saved_data["made"] = (int64_t)(!ours ? NO : captured(logits) ? IN_GRAPH : EAGERLY);
     if (ours) dlogits = empty(logits, {0}, logits.scalar_type());
     if (!keep) rows = rows.narrow(0, 0, 1);
     ctx->mark_non_differentiable({logp, rows, dlogits});
@@ -556,9 +558,9 @@ struct PolicyFunction : torch::autograd::Function<PolicyFunction> {
       // graph makes its own from the logits, as does one that may run again without its forward
       // pass: one that is watched, or captured alone. What is handed over has a version of its own:
       // what its taker does to it is no change of what this graph saved.
-      if (ctx->saved_data["made"].toBool() && !watched() &&
-          (ctx->saved_data["captured"].toBool() || !captured(s[0]))) {
-        ctx->saved_data["made"] = false;
+      auto& made = ctx->saved_data["made"];
+      if (made.toInt() != NO && !watched() && (made.toInt() == IN_GRAPH || !captured(s[0]))) {
+        made = (int64_t)NO;
         none[0] = s[3].variable_data();
         OP("policy_loss_rescale_", policy_rescale)
             .call(none[0], grads[0], s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble());
