@@ -490,7 +490,7 @@ constexpr int64_t MAX_DIM = 1024;
 
 // Argument checks shared by both directions. Returns a status; *empty: nothing to do.
 int check(const char* what, Args& a, int dtype, int64_t batch, int64_t T, int64_t q_heads,
-          int64_t k_heads, int64_t D, int64_t R, bool* empty) {
+          int64_t k_heads, int64_t D, int64_t R, int pos_bits, bool* empty) {
   if (!io_ok(dtype) || ((a.s[0].w || a.s[1].w) && !io_ok(a.wdt))) {
     muon_set_error("%s: unsupported dtype (%d, weights %d)", what, dtype, a.wdt);
     return MUON_ERR_DTYPE;
@@ -502,6 +502,10 @@ int check(const char* what, Args& a, int dtype, int64_t batch, int64_t T, int64_
                    (long long)q_heads, (long long)k_heads, (long long)D, (long long)MAX_DIM,
                    (long long)R);
     return MUON_ERR_SHAPE;
+  }
+  if (a.pos && pos_bits != 32 && pos_bits != 64) {
+    muon_set_error("%s: positions of %d bits", what, pos_bits);
+    return MUON_ERR_ARG;
   }
   *empty = batch * T == 0 || q_heads + k_heads == 0;
   if (*empty) return MUON_OK;
@@ -598,7 +602,8 @@ int muon_qk_norm_rope(const void* q, const void* k, const int64_t* strides, cons
   a.pos = positions; a.pos64 = pos_bits == 64; a.pos_sb = pos_batch_stride;
   a.inter = interleaved; a.wdt = w_dtype; a.eps = eps;
   bool empty = false;
-  const int rc = check("qk_norm_rope", a, dtype, batch, tokens, q_heads, k_heads, dim, rotary, &empty);
+  const int rc = check("qk_norm_rope", a, dtype, batch, tokens, q_heads, k_heads, dim, rotary,
+                       pos_bits, &empty);
   if (rc || empty) return rc;
   int lanes = 0;
   const Form form = form_for(a, dtype, &lanes);
@@ -637,7 +642,7 @@ int muon_qk_norm_rope_backward(const void* q, const void* k, const void* dq_out,
   a.inter = interleaved; a.wdt = w_dtype; a.eps = eps; a.part = (float*)ws;
   bool empty = false;
   const int rc = check("qk_norm_rope_backward", a, dtype, batch, tokens, q_heads, k_heads, dim,
-                       rotary, &empty);
+                       rotary, pos_bits, &empty);
   if (rc) return rc;
   const bool dw = dq_weight || dk_weight;
   if ((dq_weight && !q_weight) || (dk_weight && !k_weight) || (dw && !ws) ||

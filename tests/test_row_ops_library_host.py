@@ -34,6 +34,18 @@ def test_rescale_of_no_rows_returns_ok():
     assert _lib.load().muon_policy_loss_rescale(None, 1, 4, 0, 4, None, 1.0, None, None, None, None, None) == 0
 
 
+@pytest.mark.parametrize("bits", [0, 8, 16, 128])
+def test_positions_are_of_32_or_64_bits(bits):
+    """The kernels read positions of no other width: the call would read past their end."""
+    lib, s = _lib.load(), _lib.i64_array([8] * 12)
+    assert lib.muon_qk_norm_rope(1, 1, s, None, None, 0, 1, 1, 9, 1, bits, 0, 1, 1, 1, 1, 1, 1, 1, 8, 8, 0,
+                                 1e-6, None) == 5
+    assert "positions" in _lib.last_error()
+    assert lib.muon_qk_norm_rope_backward(1, 1, 1, 1, s, None, None, 0, 1, 1, 9, 1, bits, 0, 1, 1, None, None,
+                                          None, 1, 1, 1, 1, 1, 8, 8, 0, 1e-6, None) == 5
+    assert "positions" in _lib.last_error()
+
+
 def run_python(code):
     path = os.path.join(ROOT, "dtensor-muon_amd")
     return subprocess.run([sys.executable, "-c", code, path], capture_output=True, text=True, timeout=300)
