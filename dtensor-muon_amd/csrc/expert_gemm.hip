@@ -1,0 +1,531 @@
+// Products of the experts' matrices with their own rows (muon_expert_linear and its gradients). The
+// rows of expert e are offsets[e] .. offsets[e + 1] - 1 of all; weights are (E, out, in):
+//   FWD:  y_e  = x_e W_e^T     (rows x out, over in)
+//   ROWS: dx_e = dy_e W_e      (rows x in, over out)
+//   WGT:  dW_e = dy_e^T x_e    (out x in, over the expert's rows)
+// Rows behind the last expert's give zeros, and reach no weight; an expert without rows gets a zero
+// gradient.
+//
+// The offsets stay on the device, so the grid is the most tiles that R rows of E experts can make, and
+// each workgroup finds its tile from the offsets; those left over end at once. 16-bit types run on
+// MFMA with fp32 accumulators, fp32 on the fp32 MFMA.
+#include <algorithm>
+#include <type_traits>
+
+#include "rowops.h"
+
+namespace {
+
+enum { FWD = 0, ROWS = 1, WGT = 2 };
+
+struct GArgs {
+  const void* a;  // FWD: rows; ROWS, WGT: dy
+  const void* b;  // FWD, ROWS: weights; WGT: rows
+  void* c;        // contiguous
+  int64_t lda, ldb;  // strides in elements: of the rows of a; of the rows of b
+  int64_t sb;        // FWD, ROWS: elements of an expert's weights; WGT: unused
+  const int32_t* offsets;
+  int64_t R;  // rows in all
+  int E, N, K, M;  // FWD: N out, K in; ROWS: N in, K out; WGT: M out, N in
+  int tiles_m, tiles_n;  // FWD, ROWS: the most row tiles there can be
+};
+
+// The bounds of expert e's rows, whatever the offsets hold: within 0 .. R, the end no less than the
+// start; the first expert's start at 0. e == E: the rows behind the last expert's.
+MUON_DEVICE void bounds(const GArgs& g, int e, int& start, int& n) {
+  const int R = (int)g.R;
+  start = e ? std::min(std::max(g.offsets[e], 0), R) : 0;
+  n = (e < g.E ? std::min(std::max(g.offsets[e + 1], start), R) : R) - start;
+}
+
+// Workgroup L's tile of `total`: one contiguous range of tiles for each of the 8 XCDs (consecutive
+// workgroups are dealt round robin), so those that share panels share an L2. -1: none is left.
+MUON_DEVICE int xcd_range(int L, int total) {
+  const int x = L & 7, i = L >> 3, q = total >> 3, r = total & 7;
+  return i < q + (x < r) ? x * q + std::min(x, r) + i : -1;
+}
+// A tile's row and column: GM rows of tiles for each column after the other.
+MUON_DEVICE void tile_of(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
+  constexpr int GM = 8;
+  const int group = t / (GM * tiles_n), first = group * GM, size = std::min(tiles_m - first, GM);
+  const int local = t - group * (GM * tiles_n);
+  tm = first + local % size;
+  tn = local / size;
+}
+
+// Workgroup L's row tile of the experts one after another (g.tiles_n tiles of columns each) -> expert,
+// first row, rows left of the expert from there, and column tile. Each lane counts the tiles of a few
+// experts in a row; a scan over the wave gives their number, over which the workgroups are dealt, and
+// the lane that has the tile. False where a workgroup is left over.
+template <int BM>
+MUON_DEVICE bool find_tile(const GArgs& g, int L, int& e, int& row0, int& left, int& tn) {
+  const int lane = threadIdx.x & 63, per = (g.E + 64) / 64;
+  const int e0 = lane * per, e1 = std::min(e0 + per, g.E + 1);
+  int mine = 0, start, n;
+  for (int i = e0; i < e1; ++i) {
+    bounds(g, i, start, n);
+    mine += (n + BM - 1) / BM;
+  }
+  int incl = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int v = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += v;
+  }
+  const int tiles_m = __shfl(incl, 63, 64);
+  int t;
+  L = xcd_range(L, tiles_m * g.tiles_n);
+  if (L < 0) return false;
+  tile_of(L, tiles_m, g.tiles_n, t, tn);
+  const uint64_t past = __ballot(incl > t);
+  if (!past) return false;  // offsets that do not rise can count beyond 32 bits
+  const int src = __builtin_ctzll(past);
+  int first = __shfl(incl - mine, src, 64);
+  e = src * per;
+  for (;; ++e) {
+    bounds(g, e, start, n);
+    const int tiles = (n + BM - 1) / BM;
+    if (t < first + tiles || e >= g.E) break;
+    first += tiles;
+  }
+  e = __builtin_amdgcn_readfirstlane(e);
+  const int skip = (t - first) * BM;
+  row0 = __builtin_amdgcn_readfirstlane(start + skip);
+  left = __builtin_amdgcn_readfirstlane(n - skip);
+  return true;
+}
+
+template <int DT>
+MUON_DEVICE f32x4 mfma16(muon_u4 a, muon_u4 b, f32x4 c) {
+  if constexpr (DT == MUON_DT_BF16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_mfma, a),
+                                                   __builtin_bit_cast(bf16x8_mfma, b), c, 0, 0, 0);
+  } else {
+    typedef __attribute__((ext_vector_type(8))) _Float16 h8;
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  }
+}
+
+// Two values to 16 bits each, to nearest even.
+template <int DT>
+MUON_DEVICE uint32_t pack2(float x, float y) {
+  if constexpr (DT == MUON_DT_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(muon_f2x{x, y}, muon_bf2x));
+  else
+    return (uint32_t)f32_to_f16(x) | ((uint32_t)f32_to_f16(y) << 16);
+}
+
+// ---- 16-bit types ---------------------------------------------------------------------------
+//
+// Panels in LDS, one K-tile of 64 at a time. A panel whose rows run along k (KC) holds its rows of 64 k
+// as 8 chunks of 16 bytes, chunk c of row r at place c ^ ((r >> 1) & 7); one whose rows are k (KR) holds
+// 64 rows of the tile's width, chunk c of row k at c ^ ((k & 3) << 2) ^ (((k >> 3) & 1) << 1): both spread
+// the 16 lanes of a fragment read over all banks. A KC fragment is one 16-byte read; a KR one is two
+// transposing reads, each four k of one column for every lane.
+constexpr int BK = 64;
+typedef __attribute__((ext_vector_type(4))) short i16x4;
+typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
+
+MUON_DEVICE int swz_kc(int r) { return (r >> 1) & 7; }
+MUON_DEVICE int swz_kr(int k) { return ((k & 3) << 2) ^ (((k >> 3) & 1) << 1); }
+
+// One operand's share of a K-tile: PANEL rows (KC) or columns (KR) of the tile, NT threads.
+template <int PANEL, bool KR, int NT, bool ALIGNED>
+struct Stage {
+  static constexpr int CHUNKS = PANEL * BK / 8 / NT;  // 16-byte chunks of a thread
+  static constexpr int PER_ROW = KR ? PANEL / 8 : 8;
+  static constexpr int ROWS_PASS = NT / PER_ROW;
+  muon_u4 w[CHUNKS];
+
+  // base: the panel's first row and column at k = 0; `in`: valid rows (KC) or columns (KR) from
+  // there, k left: valid k from k0 on
+  MUON_DEVICE void load(const uint16_t* base, int64_t ld, int in, int k0, int kleft) {
+    const int row = threadIdx.x / PER_ROW, ch = threadIdx.x % PER_ROW * 8;
+#pragma unroll
+    for (int q = 0; q < CHUNKS; ++q) {
+      const int r = row + q * ROWS_PASS;
+      const bool ok = KR ? r < kleft : r < in;
+      const int have = ok ? (KR ? in : kleft) - ch : 0;
+      const uint16_t* p = KR ? base + (k0 + r) * ld + ch : base + r * ld + k0 + ch;
+      if (have >= 8) {
+        if constexpr (ALIGNED) w[q] = *(const muon_u4*)p;
+        else w[q] = load_u4(p);
+      } else {
+        uint32_t u[4] = {0, 0, 0, 0};
+        if constexpr (!ALIGNED) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < have) u[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
+        }
+        w[q] = muon_u4{u[0], u[1], u[2], u[3]};
+      }
+    }
+  }
+  MUON_DEVICE void store(uint8_t* lds) const {
+    const int row = threadIdx.x / PER_ROW, c = threadIdx.x % PER_ROW;
+#pragma unroll
+    for (int q = 0; q < CHUNKS; ++q) {
+      const int r = row + q * ROWS_PASS;
+      const int at = KR ? r * PANEL * 2 + ((c ^ swz_kr(r)) << 4) : r * BK * 2 + ((c ^ swz_kc(r)) << 4);
+      *(muon_u4*)(lds + at) = w[q];
+    }
+  }
+};
+
+// 8 consecutive k (ks 32-k substep, lane / 16) of row or column r0 + lane % 16.
+template <int PANEL, bool KR>
+MUON_DEVICE muon_u4 fragment(uint8_t* lds, int r0, int ks) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  if constexpr (!KR) {
+    const int row = r0 + r;
+    return *(const muon_u4*)(lds + row * BK * 2 + (((ks * 4 + g) ^ swz_kc(row)) << 4));
+  } else {
+    const int c = r0 / 8 + ((r & 3) >> 1), in = (r & 1) * 8;
+    const int k = ks * 32 + g * 8 + (r >> 2);
+    const uint8_t* lo = lds + k * PANEL * 2 + ((c ^ swz_kr(k)) << 4) + in;
+    const uint8_t* hi = lds + (k + 4) * PANEL * 2 + ((c ^ swz_kr(k + 4)) << 4) + in;
+    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)lo);
+    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)hi);
+    const uint64_t ua = __builtin_bit_cast(uint64_t, a), ub = __builtin_bit_cast(uint64_t, b);
+    return muon_u4{(uint32_t)ua, (uint32_t)(ua >> 32), (uint32_t)ub, (uint32_t)(ub >> 32)};
+  }
+}
+
+// A BM x BN tile by WM x WN waves.
+template <int DT, int FORM, int BM, int BN, int WM, int WN, bool ALIGNED>
+__global__ __launch_bounds__(64 * WM * WN, 1) void expert_gemm_kernel(GArgs g) {
+  constexpr int NT = 64 * WM * WN;
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  constexpr bool KRA = FORM == WGT, KRB = FORM != FWD;
+  constexpr int PANEL_A = BM * BK * 2, STAGE = (BM + BN) * BK * 2;
+  extern __shared__ __align__(16) uint8_t smem[];
+
+  int e, tm, tn, row0 = 0, left = 0, K, M;
+  if constexpr (FORM == WGT) {
+    const int per = g.tiles_m * g.tiles_n, L = xcd_range(blockIdx.x, gridDim.x);
+    e = L / per;
+    tile_of(L - e * per, g.tiles_m, g.tiles_n, tm, tn);
+    bounds(g, e, row0, K);
+    M = std::min(g.M - tm * BM, BM);
+  } else {
+    if (!find_tile<BM>(g, blockIdx.x, e, row0, left, tn)) return;
+    M = std::min(left, BM);
+    K = e < g.E ? g.K : 0;
+    tm = 0;
+  }
+  const int N = std::min(g.N - tn * BN, BN);
+  const uint16_t* A = (const uint16_t*)g.a + (int64_t)row0 * g.lda + (FORM == WGT ? tm * BM : 0);
+  const uint16_t* B = (const uint16_t*)g.b;
+  if constexpr (FORM == FWD) B += e * g.sb + (int64_t)tn * BN * g.ldb;
+  if constexpr (FORM == ROWS) B += e * g.sb + tn * BN;
+  if constexpr (FORM == WGT) B += (int64_t)row0 * g.ldb + tn * BN;
+
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wm = wave % WM, wn = wave / WM;
+  Stage<BM, KRA, NT, ALIGNED> sa;
+  Stage<BN, KRB, NT, ALIGNED> sb;
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  const int KT = (K + BK - 1) / BK;
+  if (KT) {
+    sa.load(A, g.lda, M, 0, K);
+    sb.load(B, g.ldb, N, 0, K);
+    sa.store(smem);
+    sb.store(smem + PANEL_A);
+  }
+  __syncthreads();
+  for (int kt = 0; kt < KT; ++kt) {
+    uint8_t* st = smem + (kt & 1) * STAGE;
+    const bool more = kt + 1 < KT;
+    if (more) {
+      sa.load(A, g.lda, M, (kt + 1) * BK, K - (kt + 1) * BK);
+      sb.load(B, g.ldb, N, (kt + 1) * BK, K - (kt + 1) * BK);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      muon_u4 fa[FM], fb[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fa[i] = fragment<BM, KRA>(st, wm * FM * 16 + i * 16, ks);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fb[j] = fragment<BN, KRB>(st + PANEL_A, wn * FN * 16 + j * 16, ks);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma16<DT>(fb[j], fa[i], acc[i][j]);
+    }
+    if (more) {
+      uint8_t* nx = smem + ((kt + 1) & 1) * STAGE;
+      sa.store(nx);
+      sb.store(nx + PANEL_A);
+    }
+    __syncthreads();
+  }
+
+  // the b fragment is the first operand: a lane holds four consecutive columns of one row
+  const int r = lane & 15, gq = lane >> 4;
+  uint16_t* C = (uint16_t*)g.c + (FORM == WGT ? ((int64_t)e * g.M + tm * BM) * g.N : (int64_t)row0 * g.N);
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = wm * FM * 16 + i * 16 + r;
+    if (m >= M) continue;
+    uint16_t* out = C + (int64_t)m * g.N + tn * BN;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int n = wn * FN * 16 + j * 16 + gq * 4;
+      const uint32_t lo = pack2<DT>(acc[i][j][0], acc[i][j][1]), hi = pack2<DT>(acc[i][j][2], acc[i][j][3]);
+      if (ALIGNED ? n < N : n + 4 <= N) {
+        if constexpr (ALIGNED) {
+          *(uint2*)(out + n) = make_uint2(lo, hi);
+        } else {
+          const uint2 v = make_uint2(lo, hi);
+          __builtin_memcpy(out + n, &v, 8);
+        }
+      } else if (!ALIGNED) {
+        const uint32_t u[2] = {lo, hi};
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (n + q < N) out[n + q] = (uint16_t)(u[q / 2] >> (16 * (q & 1)));
+      }
+    }
+  }
+}
+
+// ---- fp32 -----------------------------------------------------------------------------------
+//
+// 128 x 128 tile, K-tiles of 16, four waves of 64 x 64 on v_mfma_f32_32x32x2_f32. Both panels stand in LDS
+// as rows of k, whatever their order in memory, so a fragment is one value of a column for each lane.
+constexpr int F_B = 128, F_K = 16, F_P = F_B + 4;
+
+// Eight values of a thread: KR: row k, columns 8 c ..; KC: row r, k 8 c ..
+template <bool KR>
+MUON_DEVICE void f32_load(float (&w)[8], const float* base, int64_t ld, int in, int k0, int kleft) {
+  const int tid = threadIdx.x;
+  const int row = KR ? tid / 16 : tid / 2, ch = KR ? tid % 16 * 8 : tid % 2 * 8;
+  const bool ok = KR ? row < kleft : row < in;
+  const int have = ok ? (KR ? in : kleft) - ch : 0;
+  const float* p = KR ? base + (k0 + row) * ld + ch : base + row * ld + k0 + ch;
+  if (have >= 8) {
+    __builtin_memcpy(w, p, 32);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = j < have ? p[j] : 0.0f;
+  }
+}
+template <bool KR>
+MUON_DEVICE void f32_store(float* lds, const float (&w)[8]) {
+  const int tid = threadIdx.x;
+  if constexpr (KR) {
+    float* p = lds + tid / 16 * F_P + tid % 16 * 8;
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) *(float4*)(p + j) = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) lds[(tid % 2 * 8 + j) * F_P + tid / 2] = w[j];
+  }
+}
+
+template <int FORM>
+__global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
+  constexpr bool KRA = FORM == WGT, KRB = FORM != FWD;
+  __shared__ __align__(16) float lds[2][2][F_K * F_P];
+  int e, tm, tn, row0 = 0, left = 0, K, M;
+  if constexpr (FORM == WGT) {
+    const int per = g.tiles_m * g.tiles_n, L = xcd_range(blockIdx.x, gridDim.x);
+    e = L / per;
+    tile_of(L - e * per, g.tiles_m, g.tiles_n, tm, tn);
+    bounds(g, e, row0, K);
+    M = std::min(g.M - tm * F_B, F_B);
+  } else {
+    if (!find_tile<F_B>(g, blockIdx.x, e, row0, left, tn)) return;
+    M = std::min(left, F_B);
+    K = e < g.E ? g.K : 0;
+    tm = 0;
+  }
+  const int N = std::min(g.N - tn * F_B, F_B);
+  const float* A = (const float*)g.a + (int64_t)row0 * g.lda + (FORM == WGT ? tm * F_B : 0);
+  const float* B = (const float*)g.b;
+  if constexpr (FORM == FWD) B += e * g.sb + (int64_t)tn * F_B * g.ldb;
+  if constexpr (FORM == ROWS) B += e * g.sb + tn * F_B;
+  if constexpr (FORM == WGT) B += (int64_t)row0 * g.ldb + tn * F_B;
+
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave & 1, wn = wave >> 1;
+  const int fr = lane & 31, fk = lane >> 5;
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+  float wa[8], wb[8];
+  const int KT = (K + F_K - 1) / F_K;
+  if (KT) {
+    f32_load<KRA>(wa, A, g.lda, M, 0, K);
+    f32_load<KRB>(wb, B, g.ldb, N, 0, K);
+    f32_store<KRA>(lds[0][0], wa);
+    f32_store<KRB>(lds[0][1], wb);
+  }
+  __syncthreads();
+  for (int kt = 0; kt < KT; ++kt) {
+    const bool more = kt + 1 < KT;
+    if (more) {
+      f32_load<KRA>(wa, A, g.lda, M, (kt + 1) * F_K, K - (kt + 1) * F_K);
+      f32_load<KRB>(wb, B, g.ldb, N, (kt + 1) * F_K, K - (kt + 1) * F_K);
+    }
+    const float* la = lds[kt & 1][0] + wm * 64 + fr;
+    const float* lb = lds[kt & 1][1] + wn * 64 + fr;
+#pragma unroll
+    for (int k = 0; k < F_K; k += 2) {
+      float fa[2], fb[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fa[i] = la[(k + fk) * F_P + i * 32];
+        fb[i] = lb[(k + fk) * F_P + i * 32];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j], fa[i], acc[i][j], 0, 0, 0);
+    }
+    if (more) {
+      f32_store<KRA>(lds[(kt + 1) & 1][0], wa);
+      f32_store<KRB>(lds[(kt + 1) & 1][1], wb);
+    }
+    __syncthreads();
+  }
+  // a lane holds row fr, columns 8 (q / 4) + 4 fk + q % 4 of each 32 x 32 block
+  float* C = (float*)g.c + (FORM == WGT ? ((int64_t)e * g.M + tm * F_B) * g.N : (int64_t)row0 * g.N);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int m = wm * 64 + i * 32 + fr;
+    if (m >= M) continue;
+    float* out = C + (int64_t)m * g.N + tn * F_B;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = wn * 64 + j * 32 + q * 8 + fk * 4;
+        if (n + 4 <= N) {
+          const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          __builtin_memcpy(out + n, v, 16);
+        } else {
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+            if (n + p < N) out[n + p] = acc[i][j][4 * q + p];
+        }
+      }
+  }
+}
+
+// ---- launch ---------------------------------------------------------------------------------
+
+// The most tiles of bm rows that R rows of E experts, and what lies behind them, can make.
+int64_t most_tiles(int64_t R, int64_t E, int bm) { return R / bm + std::min(R, E + 1); }
+
+template <int DT, int FORM, int BM, int BN, int WM, int WN>
+int launch16(GArgs g, bool aligned, hipStream_t s) {
+  g.tiles_m = (int)(FORM == WGT ? (g.M + BM - 1) / BM : most_tiles(g.R, g.E, BM));
+  g.tiles_n = (g.N + BN - 1) / BN;
+  const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * (FORM == WGT ? g.E : 1);
+  if (grid > INT32_MAX) {
+    muon_set_error("muon_expert_linear: too many tiles");
+    return MUON_ERR_SHAPE;
+  }
+  constexpr int LDS = 2 * (BM + BN) * BK * 2;
+  auto run = [&](auto* kernel) {
+    if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {
+      muon_set_error("muon_expert_linear: %d bytes of LDS refused", LDS);
+      return MUON_ERR_LAUNCH;
+    }
+    kernel<<<(unsigned)grid, 64 * WM * WN, LDS, s>>>(g);
+    MUON_CHECK_LAUNCH("muon_expert_linear");
+    return MUON_OK;
+  };
+  return aligned ? run(expert_gemm_kernel<DT, FORM, BM, BN, WM, WN, true>)
+                 : run(expert_gemm_kernel<DT, FORM, BM, BN, WM, WN, false>);
+}
+
+template <int FORM>
+int launch32(GArgs g, hipStream_t s) {
+  g.tiles_m = (int)(FORM == WGT ? (g.M + F_B - 1) / F_B : most_tiles(g.R, g.E, F_B));
+  g.tiles_n = (g.N + F_B - 1) / F_B;
+  const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * (FORM == WGT ? g.E : 1);
+  if (grid > INT32_MAX) {
+    muon_set_error("muon_expert_linear: too many tiles");
+    return MUON_ERR_SHAPE;
+  }
+  expert_gemm_f32_kernel<FORM><<<(unsigned)grid, 256, 0, s>>>(g);
+  MUON_CHECK_LAUNCH("muon_expert_linear");
+  return MUON_OK;
+}
+
+template <int FORM>
+int launch(const GArgs& g, int dtype, hipStream_t s) {
+  if (dtype == MUON_DT_F32) return launch32<FORM>(g, s);
+  const bool aligned = ((uintptr_t)g.a | (uintptr_t)g.b | (uintptr_t)g.c) % 16 == 0 &&
+                       (g.lda | g.ldb | g.sb | g.N | g.K | g.M) % 8 == 0;
+  return dtype == MUON_DT_BF16 ? launch16<MUON_DT_BF16, FORM, 256, 256, 4, 2>(g, aligned, s)
+                               : launch16<MUON_DT_F16, FORM, 256, 256, 4, 2>(g, aligned, s);
+}
+
+int check_shapes(const char* what, int dtype, int64_t rows, int64_t experts, int64_t out, int64_t in) {
+  if (dtype != MUON_DT_F32 && dtype != MUON_DT_BF16 && dtype != MUON_DT_F16) {
+    muon_set_error("%s: unsupported dtype %d", what, dtype);
+    return MUON_ERR_DTYPE;
+  }
+  if (rows < 0 || rows > INT32_MAX || experts < 1 || experts > 1024 || out < 0 || in < 0 ||
+      out > (1 << 24) || in > (1 << 24)) {
+    muon_set_error("%s: %lld rows of %lld experts, %lld x %lld: below 2^31 rows, 1 to 1024 experts and "
+                   "extents to 2^24", what, (long long)rows, (long long)experts, (long long)out, (long long)in);
+    return MUON_ERR_SHAPE;
+  }
+  return MUON_OK;
+}
+
+}  // namespace
+
+extern "C" int muon_expert_linear(const void* rows, int dtype, int64_t row_stride, int64_t nrows,
+                                  int64_t experts, int64_t out, int64_t in, const void* weight,
+                                  const int32_t* offsets, void* y, void* stream) {
+  if (int rc = check_shapes("muon_expert_linear", dtype, nrows, experts, out, in)) return rc;
+  if (!nrows || !out) return MUON_OK;
+  if (!offsets || !y || (in && (!rows || !weight))) {
+    muon_set_error("muon_expert_linear: null pointer");
+    return MUON_ERR_ARG;
+  }
+  GArgs g{rows, weight, y, row_stride, in, out * in, offsets, nrows, (int)experts, (int)out, (int)in, 0, 0, 0};
+  return launch<FWD>(g, dtype, (hipStream_t)stream);
+}
+
+extern "C" int muon_expert_linear_backward_rows(const void* dy, int dtype, int64_t dy_stride,
+                                                int64_t nrows, int64_t experts, int64_t out, int64_t in,
+                                                const void* weight, const int32_t* offsets,
+                                                void* drows, void* stream) {
+  if (int rc = check_shapes("muon_expert_linear_backward_rows", dtype, nrows, experts, out, in)) return rc;
+  if (!nrows || !in) return MUON_OK;
+  if (!offsets || !drows || (out && (!dy || !weight))) {
+    muon_set_error("muon_expert_linear_backward_rows: null pointer");
+    return MUON_ERR_ARG;
+  }
+  GArgs g{dy, weight, drows, dy_stride, in, out * in, offsets, nrows, (int)experts, (int)in, (int)out, 0, 0, 0};
+  return launch<ROWS>(g, dtype, (hipStream_t)stream);
+}
+
+extern "C" int muon_expert_linear_backward_weight(const void* dy, int dtype, int64_t dy_stride,
+                                                  const void* rows, int64_t row_stride, int64_t nrows,
+                                                  int64_t experts, int64_t out, int64_t in,
+                                                  const int32_t* offsets, void* dweight, void* stream) {
+  if (int rc = check_shapes("muon_expert_linear_backward_weight", dtype, nrows, experts, out, in)) return rc;
+  if (!out || !in) return MUON_OK;
+  if (!offsets || !dweight || (nrows && (!dy || !rows))) {
+    muon_set_error("muon_expert_linear_backward_weight: null pointer");
+    return MUON_ERR_ARG;
+  }
+  GArgs g{dy, rows, dweight, dy_stride, row_stride, 0, offsets, nrows, (int)experts, (int)in, 0, (int)out, 0, 0};
+  return launch<WGT>(g, dtype, (hipStream_t)stream);
+}

@@ -1,0 +1,433 @@
+// Tokens to their experts and back (muon_expert_order, muon_dispatch, muon_combine and the latter's
+// gradient): the order of the (token, choice) pairs by expert, each token's row at the places of its
+// choices, and the sum of the experts' rows with the token's gates.
+//
+// The order is a stable counting sort of the choices by expert; what names no expert comes last:
+//   slot(t, j) = choices of lower experts + earlier choices of the same one       (row of the choice)
+//   slot(t, j) = -1 - row for an empty choice, row = kept choices + earlier empty ones.
+// So every row of the sorted order belongs to one choice, and who writes all choices has written all
+// rows. With s = slot(t, j):
+//   dispatch: rows[s] = x[t], 0 for an empty choice      gradient: dx[t] = sum_j drows[s]  (combine, no gates)
+//   combine:  y[t] = sum_j g_tj rows[s] over the kept ones
+//   gradient: drows[s] = g_tj dy[t], 0 for an empty one;  dg_tj = <dy[t], rows[s]>.
+//
+// All of it moves bytes. The work is laid out by tokens: a token's row is read once for all its
+// choices, and their rows are whole lines wherever they lie.
+#include <algorithm>
+
+#include "rowops.h"
+
+namespace {
+
+constexpr int ORDER_THREADS = 512;
+constexpr int ORDER_WAVES = ORDER_THREADS / 64;
+constexpr int ORDER_EMAX = 1024;
+// Choices that one workgroup orders alone: two walks over 1024 choices a wave take less than the
+// second launch.
+constexpr int64_t ORDER_ALONE = 8192;
+constexpr int64_t ORDER_CHUNK = 2048;
+constexpr int64_t ORDER_BLOCKS = 256;
+
+struct OrderArgs {
+  const int64_t* experts;
+  int64_t n, chunk;  // choices, and those of a workgroup (a multiple of 64 ORDER_WAVES)
+  int E, blocks;
+  int32_t* slots;
+  int32_t* offsets;
+  int32_t* counts;  // (blocks, E + 1): choices of each expert, and empty ones, by workgroup
+};
+
+MUON_DEVICE int expert_of(const OrderArgs& a, int64_t i) {
+  const int64_t e = a.experts[i];
+  return e >= 0 && e < a.E ? (int)e : a.E;
+}
+
+__global__ __launch_bounds__(ORDER_THREADS) void order_count_kernel(OrderArgs a) {
+  __shared__ int32_t cnt[ORDER_EMAX + 1];
+  const int tid = threadIdx.x;
+  for (int c = tid; c <= a.E; c += ORDER_THREADS) cnt[c] = 0;
+  __syncthreads();
+  const int64_t begin = blockIdx.x * a.chunk, end = std::min(begin + a.chunk, a.n);
+  for (int64_t i = begin + tid; i < end; i += ORDER_THREADS) atomicAdd(&cnt[expert_of(a, i)], 1);
+  __syncthreads();
+  for (int c = tid; c <= a.E; c += ORDER_THREADS)
+    a.counts[(int64_t)blockIdx.x * (a.E + 1) + c] = cnt[c];
+}
+
+// A workgroup's choices in order: each wave a run of them. First the counts by wave, from which each
+// wave's first place for every expert follows; then 64 choices at a time, a lane's place among the
+// lanes of its expert from one ballot for each bit of the number.
+__global__ __launch_bounds__(ORDER_THREADS) void order_place_kernel(OrderArgs a) {
+  extern __shared__ int32_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, C = a.E + 1;
+  int32_t* cnt = lds;                      // (waves, C)
+  int32_t* before = lds + ORDER_WAVES * C;  // (C): choices of the workgroups before this one
+  int32_t* total = before + C;              // (C): of all, then the experts' first rows
+  __shared__ int32_t wave_sum[ORDER_WAVES];
+  for (int c = tid; c < (ORDER_WAVES + 2) * C; c += ORDER_THREADS) lds[c] = 0;
+  __syncthreads();
+  const int64_t run = a.chunk / ORDER_WAVES;
+  const int64_t begin = blockIdx.x * a.chunk + wave * run;
+  const int64_t end = std::min(begin + run, a.n);
+  for (int64_t i = begin + lane; i < end; i += 64) atomicAdd(&cnt[wave * C + expert_of(a, i)], 1);
+  if (a.blocks > 1) {
+    const int all = a.blocks * C, mine = blockIdx.x * C;
+#pragma unroll 8
+    for (int i = tid; i < all; i += ORDER_THREADS) {
+      const int v = a.counts[i], c = i % C;
+      if (v) {
+        atomicAdd(&total[c], v);
+        if (i < mine) atomicAdd(&before[c], v);
+      }
+    }
+    __syncthreads();
+  } else {
+    __syncthreads();
+    for (int c = tid; c < C; c += ORDER_THREADS) {
+      int sum = 0;
+#pragma unroll
+      for (int w = 0; w < ORDER_WAVES; ++w) sum += cnt[w * C + c];
+      total[c] = sum;
+    }
+    __syncthreads();
+  }
+  // exclusive sums of the totals: a few experts in a row for each thread
+  const int per = (C + ORDER_THREADS - 1) / ORDER_THREADS, c0 = tid * per;
+  int sum = 0;
+  for (int c = c0; c < std::min(c0 + per, C); ++c) sum += total[c];
+  int incl = sum;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int v = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += v;
+  }
+  if (lane == 63) wave_sum[wave] = incl;
+  __syncthreads();
+  int first = incl - sum;
+  for (int w = 0; w < wave; ++w) first += wave_sum[w];
+  for (int c = c0; c < std::min(c0 + per, C); ++c) {
+    const int t = total[c];
+    if (blockIdx.x == 0) a.offsets[c] = first;
+    int place = first + before[c];
+    for (int w = 0; w < ORDER_WAVES; ++w) {
+      const int k = cnt[w * C + c];
+      cnt[w * C + c] = place;
+      place += k;
+    }
+    first += t;
+  }
+  __syncthreads();
+  const int bits = 32 - __builtin_clz(a.E | 1);
+  const uint64_t below = (1ull << lane) - 1;
+  for (int64_t i0 = begin; i0 < end; i0 += 64) {
+    const int64_t i = i0 + lane;
+    const bool in = i < end;
+    const int e = in ? expert_of(a, i) : 0;
+    uint64_t same = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t ones = __ballot(in && ((e >> b) & 1));
+      same &= ((e >> b) & 1) ? ones : ~ones;
+    }
+    const int rank = __popcll(same & below);
+    int place = 0;
+    if (in && rank == 0) place = atomicAdd(&cnt[wave * C + e], (int)__popcll(same));
+    place = __shfl(place, in ? __builtin_ctzll(same) : lane, 64) + rank;
+    if (in) a.slots[i] = e < a.E ? place : -1 - place;
+  }
+}
+
+// ---- rows -----------------------------------------------------------------------------------
+
+constexpr int ROW_THREADS = 256;
+
+struct RowArgs {
+  const void* in;  // dispatch: a token's rows; combine: the experts' rows
+  int64_t in_row;  // their stride in elements
+  int64_t T, R;    // tokens; rows of the sorted order
+  int k, W;
+  int shift;       // log2 of the lanes of a token (one workgroup's threads at most)
+  const int32_t* slots;
+  const float* gates;  // or null: ones
+  void* out;           // contiguous
+};
+
+// Columns c .. c + N - 1 of a row that ends at W (c < W): one access, or single values at its end.
+template <int DT>
+MUON_DEVICE muon_u4 load_part(const void* p, int64_t at, int left) {
+  constexpr int N = Vec16<DT>::N;
+  if (left >= N) return load_u4(elem_at<DT>(p, at));
+  float v[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = j < left ? Elem<DT>::load(p, at + j) : 0.0f;
+  return Vec16<DT>::pack(v);
+}
+template <int DT>
+MUON_DEVICE void store_part(void* p, int64_t at, int left, muon_u4 w) {
+  constexpr int N = Vec16<DT>::N;
+  if (left >= N) {
+    store_u4((void*)elem_at<DT>(p, at), w);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (j >= left) break;
+    if constexpr (DT == MUON_DT_F32)
+      ((uint32_t*)p)[at + j] = w[j];
+    else
+      ((uint16_t*)p)[at + j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(ROW_THREADS) void dispatch_kernel(RowArgs a) {
+  constexpr int N = Vec16<DT>::N;
+  const int lanes = 1 << a.shift, v0 = threadIdx.x & (lanes - 1);
+  const int64_t t = (int64_t)blockIdx.x * (ROW_THREADS >> a.shift) + (threadIdx.x >> a.shift);
+  if (t >= a.T) return;
+  const int32_t* slots = a.slots + t * a.k;
+  for (int c = v0 * N; c < a.W; c += lanes * N) {
+    const int left = a.W - c;
+    const muon_u4 w = load_part<DT>(a.in, t * a.in_row + c, left);
+    for (int j = 0; j < a.k; ++j) {
+      const int s = slots[j], row = s < 0 ? ~s : s;
+      if (row < a.R) store_part<DT>(a.out, (int64_t)row * a.W + c, left, s < 0 ? muon_u4{0, 0, 0, 0} : w);
+    }
+  }
+}
+
+constexpr int BATCH = 8;  // choices whose rows are in flight together
+
+template <int DT>
+__global__ __launch_bounds__(ROW_THREADS) void combine_kernel(RowArgs a) {
+  constexpr int N = Vec16<DT>::N;
+  const int lanes = 1 << a.shift, v0 = threadIdx.x & (lanes - 1);
+  const int64_t t = (int64_t)blockIdx.x * (ROW_THREADS >> a.shift) + (threadIdx.x >> a.shift);
+  if (t >= a.T) return;
+  for (int c = v0 * N; c < a.W; c += lanes * N) {
+    const int left = a.W - c;
+    float sum[N] = {};
+    for (int j0 = 0; j0 < a.k; j0 += BATCH) {
+      muon_u4 w[BATCH];
+      float g[BATCH];
+      bool kept[BATCH];
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        const int j = j0 + b;
+        const int s = j < a.k ? a.slots[t * a.k + j] : -1;
+        kept[b] = s >= 0 && s < a.R;
+        if (kept[b]) {
+          g[b] = a.gates ? a.gates[t * a.k + j] : 1.0f;
+          w[b] = load_part<DT>(a.in, (int64_t)s * a.in_row + c, left);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        if (!kept[b]) continue;
+        float v[N];
+        Vec16<DT>::unpack(w[b], v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] += g[b] * v[e];
+      }
+    }
+    store_part<DT>(a.out, t * a.W + c, left, Vec16<DT>::pack(sum));
+  }
+}
+
+struct BackArgs {
+  const void* dy;
+  const void* rows;
+  int64_t dy_row, rows_row;
+  int64_t T, R;
+  int k, W;
+  const int32_t* slots;
+  const float* gates;
+  void* drows;    // contiguous, or null
+  float* dgates;  // or null
+};
+
+// G lanes a token (a wave at most): the products of a choice's row are summed by each lane over its
+// columns, then over the lanes.
+template <int DT, int G>
+__global__ __launch_bounds__(ROW_THREADS) void combine_backward_kernel(BackArgs a) {
+  constexpr int N = Vec16<DT>::N;
+  const int v0 = threadIdx.x & (G - 1);
+  const int64_t t = (int64_t)blockIdx.x * (ROW_THREADS / G) + threadIdx.x / G;
+  if (t >= a.T) return;  // whole groups of lanes
+  for (int j0 = 0; j0 < a.k; j0 += BATCH) {
+    int s[BATCH];
+    float g[BATCH], dot[BATCH] = {};
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int j = j0 + b;
+      s[b] = j < a.k ? a.slots[t * a.k + j] : INT32_MAX;  // no row: R is at most that
+      g[b] = s[b] >= 0 && s[b] < a.R ? a.gates[t * a.k + j] : 0.0f;
+    }
+    for (int c = v0 * N; c < a.W; c += G * N) {
+      const int left = a.W - c;
+      float d[N];
+      Vec16<DT>::unpack(load_part<DT>(a.dy, t * a.dy_row + c, left), d);
+      if (a.dgates) {
+        muon_u4 w[BATCH];
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+          if (s[b] >= 0 && s[b] < a.R) w[b] = load_part<DT>(a.rows, (int64_t)s[b] * a.rows_row + c, left);
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+          if (!(s[b] >= 0 && s[b] < a.R)) continue;
+          float v[N];
+          Vec16<DT>::unpack(w[b], v);
+#pragma unroll
+          for (int e = 0; e < N; ++e) dot[b] += d[e] * v[e];
+        }
+      }
+      if (a.drows) {
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+          const int row = s[b] < 0 ? ~s[b] : s[b];
+          if (row >= a.R) continue;
+          float v[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[e] = s[b] < 0 ? 0.0f : g[b] * d[e];
+          store_part<DT>(a.drows, (int64_t)row * a.W + c, left, Vec16<DT>::pack(v));
+        }
+      }
+    }
+    if (a.dgates) {
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        const float sum = group_sum<G>(dot[b]);
+        if (v0 == 0 && j0 + b < a.k) a.dgates[t * a.k + j0 + b] = sum;
+      }
+    }
+  }
+}
+
+int lanes_shift(int dtype, int64_t width, int most) {
+  const int64_t runs = (width + (dtype == MUON_DT_F32 ? 3 : 7)) / (dtype == MUON_DT_F32 ? 4 : 8);
+  int shift = 0;
+  while (shift < most && (1ll << shift) < runs) ++shift;
+  return shift;
+}
+
+int64_t order_chunk(int64_t n) {
+  if (n <= ORDER_ALONE) return round_up(std::max<int64_t>(n, 1), ORDER_THREADS);
+  return std::max(ORDER_CHUNK, round_up((n + ORDER_BLOCKS - 1) / ORDER_BLOCKS, ORDER_THREADS));
+}
+int64_t order_blocks(int64_t n) { return std::max<int64_t>(1, (n + order_chunk(n) - 1) / order_chunk(n)); }
+
+bool fine_dtype(int dtype) { return dtype == MUON_DT_F32 || dtype == MUON_DT_BF16 || dtype == MUON_DT_F16; }
+
+// What the row kernels index by 32 bits: slots, columns, and workgroups.
+int check_rows(const char* what, int dtype, int64_t tokens, int64_t top, int64_t width) {
+  if (!fine_dtype(dtype)) {
+    muon_set_error("%s: unsupported dtype %d", what, dtype);
+    return MUON_ERR_DTYPE;
+  }
+  if (tokens < 0 || top < 1 || width < 0 || width > (1 << 30) || top > INT32_MAX ||
+      (tokens && top > INT32_MAX / tokens)) {
+    muon_set_error("%s: %lld tokens of %lld choices, width %lld: choices have to stay below 2^31 and the "
+                   "width up to 2^30", what, (long long)tokens, (long long)top, (long long)width);
+    return MUON_ERR_SHAPE;
+  }
+  return MUON_OK;
+}
+
+}  // namespace
+
+#define BY_TYPE(CALL)                                       \
+  switch (dtype) {                                          \
+    case MUON_DT_F32: { constexpr int DT = MUON_DT_F32; CALL; break; }   \
+    case MUON_DT_BF16: { constexpr int DT = MUON_DT_BF16; CALL; break; } \
+    default: { constexpr int DT = MUON_DT_F16; CALL; }                   \
+  }
+
+extern "C" int64_t muon_expert_order_workspace_bytes(int64_t choices, int64_t experts) {
+  if (choices < 0 || experts < 1) return 0;
+  const int64_t blocks = order_blocks(choices);
+  return blocks > 1 ? blocks * (experts + 1) * 4 : 0;
+}
+
+extern "C" int muon_expert_order(const int64_t* experts, int64_t choices, int64_t nexperts,
+                                 int32_t* slots, int32_t* offsets, void* ws, void* stream) {
+  if (choices < 0 || choices > INT32_MAX || nexperts < 1 || nexperts > ORDER_EMAX) {
+    muon_set_error("muon_expert_order: %lld choices of %lld experts: below 2^31 of at most %d",
+                   (long long)choices, (long long)nexperts, ORDER_EMAX);
+    return MUON_ERR_SHAPE;
+  }
+  if (!offsets || (choices && (!experts || !slots)) ||
+      (muon_expert_order_workspace_bytes(choices, nexperts) && !ws)) {
+    muon_set_error("muon_expert_order: null pointer");
+    return MUON_ERR_ARG;
+  }
+  OrderArgs a{experts, choices, order_chunk(choices), (int)nexperts, (int)order_blocks(choices),
+              slots, offsets, (int32_t*)ws};
+  hipStream_t s = (hipStream_t)stream;
+  if (a.blocks > 1) {
+    order_count_kernel<<<a.blocks, ORDER_THREADS, 0, s>>>(a);
+    MUON_CHECK_LAUNCH("muon_expert_order: count");
+  }
+  const int lds = (ORDER_WAVES + 2) * ((int)nexperts + 1) * 4;
+  order_place_kernel<<<a.blocks, ORDER_THREADS, lds, s>>>(a);
+  MUON_CHECK_LAUNCH("muon_expert_order: place");
+  return MUON_OK;
+}
+
+extern "C" int muon_dispatch(const void* x, int dtype, int64_t row_stride, int64_t tokens, int64_t top,
+                             int64_t width, const int32_t* slots, void* rows, void* stream) {
+  if (int rc = check_rows("muon_dispatch", dtype, tokens, top, width)) return rc;
+  if (!tokens || !width) return MUON_OK;
+  if (!x || !slots || !rows) {
+    muon_set_error("muon_dispatch: null pointer");
+    return MUON_ERR_ARG;
+  }
+  RowArgs a{x, row_stride, tokens, tokens * top, (int)top, (int)width, lanes_shift(dtype, width, 8),
+            slots, nullptr, rows};
+  const int64_t grid = (tokens + (ROW_THREADS >> a.shift) - 1) / (ROW_THREADS >> a.shift);
+  BY_TYPE((dispatch_kernel<DT><<<(unsigned)grid, ROW_THREADS, 0, (hipStream_t)stream>>>(a)))
+  MUON_CHECK_LAUNCH("muon_dispatch");
+  return MUON_OK;
+}
+
+extern "C" int muon_combine(const void* rows, int dtype, int64_t row_stride, int64_t tokens, int64_t top,
+                            int64_t width, const int32_t* slots, const float* gates, void* y,
+                            void* stream) {
+  if (int rc = check_rows("muon_combine", dtype, tokens, top, width)) return rc;
+  if (!tokens || !width) return MUON_OK;
+  if (!rows || !slots || !y) {
+    muon_set_error("muon_combine: null pointer");
+    return MUON_ERR_ARG;
+  }
+  RowArgs a{rows, row_stride, tokens, tokens * top, (int)top, (int)width, lanes_shift(dtype, width, 8),
+            slots, gates, y};
+  const int64_t grid = (tokens + (ROW_THREADS >> a.shift) - 1) / (ROW_THREADS >> a.shift);
+  BY_TYPE((combine_kernel<DT><<<(unsigned)grid, ROW_THREADS, 0, (hipStream_t)stream>>>(a)))
+  MUON_CHECK_LAUNCH("muon_combine");
+  return MUON_OK;
+}
+
+extern "C" int muon_combine_backward(const void* dy, int64_t dy_stride, const void* rows,
+                                     int64_t row_stride, int dtype, int64_t tokens, int64_t top,
+                                     int64_t width, const int32_t* slots, const float* gates,
+                                     void* drows, float* dgates, void* stream) {
+  if (int rc = check_rows("muon_combine_backward", dtype, tokens, top, width)) return rc;
+  if (!tokens || (!drows && !dgates)) return MUON_OK;
+  if (!slots || !gates || (width && (!dy || (dgates && !rows)))) {
+    muon_set_error("muon_combine_backward: null pointer");
+    return MUON_ERR_ARG;
+  }
+  BackArgs a{dy, rows, dy_stride, row_stride, tokens, tokens * top, (int)top, (int)width,
+             slots, gates, drows, dgates};
+  const int shift = std::max(3, lanes_shift(dtype, width, 6));
+  const int64_t grid = (tokens + (ROW_THREADS >> shift) - 1) / (ROW_THREADS >> shift);
+  hipStream_t s = (hipStream_t)stream;
+#define BACK(G) BY_TYPE((combine_backward_kernel<DT, G><<<(unsigned)grid, ROW_THREADS, 0, s>>>(a)))
+  switch (shift) {
+    case 3: BACK(8) break;
+    case 4: BACK(16) break;
+    case 5: BACK(32) break;
+    default: BACK(64)
+  }
+#undef BACK
+  MUON_CHECK_LAUNCH("muon_combine_backward");
+  return MUON_OK;
+}

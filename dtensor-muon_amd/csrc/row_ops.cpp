@@ -346,8 +346,176 @@ void policy_rescale(const Tensor& dlogits, const Tensor& dloss, const Tensor& lo
         "muon_policy_loss_rescale");
 }
 
-// ---- gradients --------------------------------------------------------------------------
+// ---- experts ------------------------------------------------------------------------------
 
+Tensor2 order_forward(const Tensor& experts, int64_t nexperts) {
+  const at::DeviceGuard guard(experts.device());
+  const int64_t n = experts.numel();
+  const Tensor ids = plain(experts, experts, at::kLong, n, "the experts");
+  Tensor slots = empty(experts, experts.sizes(), at::kInt);
+  Tensor offsets = empty(experts, {nexperts + 1}, at::kInt);
+  const int64_t bytes = muon_expert_order_workspace_bytes(n, nexperts);
+  Tensor ws = bytes ? scratch(experts, bytes) : Tensor();
+  check(muon_expert_order(ptr<int64_t>(ids), n, nexperts, ptr<int32_t>(slots), ptr<int32_t>(offsets),
+                          bytes ? ptr(ws) : nullptr, stream_of(experts)),
+        "muon_expert_order");
+  return {slots, offsets};
+}
+
+// (tokens, choices) slots of what is routed.
+Tensor slots_of(const Tensor& slots, const Tensor& like) {
+  TORCH_CHECK(slots.dim() == 2, "muonium_amd: slots have to be (tokens, choices); got ", slots.sizes());
+  return plain(slots, like, at::kInt, slots.numel(), "the slots");
+}
+
+Tensor dispatch_forward(const Tensor& x_, const Tensor& slots_) {
+  const at::DeviceGuard guard(x_.device());
+  const Tensor x = rows_of(x_), slots = slots_of(slots_, x_);
+  TORCH_CHECK(slots.size(0) == x.size(0), "muonium_amd: slots of ", slots.size(0), " tokens for ",
+              x.size(0));
+  Tensor rows = empty(x, {slots.numel(), x.size(1)}, x.scalar_type());
+  check(muon_dispatch(ptr(x), dtype_code(x), x.stride(0), x.size(0), slots.size(1), x.size(1),
+                      ptr<int32_t>(slots), ptr(rows), stream_of(x)),
+        "muon_dispatch");
+  return rows;
+}
+
+Tensor combine_forward(const Tensor& rows_, const Tensor& slots_, const optional<Tensor>& gates_) {
+  const at::DeviceGuard guard(rows_.device());
+  const Tensor rows = rows_of(rows_), slots = slots_of(slots_, rows_);
+  TORCH_CHECK(rows.size(0) == slots.numel(), "muonium_amd: ", rows.size(0), " rows for ",
+              slots.numel(), " choices");
+  const auto gates = plain(gates_, rows, at::kFloat, slots.numel(), "the gates");
+  Tensor y = empty(rows, {slots.size(0), rows.size(1)}, rows.scalar_type());
+  check(muon_combine(ptr(rows), dtype_code(rows), rows.stride(0), slots.size(0), slots.size(1),
+                     rows.size(1), ptr<int32_t>(slots), ptr<float>(gates), ptr(y), stream_of(rows)),
+        "muon_combine");
+  return y;
+}
+
+// Gradients that are not asked for come back empty.
+Tensor2 combine_backward(const Tensor& dy_, const Tensor& rows_, const Tensor& slots_,
+                         const Tensor& gates_, bool rows_wanted, bool gates_wanted) {
+  const at::DeviceGuard guard(rows_.device());
+  const Tensor rows = rows_of(rows_), slots = slots_of(slots_, rows_), dy = rows_of(dy_);
+  TORCH_CHECK(rows.size(0) == slots.numel() && dy.size(0) == slots.size(0) &&
+                  dy.size(1) == rows.size(1) && dy.scalar_type() == rows.scalar_type() &&
+                  dy.device() == rows.device(),
+              "muonium_amd: the gradient is not like its output");
+  const Tensor gates = plain(gates_, rows, at::kFloat, slots.numel(), "the gates");
+  Tensor drows = rows_wanted ? fresh(rows) : empty(rows, {0}, rows.scalar_type());
+  Tensor dgates = gates_wanted ? empty(rows, slots.sizes(), at::kFloat) : empty(rows, {0}, at::kFloat);
+  check(muon_combine_backward(ptr(dy), dy.stride(0), ptr(rows), rows.stride(0), dtype_code(rows),
+                              slots.size(0), slots.size(1), rows.size(1), ptr<int32_t>(slots),
+                              ptr<float>(gates), rows_wanted ? ptr(drows) : nullptr,
+                              gates_wanted ? ptr<float>(dgates) : nullptr, stream_of(rows)),
+        "muon_combine_backward");
+  return {drows, dgates};
+}
+
+// The weights and offsets of a product, and what belongs together.
+struct Experts {
+  Tensor weight, offsets;
+  int64_t n, out, in;
+
+  Experts(const Tensor& like, const Tensor& weight_, const Tensor& offsets_) {
+    TORCH_CHECK(weight_.dim() == 3 && weight_.scalar_type() == like.scalar_type() &&
+                    weight_.device() == like.device(),
+                "muonium_amd: weights have to be (experts, out, in) of the rows' type beside them");
+    weight = weight_.contiguous();
+    n = weight.size(0);
+    out = weight.size(1);
+    in = weight.size(2);
+    offsets = plain(offsets_, like, at::kInt, n + 1, "the offsets");
+  }
+};
+
+Tensor linear_forward(const Tensor& rows_, const Tensor& weight, const Tensor& offsets) {
+  const at::DeviceGuard guard(rows_.device());
+  const Tensor rows = rows_of(rows_);
+  const Experts e(rows, weight, offsets);
+  TORCH_CHECK(rows.size(1) == e.in, "muonium_amd: rows of ", rows.size(1), " values for weights of ", e.in);
+  Tensor y = empty(rows, {rows.size(0), e.out}, rows.scalar_type());
+  check(muon_expert_linear(ptr(rows), dtype_code(rows), rows.stride(0), rows.size(0), e.n, e.out, e.in,
+                           ptr(e.weight), ptr<int32_t>(e.offsets), ptr(y), stream_of(rows)),
+        "muon_expert_linear");
+  return y;
+}
+
+Tensor linear_backward_rows(const Tensor& dy_, const Tensor& weight, const Tensor& offsets) {
+  const at::DeviceGuard guard(dy_.device());
+  const Tensor dy = rows_of(dy_);
+  const Experts e(dy, weight, offsets);
+  TORCH_CHECK(dy.size(1) == e.out, "muonium_amd: the gradient is not like its output");
+  Tensor drows = empty(dy, {dy.size(0), e.in}, dy.scalar_type());
+  check(muon_expert_linear_backward_rows(ptr(dy), dtype_code(dy), dy.stride(0), dy.size(0), e.n, e.out,
+                                         e.in, ptr(e.weight), ptr<int32_t>(e.offsets), ptr(drows),
+                                         stream_of(dy)),
+        "muon_expert_linear_backward_rows");
+  return drows;
+}
+
+Tensor linear_backward_weight(const Tensor& dy_, const Tensor& rows_, const Tensor& offsets_) {
+  const at::DeviceGuard guard(dy_.device());
+  const Tensor dy = rows_of(dy_), rows = rows_of(rows_);
+  TORCH_CHECK(dy.size(0) == rows.size(0) && dy.scalar_type() == rows.scalar_type() &&
+                  dy.device() == rows.device() && offsets_.numel() > 1,
+              "muonium_amd: the gradient is not like its output");
+  const int64_t n = offsets_.numel() - 1;
+  const Tensor offsets = plain(offsets_, rows, at::kInt, n + 1, "the offsets");
+  Tensor dweight = empty(rows, {n, dy.size(1), rows.size(1)}, rows.scalar_type());
+  check(muon_expert_linear_backward_weight(ptr(dy), dtype_code(dy), dy.stride(0), ptr(rows),
+                                           rows.stride(0), rows.size(0), n, dy.size(1), rows.size(1),
+                                           ptr<int32_t>(offsets), ptr(dweight), stream_of(rows)),
+        "muon_expert_linear_backward_weight");
+  return dweight;
+}
+
+// ---- AdamW --------------------------------------------------------------------------------
+
+// One step of all tensors, on one device and of one type; without scales the moments are fp32.
+void adamw(at::TensorList params, at::TensorList grads, at::TensorList avgs, at::TensorList sqs,
+           at::TensorList avg_scales, at::TensorList sq_scales, at::TensorList steps, int64_t block,
+           double lr, double beta1, double beta2, double eps, double weight_decay, bool maximize) {
+  const size_t n = params.size();
+  const bool fp8 = block != 0;
+  TORCH_CHECK(grads.size() == n && avgs.size() == n && sqs.size() == n && steps.size() == n &&
+                  avg_scales.size() == (fp8 ? n : 0) && sq_scales.size() == (fp8 ? n : 0),
+              "muonium_amd: adamw_ takes one gradient, moment and step for each parameter");
+  if (!n) return;
+  const at::DeviceGuard guard(params[0].device());
+  std::vector<MuonAdamTensor> table(n);
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& p = params[i];
+    const int64_t numel = p.numel();
+    TORCH_CHECK(p.scalar_type() == params[0].scalar_type() && p.device() == params[0].device() &&
+                    p.is_non_overlapping_and_dense(),
+                "muonium_amd: adamw_'s parameters have to be dense, of one type and on one device");
+    TORCH_CHECK(grads[i].scalar_type() == p.scalar_type() && grads[i].device() == p.device() &&
+                    grads[i].sizes() == p.sizes() && (numel <= 1 || grads[i].strides() == p.strides()),
+                "muonium_amd: a gradient is not laid out like its parameter");
+    const auto held = [&](const Tensor& t, at::ScalarType type, int64_t count, const char* name) {
+      TORCH_CHECK(t.scalar_type() == type && t.numel() == count && t.device() == p.device() &&
+                      t.is_non_overlapping_and_dense(),
+                  "muonium_amd: ", name, " has to be ", count, " dense values of ", type, " on ", p.device());
+      return t.data_ptr();
+    };
+    table[i] = {p.data_ptr(), grads[i].data_ptr(), held(avgs[i], fp8 ? at::kByte : at::kFloat, numel, "a mean"),
+                held(sqs[i], fp8 ? at::kByte : at::kFloat, numel, "a mean square"),
+                fp8 ? (float*)held(avg_scales[i], at::kFloat, numel / block, "a scale") : nullptr,
+                fp8 ? (float*)held(sq_scales[i], at::kFloat, numel / block, "a scale") : nullptr,
+                (float*)held(steps[i], at::kFloat, 1, "a step"), numel};
+  }
+  Tensor ws = scratch(params[0], muon_adamw_workspace_bytes((int64_t)n));
+  check(muon_adamw((int64_t)n, table.data(), dtype_code(params[0]), block, lr, beta1, beta2, eps,
+                   weight_decay, maximize, ptr(ws), stream_of(params[0])),
+        "muon_adamw");
+  // what saved a parameter for its backward pass finds it changed
+  for (const Tensor& p : params)
+    if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+}
+
+// ---- gradients --------------------------------------------------------------------------
 
 #define OP(name, impl)                                                                \
   [] {                                                                                \
@@ -589,9 +757,106 @@ Tensor4 policy_autograd(const Tensor& logits, const Tensor& tokens, const Tensor
             temperature, keep, one_pass);
 }
 
+struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& slots) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({slots});
+    return {OP("dispatch", dispatch_forward).call(x, slots)};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto s = ctx->get_saved_variables();
+    Tensor d;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      d = OP("combine", combine_forward).call(grads[0], s[0], std::nullopt);
+    }
+    return once({d, Tensor()}, grads);
+  }
+};
+
+Tensor dispatch_autograd(const Tensor& x, const Tensor& slots) {
+  refuse_tangents(x);
+  if (any_needs(x)) return DispatchFunction::apply(x, slots)[0];
+  at::AutoDispatchBelowADInplaceOrView below;
+  return OP("dispatch", dispatch_forward).call(x, slots);
+}
+
+struct CombineFunction : torch::autograd::Function<CombineFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& rows, const Tensor& slots,
+                               const optional<Tensor>& gates) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    // without gates the gradient needs the slots alone
+    ctx->save_for_backward({gates ? rows : Tensor(), slots, or_undefined(gates)});
+    return {OP("combine", combine_forward).call(rows, slots, gates)};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto s = ctx->get_saved_variables();
+    variable_list out(3);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      if (!s[2].defined()) {
+        out[0] = OP("dispatch", dispatch_forward).call(grads[0], s[1]);
+      } else {
+        const bool rows = ctx->needs_input_grad(0), gates = ctx->needs_input_grad(2);
+        auto [drows, dgates] = OP("combine_backward", combine_backward)
+                                   .call(grads[0], s[0], s[1], s[2], rows, gates);
+        if (rows) out[0] = drows;
+        if (gates) out[2] = dgates;
+      }
+    }
+    return once(out, {grads[0], s[0], s[2]});
+  }
+};
+
+Tensor combine_autograd(const Tensor& rows, const Tensor& slots, const optional<Tensor>& gates) {
+  refuse_tangents(rows, gates);
+  if (any_needs(rows, gates)) return CombineFunction::apply(rows, slots, gates)[0];
+  at::AutoDispatchBelowADInplaceOrView below;
+  return OP("combine", combine_forward).call(rows, slots, gates);
+}
+
+struct LinearFunction : torch::autograd::Function<LinearFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weight,
+                               const Tensor& offsets) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({rows, weight, offsets});
+    return {OP("expert_linear", linear_forward).call(rows, weight, offsets)};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto s = ctx->get_saved_variables();
+    variable_list out(3);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      if (ctx->needs_input_grad(0))
+        out[0] = OP("expert_linear_backward_rows", linear_backward_rows).call(grads[0], s[1], s[2]);
+      if (ctx->needs_input_grad(1))
+        out[1] = OP("expert_linear_backward_weight", linear_backward_weight).call(grads[0], s[0], s[2]);
+    }
+    return once(out, {grads[0], s[0], s[1]});
+  }
+};
+
+Tensor linear_autograd(const Tensor& rows, const Tensor& weight, const Tensor& offsets) {
+  refuse_tangents(rows, weight);
+  if (any_needs(rows, weight)) return LinearFunction::apply(rows, weight, offsets)[0];
+  at::AutoDispatchBelowADInplaceOrView below;
+  return OP("expert_linear", linear_forward).call(rows, weight, offsets);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(muonium_amd, m) {
+  m.def("sort_by_expert(Tensor experts, int num_experts) -> (Tensor, Tensor)");
+  m.def("dispatch(Tensor x, Tensor slots) -> Tensor");
+  m.def("combine(Tensor rows, Tensor slots, Tensor? gates) -> Tensor");
+  m.def("combine_backward(Tensor dy, Tensor rows, Tensor slots, Tensor gates, bool rows_wanted, "
+        "bool gates_wanted) -> (Tensor, Tensor)");
+  m.def("expert_linear(Tensor rows, Tensor weight, Tensor offsets) -> Tensor");
+  m.def("expert_linear_backward_rows(Tensor dy, Tensor weight, Tensor offsets) -> Tensor");
+  m.def("expert_linear_backward_weight(Tensor dy, Tensor rows, Tensor offsets) -> Tensor");
+  m.def("adamw_(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, Tensor(c!)[] exp_avg_sqs, "
+        "Tensor(d!)[] avg_scales, Tensor(e!)[] sq_scales, Tensor(f!)[] steps, int block, float lr, "
+        "float beta1, float beta2, float eps, float weight_decay, bool maximize) -> ()");
   m.def("qk_norm_rope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor? cos, "
         "Tensor? sin, Tensor? positions, float eps, bool interleaved) -> (Tensor, Tensor)");
   m.def("qk_norm_rope_backward(Tensor dq_out, Tensor dk_out, Tensor q, Tensor k, "
@@ -624,6 +889,14 @@ TORCH_LIBRARY_IMPL(muonium_amd, CUDA, m) {
   m.impl("policy_loss", policy_forward);
   m.impl("policy_loss_backward", policy_backward);
   m.impl("policy_loss_rescale_", policy_rescale);
+  m.impl("sort_by_expert", order_forward);
+  m.impl("dispatch", dispatch_forward);
+  m.impl("combine", combine_forward);
+  m.impl("combine_backward", combine_backward);
+  m.impl("expert_linear", linear_forward);
+  m.impl("expert_linear_backward_rows", linear_backward_rows);
+  m.impl("expert_linear_backward_weight", linear_backward_weight);
+  m.impl("adamw_", adamw);
 }
 
 TORCH_LIBRARY_IMPL(muonium_amd, AutogradCUDA, m) {
@@ -631,4 +904,7 @@ TORCH_LIBRARY_IMPL(muonium_amd, AutogradCUDA, m) {
   m.impl("route", route_autograd);
   m.impl("token_logprobs", logp_autograd);
   m.impl("policy_loss", policy_autograd);
+  m.impl("dispatch", dispatch_autograd);
+  m.impl("combine", combine_autograd);
+  m.impl("expert_linear", linear_autograd);
 }

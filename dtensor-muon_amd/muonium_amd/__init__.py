@@ -6,6 +6,8 @@ Muon-family step runs hand-written gfx950 kernels from libmuon_amd.so through a 
 """
 
 from .optim import (
+    AdamW,
+    AdamWFp8,
     BufferSpec,
     Muon,
     Muon4bit,
@@ -20,6 +22,8 @@ from .optim import (
 from .orthogonalize import OrthogonalizationStrategy
 
 __all__ = [
+    "AdamW",
+    "AdamWFp8",
     "BufferSpec",
     "Muon",
     "Muon4bit",

@@ -26,6 +26,7 @@ Q_8BIT, Q_4BIT, Q_FP8 = 8, 4, 0
 MAX_TENSORS = 32
 
 _c_int, _c_i64, _c_f32, _vp = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
+_c_f64 = ctypes.c_double
 _pp = ctypes.POINTER(ctypes.c_void_p)
 _SIGNATURES = {
     "muon_amd_abi_version": (_c_int, []),
@@ -142,6 +143,29 @@ _SIGNATURES = {
         _c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_f32, _vp, _vp, _vp, _vp, _vp]
     ),
     "muon_scale_gradient": (_c_int, [_vp, _c_int, _c_i64, _vp, _vp]),
+    "muon_expert_order_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "muon_expert_order": (_c_int, [_vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp]),
+    "muon_dispatch": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp]),
+    "muon_combine": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp]),
+    "muon_combine_backward": (
+        _c_int,
+        [_vp, _c_i64, _vp, _c_i64, _c_int, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "muon_expert_linear": (
+        _c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp]
+    ),
+    "muon_expert_linear_backward_rows": (
+        _c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp]
+    ),
+    "muon_expert_linear_backward_weight": (
+        _c_int,
+        [_vp, _c_int, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp],
+    ),
+    "muon_adamw_workspace_bytes": (_c_i64, [_c_i64]),
+    "muon_adamw": (
+        _c_int,
+        [_c_i64, _vp, _c_int, _c_i64, _c_f64, _c_f64, _c_f64, _c_f64, _c_f64, _c_int, _vp, _vp],
+    ),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

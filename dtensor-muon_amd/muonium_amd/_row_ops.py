@@ -1,6 +1,7 @@
-"""The training step's row operators (include/muon_amd.h, "Row operators") as torch operators of
-namespace ``muonium_amd``: query and key norm with rotation, expert routing, token log
-probabilities, policy loss.
+"""The training step's row operators (include/muon_amd.h, "Row operators", "Experts" and "AdamW") as
+torch operators of namespace ``muonium_amd``: query and key norm with rotation, expert routing,
+token log probabilities, policy loss; tokens to their experts and back, the experts' products, and
+the AdamW step.
 
 Schemas, device implementations and gradients are in csrc/row_ops.cpp
 (``libmuon_amd_torch.so``, built beside ``libmuon_amd.so``); the fake implementations here let an
@@ -37,6 +38,11 @@ qk_norm_rope = _ops.qk_norm_rope.default
 route = _ops.route.default
 token_logprobs = _ops.token_logprobs.default
 policy_loss = _ops.policy_loss.default
+sort_by_expert = _ops.sort_by_expert.default
+dispatch = _ops.dispatch.default
+combine = _ops.combine.default
+expert_linear = _ops.expert_linear.default
+adamw_ = _ops.adamw_.default
 
 
 def unit_last(t: Tensor) -> Tensor:
@@ -115,4 +121,47 @@ def _(dloss, logits, tokens, rows, temperature):
 
 @_fake("policy_loss_rescale_")
 def _(dlogits, dloss, logits, tokens, rows, temperature):
+    return None
+
+
+@_fake("sort_by_expert")
+def _(experts, num_experts):
+    return (experts.new_empty(experts.shape, dtype=torch.int32),
+            experts.new_empty(num_experts + 1, dtype=torch.int32))
+
+
+@_fake("dispatch")
+def _(x, slots):
+    return x.new_empty((slots.size(0) * slots.size(1), x.size(1)))
+
+
+@_fake("combine")
+def _(rows, slots, gates):
+    return rows.new_empty((slots.size(0), rows.size(1)))
+
+
+@_fake("combine_backward")
+def _(dy, rows, slots, gates, rows_wanted, gates_wanted):
+    return (_like(rows) if rows_wanted else rows.new_empty(0),
+            gates.new_empty(slots.shape if gates_wanted else 0))
+
+
+@_fake("expert_linear")
+def _(rows, weight, offsets):
+    return rows.new_empty((rows.size(0), weight.size(1)))
+
+
+@_fake("expert_linear_backward_rows")
+def _(dy, weight, offsets):
+    return dy.new_empty((dy.size(0), weight.size(2)))
+
+
+@_fake("expert_linear_backward_weight")
+def _(dy, rows, offsets):
+    return rows.new_empty((offsets.size(0) - 1, dy.size(1), rows.size(1)))
+
+
+@_fake("adamw_")
+def _(params, grads, exp_avgs, exp_avg_sqs, avg_scales, sq_scales, steps, block, lr, beta1, beta2,
+      eps, weight_decay, maximize):
     return None

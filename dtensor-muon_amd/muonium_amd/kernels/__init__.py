@@ -5,11 +5,13 @@ from importlib import import_module
 
 from .gram import gram, gram_
 
-_ROW_OPERATORS = {"PolicyLoss": "logprobs", "Routing": "router", "policy_loss": "logprobs",
-                  "qk_norm_rope": "heads", "route": "router", "token_logprobs": "logprobs"}
+_ROW_OPERATORS = {"ExpertOrder": "experts", "PolicyLoss": "logprobs", "Routing": "router",
+                  "combine": "experts", "dispatch": "experts", "expert_linear": "experts",
+                  "policy_loss": "logprobs", "qk_norm_rope": "heads", "route": "router",
+                  "sort_by_expert": "experts", "token_logprobs": "logprobs"}
 
-__all__ = ["PolicyLoss", "Routing", "gram", "gram_", "policy_loss", "qk_norm_rope", "route",
-           "token_logprobs"]
+__all__ = ["ExpertOrder", "PolicyLoss", "Routing", "combine", "dispatch", "expert_linear", "gram",
+           "gram_", "policy_loss", "qk_norm_rope", "route", "sort_by_expert", "token_logprobs"]
 
 
 def __getattr__(name: str):

@@ -1,3 +1,4 @@
+from .adamw import AdamW, AdamWFp8
 from .algorithms import (
     BufferSpec,
     MuonAlgorithm,
@@ -5,10 +6,13 @@ from .algorithms import (
     register_muon_algorithm,
     registered_algorithms,
 )
+from .lp_state import OptimStateFp8
 from .optim import Muon
 from .optim_lp import Muon4bit, Muon8bit, MuonFp8, MuonLP
 
 __all__ = [
+    "AdamW",
+    "AdamWFp8",
     "BufferSpec",
     "Muon",
     "Muon4bit",
@@ -16,6 +20,7 @@ __all__ = [
     "MuonAlgorithm",
     "MuonFp8",
     "MuonLP",
+    "OptimStateFp8",
     "get_algorithm",
     "register_muon_algorithm",
     "registered_algorithms",

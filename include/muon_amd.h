@@ -342,6 +342,72 @@ int muon_policy_loss_rescale(const void* logits, int dtype, int64_t row_stride, 
                              void* dlogits, void* stream);
 int muon_scale_gradient(void* x, int dtype, int64_t n, const float* scale, void* stream);
 
+/* ---- Experts: routed tokens to their experts and back -------------------------------------
+ * No counterpart in the reference: what carries out the choices of muon_route.
+ *
+ * muon_expert_order: the rows of all choices (tokens x top, below 2^31) sorted by expert (at most
+ * 1024), in the order of choices within one: slots[i] = choice i's row; a choice whose number is none
+ * of 0 .. nexperts - 1 is empty, comes behind the last expert's, and has slots[i] = -1 - its row.
+ * offsets (nexperts + 1): the experts' first rows, and the end of the last one's.
+ * muon_dispatch: rows (tokens * top, width), contiguous, rows[slot] = x[token]; an empty choice's row
+ * is 0. muon_combine: y (tokens, width), contiguous, y[t] = sum_j gates[t, j] rows[slot(t, j)] over the
+ * kept choices (gates NULL: ones, the gradient of muon_dispatch). muon_combine_backward: drows like
+ * muon_dispatch's rows, gates[t, j] dy[t], and dgates[t, j] = <dy[t], rows[slot]>; either may be NULL.
+ * Gates and rows of empty choices are not read, their gradients are 0. A slot outside the rows is
+ * left out. Strides of rows in elements, columns contiguous; sums in fp32, rounded once. */
+int64_t muon_expert_order_workspace_bytes(int64_t choices, int64_t nexperts);
+int muon_expert_order(const int64_t* experts, int64_t choices, int64_t nexperts, int32_t* slots,
+                      int32_t* offsets, void* ws, void* stream);
+int muon_dispatch(const void* x, int dtype, int64_t row_stride, int64_t tokens, int64_t top,
+                  int64_t width, const int32_t* slots, void* rows, void* stream);
+int muon_combine(const void* rows, int dtype, int64_t row_stride, int64_t tokens, int64_t top,
+                 int64_t width, const int32_t* slots, const float* gates, void* y, void* stream);
+int muon_combine_backward(const void* dy, int64_t dy_stride, const void* rows, int64_t row_stride,
+                          int dtype, int64_t tokens, int64_t top, int64_t width,
+                          const int32_t* slots, const float* gates, void* drows, float* dgates,
+                          void* stream);
+
+/* The experts' matrices, weight (experts, out, in), contiguous, on their rows offsets[e] ..
+ * offsets[e + 1] - 1 of `nrows`: y = x W_e^T (nrows, out); drows = dy W_e (nrows, in); dweight_e =
+ * dy_e^T x_e (experts, out, in), 0 for an expert without rows; all contiguous. Rows behind
+ * offsets[experts] give zeros and reach nothing. Products of 16-bit types on the matrix cores with
+ * fp32 sums; fp32 in fp32. offsets[0] counts as 0, and the others, which have to rise, are taken
+ * into 0 .. nrows: nothing is read out of range whatever they hold. */
+int muon_expert_linear(const void* rows, int dtype, int64_t row_stride, int64_t nrows,
+                       int64_t experts, int64_t out, int64_t in, const void* weight,
+                       const int32_t* offsets, void* y, void* stream);
+int muon_expert_linear_backward_rows(const void* dy, int dtype, int64_t dy_stride, int64_t nrows,
+                                     int64_t experts, int64_t out, int64_t in, const void* weight,
+                                     const int32_t* offsets, void* drows, void* stream);
+int muon_expert_linear_backward_weight(const void* dy, int dtype, int64_t dy_stride,
+                                       const void* rows, int64_t row_stride, int64_t nrows,
+                                       int64_t experts, int64_t out, int64_t in,
+                                       const int32_t* offsets, void* dweight, void* stream);
+
+/* ---- AdamW over many tensors -------------------------------------------------------------
+ * One step of every tensor, in place: with t = ++*step (fp32, on the device),
+ *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+ *   p = (1 - lr wd) p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * (maximize: with -g), in fp32, p rounded once. Parameters and gradients are of one type and order of
+ * values. block 0: exp_avg and exp_avg_sq are fp32 m and v, the scales unused. block a power of two from
+ * 64 to 2048 that divides numel: they are float8_e4m3fn codes of m and of sqrt(v), value = float(code) *
+ * scale of its block, scale = max(absmax, 1e-12) / 448. No two tensors may share memory. ws:
+ * muon_adamw_workspace_bytes. `tensors` is host memory, read before the call returns. */
+typedef struct MuonAdamTensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* avg_scale;
+  float* sq_scale;
+  float* step;
+  int64_t numel;
+} MuonAdamTensor;
+int64_t muon_adamw_workspace_bytes(int64_t ntensors);
+int muon_adamw(int64_t ntensors, const MuonAdamTensor* tensors, int dtype, int64_t block, double lr,
+               double beta1, double beta2, double eps, double weight_decay, int maximize, void* ws,
+               void* stream);
+
 /* ---- Kernel timing (measurement support) ------------------------------------------
  * No counterpart in the reference. While enabled, every kernel the step entry points
  * launch is bracketed by hipEvents on its own stream; muon_timing_read() waits for
