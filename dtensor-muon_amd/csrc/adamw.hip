@@ -61,6 +61,7 @@ struct StepArgs {
 };
 
 constexpr int THREADS = 256;
+constexpr int64_t MOST_TENSORS = 1 << 20;
 
 // This workgroup's tensor: the last whose first piece is not behind it.
 MUON_DEVICE int find_tensor(const StepArgs& a) {
@@ -231,7 +232,7 @@ int piece_runs(int64_t total, int64_t block) {
 }  // namespace
 
 extern "C" int64_t muon_adamw_workspace_bytes(int64_t ntensors) {
-  return ntensors < 0 ? 0 : round_up(ntensors * (int64_t)sizeof(Entry), 256) + ntensors * 4;
+  return ntensors < 0 || ntensors > MOST_TENSORS ? -1 : round_up(ntensors * (int64_t)sizeof(Entry), 256) + ntensors * 4;
 }
 
 extern "C" int muon_adamw(int64_t ntensors, const MuonAdamTensor* tensors, int dtype, int64_t block,
@@ -241,7 +242,7 @@ extern "C" int muon_adamw(int64_t ntensors, const MuonAdamTensor* tensors, int d
     muon_set_error("muon_adamw: unsupported dtype %d", dtype);
     return MUON_ERR_DTYPE;
   }
-  if (ntensors < 0 || ntensors > (1 << 20) || (block && (block < 64 || block > 2048 || (block & (block - 1))))) {
+  if (ntensors < 0 || ntensors > MOST_TENSORS || (block && (block < 64 || block > 2048 || (block & (block - 1))))) {
     muon_set_error("muon_adamw: %lld tensors, blocks of %lld: to 2^20, powers of two from 64 to 2048",
                    (long long)ntensors, (long long)block);
     return MUON_ERR_SHAPE;
@@ -273,7 +274,7 @@ extern "C" int muon_adamw(int64_t ntensors, const MuonAdamTensor* tensors, int d
   int64_t work = 0;
   for (const MuonAdamTensor* t = tensors; t < tensors + ntensors; ++t)
     work += (t->numel + runs * THREADS * 8 - 1) / (runs * THREADS * 8);
-  if (work > INT32_MAX) {
+  if (work >= (1ll << 32) / THREADS) {  // a grid has to stay below 2^32 threads
     muon_set_error("muon_adamw: %lld values in one call", (long long)total);
     return MUON_ERR_SHAPE;
   }

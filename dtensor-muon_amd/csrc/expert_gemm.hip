@@ -432,7 +432,7 @@ int launch16(GArgs g, bool aligned, hipStream_t s) {
   g.tiles_m = (int)(FORM == WGT ? (g.M + BM - 1) / BM : most_tiles(g.R, g.E, BM));
   g.tiles_n = (g.N + BN - 1) / BN;
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * (FORM == WGT ? g.E : 1);
-  if (grid > INT32_MAX) {
+  if (grid >= (1ll << 32) / (64 * WM * WN)) {  // below 2^32 threads
     muon_set_error("muon_expert_linear: too many tiles");
     return MUON_ERR_SHAPE;
   }
@@ -455,7 +455,7 @@ int launch32(GArgs g, hipStream_t s) {
   g.tiles_m = (int)(FORM == WGT ? (g.M + F_B - 1) / F_B : most_tiles(g.R, g.E, F_B));
   g.tiles_n = (g.N + F_B - 1) / F_B;
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * (FORM == WGT ? g.E : 1);
-  if (grid > INT32_MAX) {
+  if (grid >= (1ll << 32) / 256) {  // below 2^32 threads
     muon_set_error("muon_expert_linear: too many tiles");
     return MUON_ERR_SHAPE;
   }

@@ -139,6 +139,8 @@ __global__ __launch_bounds__(ORDER_THREADS) void order_place_kernel(OrderArgs a)
 // ---- rows -----------------------------------------------------------------------------------
 
 constexpr int ROW_THREADS = 256;
+// Workgroups of a launch at most (a grid has to stay below 2^32 threads); each walks on by as many.
+constexpr int64_t ROW_GRID = 1 << 22;
 
 struct RowArgs {
   const void* in;  // dispatch: a token's rows; combine: the experts' rows
@@ -182,15 +184,16 @@ template <int DT>
 __global__ __launch_bounds__(ROW_THREADS) void dispatch_kernel(RowArgs a) {
   constexpr int N = Vec16<DT>::N;
   const int lanes = 1 << a.shift, v0 = threadIdx.x & (lanes - 1);
-  const int64_t t = (int64_t)blockIdx.x * (ROW_THREADS >> a.shift) + (threadIdx.x >> a.shift);
-  if (t >= a.T) return;
-  const int32_t* slots = a.slots + t * a.k;
-  for (int c = v0 * N; c < a.W; c += lanes * N) {
-    const int left = a.W - c;
-    const muon_u4 w = load_part<DT>(a.in, t * a.in_row + c, left);
-    for (int j = 0; j < a.k; ++j) {
-      const int s = slots[j], row = s < 0 ? ~s : s;
-      if (row < a.R) store_part<DT>(a.out, (int64_t)row * a.W + c, left, s < 0 ? muon_u4{0, 0, 0, 0} : w);
+  const int64_t per = ROW_THREADS >> a.shift;
+  for (int64_t t = blockIdx.x * per + (threadIdx.x >> a.shift); t < a.T; t += gridDim.x * per) {
+    const int32_t* slots = a.slots + t * a.k;
+    for (int c = v0 * N; c < a.W; c += lanes * N) {
+      const int left = a.W - c;
+      const muon_u4 w = load_part<DT>(a.in, t * a.in_row + c, left);
+      for (int j = 0; j < a.k; ++j) {
+        const int s = slots[j], row = s < 0 ? ~s : s;
+        if (row < a.R) store_part<DT>(a.out, (int64_t)row * a.W + c, left, s < 0 ? muon_u4{0, 0, 0, 0} : w);
+      }
     }
   }
 }
@@ -201,35 +204,36 @@ template <int DT>
 __global__ __launch_bounds__(ROW_THREADS) void combine_kernel(RowArgs a) {
   constexpr int N = Vec16<DT>::N;
   const int lanes = 1 << a.shift, v0 = threadIdx.x & (lanes - 1);
-  const int64_t t = (int64_t)blockIdx.x * (ROW_THREADS >> a.shift) + (threadIdx.x >> a.shift);
-  if (t >= a.T) return;
-  for (int c = v0 * N; c < a.W; c += lanes * N) {
-    const int left = a.W - c;
-    float sum[N] = {};
-    for (int j0 = 0; j0 < a.k; j0 += BATCH) {
-      muon_u4 w[BATCH];
-      float g[BATCH];
-      bool kept[BATCH];
+  const int64_t per = ROW_THREADS >> a.shift;
+  for (int64_t t = blockIdx.x * per + (threadIdx.x >> a.shift); t < a.T; t += gridDim.x * per) {
+    for (int c = v0 * N; c < a.W; c += lanes * N) {
+      const int left = a.W - c;
+      float sum[N] = {};
+      for (int j0 = 0; j0 < a.k; j0 += BATCH) {
+        muon_u4 w[BATCH];
+        float g[BATCH];
+        bool kept[BATCH];
 #pragma unroll
-      for (int b = 0; b < BATCH; ++b) {
-        const int j = j0 + b;
-        const int s = j < a.k ? a.slots[t * a.k + j] : -1;
-        kept[b] = s >= 0 && s < a.R;
-        if (kept[b]) {
-          g[b] = a.gates ? a.gates[t * a.k + j] : 1.0f;
-          w[b] = load_part<DT>(a.in, (int64_t)s * a.in_row + c, left);
+        for (int b = 0; b < BATCH; ++b) {
+          const int j = j0 + b;
+          const int s = j < a.k ? a.slots[t * a.k + j] : -1;
+          kept[b] = s >= 0 && s < a.R;
+          if (kept[b]) {
+            g[b] = a.gates ? a.gates[t * a.k + j] : 1.0f;
+            w[b] = load_part<DT>(a.in, (int64_t)s * a.in_row + c, left);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+          if (!kept[b]) continue;
+          float v[N];
+          Vec16<DT>::unpack(w[b], v);
+#pragma unroll
+          for (int e = 0; e < N; ++e) sum[e] += g[b] * v[e];
         }
       }
-#pragma unroll
-      for (int b = 0; b < BATCH; ++b) {
-        if (!kept[b]) continue;
-        float v[N];
-        Vec16<DT>::unpack(w[b], v);
-#pragma unroll
-        for (int e = 0; e < N; ++e) sum[e] += g[b] * v[e];
-      }
+      store_part<DT>(a.out, t * a.W + c, left, Vec16<DT>::pack(sum));
     }
-    store_part<DT>(a.out, t * a.W + c, left, Vec16<DT>::pack(sum));
   }
 }
 
@@ -251,52 +255,54 @@ template <int DT, int G>
 __global__ __launch_bounds__(ROW_THREADS) void combine_backward_kernel(BackArgs a) {
   constexpr int N = Vec16<DT>::N;
   const int v0 = threadIdx.x & (G - 1);
-  const int64_t t = (int64_t)blockIdx.x * (ROW_THREADS / G) + threadIdx.x / G;
-  if (t >= a.T) return;  // whole groups of lanes
-  for (int j0 = 0; j0 < a.k; j0 += BATCH) {
-    int s[BATCH];
-    float g[BATCH], dot[BATCH] = {};
-#pragma unroll
-    for (int b = 0; b < BATCH; ++b) {
-      const int j = j0 + b;
-      s[b] = j < a.k ? a.slots[t * a.k + j] : INT32_MAX;  // no row: R is at most that
-      g[b] = s[b] >= 0 && s[b] < a.R ? a.gates[t * a.k + j] : 0.0f;
-    }
-    for (int c = v0 * N; c < a.W; c += G * N) {
-      const int left = a.W - c;
-      float d[N];
-      Vec16<DT>::unpack(load_part<DT>(a.dy, t * a.dy_row + c, left), d);
-      if (a.dgates) {
-        muon_u4 w[BATCH];
-#pragma unroll
-        for (int b = 0; b < BATCH; ++b)
-          if (s[b] >= 0 && s[b] < a.R) w[b] = load_part<DT>(a.rows, (int64_t)s[b] * a.rows_row + c, left);
-#pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
-          if (!(s[b] >= 0 && s[b] < a.R)) continue;
-          float v[N];
-          Vec16<DT>::unpack(w[b], v);
-#pragma unroll
-          for (int e = 0; e < N; ++e) dot[b] += d[e] * v[e];
-        }
-      }
-      if (a.drows) {
-#pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
-          const int row = s[b] < 0 ? ~s[b] : s[b];
-          if (row >= a.R) continue;
-          float v[N];
-#pragma unroll
-          for (int e = 0; e < N; ++e) v[e] = s[b] < 0 ? 0.0f : g[b] * d[e];
-          store_part<DT>(a.drows, (int64_t)row * a.W + c, left, Vec16<DT>::pack(v));
-        }
-      }
-    }
-    if (a.dgates) {
+  // whole groups of lanes go on or end
+  const int64_t step = gridDim.x * (int64_t)(ROW_THREADS / G);
+  for (int64_t t = (int64_t)blockIdx.x * (ROW_THREADS / G) + threadIdx.x / G; t < a.T; t += step) {
+    for (int j0 = 0; j0 < a.k; j0 += BATCH) {
+      int s[BATCH];
+      float g[BATCH], dot[BATCH] = {};
 #pragma unroll
       for (int b = 0; b < BATCH; ++b) {
-        const float sum = group_sum<G>(dot[b]);
-        if (v0 == 0 && j0 + b < a.k) a.dgates[t * a.k + j0 + b] = sum;
+        const int j = j0 + b;
+        s[b] = j < a.k ? a.slots[t * a.k + j] : INT32_MAX;  // no row: R is at most that
+        g[b] = s[b] >= 0 && s[b] < a.R ? a.gates[t * a.k + j] : 0.0f;
+      }
+      for (int c = v0 * N; c < a.W; c += G * N) {
+        const int left = a.W - c;
+        float d[N];
+        Vec16<DT>::unpack(load_part<DT>(a.dy, t * a.dy_row + c, left), d);
+        if (a.dgates) {
+          muon_u4 w[BATCH];
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b)
+            if (s[b] >= 0 && s[b] < a.R) w[b] = load_part<DT>(a.rows, (int64_t)s[b] * a.rows_row + c, left);
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) {
+            if (!(s[b] >= 0 && s[b] < a.R)) continue;
+            float v[N];
+            Vec16<DT>::unpack(w[b], v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) dot[b] += d[e] * v[e];
+          }
+        }
+        if (a.drows) {
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) {
+            const int row = s[b] < 0 ? ~s[b] : s[b];
+            if (row >= a.R) continue;
+            float v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = s[b] < 0 ? 0.0f : g[b] * d[e];
+            store_part<DT>(a.drows, (int64_t)row * a.W + c, left, Vec16<DT>::pack(v));
+          }
+        }
+      }
+      if (a.dgates) {
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+          const float sum = group_sum<G>(dot[b]);
+          if (v0 == 0 && j0 + b < a.k) a.dgates[t * a.k + j0 + b] = sum;
+        }
       }
     }
   }
@@ -307,6 +313,11 @@ int lanes_shift(int dtype, int64_t width, int most) {
   int shift = 0;
   while (shift < most && (1ll << shift) < runs) ++shift;
   return shift;
+}
+
+int64_t row_grid(int64_t tokens, int shift) {
+  const int64_t per = ROW_THREADS >> shift;
+  return std::min((tokens + per - 1) / per, ROW_GRID);
 }
 
 int64_t order_chunk(int64_t n) {
@@ -342,7 +353,7 @@ int check_rows(const char* what, int dtype, int64_t tokens, int64_t top, int64_t
   }
 
 extern "C" int64_t muon_expert_order_workspace_bytes(int64_t choices, int64_t experts) {
-  if (choices < 0 || experts < 1) return 0;
+  if (choices < 0 || choices > INT32_MAX || experts < 1 || experts > ORDER_EMAX) return -1;
   const int64_t blocks = order_blocks(choices);
   return blocks > 1 ? blocks * (experts + 1) * 4 : 0;
 }
@@ -382,7 +393,7 @@ extern "C" int muon_dispatch(const void* x, int dtype, int64_t row_stride, int64
   }
   RowArgs a{x, row_stride, tokens, tokens * top, (int)top, (int)width, lanes_shift(dtype, width, 8),
             slots, nullptr, rows};
-  const int64_t grid = (tokens + (ROW_THREADS >> a.shift) - 1) / (ROW_THREADS >> a.shift);
+  const int64_t grid = row_grid(tokens, a.shift);
   BY_TYPE((dispatch_kernel<DT><<<(unsigned)grid, ROW_THREADS, 0, (hipStream_t)stream>>>(a)))
   MUON_CHECK_LAUNCH("muon_dispatch");
   return MUON_OK;
@@ -399,7 +410,7 @@ extern "C" int muon_combine(const void* rows, int dtype, int64_t row_stride, int
   }
   RowArgs a{rows, row_stride, tokens, tokens * top, (int)top, (int)width, lanes_shift(dtype, width, 8),
             slots, gates, y};
-  const int64_t grid = (tokens + (ROW_THREADS >> a.shift) - 1) / (ROW_THREADS >> a.shift);
+  const int64_t grid = row_grid(tokens, a.shift);
   BY_TYPE((combine_kernel<DT><<<(unsigned)grid, ROW_THREADS, 0, (hipStream_t)stream>>>(a)))
   MUON_CHECK_LAUNCH("muon_combine");
   return MUON_OK;
@@ -418,7 +429,7 @@ extern "C" int muon_combine_backward(const void* dy, int64_t dy_stride, const vo
   BackArgs a{dy, rows, dy_stride, row_stride, tokens, tokens * top, (int)top, (int)width,
              slots, gates, drows, dgates};
   const int shift = std::max(3, lanes_shift(dtype, width, 6));
-  const int64_t grid = (tokens + (ROW_THREADS >> shift) - 1) / (ROW_THREADS >> shift);
+  const int64_t grid = row_grid(tokens, shift);
   hipStream_t s = (hipStream_t)stream;
 #define BACK(G) BY_TYPE((combine_backward_kernel<DT, G><<<(unsigned)grid, ROW_THREADS, 0, s>>>(a)))
   switch (shift) {
