@@ -106,13 +106,14 @@ MUON_DEVICE f32x4 mfma16(muon_u4 a, muon_u4 b, f32x4 c) {
   }
 }
 
+typedef __attribute__((ext_vector_type(2))) _Float16 muon_h2x;
 // Two values to 16 bits each, to nearest even.
 template <int DT>
 MUON_DEVICE uint32_t pack2(float x, float y) {
   if constexpr (DT == MUON_DT_BF16)
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(muon_f2x{x, y}, muon_bf2x));
   else
-    return (uint32_t)f32_to_f16(x) | ((uint32_t)f32_to_f16(y) << 16);
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(muon_f2x{x, y}, muon_h2x));
 }
 
 // ---- 16-bit types ---------------------------------------------------------------------------
@@ -294,6 +295,317 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void expert_gemm_kernel(GArgs g) {
   }
 }
 
+// ---- 16-bit types, whole 16-byte runs: operands straight to LDS --------------------------------
+//
+// 256 x 256 tile, K-tiles of 64, four waves of 128 x 128 (8 x 8 accumulators of 16 x 16). The panels are
+// those above; they come by loads that write LDS themselves, two K-tiles ahead: those of K-tile k + 2 go out
+// after the barrier of K-tile k, when every wave has the last fragments of K-tile k's panels. A K-tile is two
+// substeps of 32 k; each multiplies one set of fragments while the next set is read.
+//
+// Nothing is masked beyond what the buffer's size cuts off (what lies behind it arrives as zeros): rows and
+// columns of a tile behind its own are others' values or zeros, and are not stored. Along k, a KR panel's
+// buffer ends with its last k; of a KC panel the lanes behind the last k point behind the buffer.
+constexpr int P_PANEL = 256 * BK * 2, P_STAGE = 2 * P_PANEL;
+constexpr int P_OUT_ROW = 256 + 16, P_OUT = 16 * P_OUT_ROW;  // a wave's rows on their way out
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
+
+// One load of 1 KB, 16 bytes a lane in order, to the LDS address m0.
+MUON_DEVICE void dma_1k(u32x4 rs, uint32_t vo, uint32_t so, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+               ::"v"(vo), "s"(rs), "s"(so), "s"(m0) : "m0");
+}
+
+// One operand of a tile as its loads see it.
+template <bool KR>
+struct Source {
+  const char* base;  // the panel at k = 0
+  int64_t bytes;     // from there to the end of what may be read
+  uint32_t step;     // bytes of a row
+  uint32_t vo[2];    // this lane's place: of even and odd slabs (KR), of whole and of the last K-tile (KC)
+
+  // rows: from the panel's first row (KC) or k = 0 (KR); columns: k (KC) or from the panel's first (KR)
+  MUON_DEVICE void set(const uint16_t* p, int64_t ld, int64_t rows, int columns, int K) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    base = (const char*)p;
+    step = (uint32_t)ld * 2;
+    bytes = rows && columns ? ((rows - 1) * ld + columns) * 2 : 0;
+    if constexpr (KR) {
+      const int r = wave * 2 + (lane >> 5), c = (lane & 31) ^ ((r & 3) << 2);
+      vo[0] = r * step + c * 16;
+      vo[1] = r * step + (c ^ 2) * 16;
+    } else {
+      const int r = wave * 8 + (lane >> 3), c = (lane & 7) ^ swz_kc(r);
+      vo[0] = r * step + c * 16;
+      vo[1] = c * 8 < K - (K - 1) / BK * BK ? vo[0] : 0x80000000u;
+    }
+  }
+  // The buffer of K-tile kt; without `any` it is empty, and loads of it write zeros.
+  MUON_DEVICE u32x4 buffer(int kt, bool any) const {
+    const char* b = KR ? base + (int64_t)kt * BK * step : base;
+    const int64_t left = KR ? bytes - (int64_t)kt * BK * step : bytes;
+    const uint32_t n = left <= 0 || !any ? 0u : (uint32_t)std::min<int64_t>(left, 0x7fffffff);
+    const uint64_t a = (uint64_t)b;
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)a),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) & 0xffffu,
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)n), 0x00020000u};
+  }
+  // slab q of 8 of this wave: of K-tile kt (the last of K: `last`) to LDS at `to`
+  MUON_DEVICE void load(u32x4 rs, int q, int kt, bool last, uint32_t to) const {
+    if constexpr (KR)
+      dma_1k(rs, vo[q & 1], q * 8 * step, to + q * 4096);
+    else
+      dma_1k(rs, last ? vo[1] : vo[0], q * 32 * step + kt * (BK * 2), to + q * 4096);
+  }
+};
+
+// acc += a b with the accumulator in AGPRs all along: left to the compiler, the 64 of a wave are copied
+// between registers in every K-tile.
+template <int DT>
+MUON_DEVICE void mfma_acc(f32x4& c, muon_u4 a, muon_u4 b) {
+  if constexpr (DT == MUON_DT_BF16)
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+// Reads of the accumulators by other instructions wait for the last of them, which the compiler does
+// not see, and their first use for the writes of their zeros.
+MUON_DEVICE void mfma_wait() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The tiles of a launch as its workgroups walk them. One workgroup a CU; those of XCD x (workgroups are
+// dealt to the 8 round robin) share one contiguous range of tiles, each taking every 32nd, so that
+// neighbouring tiles, whose panels are the same, meet in one L2. Ranges are of equal work: of equal
+// numbers of tiles, and for WGT, where a tile's K is its expert's rows, of K-tiles.
+constexpr int P_GROUPS = 256, P_LANE = P_GROUPS / 8;
+struct Tile {
+  int e, row0, tm, tn, M, N, K;  // row0: the first of the tile's rows (WGT: of the expert's)
+};
+template <int FORM>
+struct Walk {
+  const GArgs& g;
+  int* first;  // in LDS: row tiles (WGT: K-tiles) before each expert, E + 2 of them
+  int at, end;
+
+  MUON_DEVICE Walk(const GArgs& g_, int* lds) : g(g_), first(lds) {
+    const int lane = threadIdx.x & 63, per = (g.E + 64) / 64;
+    constexpr int UNIT = FORM == WGT ? BK : 256;
+    const int e0 = lane * per, e1 = std::min(e0 + per, g.E + 1);
+    int mine = 0, start, n;
+    for (int i = e0; i < e1; ++i) {
+      bounds(g, i, start, n);
+      mine += units(i, n, UNIT);
+    }
+    int incl = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int v = __shfl_up(incl, off, 64);
+      if (lane >= off) incl += v;
+    }
+    if (threadIdx.x < 64) {
+      int sum = incl - mine;
+      for (int i = e0; i < e1; ++i) {
+        first[i] = sum;
+        bounds(g, i, start, n);
+        sum += units(i, n, UNIT);
+      }
+      if (e1 == g.E + 1 && e0 < e1) first[g.E + 1] = sum;
+    }
+    __syncthreads();
+    const int x = blockIdx.x & 7, total = first[g.E + 1];
+    at = __builtin_amdgcn_readfirstlane(border(x, total)) + (int)(blockIdx.x >> 3);
+    end = __builtin_amdgcn_readfirstlane(border(x + 1, total));
+  }
+  // Row tiles, or K-tiles of one tile (an expert without rows has one, of nothing), of expert i.
+  static MUON_DEVICE int units(const GArgs& g, int i, int n, int unit) {
+    if (FORM == WGT) return i < g.E ? std::max(1, (n + unit - 1) / unit) : 0;
+    return (n + unit - 1) / unit;
+  }
+  MUON_DEVICE int units(int i, int n, int unit) const { return units(g, i, n, unit); }
+  // The expert whose row tiles (K-tiles) hold number t.
+  MUON_DEVICE int expert(int t) const {
+    const int lane = threadIdx.x & 63, per = (g.E + 64) / 64;
+    const int seg = __popcll(__ballot(lane * per <= g.E && first[std::min(lane * per, g.E)] <= t)) - 1;
+    const int i = seg * per + lane;
+    const int in = __popcll(__ballot(lane < per && i <= g.E && first[std::min(i, g.E)] <= t));
+    return std::max(0, std::min(seg * per + in - 1, g.E));
+  }
+  MUON_DEVICE int border(int x, int total) const {
+    if constexpr (FORM == WGT) {
+      const int per = g.tiles_m * g.tiles_n;
+      if (x == 8) return g.E * per;
+      const int64_t work = (int64_t)total * per * x / 8;
+      const int e = __builtin_amdgcn_readfirstlane(std::min(expert((int)(work / per)), g.E - 1));
+      const int k = first[e + 1] - first[e];
+      return e * per + std::min<int64_t>((work - (int64_t)first[e] * per) / k, per);
+    } else {
+      return (int)((int64_t)total * g.tiles_n * x / 8);
+    }
+  }
+  MUON_DEVICE bool tile(int t, Tile& o) const {
+    if (t >= end) return false;
+    if constexpr (FORM == WGT) {
+      const int per = g.tiles_m * g.tiles_n;
+      o.e = t / per;
+      tile_of(t - o.e * per, g.tiles_m, g.tiles_n, o.tm, o.tn);
+      bounds(g, o.e, o.row0, o.K);
+      o.M = std::min(g.M - o.tm * 256, 256);
+    } else {
+      const int total = first[g.E + 1];
+      int row;
+      tile_of(t, total, g.tiles_n, row, o.tn);
+      int start, n;
+      o.e = expert(row);
+      bounds(g, o.e, start, n);
+      const int skip = (row - first[o.e]) * 256;
+      o.row0 = start + skip;
+      o.M = std::min(n - skip, 256);
+      o.K = o.e < g.E ? g.K : 0;
+      o.tm = 0;
+    }
+    o.N = std::min(g.N - o.tn * 256, 256);
+#define UNIFORM(X) o.X = __builtin_amdgcn_readfirstlane(o.X)
+    UNIFORM(e); UNIFORM(row0); UNIFORM(tm); UNIFORM(tn); UNIFORM(M); UNIFORM(N); UNIFORM(K);
+#undef UNIFORM
+    return true;
+  }
+};
+
+template <int DT, int FORM>
+__global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
+  constexpr int BM = 256, BN = 256;
+  constexpr bool KRA = FORM == WGT, KRB = FORM != FWD;
+  extern __shared__ __align__(16) uint8_t smem[];
+  Walk<FORM> walk(g, (int*)(smem + 2 * P_STAGE + 4 * P_OUT));
+  Tile t;
+  if (!walk.tile(walk.at, t)) return;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = wave & 1, wn = wave >> 1;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem + wave * 1024;
+
+  // What the loads are at: a tile's sources, and its next K-tile. They run two K-tiles ahead of the
+  // products, across tiles.
+  Source<KRA> a;
+  Source<KRB> b;
+  int next = walk.at, kt_next = 0, kt_all = 0;
+  auto open = [&](const Tile& o) {
+    const uint16_t *A = (const uint16_t*)g.a, *B = (const uint16_t*)g.b;
+    if constexpr (FORM == WGT) {
+      a.set(A + (int64_t)o.row0 * g.lda + o.tm * BM, g.lda, o.K, g.M - o.tm * BM, o.K);
+      b.set(B + (int64_t)o.row0 * g.ldb + o.tn * BN, g.ldb, o.K, g.N - o.tn * BN, o.K);
+    } else {
+      a.set(A + (int64_t)o.row0 * g.lda, g.lda, o.K ? g.R - o.row0 : 0, g.K, o.K);
+      if constexpr (FORM == FWD)
+        b.set(B + o.e * g.sb + (int64_t)o.tn * BN * g.ldb, g.ldb,
+              o.K ? (int64_t)(g.E - o.e) * g.N - o.tn * BN : 0, g.K, o.K);
+      else
+        b.set(B + o.e * g.sb + o.tn * BN, g.ldb, o.K, g.N - o.tn * BN, o.K);
+    }
+    kt_next = 0;
+    kt_all = std::max(1, (o.K + BK - 1) / BK);
+  };
+  // to the next K-tile; kt_all = 0: there is none, and loads write zeros
+  auto advance = [&] {
+    if (++kt_next < kt_all) return;
+    next += P_LANE;
+    Tile o;
+    if (walk.tile(next, o)) open(o);
+    else kt_all = 0;
+  };
+  u32x4 ra, rb;
+  auto load = [&](int q, int st) {
+    a.load(ra, q, kt_next, kt_next + 1 == kt_all, lds0 + st * P_STAGE);
+    b.load(rb, q, kt_next, kt_next + 1 == kt_all, lds0 + st * P_STAGE + P_PANEL);
+  };
+  auto buffers = [&] {
+    ra = a.buffer(kt_next, kt_all != 0);
+    rb = b.buffer(kt_next, kt_all != 0);
+  };
+  f32x4 acc[8][8];
+  muon_u4 fa[2][8], fb[2][8];
+  auto read = [&](int to, int st, int ks, int i) {
+    uint8_t* p = smem + st * P_STAGE;
+    fa[to][i] = fragment<BM, KRA>(p, wm * 128 + i * 16, ks);
+    fb[to][i] = fragment<BN, KRB>(p + P_PANEL, wn * 128 + i * 16, ks);
+  };
+  open(t);
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    buffers();
+#pragma unroll
+    for (int q = 0; q < 8; ++q) load(q, st);
+    advance();
+  }
+  asm volatile("s_waitcnt vmcnt(16)\n\ts_barrier" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) read(0, 0, 0, i);
+
+  int st = 0;
+  for (int at = walk.at;;) {
+    const int KT = std::max(1, (t.K + BK - 1) / BK);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    mfma_wait();
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        read(1, st, 1, i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mfma_acc<DT>(acc[i][j], fb[0][j], fa[0][i]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      buffers();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        load(i, st);
+        read(0, st ^ 1, 0, i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mfma_acc<DT>(acc[i][j], fb[1][j], fa[1][i]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      st ^= 1;
+      advance();
+    }
+    mfma_wait();
+
+    // 16 rows of the wave's 128 columns at a time through its own LDS: a lane has four consecutive columns
+    // of one row, and stores 16 bytes of a line
+    int r = lane & 15, l = lane >> 4;
+    asm volatile("" : "+v"(r), "+v"(l));  // or their products are made before the loop, and spilled
+    uint8_t* mine = smem + 2 * P_STAGE + wave * P_OUT;
+    const int c = wn * 128 + r * 8;
+    char* out = (char*)((uint16_t*)g.c + (FORM == WGT ? (int64_t)t.e * g.M + t.tm * BM : (int64_t)t.row0) * g.N +
+                        (int64_t)(wm * 128 + l) * g.N + t.tn * BN + c);
+    int row = c < t.N ? wm * 128 + l : BM;
+    const int64_t four = (int64_t)g.N * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        *(uint2*)(mine + r * P_OUT_ROW + j * 32 + l * 8) =
+            make_uint2(pack2<DT>(acc[i][j][0], acc[i][j][1]), pack2<DT>(acc[i][j][2], acc[i][j][3]));
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const muon_u4 w = *(const muon_u4*)(mine + (p * 4 + l) * P_OUT_ROW + r * 16);
+        if (row < t.M) *(muon_u4*)out = w;
+        out += four;
+        row += 4;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    at += P_LANE;
+    if (!walk.tile(at, t)) break;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last loads, of nothing, into this LDS
+}
+
 // ---- fp32 -----------------------------------------------------------------------------------
 //
 // 128 x 128 tile, K-tiles of 16, four waves of 64 x 64 on v_mfma_f32_32x32x2_f32. Both panels stand in LDS
@@ -450,6 +762,29 @@ int launch16(GArgs g, bool aligned, hipStream_t s) {
                  : run(expert_gemm_kernel<DT, FORM, BM, BN, WM, WN, false>);
 }
 
+// What the direct loads index by 32 bits: 256 rows of a panel, 64 of one along k.
+constexpr int64_t P_MOST = 1 << 20;
+
+template <int DT, int FORM>
+int launch_pipe(GArgs g, hipStream_t s) {
+  g.tiles_m = (int)(FORM == WGT ? (g.M + 255) / 256 : 0);  // of rows: counted on the device
+  g.tiles_n = (g.N + 255) / 256;
+  const int64_t most = (FORM == WGT ? (int64_t)g.tiles_m * g.E : most_tiles(g.R, g.E, 256)) * g.tiles_n;
+  if (most > INT32_MAX) {
+    muon_set_error("muon_expert_linear: too many tiles");
+    return MUON_ERR_SHAPE;
+  }
+  const int lds = 2 * P_STAGE + 4 * P_OUT + (g.E + 2) * 4;
+  if (hipFuncSetAttribute((const void*)expert_gemm_pipe_kernel<DT, FORM>,
+                          hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+    muon_set_error("muon_expert_linear: %d bytes of LDS refused", lds);
+    return MUON_ERR_LAUNCH;
+  }
+  expert_gemm_pipe_kernel<DT, FORM><<<P_GROUPS, 256, lds, s>>>(g);
+  MUON_CHECK_LAUNCH("muon_expert_linear");
+  return MUON_OK;
+}
+
 template <int FORM>
 int launch32(GArgs g, hipStream_t s) {
   g.tiles_m = (int)(FORM == WGT ? (g.M + F_B - 1) / F_B : most_tiles(g.R, g.E, F_B));
@@ -469,6 +804,9 @@ int launch(const GArgs& g, int dtype, hipStream_t s) {
   if (dtype == MUON_DT_F32) return launch32<FORM>(g, s);
   const bool aligned = ((uintptr_t)g.a | (uintptr_t)g.b | (uintptr_t)g.c) % 16 == 0 &&
                        (g.lda | g.ldb | g.sb | g.N | g.K | g.M) % 8 == 0;
+  const int64_t wa = FORM == WGT ? g.M : g.K, wb = FORM == FWD ? g.K : g.N;
+  if (aligned && g.lda >= wa && g.ldb >= wb && std::max(g.lda, g.ldb) <= P_MOST)
+    return dtype == MUON_DT_BF16 ? launch_pipe<MUON_DT_BF16, FORM>(g, s) : launch_pipe<MUON_DT_F16, FORM>(g, s);
   return dtype == MUON_DT_BF16 ? launch16<MUON_DT_BF16, FORM, 256, 256, 4, 2>(g, aligned, s)
                                : launch16<MUON_DT_F16, FORM, 256, 256, 4, 2>(g, aligned, s);
 }
