@@ -309,7 +309,7 @@ constexpr int P_PANEL = 256 * BK * 2, P_STAGE = 2 * P_PANEL;
 constexpr int P_OUT_ROW = 256 + 16, P_OUT = 16 * P_OUT_ROW;  // a wave's rows on their way out
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
 
-// One load of 1 KB, 16 bytes a lane in order, to the LDS address m0.
+// One load of 1 KB, 16 bytes a lane in order, to the LDS address m0, which takes a wait state.
 MUON_DEVICE void dma_1k(u32x4 rs, uint32_t vo, uint32_t so, uint32_t m0) {
   asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
                ::"v"(vo), "s"(rs), "s"(so), "s"(m0) : "m0");
@@ -386,10 +386,12 @@ struct Tile {
 template <int FORM>
 struct Walk {
   const GArgs& g;
-  int* first;  // in LDS: row tiles (WGT: K-tiles) before each expert, E + 2 of them
+  // in LDS, E + 2 of each: row tiles (WGT: K-tiles) before each expert, its first row and its rows
+  int *first, *start_of, *rows_of;
   int at, end;
 
-  MUON_DEVICE Walk(const GArgs& g_, int* lds) : g(g_), first(lds) {
+  MUON_DEVICE Walk(const GArgs& g_, int* lds)
+      : g(g_), first(lds), start_of(lds + g_.E + 2), rows_of(lds + 2 * (g_.E + 2)) {
     const int lane = threadIdx.x & 63, per = (g.E + 64) / 64;
     constexpr int UNIT = FORM == WGT ? BK : 256;
     const int e0 = lane * per, e1 = std::min(e0 + per, g.E + 1);
@@ -409,6 +411,8 @@ struct Walk {
       for (int i = e0; i < e1; ++i) {
         first[i] = sum;
         bounds(g, i, start, n);
+        start_of[i] = start;
+        rows_of[i] = n;
         sum += units(i, n, UNIT);
       }
       if (e1 == g.E + 1 && e0 < e1) first[g.E + 1] = sum;
@@ -450,18 +454,17 @@ struct Walk {
       const int per = g.tiles_m * g.tiles_n;
       o.e = t / per;
       tile_of(t - o.e * per, g.tiles_m, g.tiles_n, o.tm, o.tn);
-      bounds(g, o.e, o.row0, o.K);
+      o.row0 = start_of[o.e];
+      o.K = rows_of[o.e];
       o.M = std::min(g.M - o.tm * 256, 256);
     } else {
       const int total = first[g.E + 1];
       int row;
       tile_of(t, total, g.tiles_n, row, o.tn);
-      int start, n;
       o.e = expert(row);
-      bounds(g, o.e, start, n);
       const int skip = (row - first[o.e]) * 256;
-      o.row0 = start + skip;
-      o.M = std::min(n - skip, 256);
+      o.row0 = start_of[o.e] + skip;
+      o.M = std::min(rows_of[o.e] - skip, 256);
       o.K = o.e < g.E ? g.K : 0;
       o.tm = 0;
     }
@@ -516,8 +519,8 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
     else kt_all = 0;
   };
   u32x4 ra, rb;
-  auto load = [&](int q, int st) {
-    a.load(ra, q, kt_next, kt_next + 1 == kt_all, lds0 + st * P_STAGE);
+  auto load_a = [&](int q, int st) { a.load(ra, q, kt_next, kt_next + 1 == kt_all, lds0 + st * P_STAGE); };
+  auto load_b = [&](int q, int st) {
     b.load(rb, q, kt_next, kt_next + 1 == kt_all, lds0 + st * P_STAGE + P_PANEL);
   };
   auto buffers = [&] {
@@ -526,22 +529,51 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
   };
   f32x4 acc[8][8];
   muon_u4 fa[2][8], fb[2][8];
-  auto read = [&](int to, int st, int ks, int i) {
+  // fragment n of the 16 of a substep, those of b first: its first products take all of them
+  auto read = [&](int to, int st, int ks, int n) {
     uint8_t* p = smem + st * P_STAGE;
-    fa[to][i] = fragment<BM, KRA>(p, wm * 128 + i * 16, ks);
-    fb[to][i] = fragment<BN, KRB>(p + P_PANEL, wn * 128 + i * 16, ks);
+    if (n < 8) fb[to][n] = fragment<BN, KRB>(p + P_PANEL, wn * 128 + n * 16, ks);
+    else fa[to][n - 8] = fragment<BM, KRA>(p, wm * 128 + (n - 8) * 16, ks);
   };
+  // One substep: 64 products on one set of fragments, the other set read between those of the first
+  // six rows, and the loads of a slab of either panel between those of every row. A wave issues in
+  // order, and each product leaves three slots before the next can start: what stands together
+  // between two products holds the second one up.
+  auto substep = [&](auto from_c, int st, auto loads_c, int load_st) {
+    constexpr int from = decltype(from_c)::value, to = from ^ 1;
+    constexpr bool loads = decltype(loads_c)::value;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        mfma_acc<DT>(acc[i][j], fb[from][j], fa[from][i]);
+        const int n = i * 3 + j / 2;
+        if (j % 2 == 0 && j < 6 && n < 16) {
+          __builtin_amdgcn_sched_barrier(0);
+          read(to, st, to, n);
+        }
+        if (loads && j == 5) load_a(i, load_st);
+        if (loads && j == 7) load_b(i, load_st);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  typedef std::integral_constant<int, 0> Zero;
+  typedef std::integral_constant<int, 1> One;
   open(t);
 #pragma unroll
   for (int st = 0; st < 2; ++st) {
     buffers();
 #pragma unroll
-    for (int q = 0; q < 8; ++q) load(q, st);
+    for (int q = 0; q < 8; ++q) {
+      load_a(q, st);
+      load_b(q, st);
+    }
     advance();
   }
   asm volatile("s_waitcnt vmcnt(16)\n\ts_barrier" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 8; ++i) read(0, 0, 0, i);
+  for (int n = 0; n < 16; ++n) read(0, 0, 0, n);
 
   int st = 0;
   for (int at = walk.at;;) {
@@ -552,24 +584,11 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
       for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
     mfma_wait();
     for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        read(1, st, 1, i);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mfma_acc<DT>(acc[i][j], fb[0][j], fa[0][i]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+substep(Zero{}, st, std::false_type{}, 0);
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
       buffers();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        load(i, st);
-        read(0, st ^ 1, 0, i);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mfma_acc<DT>(acc[i][j], fb[1][j], fa[1][i]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      substep(One{}, st ^ 1, std::true_type{}, st);
       st ^= 1;
       advance();
     }
@@ -774,7 +793,7 @@ int launch_pipe(GArgs g, hipStream_t s) {
     muon_set_error("muon_expert_linear: too many tiles");
     return MUON_ERR_SHAPE;
   }
-  const int lds = 2 * P_STAGE + 4 * P_OUT + (g.E + 2) * 4;
+  const int lds = 2 * P_STAGE + 4 * P_OUT + 3 * (g.E + 2) * 4;
   if (hipFuncSetAttribute((const void*)expert_gemm_pipe_kernel<DT, FORM>,
                           hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
     muon_set_error("muon_expert_linear: %d bytes of LDS refused", lds);
