@@ -297,31 +297,58 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void expert_gemm_kernel(GArgs g) {
 
 // ---- 16-bit types, whole 16-byte runs: operands straight to LDS --------------------------------
 //
-// 256 x 256 tile, K-tiles of 64, four waves of 128 x 128 (8 x 8 accumulators of 16 x 16). The panels are
-// those above; they come by loads that write LDS themselves, two K-tiles ahead: those of K-tile k + 2 go out
-// after the barrier of K-tile k, when every wave has the last fragments of K-tile k's panels. A K-tile is two
-// substeps of 32 k; each multiplies one set of fragments while the next set is read.
+// 256 x 256 tile, four waves of 128 x 128 (8 x 8 accumulators of 16 x 16), 32 k a step. The panels of four
+// steps stand in LDS; they come by loads that write LDS themselves, four steps ahead: those of step s + 4
+// go out during step s, into the place of step s, whose fragments every wave has by the barrier before it,
+// and are waited for at the end of step s + 2. A step multiplies one set of fragments while the next
+// step's are read.
+//
+// A KC panel has rows of 32 k, 64 bytes, chunk c of row r at c ^ ((r >> 2) & 3); a KR panel is as above.
 //
 // Nothing is masked beyond what the buffer's size cuts off (what lies behind it arrives as zeros): rows and
-// columns of a tile behind its own are others' values or zeros, and are not stored. Along k, a KR panel's
-// buffer ends with its last k; of a KC panel the lanes behind the last k point behind the buffer.
-constexpr int P_PANEL = 256 * BK * 2, P_STAGE = 2 * P_PANEL;
+// columns of a tile behind its own are others' values or zeros, and are not stored. Along k, whose steps
+// come in pairs, a KR panel's buffer ends with its last k; of a KC panel the lanes behind the last k point
+// behind the buffer.
+constexpr int P_K = 32, P_PANEL = 256 * P_K * 2, P_STAGE = 2 * P_PANEL, P_STAGES = 4;
 constexpr int P_OUT_ROW = 256 + 16, P_OUT = 16 * P_OUT_ROW;  // a wave's rows on their way out
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
 
-// One load of 1 KB, 16 bytes a lane in order, to the LDS address m0, which takes a wait state.
+// One load of 1 KB, 16 bytes a lane in order, to the LDS address m0, which takes a wait state. Scalar
+// registers that a vector instruction wrote (a readfirstlane) take five before a load reads them, which
+// the compiler does not see here: scalar_wait, or products, stand between.
 MUON_DEVICE void dma_1k(u32x4 rs, uint32_t vo, uint32_t so, uint32_t m0) {
   asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
                ::"v"(vo), "s"(rs), "s"(so), "s"(m0) : "m0");
 }
 
-// One operand of a tile as its loads see it.
+MUON_DEVICE void scalar_wait() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 7" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+MUON_DEVICE int swz_step(int r) { return (r >> 2) & 3; }
+
+// 8 consecutive k (lane / 16) of row or column r0 + lane % 16 of a step's panel.
+template <bool KR>
+MUON_DEVICE muon_u4 step_fragment(uint8_t* lds, int r0) {
+  if constexpr (KR) {
+    return fragment<256, true>(lds, r0, 0);
+  } else {
+    const int lane = threadIdx.x & 63, row = r0 + (lane & 15);
+    return *(const muon_u4*)(lds + row * P_K * 2 + (((lane >> 4) ^ swz_step(row)) << 4));
+  }
+}
+
+// One operand of a tile as its loads see it: 4 loads a step for each wave.
 template <bool KR>
 struct Source {
-  const char* base;  // the panel at k = 0
+  const char* base;  // where the buffer begins: the panel at k = 0, or a later k
   int64_t bytes;     // from there to the end of what may be read
+  u32x4 rs;          // the buffer
+  uint32_t so;       // the next pair of steps' offset in it
   uint32_t step;     // bytes of a row
-  uint32_t vo[2];    // this lane's place: of even and odd slabs (KR), of whole and of the last K-tile (KC)
+  uint32_t vo[3];    // this lane's place: of even and odd loads (KR), or (KC) of all steps, the last but one, the last
 
   // rows: from the panel's first row (KC) or k = 0 (KR); columns: k (KC) or from the panel's first (KR)
   MUON_DEVICE void set(const uint16_t* p, int64_t ld, int64_t rows, int columns, int K) {
@@ -329,32 +356,44 @@ struct Source {
     base = (const char*)p;
     step = (uint32_t)ld * 2;
     bytes = rows && columns ? ((rows - 1) * ld + columns) * 2 : 0;
+    buffer();
     if constexpr (KR) {
       const int r = wave * 2 + (lane >> 5), c = (lane & 31) ^ ((r & 3) << 2);
       vo[0] = r * step + c * 16;
       vo[1] = r * step + (c ^ 2) * 16;
     } else {
-      const int r = wave * 8 + (lane >> 3), c = (lane & 7) ^ swz_kc(r);
+      const int r = wave * 16 + (lane >> 2), c = (lane & 3) ^ swz_step(r);
+      const int rest = K - std::max(0, (K - 1) / (2 * P_K)) * (2 * P_K);  // k of the last two steps
       vo[0] = r * step + c * 16;
-      vo[1] = c * 8 < K - (K - 1) / BK * BK ? vo[0] : 0x80000000u;
+      vo[1] = c * 8 < rest ? vo[0] : 0x80000000u;
+      vo[2] = c * 8 + P_K < rest ? vo[0] : 0x80000000u;
     }
   }
-  // The buffer of K-tile kt; without `any` it is empty, and loads of it write zeros.
-  MUON_DEVICE u32x4 buffer(int kt, bool any) const {
-    const char* b = KR ? base + (int64_t)kt * BK * step : base;
-    const int64_t left = KR ? bytes - (int64_t)kt * BK * step : bytes;
-    const uint32_t n = left <= 0 || !any ? 0u : (uint32_t)std::min<int64_t>(left, 0x7fffffff);
-    const uint64_t a = (uint64_t)b;
-    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)a),
-                 (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) & 0xffffu,
-                 (uint32_t)__builtin_amdgcn_readfirstlane((int)n), 0x00020000u};
+  MUON_DEVICE void buffer() {
+    const uint64_t a = (uint64_t)base;
+    const uint32_t n = bytes <= 0 ? 0u : (uint32_t)std::min<int64_t>(bytes, 0x7fffffff);
+    rs = u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)a),
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) & 0xffffu,
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)n), 0x00020000u};
+    so = 0;
   }
-  // slab q of 8 of this wave: of K-tile kt (the last of K: `last`) to LDS at `to`
-  MUON_DEVICE void load(u32x4 rs, int q, int kt, bool last, uint32_t to) const {
+  // Nothing is left: loads write zeros.
+  MUON_DEVICE void close() { rs[2] = 0; }
+  // To the next pair of steps; long before the offset leaves 31 bits the buffer begins anew.
+  MUON_DEVICE void advance() {
+    so += KR ? 2 * P_K * step : 4 * P_K;
+    if (KR && so >= (1u << 30)) {
+      base += so;
+      bytes -= so;
+      buffer();
+    }
+  }
+  // load q of 4 of this wave: of half h of the pair (`last`: K's last) to LDS at `to`
+  MUON_DEVICE void load(int q, int h, bool last, uint32_t to) const {
     if constexpr (KR)
-      dma_1k(rs, vo[q & 1], q * 8 * step, to + q * 4096);
+      dma_1k(rs, vo[q & 1], so + (q * 8 + h * P_K) * step, to + q * 4096);
     else
-      dma_1k(rs, last ? vo[1] : vo[0], q * 32 * step + kt * (BK * 2), to + q * 4096);
+      dma_1k(rs, last ? vo[1 + h] : vo[0], so + q * 64 * step + h * (P_K * 2), to + q * 4096);
   }
 };
 
@@ -367,8 +406,17 @@ MUON_DEVICE void mfma_acc(f32x4& c, muon_u4 a, muon_u4 b) {
   else
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
-// Reads of the accumulators by other instructions wait for the last of them, which the compiler does
-// not see, and their first use for the writes of their zeros.
+// c = 0, by a product of zeros: what other instructions wrote would have to be waited for, and the
+// compiler, which does not see that, puts such writes right before the products.
+template <int DT>
+MUON_DEVICE void mfma_zero(f32x4& c, muon_u4 zero) {
+  if constexpr (DT == MUON_DT_BF16)
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %1, 0" : "=a"(c) : "v"(zero));
+  else
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %1, 0" : "=a"(c) : "v"(zero));
+}
+// Reads of the accumulators by other instructions wait for the last product, as do vector
+// instructions' results that products read.
 MUON_DEVICE void mfma_wait() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
@@ -481,7 +529,7 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
   constexpr int BM = 256, BN = 256;
   constexpr bool KRA = FORM == WGT, KRB = FORM != FWD;
   extern __shared__ __align__(16) uint8_t smem[];
-  Walk<FORM> walk(g, (int*)(smem + 2 * P_STAGE + 4 * P_OUT));
+  Walk<FORM> walk(g, (int*)(smem + P_STAGES * P_STAGE + 4 * P_OUT));
   Tile t;
   if (!walk.tile(walk.at, t)) return;
 
@@ -489,11 +537,11 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
   const int wm = wave & 1, wn = wave >> 1;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem + wave * 1024;
 
-  // What the loads are at: a tile's sources, and its next K-tile. They run two K-tiles ahead of the
+  // What the loads are at: a tile's sources, and its next pair of steps. They run four steps ahead of the
   // products, across tiles.
   Source<KRA> a;
   Source<KRB> b;
-  int next = walk.at, kt_next = 0, kt_all = 0;
+  int next = walk.at, pair = 0, pairs = 0;
   auto open = [&](const Tile& o) {
     const uint16_t *A = (const uint16_t*)g.a, *B = (const uint16_t*)g.b;
     if constexpr (FORM == WGT) {
@@ -507,118 +555,124 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
       else
         b.set(B + o.e * g.sb + o.tn * BN, g.ldb, o.K, g.N - o.tn * BN, o.K);
     }
-    kt_next = 0;
-    kt_all = std::max(1, (o.K + BK - 1) / BK);
+    pair = 0;
+    pairs = std::max(1, (o.K + BK - 1) / BK);
   };
-  // to the next K-tile; kt_all = 0: there is none, and loads write zeros
+  // to the next pair of steps, of the next tile where this one has no more
   auto advance = [&] {
-    if (++kt_next < kt_all) return;
+    a.advance();
+    b.advance();
+    if (++pair < pairs) return;
     next += P_LANE;
     Tile o;
-    if (walk.tile(next, o)) open(o);
-    else kt_all = 0;
+    if (walk.tile(next, o)) {
+      open(o);
+    } else {
+      a.close();
+      b.close();
+    }
   };
-  u32x4 ra, rb;
-  auto load_a = [&](int q, int st) { a.load(ra, q, kt_next, kt_next + 1 == kt_all, lds0 + st * P_STAGE); };
-  auto load_b = [&](int q, int st) {
-    b.load(rb, q, kt_next, kt_next + 1 == kt_all, lds0 + st * P_STAGE + P_PANEL);
-  };
-  auto buffers = [&] {
-    ra = a.buffer(kt_next, kt_all != 0);
-    rb = b.buffer(kt_next, kt_all != 0);
-  };
+  auto load_a = [&](int q, int h, int st) { a.load(q, h, pair + 1 == pairs, lds0 + st * P_STAGE); };
+  auto load_b = [&](int q, int h, int st) { b.load(q, h, pair + 1 == pairs, lds0 + st * P_STAGE + P_PANEL); };
   f32x4 acc[8][8];
   muon_u4 fa[2][8], fb[2][8];
-  // fragment n of the 16 of a substep, those of b first: its first products take all of them
-  auto read = [&](int to, int st, int ks, int n) {
+  // fragment n of the 16 of a step, those of b first: its first products take all of them
+  auto read = [&](int to, int st, int n) {
     uint8_t* p = smem + st * P_STAGE;
-    if (n < 8) fb[to][n] = fragment<BN, KRB>(p + P_PANEL, wn * 128 + n * 16, ks);
-    else fa[to][n - 8] = fragment<BM, KRA>(p, wm * 128 + (n - 8) * 16, ks);
+    if (n < 8) fb[to][n] = step_fragment<KRB>(p + P_PANEL, wn * 128 + n * 16);
+    else fa[to][n - 8] = step_fragment<KRA>(p, wm * 128 + (n - 8) * 16);
   };
-  // One substep: 64 products on one set of fragments, the other set read between those of the first
-  // six rows, and the loads of a slab of either panel between those of every row. A wave issues in
-  // order, and each product leaves three slots before the next can start: what stands together
-  // between two products holds the second one up.
-  auto substep = [&](auto from_c, int st, auto loads_c, int load_st) {
-    constexpr int from = decltype(from_c)::value, to = from ^ 1;
-    constexpr bool loads = decltype(loads_c)::value;
+  // Step h of a pair, whose panels stood in place st: 64 products on one set of fragments, the other
+  // set, of the next step, read between those of the first six rows, and the loads of the step four ahead
+  // between those of every row. A wave issues in order, and each product leaves three slots before
+  // the next can start: what stands together between two products holds the second one up.
+  int stores = 0;  // a bit for each step whose end does not wait for a finished tile's stores
+  auto step = [&](auto half, int st) {
+    constexpr int h = decltype(half)::value, to = h ^ 1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        mfma_acc<DT>(acc[i][j], fb[from][j], fa[from][i]);
+        mfma_acc<DT>(acc[i][j], fb[h][j], fa[h][i]);
         const int n = i * 3 + j / 2;
         if (j % 2 == 0 && j < 6 && n < 16) {
           __builtin_amdgcn_sched_barrier(0);
-          read(to, st, to, n);
+          read(to, (st + 1) & 3, n);
         }
-        if (loads && j == 5) load_a(i, load_st);
-        if (loads && j == 7) load_b(i, load_st);
+        if (j == 7 && i < 4) load_a(i, h, st);
+        if (j == 7 && i >= 4) load_b(i - 4, h, st);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    // of this wave's loads those of the last two steps may be under way, and the 32 stores of a tile
+    // that ended before them
+    asm volatile("s_waitcnt vmcnt(48) lgkmcnt(0)\n\ts_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 .Lstores%=\n\t"
+                 "s_waitcnt vmcnt(16)\n.Lstores%=:\n\ts_barrier" ::"s"(stores) : "scc", "memory");
+    stores >>= 1;
+    __builtin_amdgcn_sched_barrier(0);
   };
-  typedef std::integral_constant<int, 0> Zero;
-  typedef std::integral_constant<int, 1> One;
   open(t);
 #pragma unroll
-  for (int st = 0; st < 2; ++st) {
-    buffers();
+  for (int st = 0; st < P_STAGES; ++st) {
+    scalar_wait();
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      load_a(q, st);
-      load_b(q, st);
-    }
-    advance();
+    for (int q = 0; q < 4; ++q) load_a(q, st & 1, st);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) load_b(q, st & 1, st);
+    if (st & 1) advance();
   }
   asm volatile("s_waitcnt vmcnt(16)\n\ts_barrier" ::: "memory");
 #pragma unroll
-  for (int n = 0; n < 16; ++n) read(0, 0, 0, n);
+  for (int n = 0; n < 16; ++n) read(0, 0, n);
+  // every wave has the first step's fragments before their place is loaded anew
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
   int st = 0;
   for (int at = walk.at;;) {
     const int KT = std::max(1, (t.K + BK - 1) / BK);
+    const muon_u4 zero = {0, 0, 0, 0};
+    mfma_wait();
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    mfma_wait();
+      for (int j = 0; j < 8; ++j) mfma_zero<DT>(acc[i][j], zero);
+#pragma clang loop unroll(disable)
     for (int kt = 0; kt < KT; ++kt) {
-substep(Zero{}, st, std::false_type{}, 0);
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-      buffers();
-      substep(One{}, st ^ 1, std::true_type{}, st);
-      st ^= 1;
+      step(std::integral_constant<int, 0>{}, st);
+      step(std::integral_constant<int, 1>{}, st + 1);
+      st ^= 2;
       advance();
     }
     mfma_wait();
 
     // 16 rows of the wave's 128 columns at a time through its own LDS: a lane has four consecutive columns
-    // of one row, and stores 16 bytes of a line
+    // of one row, and stores 16 bytes of a line; what is none of the tile's points behind the buffer,
+    // so that every wave has 32 stores
     int r = lane & 15, l = lane >> 4;
     asm volatile("" : "+v"(r), "+v"(l));  // or their products are made before the loop, and spilled
-    uint8_t* mine = smem + 2 * P_STAGE + wave * P_OUT;
-    const int c = wn * 128 + r * 8;
-    char* out = (char*)((uint16_t*)g.c + (FORM == WGT ? (int64_t)t.e * g.M + t.tm * BM : (int64_t)t.row0) * g.N +
-                        (int64_t)(wm * 128 + l) * g.N + t.tn * BN + c);
-    int row = c < t.N ? wm * 128 + l : BM;
-    const int64_t four = (int64_t)g.N * 8;
+    uint8_t* mine = smem + P_STAGES * P_STAGE + wave * P_OUT;
+    const int c = wn * 128 + r * 8, m = t.M - wm * 128 - l;
+    const uint64_t out = (uint64_t)((uint16_t*)g.c + (FORM == WGT ? (int64_t)t.e * g.M + t.tm * BM : (int64_t)t.row0) * g.N +
+                                    (int64_t)(wm * 128) * g.N + t.tn * BN);
+    const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)out, 0, 0x7fffffff, 0x00020000);
+    const uint32_t vo = c < t.N ? (uint32_t)l * g.N * 2 + c * 2 : 0x80000000u;
+    const uint32_t four = (uint32_t)g.N * 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        *(uint2*)(mine + r * P_OUT_ROW + j * 32 + l * 8) =
-            make_uint2(pack2<DT>(acc[i][j][0], acc[i][j][1]), pack2<DT>(acc[i][j][2], acc[i][j][3]));
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t w[2] = {pack2<DT>(acc[i][j][0], acc[i][j][1]), pack2<DT>(acc[i][j][2], acc[i][j][3])};
+        __builtin_memcpy(__builtin_assume_aligned(mine + r * P_OUT_ROW + j * 32 + l * 8, 8), w, 8);
+      }
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        const muon_u4 w = *(const muon_u4*)(mine + (p * 4 + l) * P_OUT_ROW + r * 16);
-        if (row < t.M) *(muon_u4*)out = w;
-        out += four;
-        row += 4;
+        muon_u4 w;
+        __builtin_memcpy(&w, __builtin_assume_aligned(mine + (p * 4 + l) * P_OUT_ROW + r * 16, 16), 16);
+        __builtin_amdgcn_raw_buffer_store_b128(w, rc, i * 16 + p * 4 < m ? vo : 0x80000000u, (i * 4 + p) * four, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    stores = 3;
     at += P_LANE;
     if (!walk.tile(at, t)) break;
   }
@@ -793,7 +847,7 @@ int launch_pipe(GArgs g, hipStream_t s) {
     muon_set_error("muon_expert_linear: too many tiles");
     return MUON_ERR_SHAPE;
   }
-  const int lds = 2 * P_STAGE + 4 * P_OUT + 3 * (g.E + 2) * 4;
+  const int lds = P_STAGES * P_STAGE + 4 * P_OUT + 3 * (g.E + 2) * 4;
   if (hipFuncSetAttribute((const void*)expert_gemm_pipe_kernel<DT, FORM>,
                           hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
     muon_set_error("muon_expert_linear: %d bytes of LDS refused", lds);
