@@ -297,19 +297,20 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void expert_gemm_kernel(GArgs g) {
 
 // ---- 16-bit types, whole 16-byte runs: operands straight to LDS --------------------------------
 //
-// 256 x 256 tile, four waves of 128 x 128 (8 x 8 accumulators of 16 x 16), 32 k a step. The panels of four
-// steps stand in LDS; they come by loads that write LDS themselves, four steps ahead: those of step s + 4
-// go out during step s, into the place of step s, whose fragments every wave has by the barrier before it,
-// and are waited for at the end of step s + 2. A step multiplies one set of fragments while the next
-// step's are read.
-//
-// A KC panel has rows of 32 k, 64 bytes, chunk c of row r at c ^ ((r >> 2) & 3); a KR panel is as above.
+// 256 x 256 tile, K-tiles of 64, four waves of 128 x 128 (8 x 8 accumulators of 16 x 16). A K-tile is two
+// steps, of the upper and of the lower 64 rows of every wave, over all 64 k. The panels of two K-tiles
+// stand in LDS, that of a as two halves of the rows of one step each; they come by loads that write LDS
+// themselves. A step multiplies one set of fragments while the next step's are read, so that during K-tile t
+//   step 0 reads the lower a of t, and loads the b of t + 2 into the place of t's;
+//   step 1 reads the b and the upper a of t + 1, and loads the a of t + 2 into the places of t's:
+// each load has two to three steps to arrive, and covers whole lines of 128 bytes along k. (With steps
+// of 32 k of all rows, whose loads take half lines of a KC panel, FWD ran at 1141 TFLOP/s where WGT did
+// at 1228.)
 //
 // Nothing is masked beyond what the buffer's size cuts off (what lies behind it arrives as zeros): rows and
-// columns of a tile behind its own are others' values or zeros, and are not stored. Along k, whose steps
-// come in pairs, a KR panel's buffer ends with its last k; of a KC panel the lanes behind the last k point
-// behind the buffer.
-constexpr int P_K = 32, P_PANEL = 256 * P_K * 2, P_STAGE = 2 * P_PANEL, P_STAGES = 4;
+// columns of a tile behind its own are others' values or zeros, and are not stored. Along k, a KR panel's
+// buffer ends with its last k; of a KC panel the lanes behind the last k point behind the buffer.
+constexpr int P_HALF = 128 * BK * 2, P_PANEL = 2 * P_HALF, P_STAGE = 2 * P_PANEL;
 constexpr int P_OUT_ROW = 256 + 16, P_OUT = 16 * P_OUT_ROW;  // a wave's rows on their way out
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
 
@@ -327,28 +328,16 @@ MUON_DEVICE void scalar_wait() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-MUON_DEVICE int swz_step(int r) { return (r >> 2) & 3; }
-
-// 8 consecutive k (lane / 16) of row or column r0 + lane % 16 of a step's panel.
-template <bool KR>
-MUON_DEVICE muon_u4 step_fragment(uint8_t* lds, int r0) {
-  if constexpr (KR) {
-    return fragment<256, true>(lds, r0, 0);
-  } else {
-    const int lane = threadIdx.x & 63, row = r0 + (lane & 15);
-    return *(const muon_u4*)(lds + row * P_K * 2 + (((lane >> 4) ^ swz_step(row)) << 4));
-  }
-}
-
-// One operand of a tile as its loads see it: 4 loads a step for each wave.
-template <bool KR>
+// One operand of a tile as its loads see it, 8 a K-tile for each wave. SPLIT: the a panel, in halves of
+// the first and the second 64 of every 128 rows (KC) or columns (KR).
+template <bool KR, bool SPLIT>
 struct Source {
   const char* base;  // where the buffer begins: the panel at k = 0, or a later k
   int64_t bytes;     // from there to the end of what may be read
   u32x4 rs;          // the buffer
-  uint32_t so;       // the next pair of steps' offset in it
+  uint32_t so;       // the next K-tile's offset in it
   uint32_t step;     // bytes of a row
-  uint32_t vo[3];    // this lane's place: of even and odd loads (KR), or (KC) of all steps, the last but one, the last
+  uint32_t vo[2];    // this lane's place: of even and odd loads (KR), or of all K-tiles and of the last (KC)
 
   // rows: from the panel's first row (KC) or k = 0 (KR); columns: k (KC) or from the panel's first (KR)
   MUON_DEVICE void set(const uint16_t* p, int64_t ld, int64_t rows, int columns, int K) {
@@ -357,16 +346,17 @@ struct Source {
     step = (uint32_t)ld * 2;
     bytes = rows && columns ? ((rows - 1) * ld + columns) * 2 : 0;
     buffer();
-    if constexpr (KR) {
+    if constexpr (KR && SPLIT) {  // four k a load, 16 chunks of each
+      const int r = wave * 4 + (lane >> 4), c = (lane & 15) ^ swz_kr(r);
+      vo[0] = vo[1] = r * step + (c & 7) * 16 + (c >> 3) * 256;
+    } else if constexpr (KR) {  // two k a load, 32 chunks
       const int r = wave * 2 + (lane >> 5), c = (lane & 31) ^ ((r & 3) << 2);
       vo[0] = r * step + c * 16;
       vo[1] = r * step + (c ^ 2) * 16;
-    } else {
-      const int r = wave * 16 + (lane >> 2), c = (lane & 3) ^ swz_step(r);
-      const int rest = K - std::max(0, (K - 1) / (2 * P_K)) * (2 * P_K);  // k of the last two steps
+    } else {  // eight rows a load, 8 chunks
+      const int r = wave * 8 + (lane >> 3), c = (lane & 7) ^ swz_kc(r);
       vo[0] = r * step + c * 16;
-      vo[1] = c * 8 < rest ? vo[0] : 0x80000000u;
-      vo[2] = c * 8 + P_K < rest ? vo[0] : 0x80000000u;
+      vo[1] = c * 8 < K - std::max(0, (K - 1) / BK) * BK ? vo[0] : 0x80000000u;
     }
   }
   MUON_DEVICE void buffer() {
@@ -379,21 +369,24 @@ struct Source {
   }
   // Nothing is left: loads write zeros.
   MUON_DEVICE void close() { rs[2] = 0; }
-  // To the next pair of steps; long before the offset leaves 31 bits the buffer begins anew.
+  // To the next K-tile; long before the offset leaves 31 bits the buffer begins anew.
   MUON_DEVICE void advance() {
-    so += KR ? 2 * P_K * step : 4 * P_K;
+    so += KR ? BK * step : BK * 2;
     if (KR && so >= (1u << 30)) {
       base += so;
       bytes -= so;
       buffer();
     }
   }
-  // load q of 4 of this wave: of half h of the pair (`last`: K's last) to LDS at `to`
-  MUON_DEVICE void load(int q, int h, bool last, uint32_t to) const {
-    if constexpr (KR)
-      dma_1k(rs, vo[q & 1], so + (q * 8 + h * P_K) * step, to + q * 4096);
-    else
-      dma_1k(rs, last ? vo[1 + h] : vo[0], so + q * 64 * step + h * (P_K * 2), to + q * 4096);
+  // load q of 8 of this wave (SPLIT: 4 of either half; `last`: K's last K-tile) to LDS at `to`
+  MUON_DEVICE void load(int q, bool last, uint32_t to) const {
+    const int h = q >> 2, p = q & 3;
+    uint32_t at;
+    if constexpr (KR && SPLIT) at = p * 16 * step + h * 128;
+    else if constexpr (KR) at = q * 8 * step;
+    else if constexpr (SPLIT) at = ((p >> 1) * 128 + h * 64 + (p & 1) * 32) * step;
+    else at = q * 32 * step;
+    dma_1k(rs, KR ? vo[q & 1] : last ? vo[1] : vo[0], so + at, to + q * 4096);
   }
 };
 
@@ -441,7 +434,7 @@ struct Walk {
   MUON_DEVICE Walk(const GArgs& g_, int* lds)
       : g(g_), first(lds), start_of(lds + g_.E + 2), rows_of(lds + 2 * (g_.E + 2)) {
     const int lane = threadIdx.x & 63, per = (g.E + 64) / 64;
-    constexpr int UNIT = FORM == WGT ? BK : 256;
+    constexpr int UNIT = FORM == WGT ? 2 * BK : 256;
     const int e0 = lane * per, e1 = std::min(e0 + per, g.E + 1);
     int mine = 0, start, n;
     for (int i = e0; i < e1; ++i) {
@@ -524,12 +517,16 @@ struct Walk {
   }
 };
 
+// K-tiles go by twos, since two sets of b fragments take turns; one at least, of nothing, so that every
+// tile is written.
+MUON_DEVICE int k_pairs(int K) { return std::max(1, (K + 2 * BK - 1) / (2 * BK)); }
+
 template <int DT, int FORM>
 __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
   constexpr int BM = 256, BN = 256;
   constexpr bool KRA = FORM == WGT, KRB = FORM != FWD;
   extern __shared__ __align__(16) uint8_t smem[];
-  Walk<FORM> walk(g, (int*)(smem + P_STAGES * P_STAGE + 4 * P_OUT));
+  Walk<FORM> walk(g, (int*)(smem + 2 * P_STAGE + 4 * P_OUT));
   Tile t;
   if (!walk.tile(walk.at, t)) return;
 
@@ -537,11 +534,11 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
   const int wm = wave & 1, wn = wave >> 1;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem + wave * 1024;
 
-  // What the loads are at: a tile's sources, and its next pair of steps. They run four steps ahead of the
+  // What the loads are at: a tile's sources, and its next K-tile. They run two K-tiles ahead of the
   // products, across tiles.
-  Source<KRA> a;
-  Source<KRB> b;
-  int next = walk.at, pair = 0, pairs = 0;
+  Source<KRA, true> a;
+  Source<KRB, false> b;
+  int next = walk.at, kt_next = 0, kt_last = 0, kt_all = 0;
   auto open = [&](const Tile& o) {
     const uint16_t *A = (const uint16_t*)g.a, *B = (const uint16_t*)g.b;
     if constexpr (FORM == WGT) {
@@ -555,81 +552,95 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
       else
         b.set(B + o.e * g.sb + o.tn * BN, g.ldb, o.K, g.N - o.tn * BN, o.K);
     }
-    pair = 0;
-    pairs = std::max(1, (o.K + BK - 1) / BK);
+    kt_next = 0;
+    kt_last = (o.K + BK - 1) / BK - 1;
+    kt_all = 2 * k_pairs(o.K);
   };
-  // to the next pair of steps, of the next tile where this one has no more
+  // to the next K-tile, of the next tile where this one has no more
   auto advance = [&] {
     a.advance();
     b.advance();
-    if (++pair < pairs) return;
-    next += P_LANE;
-    Tile o;
-    if (walk.tile(next, o)) {
-      open(o);
-    } else {
-      a.close();
-      b.close();
-    }
-  };
-  auto load_a = [&](int q, int h, int st) { a.load(q, h, pair + 1 == pairs, lds0 + st * P_STAGE); };
-  auto load_b = [&](int q, int h, int st) { b.load(q, h, pair + 1 == pairs, lds0 + st * P_STAGE + P_PANEL); };
-  f32x4 acc[8][8];
-  muon_u4 fa[2][8], fb[2][8];
-  // fragment n of the 16 of a step, those of b first: its first products take all of them
-  auto read = [&](int to, int st, int n) {
-    uint8_t* p = smem + st * P_STAGE;
-    if (n < 8) fb[to][n] = step_fragment<KRB>(p + P_PANEL, wn * 128 + n * 16);
-    else fa[to][n - 8] = step_fragment<KRA>(p, wm * 128 + (n - 8) * 16);
-  };
-  // Step h of a pair, whose panels stood in place st: 64 products on one set of fragments, the other
-  // set, of the next step, read between those of the first six rows, and the loads of the step four ahead
-  // between those of every row. A wave issues in order, and each product leaves three slots before
-  // the next can start: what stands together between two products holds the second one up.
-  int stores = 0;  // a bit for each step whose end does not wait for a finished tile's stores
-  auto step = [&](auto half, int st) {
-    constexpr int h = decltype(half)::value, to = h ^ 1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        mfma_acc<DT>(acc[i][j], fb[h][j], fa[h][i]);
-        const int n = i * 3 + j / 2;
-        if (j % 2 == 0 && j < 6 && n < 16) {
-          __builtin_amdgcn_sched_barrier(0);
-          read(to, (st + 1) & 3, n);
-        }
-        if (j == 7 && i < 4) load_a(i, h, st);
-        if (j == 7 && i >= 4) load_b(i - 4, h, st);
-        __builtin_amdgcn_sched_barrier(0);
+    if (++kt_next <= kt_last) return;
+    if (kt_next >= kt_all) {
+      next += P_LANE;
+      Tile o;
+      if (walk.tile(next, o)) {
+        open(o);
+        return;
       }
     }
-    // of this wave's loads those of the last two steps may be under way, and the 32 stores of a tile
-    // that ended before them
-    asm volatile("s_waitcnt vmcnt(48) lgkmcnt(0)\n\ts_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 .Lstores%=\n\t"
-                 "s_waitcnt vmcnt(16)\n.Lstores%=:\n\ts_barrier" ::"s"(stores) : "scc", "memory");
+    a.close();  // the second of a pair that has one, or no more tiles
+    b.close();
+  };
+  auto load_a = [&](int q, int st) { a.load(q, kt_next == kt_last, lds0 + st * P_STAGE); };
+  auto load_b = [&](int q, int st) { b.load(q, kt_next == kt_last, lds0 + st * P_STAGE + P_PANEL); };
+  f32x4 acc[8][8];
+  muon_u4 fa[2][8], fb[2][16];  // [k half * 4 + i], [k half * 8 + j], of two steps and of two K-tiles
+  auto read_a = [&](int half, int st, int n) {
+    fa[half][n] = fragment<KRA ? 128 : 256, KRA>(smem + st * P_STAGE + half * P_HALF, wm * 64 + (n & 3) * 16, n >> 2);
+  };
+  auto read_b = [&](int to, int st, int n) {
+    fb[to][n] = fragment<BN, KRB>(smem + st * P_STAGE + P_PANEL, wn * 128 + (n & 7) * 16, n >> 3);
+  };
+  // Step `half` of the K-tile in place st (`set`, the b fragments): 64 products, and between them the reads
+  // of the next step's fragments and the loads. A wave issues in order, and each product leaves
+  // three slots before the next can start: what stands together between two products holds the
+  // second one up.
+  int stores = 0;  // a bit for each step whose end does not wait for a finished tile's stores
+  auto step = [&](auto half_c, auto set_c) {
+    constexpr int half = decltype(half_c)::value, set = decltype(set_c)::value;
+#pragma unroll
+    for (int n = 0; n < 64; ++n) {
+      const int ks = n >> 5, i = (n >> 3) & 3, j = n & 7;
+      mfma_acc<DT>(acc[half * 4 + i][j], fb[set][ks * 8 + j], fa[half][ks * 4 + i]);
+      if (half == 0 && n % 4 == 1 && n < 32) {
+        __builtin_amdgcn_sched_barrier(0);
+        read_a(1, set, n / 4);
+      }
+      if (half == 1 && n % 2 == 1 && n < 48) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (n < 32) read_b(set ^ 1, set ^ 1, n / 2);
+        else read_a(0, set ^ 1, n / 2 - 16);
+      }
+      if (n % 8 == 6) {
+        if (half == 0) load_b(n / 8, set);
+        else load_a(n / 8, set);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // What the next step reads has arrived: at the end of step 0 the b and upper a of the next K-tile, at
+    // that of step 1 its lower a. Newer than those are 4 + 8 or 8 + 8 loads, and, right after a tile, its 32 stores.
+    if constexpr (half == 0)
+      asm volatile("s_waitcnt vmcnt(44) lgkmcnt(0)\n\ts_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 .Lstores%=\n\t"
+                   "s_waitcnt vmcnt(12)\n.Lstores%=:\n\ts_barrier" ::"s"(stores) : "scc", "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(48) lgkmcnt(0)\n\ts_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 .Lstores%=\n\t"
+                   "s_waitcnt vmcnt(16)\n.Lstores%=:\n\ts_barrier" ::"s"(stores) : "scc", "memory");
     stores >>= 1;
     __builtin_amdgcn_sched_barrier(0);
   };
+  typedef std::integral_constant<int, 0> Zero;
+  typedef std::integral_constant<int, 1> One;
   open(t);
 #pragma unroll
-  for (int st = 0; st < P_STAGES; ++st) {
+  for (int st = 0; st < 2; ++st) {
     scalar_wait();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) load_a(q, st & 1, st);
+    for (int q = 0; q < 8; ++q) load_b(q, st);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) load_b(q, st & 1, st);
-    if (st & 1) advance();
+    for (int q = 0; q < 8; ++q) load_a(q, st);
+    advance();
   }
   asm volatile("s_waitcnt vmcnt(16)\n\ts_barrier" ::: "memory");
 #pragma unroll
-  for (int n = 0; n < 16; ++n) read(0, 0, n);
-  // every wave has the first step's fragments before their place is loaded anew
+  for (int n = 0; n < 16; ++n) read_b(0, 0, n);
+#pragma unroll
+  for (int n = 0; n < 8; ++n) read_a(0, 0, n);
+  // every wave has these fragments before their place is loaded anew
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
-  int st = 0;
   for (int at = walk.at;;) {
-    const int KT = std::max(1, (t.K + BK - 1) / BK);
+    const int pairs = k_pairs(t.K);
     const muon_u4 zero = {0, 0, 0, 0};
     mfma_wait();
 #pragma unroll
@@ -637,10 +648,12 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) mfma_zero<DT>(acc[i][j], zero);
 #pragma clang loop unroll(disable)
-    for (int kt = 0; kt < KT; ++kt) {
-      step(std::integral_constant<int, 0>{}, st);
-      step(std::integral_constant<int, 1>{}, st + 1);
-      st ^= 2;
+    for (int p = 0; p < pairs; ++p) {
+      step(Zero{}, Zero{});
+      step(One{}, Zero{});
+      advance();
+      step(Zero{}, One{});
+      step(One{}, One{});
       advance();
     }
     mfma_wait();
@@ -650,7 +663,7 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
     // so that every wave has 32 stores
     int r = lane & 15, l = lane >> 4;
     asm volatile("" : "+v"(r), "+v"(l));  // or their products are made before the loop, and spilled
-    uint8_t* mine = smem + P_STAGES * P_STAGE + wave * P_OUT;
+    uint8_t* mine = smem + 2 * P_STAGE + wave * P_OUT;
     const int c = wn * 128 + r * 8, m = t.M - wm * 128 - l;
     const uint64_t out = (uint64_t)((uint16_t*)g.c + (FORM == WGT ? (int64_t)t.e * g.M + t.tm * BM : (int64_t)t.row0) * g.N +
                                     (int64_t)(wm * 128) * g.N + t.tn * BN);
@@ -847,7 +860,7 @@ int launch_pipe(GArgs g, hipStream_t s) {
     muon_set_error("muon_expert_linear: too many tiles");
     return MUON_ERR_SHAPE;
   }
-  const int lds = P_STAGES * P_STAGE + 4 * P_OUT + 3 * (g.E + 2) * 4;
+  const int lds = 2 * P_STAGE + 4 * P_OUT + 3 * (g.E + 2) * 4;
   if (hipFuncSetAttribute((const void*)expert_gemm_pipe_kernel<DT, FORM>,
                           hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
     muon_set_error("muon_expert_linear: %d bytes of LDS refused", lds);
