@@ -203,7 +203,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void expert_gemm_kernel(GArgs g) {
 
   int e, tm, tn, row0 = 0, left = 0, K, M;
   if constexpr (FORM == WGT) {
-    const int per = g.tiles_m * g.tiles_n, L = xcd_range(blockIdx.x, gridDim.x);
+    // an expert's tiles, which take as long as its rows, on all XCDs
+    const int per = g.tiles_m * g.tiles_n, L = blockIdx.x;
     e = L / per;
     tile_of(L - e * per, g.tiles_m, g.tiles_n, tm, tn);
     bounds(g, e, row0, K);
@@ -692,47 +693,124 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last loads, of nothing, into this LDS
 }
 
+// ---- 16-bit types, few rows an expert ---------------------------------------------------------
+//
+// y = x W_e^T where every expert has a few rows (single tokens): the weights are read once and nothing
+// else counts. A workgroup has 16 rows of an expert and 32 columns of its output, its four waves a quarter
+// of k each. Fragments come from memory as the products take them, 16 weight rows by 64 bytes a load,
+// several of them under way in every wave; the four sums are joined through LDS in fixed order.
+constexpr int R_N = 32, R_DEEP = 4;  // columns of a workgroup; k fragments under way
+
+// 8 values of a row from k on, 0 behind K.
+template <bool ALIGNED>
+MUON_DEVICE muon_u4 row_fragment(const uint16_t* row, int k, int K) {
+  if (k + 8 <= K) {
+    if constexpr (ALIGNED) return *(const muon_u4*)(row + k);
+    else return load_u4(row + k);
+  }
+  uint32_t u[4] = {0, 0, 0, 0};
+  if constexpr (!ALIGNED) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k + j < K) u[j / 2] |= (uint32_t)row[k + j] << (16 * (j & 1));
+  }
+  return muon_u4{u[0], u[1], u[2], u[3]};
+}
+
+template <int DT, bool ALIGNED>
+__global__ __launch_bounds__(256) void expert_rows_kernel(GArgs g) {
+  __shared__ f32x4 part[4][2][64];
+  int e, row0, left, tn;
+  if (!find_tile<16>(g, blockIdx.x, e, row0, left, tn)) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, gq = lane >> 4;
+  const int K = e < g.E ? g.K : 0, n0 = tn * R_N;
+  // rows and columns behind the last ones repeat them, and are not stored
+  const uint16_t* w[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    w[j] = (const uint16_t*)g.b + (e < g.E ? e : 0) * g.sb + (int64_t)std::min(n0 + j * 16 + r, g.N - 1) * g.ldb;
+  const uint16_t* x = (const uint16_t*)g.a + (int64_t)(row0 + std::min(r, left - 1)) * g.lda;
+  f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  const int quarter = (K + 127) / 128 * 32;
+  const int end = std::min((wave + 1) * quarter, K);
+  for (int k0 = wave * quarter; k0 < end; k0 += 32 * R_DEEP) {
+    muon_u4 fw[R_DEEP][2], fx[R_DEEP];
+#pragma unroll
+    for (int d = 0; d < R_DEEP; ++d) {
+      const int k = k0 + d * 32 + gq * 8;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) fw[d][j] = row_fragment<ALIGNED>(w[j], k, end);
+      fx[d] = row_fragment<ALIGNED>(x, k, end);
+    }
+#pragma unroll
+    for (int d = 0; d < R_DEEP; ++d)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[j] = mfma16<DT>(fw[d][j], fx[d], acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) part[wave][j][lane] = acc[j];
+  __syncthreads();
+  if (wave >= 2 || r >= left) return;
+  f32x4 v = part[0][wave][lane];
+#pragma unroll
+  for (int q = 1; q < 4; ++q) v += part[q][wave][lane];
+  const int n = n0 + wave * 16 + gq * 4;
+  uint16_t* out = (uint16_t*)g.c + (int64_t)(row0 + r) * g.N + n;
+  const uint32_t u[2] = {pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+  if (n + 4 <= g.N) {
+    __builtin_memcpy(out, u, 8);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (n + q < g.N) out[q] = (uint16_t)(u[q / 2] >> (16 * (q & 1)));
+  }
+}
+
 // ---- fp32 -----------------------------------------------------------------------------------
 //
-// 128 x 128 tile, K-tiles of 16, four waves of 64 x 64 on v_mfma_f32_32x32x2_f32. Both panels stand in LDS
-// as rows of k, whatever their order in memory, so a fragment is one value of a column for each lane.
-constexpr int F_B = 128, F_K = 16, F_P = F_B + 4;
+// 128 x 128 or 64 x 64 tile (S blocks of 32 a wave and side, 2 or 1), K-tiles of 16, four waves on
+// v_mfma_f32_32x32x2_f32. Both panels stand in LDS as rows of k, whatever their order in memory, so a fragment
+// is one value of a column for each lane.
+constexpr int F_K = 16;
 
-// Eight values of a thread: KR: row k, columns 8 c ..; KC: row r, k 8 c ..
-template <bool KR>
-MUON_DEVICE void f32_load(float (&w)[8], const float* base, int64_t ld, int in, int k0, int kleft) {
+// A thread's V = 4 S values: KR: of row k; KC: of row r, V k in a row.
+template <bool KR, int V>
+MUON_DEVICE void f32_load(float (&w)[V], const float* base, int64_t ld, int in, int k0, int kleft) {
   const int tid = threadIdx.x;
-  const int row = KR ? tid / 16 : tid / 2, ch = KR ? tid % 16 * 8 : tid % 2 * 8;
+  constexpr int EACH = F_K / V;  // threads of a KC row
+  const int row = KR ? tid / 16 : tid / EACH, ch = KR ? tid % 16 * V : tid % EACH * V;
   const bool ok = KR ? row < kleft : row < in;
   const int have = ok ? (KR ? in : kleft) - ch : 0;
   const float* p = KR ? base + (k0 + row) * ld + ch : base + row * ld + k0 + ch;
-  if (have >= 8) {
-    __builtin_memcpy(w, p, 32);
+  if (have >= V) {
+    __builtin_memcpy(w, p, 4 * V);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = j < have ? p[j] : 0.0f;
+    for (int j = 0; j < V; ++j) w[j] = j < have ? p[j] : 0.0f;
   }
 }
-template <bool KR>
-MUON_DEVICE void f32_store(float* lds, const float (&w)[8]) {
+template <bool KR, int V>
+MUON_DEVICE void f32_store(float* lds, const float (&w)[V]) {
+  constexpr int P = 16 * V + 4, EACH = F_K / V;
   const int tid = threadIdx.x;
   if constexpr (KR) {
-    float* p = lds + tid / 16 * F_P + tid % 16 * 8;
+    float* p = lds + tid / 16 * P + tid % 16 * V;
 #pragma unroll
-    for (int j = 0; j < 8; j += 4) *(float4*)(p + j) = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+    for (int j = 0; j < V; j += 4) *(float4*)(p + j) = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) lds[(tid % 2 * 8 + j) * F_P + tid / 2] = w[j];
+    for (int j = 0; j < V; ++j) lds[(tid % EACH * V + j) * P + tid / EACH] = w[j];
   }
 }
 
-template <int FORM>
+template <int FORM, int S>
 __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
+  constexpr int F_B = 64 * S, F_P = F_B + 4, V = 4 * S;
   constexpr bool KRA = FORM == WGT, KRB = FORM != FWD;
   __shared__ __align__(16) float lds[2][2][F_K * F_P];
   int e, tm, tn, row0 = 0, left = 0, K, M;
   if constexpr (FORM == WGT) {
-    const int per = g.tiles_m * g.tiles_n, L = xcd_range(blockIdx.x, gridDim.x);
+    const int per = g.tiles_m * g.tiles_n, L = blockIdx.x;
     e = L / per;
     tile_of(L - e * per, g.tiles_m, g.tiles_n, tm, tn);
     bounds(g, e, row0, K);
@@ -752,62 +830,62 @@ __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
 
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave & 1, wn = wave >> 1;
   const int fr = lane & 31, fk = lane >> 5;
-  f32x16 acc[2][2];
+  f32x16 acc[S][S];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < S; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < S; ++j)
 #pragma unroll
       for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
-  float wa[8], wb[8];
+  float wa[V], wb[V];
   const int KT = (K + F_K - 1) / F_K;
   if (KT) {
-    f32_load<KRA>(wa, A, g.lda, M, 0, K);
-    f32_load<KRB>(wb, B, g.ldb, N, 0, K);
-    f32_store<KRA>(lds[0][0], wa);
-    f32_store<KRB>(lds[0][1], wb);
+    f32_load<KRA, V>(wa, A, g.lda, M, 0, K);
+    f32_load<KRB, V>(wb, B, g.ldb, N, 0, K);
+    f32_store<KRA, V>(lds[0][0], wa);
+    f32_store<KRB, V>(lds[0][1], wb);
   }
   __syncthreads();
   for (int kt = 0; kt < KT; ++kt) {
     const bool more = kt + 1 < KT;
     if (more) {
-      f32_load<KRA>(wa, A, g.lda, M, (kt + 1) * F_K, K - (kt + 1) * F_K);
-      f32_load<KRB>(wb, B, g.ldb, N, (kt + 1) * F_K, K - (kt + 1) * F_K);
+      f32_load<KRA, V>(wa, A, g.lda, M, (kt + 1) * F_K, K - (kt + 1) * F_K);
+      f32_load<KRB, V>(wb, B, g.ldb, N, (kt + 1) * F_K, K - (kt + 1) * F_K);
     }
-    const float* la = lds[kt & 1][0] + wm * 64 + fr;
-    const float* lb = lds[kt & 1][1] + wn * 64 + fr;
+    const float* la = lds[kt & 1][0] + wm * 32 * S + fr;
+    const float* lb = lds[kt & 1][1] + wn * 32 * S + fr;
 #pragma unroll
     for (int k = 0; k < F_K; k += 2) {
-      float fa[2], fb[2];
+      float fa[S], fb[S];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < S; ++i) {
         fa[i] = la[(k + fk) * F_P + i * 32];
         fb[i] = lb[(k + fk) * F_P + i * 32];
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < S; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < S; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j], fa[i], acc[i][j], 0, 0, 0);
     }
     if (more) {
-      f32_store<KRA>(lds[(kt + 1) & 1][0], wa);
-      f32_store<KRB>(lds[(kt + 1) & 1][1], wb);
+      f32_store<KRA, V>(lds[(kt + 1) & 1][0], wa);
+      f32_store<KRB, V>(lds[(kt + 1) & 1][1], wb);
     }
     __syncthreads();
   }
   // a lane holds row fr, columns 8 (q / 4) + 4 fk + q % 4 of each 32 x 32 block
   float* C = (float*)g.c + (FORM == WGT ? ((int64_t)e * g.M + tm * F_B) * g.N : (int64_t)row0 * g.N);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int m = wm * 64 + i * 32 + fr;
+  for (int i = 0; i < S; ++i) {
+    const int m = wm * 32 * S + i * 32 + fr;
     if (m >= M) continue;
     float* out = C + (int64_t)m * g.N + tn * F_B;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < S; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int n = wn * 64 + j * 32 + q * 8 + fk * 4;
+        const int n = wn * 32 * S + j * 32 + q * 8 + fk * 4;
         if (n + 4 <= N) {
           const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
           __builtin_memcpy(out + n, v, 16);
@@ -848,6 +926,20 @@ int launch16(GArgs g, bool aligned, hipStream_t s) {
                  : run(expert_gemm_kernel<DT, FORM, BM, BN, WM, WN, false>);
 }
 
+template <int DT>
+int launch_rows(GArgs g, bool aligned, hipStream_t s) {
+  g.tiles_n = (g.N + R_N - 1) / R_N;
+  const int64_t grid = most_tiles(g.R, g.E, 16) * g.tiles_n;
+  if (grid >= (1ll << 32) / 256) {  // below 2^32 threads
+    muon_set_error("muon_expert_linear: too many tiles");
+    return MUON_ERR_SHAPE;
+  }
+  if (aligned) expert_rows_kernel<DT, true><<<(unsigned)grid, 256, 0, s>>>(g);
+  else expert_rows_kernel<DT, false><<<(unsigned)grid, 256, 0, s>>>(g);
+  MUON_CHECK_LAUNCH("muon_expert_linear");
+  return MUON_OK;
+}
+
 // What the direct loads index by 32 bits: 256 rows of a panel, 64 of one along k.
 constexpr int64_t P_MOST = 1 << 20;
 
@@ -871,30 +963,52 @@ int launch_pipe(GArgs g, hipStream_t s) {
   return MUON_OK;
 }
 
-template <int FORM>
+template <int FORM, int S>
 int launch32(GArgs g, hipStream_t s) {
-  g.tiles_m = (int)(FORM == WGT ? (g.M + F_B - 1) / F_B : most_tiles(g.R, g.E, F_B));
-  g.tiles_n = (g.N + F_B - 1) / F_B;
+  g.tiles_m = (int)(FORM == WGT ? (g.M + 64 * S - 1) / (64 * S) : most_tiles(g.R, g.E, 64 * S));
+  g.tiles_n = (g.N + 64 * S - 1) / (64 * S);
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * (FORM == WGT ? g.E : 1);
   if (grid >= (1ll << 32) / 256) {  // below 2^32 threads
     muon_set_error("muon_expert_linear: too many tiles");
     return MUON_ERR_SHAPE;
   }
-  expert_gemm_f32_kernel<FORM><<<(unsigned)grid, 256, 0, s>>>(g);
+  expert_gemm_f32_kernel<FORM, S><<<(unsigned)grid, 256, 0, s>>>(g);
   MUON_CHECK_LAUNCH("muon_expert_linear");
   return MUON_OK;
 }
 
-template <int FORM>
-int launch(const GArgs& g, int dtype, hipStream_t s) {
-  if (dtype == MUON_DT_F32) return launch32<FORM>(g, s);
+// Which kernel, all sides measured on 8 to 128 experts of 1024 x 1024 to 4096 x 4096 (us):
+// * FWD of at most 8 rows an expert on the average: the kernel of few rows (64 experts of 1408 x 2048, 128
+//   and 512 rows: 58 and 85, 90 and 97 in tiles of 128).
+// * 256-row tiles for output of 64 of them or more (16 experts of 4096 x 4096, 1024 rows: 136, in tiles of
+//   128 180; 8 of 1024 x 1024, 4000 rows: 26 and 26, 2000 rows: 25 and 18); WGT also with fewer of them
+//   than CUs where they are long (8 of 1024 x 1024, 4000 rows: 26 and 26, 2000 rows 25 and 19).
+// * Else, and where rows are no whole 16-byte runs, tiles of 128.
+template <int DT, int FORM>
+int launch_typed(const GArgs& g, hipStream_t s) {
   const bool aligned = ((uintptr_t)g.a | (uintptr_t)g.b | (uintptr_t)g.c) % 16 == 0 &&
                        (g.lda | g.ldb | g.sb | g.N | g.K | g.M) % 8 == 0;
+  if (FORM == FWD && g.R <= 8 * (int64_t)g.E) return launch_rows<DT>(g, aligned, s);
   const int64_t wa = FORM == WGT ? g.M : g.K, wb = FORM == FWD ? g.K : g.N;
-  if (aligned && g.lda >= wa && g.ldb >= wb && std::max(g.lda, g.ldb) <= P_MOST)
-    return dtype == MUON_DT_BF16 ? launch_pipe<MUON_DT_BF16, FORM>(g, s) : launch_pipe<MUON_DT_F16, FORM>(g, s);
-  return dtype == MUON_DT_BF16 ? launch16<MUON_DT_BF16, FORM, 256, 256, 4, 2>(g, aligned, s)
-                               : launch16<MUON_DT_F16, FORM, 256, 256, 4, 2>(g, aligned, s);
+  const bool direct = aligned && g.lda >= wa && g.ldb >= wb && std::max(g.lda, g.ldb) <= P_MOST;
+  const int64_t area = FORM == WGT ? (int64_t)g.M * g.N * g.E : g.R * g.N, tile = 256 * 256;
+  const bool large = FORM == WGT ? area >= P_GROUPS * tile || g.R >= 512 * (int64_t)g.E : area >= P_GROUPS / 4 * tile;
+  return direct && large ? launch_pipe<DT, FORM>(g, s) : launch16<DT, FORM, 128, 128, 4, 2>(g, aligned, s);
+}
+
+template <int FORM>
+int launch(const GArgs& g, int dtype, hipStream_t s) {
+  switch (dtype) {
+    case MUON_DT_F32: {
+      // Tiles of 128 where there are several for every CU (8 experts of 1001 x 769: 32000 rows 428 us, in
+      // tiles of 64 526; 4094 rows 129 and 92), for WGT, where the largest expert's last long, more (its
+      // gradient from those rows 740 and 588, of 64 experts of 1408 x 2048 from 16384 rows 813 and 891).
+      const int64_t tiles = (FORM == WGT ? (int64_t)g.M * g.N * g.E : g.R * g.N) / (128 * 128);
+      return tiles >= (FORM == WGT ? 2048 : 1536) ? launch32<FORM, 2>(g, s) : launch32<FORM, 1>(g, s);
+    }
+    case MUON_DT_BF16: return launch_typed<MUON_DT_BF16, FORM>(g, s);
+    default: return launch_typed<MUON_DT_F16, FORM>(g, s);
+  }
 }
 
 int check_shapes(const char* what, int dtype, int64_t rows, int64_t experts, int64_t out, int64_t in) {
