@@ -32,7 +32,21 @@ def _load() -> None:
     torch.ops.load_library(_TORCH_LIB_PATH)
 
 
+def _module():
+    """The library as a Python module; None where it was built without Python's headers."""
+    import importlib.machinery
+    import importlib.util
+
+    loader = importlib.machinery.ExtensionFileLoader("libmuon_amd_torch", _TORCH_LIB_PATH)
+    try:
+        return importlib.util.module_from_spec(
+            importlib.util.spec_from_loader("libmuon_amd_torch", loader))
+    except ImportError:
+        return None
+
+
 _load()
+module = _module()
 _ops = torch.ops.muonium_amd
 qk_norm_rope = _ops.qk_norm_rope.default
 route = _ops.route.default

@@ -113,10 +113,10 @@ class AdamW(torch.optim.Optimizer):
 
     # -- the step ---------------------------------------------------------------------
 
-    def _collect(self, group: dict) -> dict:
+    def _collect(self, params: list[Tensor]) -> dict:
         """Lists of what one call takes, by device, type and block."""
         calls: dict[tuple, tuple[list, ...]] = {}
-        for p in group["params"]:
+        for p in params:
             grad = p.grad
             if grad is None:
                 continue
@@ -163,7 +163,14 @@ class AdamW(torch.optim.Optimizer):
             beta1, beta2 = group["betas"]
             numbers = (float(group["lr"]), beta1, beta2, group["eps"], float(group["wd"]),
                        group["maximize"])
-            for (device, _, block), call in self._collect(group).items():
+            params = group["params"]
+            if (_row_ops.module is not None and not torch.compiler.is_compiling()
+                    and params and params[0].is_cuda):
+                # plain parameters with fp32 moments are walked in C++; what it leaves is walked here
+                _row_ops.check_device(params[0].device)
+                left = _row_ops.module.adamw_step(params, self.state, *numbers)
+                params = params if left is None else left
+            for (device, _, block), call in self._collect(params).items():
                 _row_ops.check_device(device)
                 lists, copies = call[:7], call[7]
                 if len(lists[0]) > 1 and (copies or torch.compiler.is_compiling()
