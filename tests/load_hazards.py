@@ -60,7 +60,7 @@ def scan(lines):
                     return
                 seen.add((at, left))
                 for j in jumps.get(text, ()):
-                    back(j + 1, left, used, load, seen)
+                    back(j, left - 1, used, load, seen)
                 continue
             if re.match(r"s_branch|s_endpgm|s_setpc", text) and code[at + 1][0] == "label":
                 return  # nothing falls through
