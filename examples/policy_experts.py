@@ -1,5 +1,5 @@
-"""Policy fine-tuning of a small decoder with experts: the row operators of ``muonium_amd.kernels``
-with the ``Muon`` step, as a training loop uses them.
+"""Policy fine-tuning of a small decoder with experts: the operators of ``muonium_amd.kernels``
+with the ``Muon`` and ``AdamW`` steps, as a training loop uses them.
 
     python examples/policy_experts.py [--steps 30]
 
@@ -7,7 +7,10 @@ A decoder of two layers (grouped heads, normalized and rotated queries and keys,
 each token takes two) answers random prompts; an answer token is rewarded when it repeats the
 token three places before it. Each step samples answers with the current weights
 (``token_logprobs`` gives what they were sampled with, and what the frozen first model thinks of
-them), then takes two steps on ``policy_loss`` with the balance and z losses of ``route``.
+them), then takes two steps on ``policy_loss`` with the balance and z losses of ``route``. The routed
+tokens are brought to their experts (``sort_by_expert``, ``dispatch``), go through the experts' matrices
+(``expert_linear``) and come back with their gates (``combine``). ``Muon`` steps the matrices, ``AdamW`` the
+embedding, the head and the gains.
 """
 
 import argparse
@@ -20,8 +23,9 @@ from torch import nn
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                                 "dtensor-muon_amd"))
 
-from muonium_amd import Muon  # noqa: E402
-from muonium_amd.kernels import policy_loss, qk_norm_rope, route, token_logprobs  # noqa: E402
+from muonium_amd import AdamW, Muon  # noqa: E402
+from muonium_amd.kernels import (combine, dispatch, expert_linear, policy_loss,  # noqa: E402
+                                 qk_norm_rope, route, sort_by_expert, token_logprobs)
 
 VOCAB, WIDTH, LAYERS, HEADS, KV_HEADS, DIM, EXPERTS, TOP, HIDDEN = 64, 128, 2, 4, 2, 32, 8, 2, 128
 
@@ -51,13 +55,10 @@ class Layer(nn.Module):
         return y.transpose(1, 2).reshape(b, t, -1) @ self.out.T
 
     def experts(self, x):
-        flat = x.flatten(0, 1)
-        r = route(flat @ self.router.T, TOP)
-        # every expert on every token: a small model can afford it
-        share = torch.zeros(len(flat), EXPERTS, device=x.device).scatter(1, r.experts, r.gates)
-        hidden = torch.relu(flat @ self.up.transpose(1, 2).contiguous()).square()
-        y = (hidden @ self.down.transpose(1, 2).contiguous()).transpose(0, 1)
-        return (share[:, :, None] * y).sum(1).view_as(x), r
+        r = route(x @ self.router.T, TOP)
+        order = sort_by_expert(r.experts, EXPERTS)
+        hidden = torch.relu(expert_linear(dispatch(x, order), self.up, order.offsets)).square()
+        return combine(expert_linear(hidden, self.down, order.offsets), order, r.gates), r
 
 
 def norm(x):
@@ -103,7 +104,7 @@ def train(steps=30, batch=64, prompt=6, answer=10, seed=0, log=print):
     matrices = [p for layer in model.layers for n, p in layer.named_parameters() if p.ndim >= 2]
     rest = [model.embed, model.head, *(p for layer in model.layers for p in layer.parameters()
                                        if p.ndim < 2)]
-    optimizers = [Muon(matrices, lr=0.01, wd=0.0), torch.optim.AdamW(rest, lr=0.01, weight_decay=0.0)]
+    optimizers = [Muon(matrices, lr=0.01, wd=0.0), AdamW(rest, lr=0.01, wd=0.0, betas=(0.9, 0.999))]
     rewards = []
     for step in range(steps):
         prompts = torch.randint(VOCAB, (batch, prompt), device="cuda")
