@@ -770,8 +770,9 @@ __global__ __launch_bounds__(256) void expert_rows_kernel(GArgs g) {
 //
 // 128 x 128 or 64 x 64 tile (S blocks of 32 a wave and side, 2 or 1), K-tiles of 16, four waves on
 // v_mfma_f32_32x32x2_f32. Both panels stand in LDS as rows of k, whatever their order in memory, so a fragment
-// is one value of a column for each lane.
-constexpr int F_K = 16;
+// is one value of a column for each lane. The sums of 256 k are added up apart from the products' own: a
+// sum that runs over all of k takes a rounding of its whole size at each.
+constexpr int F_K = 16, F_SUM = 256 / F_K;
 
 // A thread's V = 4 S values: KR: of row k; KC: of row r, V k in a row.
 template <bool KR, int V>
@@ -830,13 +831,13 @@ __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
 
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave & 1, wn = wave >> 1;
   const int fr = lane & 31, fk = lane >> 5;
-  f32x16 acc[S][S];
+  f32x16 acc[S][S], sum[S][S];
 #pragma unroll
   for (int i = 0; i < S; ++i)
 #pragma unroll
     for (int j = 0; j < S; ++j)
 #pragma unroll
-      for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+      for (int q = 0; q < 16; ++q) acc[i][j][q] = sum[i][j][q] = 0.0f;
   float wa[V], wb[V];
   const int KT = (K + F_K - 1) / F_K;
   if (KT) {
@@ -868,6 +869,17 @@ __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
         for (int j = 0; j < S; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j], fa[i], acc[i][j], 0, 0, 0);
     }
+    if (kt % F_SUM == F_SUM - 1 || !more) {
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            sum[i][j][q] += acc[i][j][q];
+            acc[i][j][q] = 0.0f;
+          }
+    }
     if (more) {
       f32_store<KRA, V>(lds[(kt + 1) & 1][0], wa);
       f32_store<KRB, V>(lds[(kt + 1) & 1][1], wb);
@@ -887,12 +899,12 @@ __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
       for (int q = 0; q < 4; ++q) {
         const int n = wn * 32 * S + j * 32 + q * 8 + fk * 4;
         if (n + 4 <= N) {
-          const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          const float v[4] = {sum[i][j][4 * q], sum[i][j][4 * q + 1], sum[i][j][4 * q + 2], sum[i][j][4 * q + 3]};
           __builtin_memcpy(out + n, v, 16);
         } else {
 #pragma unroll
           for (int p = 0; p < 4; ++p)
-            if (n + p < N) out[n + p] = acc[i][j][4 * q + p];
+            if (n + p < N) out[n + p] = sum[i][j][4 * q + p];
         }
       }
   }
