@@ -417,10 +417,12 @@ MUON_DEVICE void mfma_wait() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// The tiles of a launch as its workgroups walk them. One workgroup a CU; those of XCD x (workgroups are
-// dealt to the 8 round robin) share one contiguous range of tiles, each taking every 32nd, so that
-// neighbouring tiles, whose panels are the same, meet in one L2. Ranges are of equal work: of equal
-// numbers of tiles, and for WGT, where a tile's K is its expert's rows, of K-tiles.
+// The tiles of a launch as its workgroups walk them, one workgroup a CU. Neighbouring tiles, whose panels
+// are the same, are dealt to one XCD (workgroups go to the 8 round robin), whose L2 they meet in.
+// FWD, ROWS: the XCDs have contiguous ranges of equal numbers of tiles, each workgroup every 32nd of them.
+// WGT, where a tile lasts as long as its expert has rows: the experts' tiles from the longest on, in
+// rounds of 256 that are dealt out in turn from the first workgroup on and from the last one, so that
+// what a round gives one more of the next gives it less of.
 constexpr int P_GROUPS = 256, P_LANE = P_GROUPS / 8;
 struct Tile {
   int e, row0, tm, tn, M, N, K;  // row0: the first of the tile's rows (WGT: of the expert's)
@@ -428,49 +430,58 @@ struct Tile {
 template <int FORM>
 struct Walk {
   const GArgs& g;
-  // in LDS, E + 2 of each: row tiles (WGT: K-tiles) before each expert, its first row and its rows
+  // in LDS, E + 2 of each: row tiles before each expert (WGT: the experts from the one of most rows on),
+  // its first row and its rows
   int *first, *start_of, *rows_of;
-  int at, end;
+  int at, end;  // next tile (WGT: round) of this workgroup, and the last ones' end
+
+  static constexpr int NEXT = FORM == WGT ? 1 : P_LANE;
 
   MUON_DEVICE Walk(const GArgs& g_, int* lds)
       : g(g_), first(lds), start_of(lds + g_.E + 2), rows_of(lds + 2 * (g_.E + 2)) {
-    const int lane = threadIdx.x & 63, per = (g.E + 64) / 64;
-    constexpr int UNIT = FORM == WGT ? 2 * BK : 256;
-    const int e0 = lane * per, e1 = std::min(e0 + per, g.E + 1);
-    int mine = 0, start, n;
-    for (int i = e0; i < e1; ++i) {
+    for (int i = threadIdx.x; i <= g.E; i += 256) {
+      int start, n;
       bounds(g, i, start, n);
-      mine += units(i, n, UNIT);
-    }
-    int incl = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int v = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += v;
-    }
-    if (threadIdx.x < 64) {
-      int sum = incl - mine;
-      for (int i = e0; i < e1; ++i) {
-        first[i] = sum;
-        bounds(g, i, start, n);
-        start_of[i] = start;
-        rows_of[i] = n;
-        sum += units(i, n, UNIT);
-      }
-      if (e1 == g.E + 1 && e0 < e1) first[g.E + 1] = sum;
+      start_of[i] = start;
+      rows_of[i] = n;
     }
     __syncthreads();
-    const int x = blockIdx.x & 7, total = first[g.E + 1];
-    at = __builtin_amdgcn_readfirstlane(border(x, total)) + (int)(blockIdx.x >> 3);
-    end = __builtin_amdgcn_readfirstlane(border(x + 1, total));
+    if constexpr (FORM == WGT) {
+      for (int i = threadIdx.x; i < g.E; i += 256) {
+        int rank = 0;
+        const int mine = rows_of[i];
+        for (int k = 0; k < g.E; ++k) rank += rows_of[k] > mine || (rows_of[k] == mine && k < i);
+        first[rank] = i;
+      }
+      __syncthreads();
+      at = 0;
+      end = (g.E * g.tiles_m * g.tiles_n + P_GROUPS - 1) / P_GROUPS;
+    } else {
+      const int lane = threadIdx.x & 63, per = (g.E + 64) / 64;
+      const int e0 = lane * per, e1 = std::min(e0 + per, g.E + 1);
+      int mine = 0;
+      for (int i = e0; i < e1; ++i) mine += (rows_of[i] + 255) / 256;
+      int incl = mine;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int v = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += v;
+      }
+      if (threadIdx.x < 64) {
+        int sum = incl - mine;
+        for (int i = e0; i < e1; ++i) {
+          first[i] = sum;
+          sum += (rows_of[i] + 255) / 256;
+        }
+        if (e1 == g.E + 1 && e0 < e1) first[g.E + 1] = sum;
+      }
+      __syncthreads();
+      const int64_t x = blockIdx.x & 7, all = (int64_t)__builtin_amdgcn_readfirstlane(first[g.E + 1]) * g.tiles_n;
+      at = (int)(all * x / 8) + (int)(blockIdx.x >> 3);
+      end = (int)(all * (x + 1) / 8);
+    }
   }
-  // Row tiles, or K-tiles of one tile (an expert without rows has one, of nothing), of expert i.
-  static MUON_DEVICE int units(const GArgs& g, int i, int n, int unit) {
-    if (FORM == WGT) return i < g.E ? std::max(1, (n + unit - 1) / unit) : 0;
-    return (n + unit - 1) / unit;
-  }
-  MUON_DEVICE int units(int i, int n, int unit) const { return units(g, i, n, unit); }
-  // The expert whose row tiles (K-tiles) hold number t.
+  // The expert whose row tiles hold number t.
   MUON_DEVICE int expert(int t) const {
     const int lane = threadIdx.x & 63, per = (g.E + 64) / 64;
     const int seg = __popcll(__ballot(lane * per <= g.E && first[std::min(lane * per, g.E)] <= t)) - 1;
@@ -478,31 +489,24 @@ struct Walk {
     const int in = __popcll(__ballot(lane < per && i <= g.E && first[std::min(i, g.E)] <= t));
     return std::max(0, std::min(seg * per + in - 1, g.E));
   }
-  MUON_DEVICE int border(int x, int total) const {
-    if constexpr (FORM == WGT) {
-      const int per = g.tiles_m * g.tiles_n;
-      if (x == 8) return g.E * per;
-      const int64_t work = (int64_t)total * per * x / 8;
-      const int e = __builtin_amdgcn_readfirstlane(std::min(expert((int)(work / per)), g.E - 1));
-      const int k = first[e + 1] - first[e];
-      return e * per + std::min<int64_t>((work - (int64_t)first[e] * per) / k, per);
-    } else {
-      return (int)((int64_t)total * g.tiles_n * x / 8);
-    }
-  }
   MUON_DEVICE bool tile(int t, Tile& o) const {
     if (t >= end) return false;
     if constexpr (FORM == WGT) {
       const int per = g.tiles_m * g.tiles_n;
-      o.e = t / per;
-      tile_of(t - o.e * per, g.tiles_m, g.tiles_n, o.tm, o.tn);
+      // of a round of n tiles, fewer in the last one, an XCD has an eighth
+      const int n = std::min(g.E * per - t * P_GROUPS, P_GROUPS), x = blockIdx.x & 7;
+      int k = n * x / 8 + (int)(blockIdx.x >> 3);
+      if (k >= n * (x + 1) / 8) return false;  // none in the last round
+      k = t * P_GROUPS + (t & 1 ? n - 1 - k : k);
+      const int rank = k / per;
+      o.e = __builtin_amdgcn_readfirstlane(first[rank]);
+      tile_of(k - rank * per, g.tiles_m, g.tiles_n, o.tm, o.tn);
       o.row0 = start_of[o.e];
       o.K = rows_of[o.e];
       o.M = std::min(g.M - o.tm * 256, 256);
     } else {
-      const int total = first[g.E + 1];
       int row;
-      tile_of(t, total, g.tiles_n, row, o.tn);
+      tile_of(t, __builtin_amdgcn_readfirstlane(first[g.E + 1]), g.tiles_n, row, o.tn);
       o.e = expert(row);
       const int skip = (row - first[o.e]) * 256;
       o.row0 = start_of[o.e] + skip;
@@ -563,7 +567,7 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
     b.advance();
     if (++kt_next <= kt_last) return;
     if (kt_next >= kt_all) {
-      next += P_LANE;
+      next += walk.NEXT;
       Tile o;
       if (walk.tile(next, o)) {
         open(o);
@@ -687,7 +691,7 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
       __builtin_amdgcn_sched_barrier(0);
     }
     stores = 3;
-    at += P_LANE;
+    at += walk.NEXT;
     if (!walk.tile(at, t)) break;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last loads, of nothing, into this LDS
