@@ -22,11 +22,13 @@ namespace {
 constexpr int ORDER_THREADS = 512;
 constexpr int ORDER_WAVES = ORDER_THREADS / 64;
 constexpr int ORDER_EMAX = 1024;
-// Choices that one workgroup orders alone: two walks over 1024 choices a wave take less than the
-// second launch.
-constexpr int64_t ORDER_ALONE = 8192;
+constexpr int ORDER_BATCH = 8;  // choices of a lane whose loads are under way together
+// Choices that one workgroup orders alone, in one launch (2048 of 64 experts 5.7 us, 8192 15; 16384 by
+// eight workgroups 9.0).
+constexpr int64_t ORDER_ALONE = 4096;
 constexpr int64_t ORDER_CHUNK = 2048;
-constexpr int64_t ORDER_BLOCKS = 256;
+// Every workgroup adds up the counts of all: so many counts at most, of a workgroup a CU at most.
+constexpr int64_t ORDER_COUNTS = 65536, ORDER_BLOCKS = 256;
 
 struct OrderArgs {
   const int64_t* experts;
@@ -37,7 +39,9 @@ struct OrderArgs {
   int32_t* counts;  // (blocks, E + 1): choices of each expert, and empty ones, by workgroup
 };
 
-MUON_DEVICE int expert_of(const OrderArgs& a, int64_t i) {
+// Choice i's expert, E for an empty one, -1 behind the end.
+MUON_DEVICE int expert_at(const OrderArgs& a, int64_t i, int64_t end) {
+  if (i >= end) return -1;
   const int64_t e = a.experts[i];
   return e >= 0 && e < a.E ? (int)e : a.E;
 }
@@ -48,7 +52,14 @@ __global__ __launch_bounds__(ORDER_THREADS) void order_count_kernel(OrderArgs a)
   for (int c = tid; c <= a.E; c += ORDER_THREADS) cnt[c] = 0;
   __syncthreads();
   const int64_t begin = blockIdx.x * a.chunk, end = std::min(begin + a.chunk, a.n);
-  for (int64_t i = begin + tid; i < end; i += ORDER_THREADS) atomicAdd(&cnt[expert_of(a, i)], 1);
+  for (int64_t i0 = begin + tid; i0 < end; i0 += ORDER_THREADS * ORDER_BATCH) {
+    int e[ORDER_BATCH];
+#pragma unroll
+    for (int b = 0; b < ORDER_BATCH; ++b) e[b] = expert_at(a, i0 + b * ORDER_THREADS, end);
+#pragma unroll
+    for (int b = 0; b < ORDER_BATCH; ++b)
+      if (e[b] >= 0) atomicAdd(&cnt[e[b]], 1);
+  }
   __syncthreads();
   for (int c = tid; c <= a.E; c += ORDER_THREADS)
     a.counts[(int64_t)blockIdx.x * (a.E + 1) + c] = cnt[c];
@@ -69,15 +80,26 @@ __global__ __launch_bounds__(ORDER_THREADS) void order_place_kernel(OrderArgs a)
   const int64_t run = a.chunk / ORDER_WAVES;
   const int64_t begin = blockIdx.x * a.chunk + wave * run;
   const int64_t end = std::min(begin + run, a.n);
-  for (int64_t i = begin + lane; i < end; i += 64) atomicAdd(&cnt[wave * C + expert_of(a, i)], 1);
+  for (int64_t i0 = begin + lane; i0 < end; i0 += 64 * ORDER_BATCH) {
+    int e[ORDER_BATCH];
+#pragma unroll
+    for (int b = 0; b < ORDER_BATCH; ++b) e[b] = expert_at(a, i0 + b * 64, end);
+#pragma unroll
+    for (int b = 0; b < ORDER_BATCH; ++b)
+      if (e[b] >= 0) atomicAdd(&cnt[wave * C + e[b]], 1);
+  }
   if (a.blocks > 1) {
     const int all = a.blocks * C, mine = blockIdx.x * C;
-#pragma unroll 8
-    for (int i = tid; i < all; i += ORDER_THREADS) {
-      const int v = a.counts[i], c = i % C;
-      if (v) {
-        atomicAdd(&total[c], v);
-        if (i < mine) atomicAdd(&before[c], v);
+    for (int i0 = tid; i0 < all; i0 += ORDER_THREADS * ORDER_BATCH) {
+      int v[ORDER_BATCH];
+#pragma unroll
+      for (int b = 0; b < ORDER_BATCH; ++b) v[b] = i0 + b * ORDER_THREADS < all ? a.counts[i0 + b * ORDER_THREADS] : 0;
+#pragma unroll
+      for (int b = 0; b < ORDER_BATCH; ++b) {
+        const int i = i0 + b * ORDER_THREADS;
+        if (!v[b]) continue;
+        atomicAdd(&total[i % C], v[b]);
+        if (i < mine) atomicAdd(&before[i % C], v[b]);
       }
     }
     __syncthreads();
@@ -119,20 +141,26 @@ __global__ __launch_bounds__(ORDER_THREADS) void order_place_kernel(OrderArgs a)
   __syncthreads();
   const int bits = 32 - __builtin_clz(a.E | 1);
   const uint64_t below = (1ull << lane) - 1;
-  for (int64_t i0 = begin; i0 < end; i0 += 64) {
-    const int64_t i = i0 + lane;
-    const bool in = i < end;
-    const int e = in ? expert_of(a, i) : 0;
-    uint64_t same = __ballot(in);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t ones = __ballot(in && ((e >> b) & 1));
-      same &= ((e >> b) & 1) ? ones : ~ones;
+  for (int64_t i0 = begin; i0 < end; i0 += 64 * ORDER_BATCH) {
+    int es[ORDER_BATCH];
+#pragma unroll
+    for (int b = 0; b < ORDER_BATCH; ++b) es[b] = expert_at(a, i0 + b * 64 + lane, end);
+#pragma unroll
+    for (int b = 0; b < ORDER_BATCH; ++b) {
+      if (i0 + b * 64 >= end) break;
+      const bool in = es[b] >= 0;
+      const int e = in ? es[b] : 0;
+      uint64_t same = __ballot(in);
+      for (int k = 0; k < bits; ++k) {
+        const uint64_t ones = __ballot(in && ((e >> k) & 1));
+        same &= ((e >> k) & 1) ? ones : ~ones;
+      }
+      const int rank = __popcll(same & below);
+      int place = 0;
+      if (in && rank == 0) place = atomicAdd(&cnt[wave * C + e], (int)__popcll(same));
+      place = __shfl(place, in ? __builtin_ctzll(same) : lane, 64) + rank;
+      if (in) a.slots[i0 + b * 64 + lane] = e < a.E ? place : -1 - place;
     }
-    const int rank = __popcll(same & below);
-    int place = 0;
-    if (in && rank == 0) place = atomicAdd(&cnt[wave * C + e], (int)__popcll(same));
-    place = __shfl(place, in ? __builtin_ctzll(same) : lane, 64) + rank;
-    if (in) a.slots[i] = e < a.E ? place : -1 - place;
   }
 }
 
@@ -320,11 +348,15 @@ int64_t row_grid(int64_t tokens, int shift) {
   return std::min((tokens + per - 1) / per, ROW_GRID);
 }
 
-int64_t order_chunk(int64_t n) {
+int64_t order_chunk(int64_t n, int64_t experts) {
   if (n <= ORDER_ALONE) return round_up(std::max<int64_t>(n, 1), ORDER_THREADS);
-  return std::max(ORDER_CHUNK, round_up((n + ORDER_BLOCKS - 1) / ORDER_BLOCKS, ORDER_THREADS));
+  const int64_t blocks = std::min(ORDER_COUNTS / (experts + 1), ORDER_BLOCKS);
+  return std::max(ORDER_CHUNK, round_up((n + blocks - 1) / blocks, ORDER_THREADS));
 }
-int64_t order_blocks(int64_t n) { return std::max<int64_t>(1, (n + order_chunk(n) - 1) / order_chunk(n)); }
+int64_t order_blocks(int64_t n, int64_t experts) {
+  const int64_t chunk = order_chunk(n, experts);
+  return std::max<int64_t>(1, (n + chunk - 1) / chunk);
+}
 
 bool fine_dtype(int dtype) { return dtype == MUON_DT_F32 || dtype == MUON_DT_BF16 || dtype == MUON_DT_F16; }
 
@@ -354,7 +386,7 @@ int check_rows(const char* what, int dtype, int64_t tokens, int64_t top, int64_t
 
 extern "C" int64_t muon_expert_order_workspace_bytes(int64_t choices, int64_t experts) {
   if (choices < 0 || choices > INT32_MAX || experts < 1 || experts > ORDER_EMAX) return -1;
-  const int64_t blocks = order_blocks(choices);
+  const int64_t blocks = order_blocks(choices, experts);
   return blocks > 1 ? blocks * (experts + 1) * 4 : 0;
 }
 
@@ -370,7 +402,7 @@ extern "C" int muon_expert_order(const int64_t* experts, int64_t choices, int64_
     muon_set_error("muon_expert_order: null pointer");
     return MUON_ERR_ARG;
   }
-  OrderArgs a{experts, choices, order_chunk(choices), (int)nexperts, (int)order_blocks(choices),
+  OrderArgs a{experts, choices, order_chunk(choices, nexperts), (int)nexperts, (int)order_blocks(choices, nexperts),
               slots, offsets, (int32_t*)ws};
   hipStream_t s = (hipStream_t)stream;
   if (a.blocks > 1) {

@@ -64,8 +64,9 @@ ORDERS = [
     (33, 2, 7, 1.0, "random"),       # nothing goes anywhere
     (100, 3, 1024, 0.1, "random"),
     (513, 1, 2, 0.0, "one"),
-    (1024, 8, 64, 0.1, "skewed"),    # the most that one workgroup orders
-    (1025, 8, 64, 0.1, "skewed"),    # the least that several do
+    (512, 8, 64, 0.1, "skewed"),     # the most that one workgroup orders
+    (513, 8, 64, 0.1, "skewed"),     # the least that several do
+    (1025, 8, 64, 0.1, "skewed"),
     (4099, 5, 63, 0.3, "random"),
     (3001, 4, 255, 0.2, "random"),
     (30011, 1, 1024, 0.05, "random"),
