@@ -81,7 +81,7 @@ MUON_DEVICE bool find_tile(const GArgs& g, int L, int& e, int& row0, int& left, 
   if (!past) return false;  // offsets that do not rise can count beyond 32 bits
   const int src = __builtin_ctzll(past);
   int first = __shfl(incl - mine, src, 64);
-  e = src * per;
+  e = std::min(src * per, g.E);
   for (;; ++e) {
     bounds(g, e, start, n);
     const int tiles = (n + BM - 1) / BM;
@@ -92,7 +92,7 @@ MUON_DEVICE bool find_tile(const GArgs& g, int L, int& e, int& row0, int& left, 
   const int skip = (t - first) * BM;
   row0 = __builtin_amdgcn_readfirstlane(start + skip);
   left = __builtin_amdgcn_readfirstlane(n - skip);
-  return true;
+  return skip >= 0 && left > 0;
 }
 
 template <int DT>
@@ -508,10 +508,11 @@ struct Walk {
       int row;
       tile_of(t, __builtin_amdgcn_readfirstlane(first[g.E + 1]), g.tiles_n, row, o.tn);
       o.e = expert(row);
-      const int skip = (row - first[o.e]) * 256;
-      o.row0 = start_of[o.e] + skip;
-      o.M = std::min(rows_of[o.e] - skip, 256);
-      o.K = o.e < g.E ? g.K : 0;
+      const int skip = (row - first[o.e]) * 256, rows = rows_of[o.e];
+      const bool fine = skip >= 0 && skip < rows;  // also where offsets that fall count beyond 32 bits
+      o.row0 = start_of[o.e] + (fine ? skip : 0);
+      o.M = fine ? std::min(rows - skip, 256) : 0;
+      o.K = fine && o.e < g.E ? g.K : 0;
       o.tm = 0;
     }
     o.N = std::min(g.N - o.tn * 256, 256);
@@ -956,7 +957,7 @@ int launch_rows(GArgs g, bool aligned, hipStream_t s) {
   return MUON_OK;
 }
 
-// What the direct loads index by 32 bits: 256 rows of a panel, 64 of one along k.
+// What the direct loads and stores index by 32 bits: 256 rows of a panel, 64 of one along k, 128 of a result.
 constexpr int64_t P_MOST = 1 << 20;
 
 template <int DT, int FORM>
@@ -1006,7 +1007,7 @@ int launch_typed(const GArgs& g, hipStream_t s) {
                        (g.lda | g.ldb | g.sb | g.N | g.K | g.M) % 8 == 0;
   if (FORM == FWD && g.R <= 8 * (int64_t)g.E) return launch_rows<DT>(g, aligned, s);
   const int64_t wa = FORM == WGT ? g.M : g.K, wb = FORM == FWD ? g.K : g.N;
-  const bool direct = aligned && g.lda >= wa && g.ldb >= wb && std::max(g.lda, g.ldb) <= P_MOST;
+  const bool direct = aligned && g.lda >= wa && g.ldb >= wb && std::max({g.lda, g.ldb, (int64_t)g.N}) <= P_MOST;
   const int64_t area = FORM == WGT ? (int64_t)g.M * g.N * g.E : g.R * g.N, tile = 256 * 256;
   const bool large = FORM == WGT ? area >= P_GROUPS * tile || g.R >= 512 * (int64_t)g.E : area >= P_GROUPS / 4 * tile;
   return direct && large ? launch_pipe<DT, FORM>(g, s) : launch16<DT, FORM, 128, 128, 4, 2>(g, aligned, s);

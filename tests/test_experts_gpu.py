@@ -598,3 +598,42 @@ def test_rows_behind_offsets_past_32_bits():
     want = y[at].double() @ weight[-1].double()
     scale = y[at].double().abs() @ weight[-1].double().abs()
     check(dx[at], want.cpu(), scale.cpu(), depth(8, torch.bfloat16), "dx")
+
+
+@pytest.mark.parametrize("wide", ["out", "stride"])
+def test_extents_beyond_what_direct_loads_index(wide):
+    """A result of 2^20 + 8 columns; rows 2^20 + 8 values apart: 32 bits would not do for 256 of them."""
+    n, far = 300, 2**20 + 8
+    g = gen(29)
+    rows = torch.randn(n, 16, generator=g).bfloat16().cuda()
+    offsets = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    if wide == "out":
+        weight = torch.randn(1, far, 16, generator=g).bfloat16().cuda()
+    else:
+        weight = torch.randn(1, 16384, 16, generator=g).bfloat16().cuda()
+        spread = torch.zeros(n, far, dtype=torch.bfloat16, device="cuda")
+        rows = spread[:, 8:24].copy_(rows)
+    y = expert_linear(rows, weight, offsets)
+    at = torch.cat([torch.arange(40), torch.arange(weight.shape[1] - 40, weight.shape[1])]).cuda()
+    want = rows.double() @ weight[0, at].double().T
+    scale = rows.double().abs() @ weight[0, at].double().abs().T
+    check(y[:, at], want.cpu(), scale.cpu(), depth(16, torch.bfloat16))
+
+
+def test_many_rows_of_many_experts():
+    """More row tiles than a wave counts in one go, experts of none to thousands of rows, in whole tiles."""
+    g = gen(31)
+    counts = torch.randint(0, 40, (200,), generator=g)
+    counts[::7] = torch.randint(200, 3000, (29,), generator=g)
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]).int()
+    n, out, width = int(offsets[-1]) + 100, 1032, 328
+    x, dy = (torch.randn(n, w, generator=g).bfloat16().cuda() for w in (width, out))
+    w = torch.randn(200, out, width, generator=g).bfloat16().cuda()
+    leaf, wleaf = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = expert_linear(leaf, wleaf, offsets.cuda())
+    dx, dw = torch.autograd.grad(y, (leaf, wleaf), dy)
+    assert (y[int(offsets[-1]):] == 0).all() and (dx[int(offsets[-1]):] == 0).all()
+    for e, (a, b) in enumerate(ref.spans(offsets)):
+        xe, de, we = x[a:b].double(), dy[a:b].double(), w[e].double()
+        for got, p, q in ((y[a:b], xe, we.T), (dx[a:b], de, we), (dw[e], de.T, xe)):
+            check(got, (p @ q).cpu(), (p.abs() @ q.abs()).cpu(), depth(p.shape[1], torch.bfloat16), e)
