@@ -232,9 +232,11 @@ __global__ __launch_bounds__(ROW_THREADS) void dispatch_kernel(RowArgs a) {
   }
 }
 
-constexpr int BATCH = 8;  // choices whose rows are in flight together
 
-template <int DT>
+// BATCH: choices whose rows are in flight together, 8, or fewer where a token has fewer: what is asked
+// and masked for the missing ones costs more than the bytes then (32768 tokens of 777 bf16 columns, one
+// choice: combine 28 us by eights, 19 by twos; its gradient 52 by eights, 31 by ones).
+template <int DT, int BATCH>
 __global__ __launch_bounds__(ROW_THREADS) void combine_kernel(RowArgs a) {
   constexpr int N = Vec16<DT>::N;
   const int lanes = 1 << a.shift, v0 = threadIdx.x & (lanes - 1);
@@ -285,7 +287,7 @@ struct BackArgs {
 
 // G lanes a token (a wave at most): the products of a choice's row are summed by each lane over its
 // columns, then over the lanes.
-template <int DT, int G>
+template <int DT, int G, int BATCH>
 __global__ __launch_bounds__(ROW_THREADS) void combine_backward_kernel(BackArgs a) {
   constexpr int N = Vec16<DT>::N;
   const int v0 = threadIdx.x & (G - 1);
@@ -449,7 +451,11 @@ extern "C" int muon_combine(const void* rows, int dtype, int64_t row_stride, int
   RowArgs a{rows, row_stride, tokens, tokens * top, (int)top, (int)width, lanes_shift(dtype, width, 8),
             slots, gates, y};
   const int64_t grid = row_grid(tokens, a.shift);
-  BY_TYPE((combine_kernel<DT><<<(unsigned)grid, ROW_THREADS, 0, (hipStream_t)stream>>>(a)))
+  if (top <= 2) {
+    BY_TYPE((combine_kernel<DT, 2><<<(unsigned)grid, ROW_THREADS, 0, (hipStream_t)stream>>>(a)))
+  } else {
+    BY_TYPE((combine_kernel<DT, 8><<<(unsigned)grid, ROW_THREADS, 0, (hipStream_t)stream>>>(a)))
+  }
   MUON_CHECK_LAUNCH("muon_combine");
   return MUON_OK;
 }
@@ -469,7 +475,8 @@ extern "C" int muon_combine_backward(const void* dy, int64_t dy_stride, const vo
   const int shift = std::max(3, lanes_shift(dtype, width, 6));
   const int64_t grid = row_grid(tokens, shift);
   hipStream_t s = (hipStream_t)stream;
-#define BACK(G) BY_TYPE((combine_backward_kernel<DT, G><<<(unsigned)grid, ROW_THREADS, 0, s>>>(a)))
+#define BACK_KERNEL(G, B) BY_TYPE((combine_backward_kernel<DT, G, B><<<(unsigned)grid, ROW_THREADS, 0, s>>>(a)))
+#define BACK(G) if (top == 1) { BACK_KERNEL(G, 1) } else { BACK_KERNEL(G, 8) }
   switch (shift) {
     case 3: BACK(8) break;
     case 4: BACK(16) break;
@@ -477,6 +484,7 @@ extern "C" int muon_combine_backward(const void* dy, int64_t dy_stride, const vo
     default: BACK(64)
   }
 #undef BACK
+#undef BACK_KERNEL
   MUON_CHECK_LAUNCH("muon_combine_backward");
   return MUON_OK;
 }
