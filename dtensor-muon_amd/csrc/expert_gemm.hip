@@ -130,7 +130,28 @@ typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
 MUON_DEVICE int swz_kc(int r) { return (r >> 1) & 7; }
 MUON_DEVICE int swz_kr(int k) { return ((k & 3) << 2) ^ (((k >> 3) & 1) << 1); }
 
+// w without its first n values (16 bits each), zeros behind.
+MUON_DEVICE muon_u4 drop(muon_u4 w, int n) {
+  uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
+  if (n & 4) {
+    lo = hi;
+    hi = 0;
+  }
+  const int bits = 16 * (n & 3);
+  if (bits) {
+    lo = lo >> bits | hi << (64 - bits);
+    hi >>= bits;
+  }
+  if (n >= 8) lo = hi = 0;
+  return muon_u4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
+
 // One operand's share of a K-tile: PANEL rows (KC) or columns (KR) of the tile, NT threads.
+//
+// Every chunk is one load, at an address that no condition on a lane changes: single values behind a
+// condition are waited for before the next chunk is asked for. Rows of a KC panel behind the last repeat it
+// (they are not stored), a run of columns that leaves the matrix moves back to end with it, and what
+// it brought too many is dropped on the way to LDS, where a k behind the last becomes zero.
 template <int PANEL, bool KR, int NT, bool ALIGNED>
 struct Stage {
   static constexpr int CHUNKS = PANEL * BK / 8 / NT;  // 16-byte chunks of a thread
@@ -139,37 +160,46 @@ struct Stage {
   muon_u4 w[CHUNKS];
 
   // base: the panel's first row and column at k = 0; `in`: valid rows (KC) or columns (KR) from
-  // there, k left: valid k from k0 on
-  MUON_DEVICE void load(const uint16_t* base, int64_t ld, int in, int k0, int kleft) {
+  // there, k left: valid k from k0 on; wide: a row of the matrix has eight values
+  MUON_DEVICE void load(const uint16_t* base, int64_t ld, int in, int k0, int kleft, bool wide) {
     const int row = threadIdx.x / PER_ROW, ch = threadIdx.x % PER_ROW * 8;
+    const int cols = KR ? in : kleft, last = (KR ? kleft : in) - 1;
 #pragma unroll
     for (int q = 0; q < CHUNKS; ++q) {
-      const int r = row + q * ROWS_PASS;
-      const bool ok = KR ? r < kleft : r < in;
-      const int have = ok ? (KR ? in : kleft) - ch : 0;
-      const uint16_t* p = KR ? base + (k0 + r) * ld + ch : base + r * ld + k0 + ch;
-      if (have >= 8) {
+      const int r = std::min(row + q * ROWS_PASS, last), c = std::min(ch, cols - 8);
+      const uint16_t* p = KR ? base + (k0 + r) * ld + c : base + r * ld + k0 + c;
+      if (ALIGNED || wide) {
         if constexpr (ALIGNED) w[q] = *(const muon_u4*)p;
         else w[q] = load_u4(p);
-      } else {
+      } else {  // fewer than eight columns, all of them in the first chunk
         uint32_t u[4] = {0, 0, 0, 0};
-        if constexpr (!ALIGNED) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j < have) u[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
-        }
+        for (int j = 0; j < 7; ++j)
+          if (ch == 0 && j < cols) u[j / 2] |= (uint32_t)p[j - c] << (16 * (j & 1));
         w[q] = muon_u4{u[0], u[1], u[2], u[3]};
       }
     }
   }
-  MUON_DEVICE void store(uint8_t* lds) const {
-    const int row = threadIdx.x / PER_ROW, c = threadIdx.x % PER_ROW;
+  MUON_DEVICE void store(uint8_t* lds, int in, int kleft, bool wide) const {
+    if (kleft < BK || (KR && in < PANEL)) {
+      const int c = threadIdx.x % PER_ROW * 8, cols = KR ? in : kleft;
+      const int moved = wide ? c - std::min(c, cols - 8) : 0;
 #pragma unroll
-    for (int q = 0; q < CHUNKS; ++q) {
-      const int r = row + q * ROWS_PASS;
-      const int at = KR ? r * PANEL * 2 + ((c ^ swz_kr(r)) << 4) : r * BK * 2 + ((c ^ swz_kc(r)) << 4);
-      *(muon_u4*)(lds + at) = w[q];
+      for (int q = 0; q < CHUNKS; ++q) {
+        muon_u4 v = w[q];
+        if constexpr (!ALIGNED) v = drop(v, moved);
+        if (KR ? (int)threadIdx.x / PER_ROW + q * ROWS_PASS >= kleft : ALIGNED && moved) v = muon_u4{0, 0, 0, 0};
+        put(lds, q, v);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < CHUNKS; ++q) put(lds, q, w[q]);
     }
+  }
+  static MUON_DEVICE void put(uint8_t* lds, int q, muon_u4 v) {
+    const int r = threadIdx.x / PER_ROW + q * ROWS_PASS, c = threadIdx.x % PER_ROW;
+    const int at = KR ? r * PANEL * 2 + ((c ^ swz_kr(r)) << 4) : r * BK * 2 + ((c ^ swz_kc(r)) << 4);
+    *(muon_u4*)(lds + at) = v;
   }
 };
 
@@ -233,19 +263,21 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void expert_gemm_kernel(GArgs g) {
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
   const int KT = (K + BK - 1) / BK;
+  const bool wide_a = (KRA ? g.M : g.K) >= 8, wide_b = (KRB ? g.N : g.K) >= 8;
   if (KT) {
-    sa.load(A, g.lda, M, 0, K);
-    sb.load(B, g.ldb, N, 0, K);
-    sa.store(smem);
-    sb.store(smem + PANEL_A);
+    sa.load(A, g.lda, M, 0, K, wide_a);
+    sb.load(B, g.ldb, N, 0, K, wide_b);
+    sa.store(smem, M, K, wide_a);
+    sb.store(smem + PANEL_A, N, K, wide_b);
   }
   __syncthreads();
   for (int kt = 0; kt < KT; ++kt) {
     uint8_t* st = smem + (kt & 1) * STAGE;
     const bool more = kt + 1 < KT;
+    const int k1 = (kt + 1) * BK;
     if (more) {
-      sa.load(A, g.lda, M, (kt + 1) * BK, K - (kt + 1) * BK);
-      sb.load(B, g.ldb, N, (kt + 1) * BK, K - (kt + 1) * BK);
+      sa.load(A, g.lda, M, k1, K - k1, wide_a);
+      sb.load(B, g.ldb, N, k1, K - k1, wide_b);
     }
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -261,8 +293,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void expert_gemm_kernel(GArgs g) {
     }
     if (more) {
       uint8_t* nx = smem + ((kt + 1) & 1) * STAGE;
-      sa.store(nx);
-      sb.store(nx + PANEL_A);
+      sa.store(nx, M, K - k1, wide_a);
+      sb.store(nx + PANEL_A, N, K - k1, wide_b);
     }
     __syncthreads();
   }
