@@ -9,6 +9,12 @@
 // The offsets stay on the device, so the grid is the most tiles that R rows of E experts can make, and
 // each workgroup finds its tile from the offsets; those left over end at once. 16-bit types run on
 // MFMA with fp32 accumulators, fp32 on the fp32 MFMA.
+//
+// 64 experts of 1408 x 2048 in bf16 (an 8192-cubed library product runs at 1431 TFLOP/s, a copy at 4.9 TB/s):
+//   262144 rows: FWD 1236 to 1317 us, ROWS 1264 to 1288, WGT 1186 to 1237, 1.15 to 1.27 PFLOP/s; 1408
+//     fills 5.5 tiles of 256, so the matrix units do 9% more than that;
+//   128 rows: 60 to 63 us, the bytes of the weights that they meet at 6 TB/s (part of them from the
+//     last-level cache).
 #include <algorithm>
 #include <type_traits>
 
@@ -222,7 +228,10 @@ MUON_DEVICE muon_u4 fragment(uint8_t* lds, int r0, int ks) {
   }
 }
 
-// A BM x BN tile by WM x WN waves.
+// A BM x BN tile by WM x WN waves, the next K-tile's loads under way during the products of one: for
+// few tiles and for ragged sizes (262144 rows, 64 experts of 1409 x 2041: 2844, 2625 and 2690 us, 530 to 575
+// TFLOP/s; with loads two K-tiles ahead 4361, 4253 and 4280, in registers that a second workgroup of
+// the CU needs).
 template <int DT, int FORM, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(64 * WM * WN, 1) void expert_gemm_kernel(GArgs g) {
   constexpr int NT = 64 * WM * WN;
@@ -808,7 +817,9 @@ __global__ __launch_bounds__(256) void expert_rows_kernel(GArgs g) {
 // 128 x 128 or 64 x 64 tile (S blocks of 32 a wave and side, 2 or 1), K-tiles of 16, four waves on
 // v_mfma_f32_32x32x2_f32. Both panels stand in LDS as rows of k, whatever their order in memory, so a fragment
 // is one value of a column for each lane. The sums of 256 k are added up apart from the products' own: a
-// sum that runs over all of k takes a rounding of its whole size at each.
+// sum that runs over all of k takes a rounding of its whole size at each. 4094 rows of 8 experts of
+// 1001 x 769: 94, 102 and 101 us, 62 to 67 TFLOP/s of 154 (8192 cubed): their 294 to 425 workgroups are one
+// to two for a CU, and each waits for its own loads.
 constexpr int F_K = 16, F_SUM = 256 / F_K;
 
 // A thread's V = 4 S values: KR: of row k; KC: of row r, V k in a row.

