@@ -87,9 +87,9 @@ def combine(rows: Tensor, order: ExpertOrder, gates: Tensor | None = None) -> Te
         rows: ``(tokens * k, width)`` in the order's order, fp32, bf16 or fp16; rows may be strided.
         order: of :func:`sort_by_expert`.
         gates: ``(..., k)`` fp32, as :func:`route` gives them, or None for ones. Those of empty choices
-            are not read, nor are the rows behind the last expert's.
+            and the rows behind the last expert's reach nothing.
 
-    Differentiable in rows and gates (zeros for what is not read); sums in fp32, rounded once."""
+    Differentiable in rows and gates (zeros for what reaches nothing); sums in fp32, rounded once."""
     slots = _slots(order, rows)
     if rows.dim() != 2 or rows.shape[0] != slots.numel():
         raise ValueError(f"rows are ({slots.numel()}, width); got {tuple(rows.shape)}")

@@ -353,7 +353,7 @@ int muon_scale_gradient(void* x, int dtype, int64_t n, const float* scale, void*
  * is 0. muon_combine: y (tokens, width), contiguous, y[t] = sum_j gates[t, j] rows[slot(t, j)] over the
  * kept choices (gates NULL: ones, the gradient of muon_dispatch). muon_combine_backward: drows like
  * muon_dispatch's rows, gates[t, j] dy[t], and dgates[t, j] = <dy[t], rows[slot]>; either may be NULL.
- * Gates and rows of empty choices are not read, their gradients are 0. A slot outside the rows is
+ * Gates and rows of empty choices reach nothing, their gradients are 0. A slot outside the rows is
  * left out. Strides of rows in elements, columns contiguous; sums in fp32, rounded once. */
 int64_t muon_expert_order_workspace_bytes(int64_t choices, int64_t nexperts);
 int muon_expert_order(const int64_t* experts, int64_t choices, int64_t nexperts, int32_t* slots,

@@ -273,6 +273,35 @@ def test_infinities_and_nan_go_where_they_belong():
     assert y[0].isnan().all() and y[1:].isfinite().all()
 
 
+def among_nan(t, after=5):
+    """t on the GPU, in the middle of rows of NaN."""
+    wide = torch.full((t.shape[0], t.shape[1] + 2 + after), math.nan, dtype=t.dtype)
+    wide[:, 2:2 + t.shape[1]] = t
+    return wide.cuda()[:, 2:2 + t.shape[1]]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", [1, 2, 3, 8])
+@pytest.mark.parametrize("width", [3, 4, 5, 8, 9, 13, 15, 31, 517])
+def test_ends_of_rows(width, k, dtype):
+    """The last columns, which two lanes may have, count once, and what lies beside a row is not read."""
+    e, slots, _, x, rows, gates, dy = rows_case(41, k, width, 6, dtype)
+    rows[::5, -1], dy[3::7, -2] = math.inf, -math.inf
+    rows[2::9, max(0, width - 6)] = math.nan
+    order = sort_by_expert(e.cuda(), 6)
+    assert torch.equal(dispatch(among_nan(dy), order).cpu().double(), ref.dispatch(dy, slots))
+    leaf, g = among_nan(rows).requires_grad_(), gates.cuda().requires_grad_()
+    y = combine(leaf, order, g)
+    got = (y, *torch.autograd.grad(y, (leaf, g), among_nan(dy)))
+    want, scale = ref.combine(rows, slots, gates)
+    want_rows, want_gates, scale_gates = ref.combine_grad(rows, slots, gates, dy)
+    for a, b, c, n, what in ((got[0], want, scale, k + 1, "y"), (got[1], want_rows, want_rows.abs(), 1, "drows"),
+                             (got[2], want_gates, scale_gates, 2 * 16 + 6, "dgates")):
+        inf = b.isinf()
+        assert torch.equal(a.cpu().double()[inf], b[inf]), what
+        check(a.cpu().masked_fill(inf, 0), b.masked_fill(inf, 0), c.masked_fill(inf, 0), n, what)
+
+
 # ---- products -------------------------------------------------------------------------------
 
 PRODUCTS = [
@@ -354,6 +383,22 @@ def test_products_of_other_strides(dtype):
     want_x, scale_x, want_w, scale_w = ref.linear_grad(rows, weight, offsets, torch.ones(dy.shape))
     check(x.grad, want_x, scale_x, depth(48, dtype), "dx")
     check(w.grad, want_w, scale_w, depth(41, dtype), "dw")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("out, width", [(1, 7), (7, 8), (8, 9), (9, 15), (15, 65), (65, 71), (72, 127),
+                                        (127, 129), (129, 136), (136, 1), (130, 250)])
+def test_products_among_nan(out, width, dtype):
+    """Runs that end with a matrix's row bring nothing of what lies beside it."""
+    rows, weight, offsets, dy = product_case([70, 0, 61, 3], 2, out, width, dtype)
+    x, d, w = among_nan(rows), among_nan(dy), weight.cuda().requires_grad_()
+    y = expert_linear(x.requires_grad_(), w, offsets.cuda())
+    want, scale = ref.linear(rows, weight, offsets)
+    check(y, want, scale, depth(width, dtype), "y")
+    dx, dw = torch.autograd.grad(y, (x, w), d)
+    want_x, scale_x, want_w, scale_w = ref.linear_grad(rows, weight, offsets, dy)
+    check(dx, want_x, scale_x, depth(out, dtype), "dx")
+    check(dw, want_w, scale_w, depth(70, dtype), "dw")
 
 
 @pytest.mark.parametrize("dtype", TYPES)
