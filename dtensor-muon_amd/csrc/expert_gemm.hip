@@ -815,8 +815,9 @@ __global__ __launch_bounds__(256) void expert_rows_kernel(GArgs g) {
 // ---- fp32 -----------------------------------------------------------------------------------
 //
 // 128 x 128 or 64 x 64 tile (S blocks of 32 a wave and side, 2 or 1), K-tiles of 16, four waves on
-// v_mfma_f32_32x32x2_f32. Both panels stand in LDS as rows of k, whatever their order in memory, so a fragment
-// is one value of a column for each lane. The sums of 256 k are added up apart from the products' own: a
+// v_mfma_f32_32x32x2_f32. Panels stand in LDS as they do in memory, rows 4 values apart from whole ones. A
+// lane holds four k in a row for four products, the other half of the wave the next four: in that order a KC
+// fragment of all four is one read. The sums of 256 k are added up apart from the products' own: a
 // sum that runs over all of k takes a rounding of its whole size at each. 4094 rows of 8 experts of
 // 1001 x 769: 94, 102 and 101 us, 62 to 67 TFLOP/s of 154 (8192 cubed): their 294 to 425 workgroups are one
 // to two for a CU, and each waits for its own loads.
@@ -840,23 +841,62 @@ MUON_DEVICE void f32_load(float (&w)[V], const float* base, int64_t ld, int in, 
 }
 template <bool KR, int V>
 MUON_DEVICE void f32_store(float* lds, const float (&w)[V]) {
-  constexpr int P = 16 * V + 4, EACH = F_K / V;
-  const int tid = threadIdx.x;
-  if constexpr (KR) {
-    float* p = lds + tid / 16 * P + tid % 16 * V;
+  constexpr int EACH = KR ? 16 : F_K / V, P = KR ? 16 * V + 4 : F_K + 4;
+  float* p = lds + (int)threadIdx.x / EACH * P + threadIdx.x % EACH * V;
 #pragma unroll
-    for (int j = 0; j < V; j += 4) *(float4*)(p + j) = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) lds[(tid % EACH * V + j) * P + tid / EACH] = w[j];
+  for (int j = 0; j < V; j += 4) *(float4*)(p + j) = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+}
+// A thread's values of whole K-tiles, whose loads no condition delays: rows behind the last repeat it, and a
+// run of columns that would leave the matrix moves back to end with it (`moved` values) and drops them on
+// the way to LDS.
+template <bool KR, int V>
+struct F32Source {
+  const float* p;
+  int64_t step;
+  int moved;
+  float w[2][V];  // K-tiles under way
+
+  MUON_DEVICE void set(const float* base, int64_t ld, int in) {
+    constexpr int EACH = KR ? 16 : F_K / V;
+    const int row = threadIdx.x / EACH, ch = threadIdx.x % EACH * V, c = KR ? std::min(ch, in - V) : ch;
+    p = base + (KR ? row : std::min(row, in - 1)) * ld + c;
+    step = KR ? F_K * ld : F_K;
+    moved = KR && in < 16 * V ? ch - c : 0;
   }
+  // the K-tile at p, and on to the next one if there is one
+  template <int TO>
+  MUON_DEVICE void load(bool on) {
+    __builtin_memcpy(w[TO], p, 4 * V);
+    p += on ? step : 0;
+  }
+  template <int FROM>
+  MUON_DEVICE void store(float* lds, bool ragged) {
+    if (ragged) {
+#pragma unroll
+      for (int bit = 1; bit < V; bit *= 2)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (moved & bit) w[FROM][j] = j + bit < V ? w[FROM][j + bit] : 0.0f;
+    }
+    f32_store<KR, V>(lds, w[FROM]);
+  }
+};
+// Values k .. k + 3 of row or column r of a panel.
+template <bool KR, int V>
+MUON_DEVICE f32x4 f32_fragment(const float* lds, int r, int k) {
+  constexpr int P = KR ? 16 * V + 4 : F_K + 4;
+  if constexpr (!KR) return *(const f32x4*)(lds + r * P + k);
+  f32x4 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = lds[(k + j) * P + r];
+  return v;
 }
 
 template <int FORM, int S>
 __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
-  constexpr int F_B = 64 * S, F_P = F_B + 4, V = 4 * S;
+  constexpr int F_B = 64 * S, V = 4 * S;
   constexpr bool KRA = FORM == WGT, KRB = FORM != FWD;
-  __shared__ __align__(16) float lds[2][2][F_K * F_P];
+  __shared__ __align__(16) float lds[2][2][F_B * (F_K + 4)];
   int e, tm, tn, row0 = 0, left = 0, K, M;
   if constexpr (FORM == WGT) {
     const int per = g.tiles_m * g.tiles_n, L = blockIdx.x;
@@ -886,38 +926,26 @@ __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
     for (int j = 0; j < S; ++j)
 #pragma unroll
       for (int q = 0; q < 16; ++q) acc[i][j][q] = sum[i][j][q] = 0.0f;
-  float wa[V], wb[V];
-  const int KT = (K + F_K - 1) / F_K;
-  if (KT) {
-    f32_load<KRA, V>(wa, A, g.lda, M, 0, K);
-    f32_load<KRB, V>(wb, B, g.ldb, N, 0, K);
-    f32_store<KRA, V>(lds[0][0], wa);
-    f32_store<KRB, V>(lds[0][1], wb);
-  }
-  __syncthreads();
-  for (int kt = 0; kt < KT; ++kt) {
-    const bool more = kt + 1 < KT;
-    if (more) {
-      f32_load<KRA, V>(wa, A, g.lda, M, (kt + 1) * F_K, K - (kt + 1) * F_K);
-      f32_load<KRB, V>(wb, B, g.ldb, N, (kt + 1) * F_K, K - (kt + 1) * F_K);
-    }
-    const float* la = lds[kt & 1][0] + wm * 32 * S + fr;
-    const float* lb = lds[kt & 1][1] + wn * 32 * S + fr;
+  auto multiply = [&](int kt) {
+    const float* la = lds[kt & 1][0];
+    const float* lb = lds[kt & 1][1];
 #pragma unroll
-    for (int k = 0; k < F_K; k += 2) {
-      float fa[S], fb[S];
+    for (int k = 0; k < F_K; k += 8) {
+      f32x4 fa[S], fb[S];
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        fa[i] = la[(k + fk) * F_P + i * 32];
-        fb[i] = lb[(k + fk) * F_P + i * 32];
+        fa[i] = f32_fragment<KRA, V>(la, wm * 32 * S + i * 32 + fr, k + fk * 4);
+        fb[i] = f32_fragment<KRB, V>(lb, wn * 32 * S + i * 32 + fr, k + fk * 4);
       }
 #pragma unroll
-      for (int i = 0; i < S; ++i)
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int j = 0; j < S; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j], fa[i], acc[i][j], 0, 0, 0);
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+          for (int j = 0; j < S; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j][q], fa[i][q], acc[i][j], 0, 0, 0);
     }
-    if (kt % F_SUM == F_SUM - 1 || !more) {
+    if (kt % F_SUM == F_SUM - 1) {
 #pragma unroll
       for (int i = 0; i < S; ++i)
 #pragma unroll
@@ -928,12 +956,59 @@ __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
             acc[i][j][q] = 0.0f;
           }
     }
-    if (more) {
-      f32_store<KRA, V>(lds[(kt + 1) & 1][0], wa);
-      f32_store<KRB, V>(lds[(kt + 1) & 1][1], wb);
-    }
+  };
+  // Whole K-tiles: while one is multiplied the next two are under way. The last loads repeat the last K-tile, so
+  // that as many are under way in every turn.
+  const int KT = (K + F_K - 1) / F_K;
+  const int whole = (KRA ? g.M >= V : true) && (KRB ? g.N >= V : true) ? K / F_K / 2 * 2 : 0;
+  if (whole) {
+    F32Source<KRA, V> sa;
+    F32Source<KRB, V> sb;
+    sa.set(A, g.lda, M);
+    sb.set(B, g.ldb, N);
+    const bool ra = KRA && M < F_B, rb = KRB && N < F_B;
+    auto load = [&](auto to, int kt) {
+      sa.template load<decltype(to)::value>(kt + 1 < whole);
+      sb.template load<decltype(to)::value>(kt + 1 < whole);
+    };
+    auto store = [&](auto from, int kt) {
+      sa.template store<decltype(from)::value>(lds[kt & 1][0], ra);
+      sb.template store<decltype(from)::value>(lds[kt & 1][1], rb);
+    };
+    typedef std::integral_constant<int, 0> Zero;
+    typedef std::integral_constant<int, 1> One;
+    load(Zero{}, 0);
+    load(One{}, 1);
+    store(Zero{}, 0);
+    load(Zero{}, 2);
     __syncthreads();
+#pragma unroll 1
+    for (int kt = 0; kt < whole; kt += 2) {
+      multiply(kt);
+      store(One{}, kt + 1);
+      load(One{}, kt + 3);
+      __syncthreads();
+      multiply(kt + 1);
+      store(Zero{}, kt + 2);
+      load(Zero{}, kt + 4);
+      __syncthreads();
+    }
   }
+  for (int kt = whole; kt < KT; ++kt) {
+    float wa[V], wb[V];
+    f32_load<KRA, V>(wa, A, g.lda, M, kt * F_K, K - kt * F_K);
+    f32_load<KRB, V>(wb, B, g.ldb, N, kt * F_K, K - kt * F_K);
+    f32_store<KRA, V>(lds[kt & 1][0], wa);
+    f32_store<KRB, V>(lds[kt & 1][1], wb);
+    __syncthreads();
+    multiply(kt);
+  }
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) sum[i][j][q] += acc[i][j][q];
   // a lane holds row fr, columns 8 (q / 4) + 4 fk + q % 4 of each 32 x 32 block
   float* C = (float*)g.c + (FORM == WGT ? ((int64_t)e * g.M + tm * F_B) * g.N : (int64_t)row0 * g.N);
 #pragma unroll
