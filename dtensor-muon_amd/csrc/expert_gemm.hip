@@ -819,8 +819,10 @@ __global__ __launch_bounds__(256) void expert_rows_kernel(GArgs g) {
 // lane holds four k in a row for four products, the other half of the wave the next four: in that order a KC
 // fragment of all four is one read. The sums of 256 k are added up apart from the products' own: a
 // sum that runs over all of k takes a rounding of its whole size at each. 4094 rows of 8 experts of
-// 1001 x 769: 94, 102 and 101 us, 62 to 67 TFLOP/s of 154 (8192 cubed): their 294 to 425 workgroups are one
-// to two for a CU, and each waits for its own loads.
+// 1001 x 769: 80 to 86 us each, 73 to 79 TFLOP/s of 154 (8192 cubed): about 1090 tiles of 64, so that some
+// CUs have five of them and others four, whose edges hold a tenth of nothing. Two K-tiles are under way, in
+// counted loads; with one, behind conditions, 91, 94 and 84 us. More of these workgroups on a CU
+// help, wider tiles and K-tiles do not.
 constexpr int F_K = 16, F_SUM = 256 / F_K;
 
 // A thread's V = 4 S values: KR: of row k; KC: of row r, V k in a row.
@@ -1135,11 +1137,11 @@ template <int FORM>
 int launch(const GArgs& g, int dtype, hipStream_t s) {
   switch (dtype) {
     case MUON_DT_F32: {
-      // Tiles of 128 where there are several for every CU (8 experts of 1001 x 769: 32000 rows 428 us, in
-      // tiles of 64 526; 4094 rows 129 and 92), for WGT, where the largest expert's last long, more (its
-      // gradient from those rows 740 and 588, of 64 experts of 1408 x 2048 from 16384 rows 813 and 891).
+      // Tiles of 128 where there are ten for every CU (16 experts of 1024 x 1024: 64000 rows 1121 us, in
+      // tiles of 64 1142, their gradient 1026 and 1111; 16000 rows 346 and 312); for WGT, whose experts are
+      // tiled alone, by the weights (8 of 2048 x 2048, 4000 rows: 270 and 306; 8 of 1001 x 769, 32000 rows: 641 and 517).
       const int64_t tiles = (FORM == WGT ? (int64_t)g.M * g.N * g.E : g.R * g.N) / (128 * 128);
-      return tiles >= (FORM == WGT ? 2048 : 1536) ? launch32<FORM, 2>(g, s) : launch32<FORM, 1>(g, s);
+      return tiles >= (FORM == WGT ? 2048 : 2560) ? launch32<FORM, 2>(g, s) : launch32<FORM, 1>(g, s);
     }
     case MUON_DT_BF16: return launch_typed<MUON_DT_BF16, FORM>(g, s);
     default: return launch_typed<MUON_DT_F16, FORM>(g, s);
