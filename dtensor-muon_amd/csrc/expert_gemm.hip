@@ -209,6 +209,48 @@ struct Stage {
   }
 };
 
+// The same of whole K-tiles, two of which are under way: the pointers move on, and nothing depends on a
+// lane, so that loads are waited for by count.
+template <int PANEL, bool KR, int NT, bool ALIGNED>
+struct Runs {
+  typedef Stage<PANEL, KR, NT, ALIGNED> One;
+  const uint16_t* p[One::CHUNKS];
+  int64_t step;
+  int moved;
+  muon_u4 w[2][One::CHUNKS];
+
+  MUON_DEVICE void set(const uint16_t* base, int64_t ld, int in) {
+    const int row = threadIdx.x / One::PER_ROW, ch = threadIdx.x % One::PER_ROW * 8;
+    const int c = KR ? std::min(ch, in - 8) : ch;
+#pragma unroll
+    for (int q = 0; q < One::CHUNKS; ++q) {
+      const int r = row + q * One::ROWS_PASS;
+      p[q] = base + (KR ? r : std::min(r, in - 1)) * ld + c;
+    }
+    step = KR ? BK * ld : BK;
+    moved = !ALIGNED && KR && in < PANEL ? ch - c : 0;
+  }
+  // the K-tile at p, and on to the next one if there is one
+  template <int TO>
+  MUON_DEVICE void load(bool on) {
+#pragma unroll
+    for (int q = 0; q < One::CHUNKS; ++q) {
+      if constexpr (ALIGNED) w[TO][q] = *(const muon_u4*)p[q];
+      else w[TO][q] = load_u4(p[q]);
+      p[q] += on ? step : 0;
+    }
+  }
+  template <int FROM>
+  MUON_DEVICE void store(uint8_t* lds, bool ragged) {
+#pragma unroll
+    for (int q = 0; q < One::CHUNKS; ++q) {
+      muon_u4 v = w[FROM][q];
+      if (!ALIGNED && ragged) v = drop(v, moved);
+      One::put(lds, q, v);
+    }
+  }
+};
+
 // 8 consecutive k (ks 32-k substep, lane / 16) of row or column r0 + lane % 16.
 template <int PANEL, bool KR>
 MUON_DEVICE muon_u4 fragment(uint8_t* lds, int r0, int ks) {
@@ -228,12 +270,10 @@ MUON_DEVICE muon_u4 fragment(uint8_t* lds, int r0, int ks) {
   }
 }
 
-// A BM x BN tile by WM x WN waves, the next K-tile's loads under way during the products of one: for
-// few tiles and for ragged sizes (262144 rows, 64 experts of 1409 x 2041: 2844, 2625 and 2690 us, 530 to 575
-// TFLOP/s; with loads two K-tiles ahead 4361, 4253 and 4280, in registers that a second workgroup of
-// the CU needs).
+// A BM x BN tile by WM x WN waves: for few tiles and for ragged sizes (262144 rows, 64 experts of 1409 x
+// 2041: 2835, 2654 and 2729 us, 530 to 570 TFLOP/s). Four waves a SIMD, two workgroups a CU.
 template <int DT, int FORM, int BM, int BN, int WM, int WN, bool ALIGNED>
-__global__ __launch_bounds__(64 * WM * WN, 1) void expert_gemm_kernel(GArgs g) {
+__global__ __launch_bounds__(64 * WM * WN, 4) void expert_gemm_kernel(GArgs g) {
   constexpr int NT = 64 * WM * WN;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr bool KRA = FORM == WGT, KRB = FORM != FWD;
@@ -263,31 +303,14 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void expert_gemm_kernel(GArgs g) {
 
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int wm = wave % WM, wn = wave / WM;
-  Stage<BM, KRA, NT, ALIGNED> sa;
-  Stage<BN, KRB, NT, ALIGNED> sb;
   f32x4 acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
-  const int KT = (K + BK - 1) / BK;
-  const bool wide_a = (KRA ? g.M : g.K) >= 8, wide_b = (KRB ? g.N : g.K) >= 8;
-  if (KT) {
-    sa.load(A, g.lda, M, 0, K, wide_a);
-    sb.load(B, g.ldb, N, 0, K, wide_b);
-    sa.store(smem, M, K, wide_a);
-    sb.store(smem + PANEL_A, N, K, wide_b);
-  }
-  __syncthreads();
-  for (int kt = 0; kt < KT; ++kt) {
+  auto multiply = [&](int kt) {
     uint8_t* st = smem + (kt & 1) * STAGE;
-    const bool more = kt + 1 < KT;
-    const int k1 = (kt + 1) * BK;
-    if (more) {
-      sa.load(A, g.lda, M, k1, K - k1, wide_a);
-      sb.load(B, g.ldb, N, k1, K - k1, wide_b);
-    }
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       muon_u4 fa[FM], fb[FN];
@@ -300,12 +323,68 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void expert_gemm_kernel(GArgs g) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = mfma16<DT>(fb[j], fa[i], acc[i][j]);
     }
-    if (more) {
-      uint8_t* nx = smem + ((kt + 1) & 1) * STAGE;
-      sa.store(nx, M, K - k1, wide_a);
-      sb.store(nx + PANEL_A, N, K - k1, wide_b);
-    }
+  };
+  const int KT = (K + BK - 1) / BK;
+  const bool wide_a = (KRA ? g.M : g.K) >= 8, wide_b = (KRB ? g.N : g.K) >= 8;
+  // Pairs of whole K-tiles; the last loads repeat the last of them, so that as many are under way in every
+  // turn. (Few tiles gain: 8 experts of 100 x 4001, 6000 rows 76 -> 50 us, 64 of 1408 x 2048, 1024 rows 98 -> 80.
+  // WGT does not, nor do ragged columns, whose runs are shifted in registers that are short then: 262144
+  // rows of 64 experts of 1409 x 2041 2729 -> 3172.)
+  constexpr bool AHEAD = FORM == FWD || (FORM == ROWS && ALIGNED);
+  const int whole = AHEAD && (!KRB || wide_b) ? K / BK / 2 * 2 : 0;
+  if (whole) {
+    Runs<BM, KRA, NT, ALIGNED> ra;
+    Runs<BN, KRB, NT, ALIGNED> rb;
+    ra.set(A, g.lda, M);
+    rb.set(B, g.ldb, N);
+    auto load = [&](auto to, int kt) {
+      ra.template load<decltype(to)::value>(kt + 1 < whole);
+      rb.template load<decltype(to)::value>(kt + 1 < whole);
+    };
+    auto store = [&](auto from, int kt) {
+      ra.template store<decltype(from)::value>(smem + (kt & 1) * STAGE, KRA && M < BM);
+      rb.template store<decltype(from)::value>(smem + (kt & 1) * STAGE + PANEL_A, KRB && N < BN);
+    };
+    typedef std::integral_constant<int, 0> Zero;
+    typedef std::integral_constant<int, 1> One;
+    load(Zero{}, 0);
+    load(One{}, 1);
+    store(Zero{}, 0);
+    load(Zero{}, 2);
     __syncthreads();
+#pragma unroll 1
+    for (int kt = 0; kt < whole; kt += 2) {
+      multiply(kt);
+      store(One{}, kt + 1);
+      load(One{}, kt + 3);
+      __syncthreads();
+      multiply(kt + 1);
+      store(Zero{}, kt + 2);
+      load(Zero{}, kt + 4);
+      __syncthreads();
+    }
+  }
+  if (whole < KT) {
+    Stage<BM, KRA, NT, ALIGNED> sa;
+    Stage<BN, KRB, NT, ALIGNED> sb;
+    auto load = [&](int kt) {
+      sa.load(A, g.lda, M, kt * BK, K - kt * BK, wide_a);
+      sb.load(B, g.ldb, N, kt * BK, K - kt * BK, wide_b);
+    };
+    auto store = [&](int kt) {
+      sa.store(smem + (kt & 1) * STAGE, M, K - kt * BK, wide_a);
+      sb.store(smem + (kt & 1) * STAGE + PANEL_A, N, K - kt * BK, wide_b);
+    };
+    load(whole);
+    store(whole);
+    __syncthreads();
+#pragma unroll 1
+    for (int kt = whole; kt < KT; ++kt) {
+      if (kt + 1 < KT) load(kt + 1);
+      multiply(kt);
+      if (kt + 1 < KT) store(kt + 1);
+      __syncthreads();
+    }
   }
 
   // the b fragment is the first operand: a lane holds four consecutive columns of one row
