@@ -1196,9 +1196,12 @@ int launch32(GArgs g, hipStream_t s) {
 // Which kernel, all sides measured on 8 to 128 experts of 1024 x 1024 to 4096 x 4096 (us):
 // * FWD of at most 8 rows an expert on the average: the kernel of few rows (64 experts of 1408 x 2048, 128
 //   and 512 rows: 58 and 85, 90 and 97 in tiles of 128).
-// * 256-row tiles for output of 64 of them or more (16 experts of 4096 x 4096, 1024 rows: 136, in tiles of
-//   128 180; 8 of 1024 x 1024, 4000 rows: 26 and 26, 2000 rows: 25 and 18); WGT also with fewer of them
-//   than CUs where they are long (8 of 1024 x 1024, 4000 rows: 26 and 26, 2000 rows 25 and 19).
+// * FWD and ROWS in tiles of 256 from 112 of them on (8 experts of 1024 x 1024, 8000 rows: 27 and 27, in
+//   tiles of 128 33 and 35; 6000 rows: 27 and 26, 23 and 25), if there are 192 rows an expert: with fewer the weights'
+//   bytes count, which more workgroups fetch faster (64 of 1408 x 2048, 8192 rows: 123 and 117, 114 and
+//   114; 16384 rows: 160 and 151, 176 and 182).
+// * WGT where there is one for every CU (4 experts of 2048 x 2048, 4000 rows 73 and 91), or where fewer
+//   of them are very long (2 of 2048 x 2048, 8000 rows: 122 and 98, 32000 rows: 279 and 349).
 // * Else, and where rows are no whole 16-byte runs, tiles of 128.
 template <int DT, int FORM>
 int launch_typed(const GArgs& g, hipStream_t s) {
@@ -1208,7 +1211,8 @@ int launch_typed(const GArgs& g, hipStream_t s) {
   const int64_t wa = FORM == WGT ? g.M : g.K, wb = FORM == FWD ? g.K : g.N;
   const bool direct = aligned && g.lda >= wa && g.ldb >= wb && std::max({g.lda, g.ldb, (int64_t)g.N}) <= P_MOST;
   const int64_t area = FORM == WGT ? (int64_t)g.M * g.N * g.E : g.R * g.N, tile = 256 * 256;
-  const bool large = FORM == WGT ? area >= P_GROUPS * tile || g.R >= 512 * (int64_t)g.E : area >= P_GROUPS / 4 * tile;
+  const bool large = FORM == WGT ? area >= P_GROUPS * tile || g.R >= 8192 * (int64_t)g.E
+                                 : area >= 112 * tile && g.R >= 192 * (int64_t)g.E;
   return direct && large ? launch_pipe<DT, FORM>(g, s) : launch16<DT, FORM, 128, 128, 4, 2>(g, aligned, s);
 }
 

@@ -401,6 +401,36 @@ def test_products_among_nan(out, width, dtype):
     check(dw, want_w, scale_w, depth(70, dtype), "dw")
 
 
+MANY = [
+    # outputs and gradients of so many rows, or of so large weights, that wider tiles are taken
+    ([0, 1, 3000, 255, 4001, 257], 30, 1000, 72, TYPES),
+    ([0, 1, 3000, 255, 4001, 257], 30, 72, 1000, TYPES),
+    ([7400, 300], 0, 1032, 8, TYPES),
+    ([3000, 0, 1, 255, 4001, 257], 1, 968, 1032, TYPES),       # whole K-tiles and a part
+    ([0, 1, 70, 64, 65, 513, 0, 8] * 8, 3, 520, 512, TYPES),
+    ([8200], 0, 264, 40, TYPES),                                # one expert's long gradient
+    ([1, 20000, 0, 22000], 5, 1024, 20, [torch.float32]),
+    ([1, 20000, 0, 22000], 5, 17, 1027, [torch.float32]),
+    ([5, 0, 40, 33] * 2, 2, 2050, 2047, [torch.float32]),
+]
+
+
+@pytest.mark.parametrize("case, dtype", [(i, t) for i, c in enumerate(MANY) for t in c[4]])
+def test_many_rows_and_large_weights(case, dtype):
+    counts, rest, out, width, _ = MANY[case]
+    rows, weight, offsets, dy = product_case(counts, rest, out, width, dtype)
+    end = int(offsets[-1])
+    rows[end:], dy[end:] = math.nan, math.inf
+    x, w = rows.cuda().requires_grad_(), weight.cuda().requires_grad_()
+    y = expert_linear(x, w, offsets.cuda())
+    want, scale = ref.linear(rows, weight, offsets)
+    check(y, want, scale, depth(width, dtype), "y")
+    dx, dw = torch.autograd.grad(y, (x, w), dy.cuda())
+    want_x, scale_x, want_w, scale_w = ref.linear_grad(rows, weight, offsets, dy)
+    check(dx, want_x, scale_x, depth(out, dtype), "dx")
+    check(dw, want_w, scale_w, depth(max(counts), dtype), "dw")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows, out, width", [(0, 8, 16), (5, 0, 16), (5, 8, 0)])
 def test_products_of_nothing(rows, out, width, dtype):
