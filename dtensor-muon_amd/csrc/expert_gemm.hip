@@ -11,7 +11,7 @@
 // MFMA with fp32 accumulators, fp32 on the fp32 MFMA.
 //
 // 64 experts of 1408 x 2048 in bf16 (an 8192-cubed library product runs at 1431 TFLOP/s, a copy at 4.9 TB/s):
-//   262144 rows: FWD 1236 to 1317 us, ROWS 1264 to 1288, WGT 1186 to 1237, 1.15 to 1.27 PFLOP/s; 1408
+//   262144 rows: FWD 1217 to 1346 us, ROWS 1259 to 1308, WGT 1186 to 1257, 1.12 to 1.27 PFLOP/s; 1408
 //     fills 5.5 tiles of 256, so the matrix units do 9% more than that;
 //   128 rows: 60 to 63 us, the bytes of the weights that they meet at 6 TB/s (part of them from the
 //     last-level cache).
