@@ -1194,8 +1194,10 @@ int launch32(GArgs g, hipStream_t s) {
 }
 
 // Which kernel, all sides measured on 8 to 128 experts of 1024 x 1024 to 4096 x 4096 (us):
-// * FWD of at most 8 rows an expert on the average: the kernel of few rows (64 experts of 1408 x 2048, 128
-//   and 512 rows: 58 and 85, 90 and 97 in tiles of 128).
+// * FWD of at most 4 rows an expert on the average: the kernel of few rows (64 experts of 1408 x 2048, 128 and
+//   256 rows: 60 and 67, 72 and 73 in tiles of 128; 512 rows 85 and 78). Short rows of many experts
+//   are an exception (128 of 2048 x 768, 512 rows: 90 and 73), few tiles another, up to 16 rows (8 of
+//   1024 x 1024, 128 rows: 9 and 11; ragged ones, 8 of 1001 x 769, 64 rows: 17 and 15).
 // * FWD and ROWS in tiles of 256 from 112 of them on (8 experts of 1024 x 1024, 8000 rows: 27 and 27, in
 //   tiles of 128 33 and 35; 6000 rows: 27 and 26, 23 and 25), if there are 192 rows an expert: with fewer the weights'
 //   bytes count, which more workgroups fetch faster (64 of 1408 x 2048, 8192 rows: 123 and 117, 114 and
@@ -1207,7 +1209,8 @@ template <int DT, int FORM>
 int launch_typed(const GArgs& g, hipStream_t s) {
   const bool aligned = ((uintptr_t)g.a | (uintptr_t)g.b | (uintptr_t)g.c) % 16 == 0 &&
                        (g.lda | g.ldb | g.sb | g.N | g.K | g.M) % 8 == 0;
-  if (FORM == FWD && g.R <= 8 * (int64_t)g.E) return launch_rows<DT>(g, aligned, s);
+  const int64_t columns = (int64_t)g.E * g.N, few = aligned && columns <= 16384 ? 16 : g.K >= 1024 || columns <= 65536 ? 4 : 0;
+  if (FORM == FWD && g.R <= few * g.E) return launch_rows<DT>(g, aligned, s);
   const int64_t wa = FORM == WGT ? g.M : g.K, wb = FORM == FWD ? g.K : g.N;
   const bool direct = aligned && g.lda >= wa && g.ldb >= wb && std::max({g.lda, g.ldb, (int64_t)g.N}) <= P_MOST;
   const int64_t area = FORM == WGT ? (int64_t)g.M * g.N * g.E : g.R * g.N, tile = 256 * 256;
