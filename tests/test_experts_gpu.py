@@ -575,6 +575,40 @@ def test_captured_layer(dtype):
             assert torch.equal(a, b)
 
 
+def test_captured_products_of_many_rows():
+    """Products and gradients in wide tiles, replayed on other rows and other offsets."""
+    g = gen(37)
+    n, experts, out, width = 7500, 16, 1024, 1032
+
+    def inputs():
+        at = torch.randint(0, n, (experts - 1,), generator=g).sort().values
+        return (torch.randn(n, width, generator=g).bfloat16(), torch.randn(experts, out, width, generator=g).bfloat16(),
+                torch.cat([torch.zeros(1, dtype=torch.int64), at, torch.tensor([n - 3])]).clamp(max=n - 3).int(),
+                torch.randn(n, out, generator=g).bfloat16())
+
+    def run(x, w, offsets, dy):
+        leaf, wleaf = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = expert_linear(leaf, wleaf, offsets)
+        return (y.detach(), *torch.autograd.grad(y, (leaf, wleaf), dy))
+
+    held = [t.cuda() for t in inputs()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(*held)
+    for _ in range(3):
+        for to, t in zip(held, inputs()):
+            to.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, run(*held)):
+            assert torch.equal(a, b)
+
+
 def test_two_streams_at_once():
     g = gen(19)
     cases = []
