@@ -160,12 +160,29 @@ MUON_DEVICE void decode8(uint2 c, float scale, float (&x)[8]) {
     x[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(w, 3) * scale;
   }
 }
-MUON_DEVICE uint2 encode8(const float (&x)[8], float inv) {
+// The quotient x / scale, correctly rounded: inv = 1 / scale gives it up to an ulp, and the exact remainder
+// of that moves it to the rounded one (P. Markstein, IBM J. Res. Dev. 34(1), 1990). A finite scale is 2^-49
+// to 2^120, and only quotients from 2^-10 on have a code, so what such a value goes through is normal. Of an
+// infinite or NaN scale, whose values are all NaN, the product with its inverse has the quotient's code.
+struct Quotient {
+  float inv, neg, back;
+  MUON_DEVICE explicit Quotient(float scale) : inv(1.0f / scale) {
+    const bool finite = scale <= 3.40282347e38f;
+    neg = finite ? -scale : 0.0f;
+    back = finite ? inv : 0.0f;
+  }
+  MUON_DEVICE float operator()(float x) const {
+#pragma clang fp contract(off)
+    const float q = x * inv;
+    return __builtin_fmaf(__builtin_fmaf(neg, q, x), back, q);
+  }
+};
+MUON_DEVICE uint2 encode8(const float (&x)[8], const Quotient& by) {
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * h] * inv, x[4 * h + 1] * inv, 0, false);
-    w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * h + 2] * inv, x[4 * h + 3] * inv, c, true);
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(by(x[4 * h]), by(x[4 * h + 1]), 0, false);
+    w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(by(x[4 * h + 2]), by(x[4 * h + 3]), c, true);
   }
   return make_uint2(w[0], w[1]);
 }
@@ -212,12 +229,11 @@ __global__ __launch_bounds__(THREADS) void adamw_fp8_kernel(StepArgs a) {
     }
     const auto larger = [](uint32_t x, uint32_t y) { return std::max(x, y); };
     const float mn = block_scale(group_reduce<G>(mt, larger)), vn = block_scale(group_reduce<G>(vt, larger));
-    // the product with the inverse differs from the quotient by a rounding of 2^-24, where a code's is 2^-4
-    const float mi = 1.0f / mn, vi = 1.0f / vn;
+    const Quotient by_m(mn), by_v(vn);
 #pragma unroll
     for (int q = 0; q < RUNS; ++q) {
       const int64_t e = e0 + q * 512;
-      const uint2 cm = encode8(m[q], mi), cv = encode8(root[q], vi);
+      const uint2 cm = encode8(m[q], by_m), cv = encode8(root[q], by_v);
       __builtin_memcpy((uint8_t*)t.m + e, &cm, 8);
       __builtin_memcpy((uint8_t*)t.v + e, &cv, 8);
     }
