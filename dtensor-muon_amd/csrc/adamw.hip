@@ -2,9 +2,11 @@
 //   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
 //   p = (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // in fp32, p rounded once to its type. The moments are fp32, or fp8: e4m3 codes with one scale
-// (absmax / 448) for each block of values. In fp8 the second moment is held as its root: |m| is at
-// most a small multiple of sqrt(v), so where the root falls below e4m3's 17 binades under its block's
-// largest the mean does too, while v itself would vanish at half of them and leave m / eps.
+// (absmax / 448) for each block of values. In fp8 the second moment is held as its root, which spans half
+// the binades that v does: e4m3 has 17 of them under a block's largest. Mean and root have scales of their
+// own, and a block's mean can be far below its root (a large gradient whose sign alternates, or one that
+// is past), so a root can be too small for a code where its mean has one, and would leave m / eps for
+// the next step: the root's code is at least 1 where the mean's is not 0.
 //
 // Two kinds of launches: a table of the tensors (pointers, first piece of work, and the two factors that
 // depend on t, whose counters it moves on), as many as a launch's arguments hold at a time; then one
@@ -186,6 +188,11 @@ MUON_DEVICE uint2 encode8(const float (&x)[8], const Quotient& by) {
   }
   return make_uint2(w[0], w[1]);
 }
+// The codes v of roots, the least one in place of 0 where the mean's code in m is not 0.
+MUON_DEVICE uint32_t least_root(uint32_t v, uint32_t m) {
+  constexpr uint32_t low = 0x7f7f7f7fu, top = 0x80808080u;  // a byte of 7 bits and low: top set if it is not 0
+  return v | (((m & low) + low) & ~((v & low) + low) & top) >> 7;
+}
 // absmax / 448 of a block; bits are compared as integers, so that a NaN is the largest
 MUON_DEVICE float block_scale(uint32_t bits) {
   const float top = __uint_as_float(bits);
@@ -233,7 +240,8 @@ __global__ __launch_bounds__(THREADS) void adamw_fp8_kernel(StepArgs a) {
 #pragma unroll
     for (int q = 0; q < RUNS; ++q) {
       const int64_t e = e0 + q * 512;
-      const uint2 cm = encode8(m[q], by_m), cv = encode8(root[q], by_v);
+      const uint2 cm = encode8(m[q], by_m), cr = encode8(root[q], by_v);
+      const uint2 cv = make_uint2(least_root(cr.x, cm.x), least_root(cr.y, cm.y));
       __builtin_memcpy((uint8_t*)t.m + e, &cm, 8);
       __builtin_memcpy((uint8_t*)t.v + e, &cv, 8);
     }

@@ -194,8 +194,9 @@ class AdamWFp8(AdamW):
     """AdamW with the moments in 8 bits: float8_e4m3fn codes, with one fp32 scale for each block of
     ``block_size`` consecutive values (:class:`OptimStateFp8`, the largest value of a block at 448).
 
-    The state is ``step``, ``exp_avg`` and ``exp_avg_sq_root``, the second moment's root: in e4m3 v itself
-    would vanish beside its block's largest at half the binades where m does, and leave m / eps.
+    The state is ``step``, ``exp_avg`` and ``exp_avg_sq_root``, the second moment's root, which spans half the
+    binades that v does. A root that is too small for a code beside its block's largest has the least one
+    where its mean has a code, so that no step is m / eps.
     Parameters of fewer than 4096 values, or not a multiple of ``block_size`` (``MuonLP``'s rule), have
     fp32 moments as in :class:`AdamW`.
 
