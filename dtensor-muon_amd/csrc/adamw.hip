@@ -8,6 +8,13 @@
 // is past), so a root can be too small for a code where its mean has one, and would leave m / eps for
 // the next step: the root's code is at least 1 where the mean's is not 0.
 //
+// Codes are rounded to nearest while a moment moves by more than that holds back: without a gradient, a mean
+// by 1 - b1 and a root by 1 - sqrt(b2), where half a step of a code is 2^-5 to 2^-4. Up to b2 = 0.95 a block's
+// scale, which its largest value moves, shifts the codes enough for the roots to follow. Beyond that they
+// stay (b2 = 0.99, gradients that fall from 0.5 to 0.005 beside others: roots 59 times too large), and
+// from b1 = 15/16 on a mean does: codes are rounded up or down at random then, by a number made from the
+// step and the value's place, with the chance that keeps the value on the average.
+//
 // Two kinds of launches: a table of the tensors (pointers, first piece of work, and the two factors that
 // depend on t, whose counters it moves on), as many as a launch's arguments hold at a time; then one
 // over all values, whose workgroups find their tensor in the table. Everything that changes from step
@@ -24,7 +31,7 @@
 
 namespace {
 
-// A tensor in the table, 64 bytes.
+// A tensor in the table.
 struct Entry {
   void* p;
   const void* g;
@@ -34,6 +41,7 @@ struct Entry {
   float* v_scale;
   int64_t n;
   float size, scale;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  uint32_t seed;      // of the step's random numbers
 };
 
 constexpr int TABLE_MAX = 48;  // tensors of one table launch: 3.5 KB of arguments
@@ -46,6 +54,13 @@ struct TableArgs {
   double lr, log2_b1, log2_b2;
 };
 
+// 32 bits that change with every bit of x: the odd numbers are 2^32 over the golden ratio and 2^31.5.
+MUON_DEVICE uint32_t scatter(uint32_t x) {
+  x = (x ^ x >> 16) * 0xb504f333u;
+  x = (x ^ x >> 15) * 0x9e3779b1u;
+  return x ^ x >> 16;
+}
+
 __global__ __launch_bounds__(64) void adamw_table_kernel(TableArgs a) {
   const int i = threadIdx.x;
   if (i >= a.n) return;
@@ -55,7 +70,7 @@ __global__ __launch_bounds__(64) void adamw_table_kernel(TableArgs a) {
   // b^t by a power of two; b = 0 has log2 -inf and gives 0
   const double c1 = 1.0 - exp2(step * a.log2_b1), c2 = 1.0 - exp2(step * a.log2_b2);
   a.table[a.at + i] = Entry{t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.avg_scale, t.sq_scale, t.numel,
-                            (float)(a.lr / c1), (float)(1.0 / sqrt(c2))};
+                            (float)(a.lr / c1), (float)(1.0 / sqrt(c2)), scatter(__float_as_uint(step))};
   a.pieces[a.at + i] = a.first[i];
 }
 
@@ -188,6 +203,36 @@ MUON_DEVICE uint2 encode8(const float (&x)[8], const Quotient& by) {
   }
   return make_uint2(w[0], w[1]);
 }
+// A quotient as one of the two values of a code around it, up if random bits carry: a code has 3 bits of a
+// float's 23, and below 2^-6 steps of 2^-9, which 2^-6 more makes the same. 16 of the 20 bits behind a code's
+// are random and the last ones their middle: a move of a 2^-11th of a step (b2 = 0.9999) is off by 2% at most.
+MUON_DEVICE float to_code(float y, uint32_t random16) {
+  const float a = fabsf(y), more = a >= 0x1p-6f ? 0.0f : 0x1p-6f;
+  const float c = __uint_as_float((__float_as_uint(a + more) + (random16 << 4 | 8)) & 0xfff00000u) - more;
+  return copysignf(c > 448.0f ? 448.0f : c, y);
+}
+// The codes of eight means and roots at random, by a number for each place.
+MUON_DEVICE void encode8_random(const float (&m)[8], const Quotient& by_m, const float (&v)[8], const Quotient& by_v,
+                                uint32_t seed, uint2& cm, uint2& cv) {
+  uint32_t wm[2], wv[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float x[4], y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t r = scatter(seed + (4 * h + j) * 0x9e3779b1u);
+      x[j] = to_code(by_m(m[4 * h + j]), r & 0xffffu);
+      y[j] = to_code(by_v(v[4 * h + j]), r >> 16);
+    }
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    wm[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], c, true);
+    c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    wv[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
+  }
+  cm = make_uint2(wm[0], wm[1]);
+  cv = make_uint2(wv[0], wv[1]);
+}
+
 // The codes v of roots, the least one in place of 0 where the mean's code in m is not 0.
 MUON_DEVICE uint32_t least_root(uint32_t v, uint32_t m) {
   constexpr uint32_t low = 0x7f7f7f7fu, top = 0x80808080u;  // a byte of 7 bits and low: top set if it is not 0
@@ -201,7 +246,7 @@ MUON_DEVICE float block_scale(uint32_t bits) {
 
 // fp8 moments: a wave holds RUNS runs of 512 values, a block is G lanes of one run (G = 64: of all of
 // them). Tensors are whole blocks, so the lanes of a block are all in or all out.
-template <int DT, int G, int RUNS>
+template <int DT, int G, int RUNS, bool RANDOM>
 __global__ __launch_bounds__(THREADS) void adamw_fp8_kernel(StepArgs a) {
   const int i = find_tensor(a);
   const Entry t = a.table[i];
@@ -240,7 +285,14 @@ __global__ __launch_bounds__(THREADS) void adamw_fp8_kernel(StepArgs a) {
 #pragma unroll
     for (int q = 0; q < RUNS; ++q) {
       const int64_t e = e0 + q * 512;
-      const uint2 cm = encode8(m[q], by_m), cr = encode8(root[q], by_v);
+      uint2 cm, cr;
+      if constexpr (RANDOM) {
+        const uint32_t seed = t.seed + (uint32_t)e * 0x9e3779b1u + (uint32_t)(e >> 32) * 0xb504f333u;
+        encode8_random(m[q], by_m, root[q], by_v, seed, cm, cr);
+      } else {
+        cm = encode8(m[q], by_m);
+        cr = encode8(root[q], by_v);
+      }
       const uint2 cv = make_uint2(least_root(cr.x, cm.x), least_root(cr.y, cm.y));
       __builtin_memcpy((uint8_t*)t.m + e, &cm, 8);
       __builtin_memcpy((uint8_t*)t.v + e, &cv, 8);
@@ -328,6 +380,7 @@ extern "C" int muon_adamw(int64_t ntensors, const MuonAdamTensor* tensors, int d
   if (!piece) return MUON_OK;
   const StepArgs a{table, pieces, (int)ntensors, runs, (float)beta1, (float)(1.0 - beta1), (float)beta2,
                    (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay), maximize};
+  const bool random = beta1 >= 0.9375 || beta2 > 0.95;
   const unsigned grid = (unsigned)piece;
 #define STEP(KERNEL)                                                                       \
   switch (dtype) {                                                                         \
@@ -335,15 +388,23 @@ extern "C" int muon_adamw(int64_t ntensors, const MuonAdamTensor* tensors, int d
     case MUON_DT_BF16: { constexpr int DT = MUON_DT_BF16; KERNEL<<<grid, THREADS, 0, s>>>(a); break; } \
     default: { constexpr int DT = MUON_DT_F16; KERNEL<<<grid, THREADS, 0, s>>>(a); }                   \
   }
+#define STEP_FP8(G, RUNS)                                \
+  if (random) {                                          \
+    STEP((adamw_fp8_kernel<DT, G, RUNS, true>))          \
+  } else {                                               \
+    STEP((adamw_fp8_kernel<DT, G, RUNS, false>))         \
+  }                                                      \
+  break;
   switch (block) {
     case 0: STEP((adamw_kernel<DT>)) break;
-    case 64: STEP((adamw_fp8_kernel<DT, 8, 1>)) break;
-    case 128: STEP((adamw_fp8_kernel<DT, 16, 1>)) break;
-    case 256: STEP((adamw_fp8_kernel<DT, 32, 1>)) break;
-    case 512: STEP((adamw_fp8_kernel<DT, 64, 1>)) break;
-    case 1024: STEP((adamw_fp8_kernel<DT, 64, 2>)) break;
-    default: STEP((adamw_fp8_kernel<DT, 64, 4>))
+    case 64: STEP_FP8(8, 1)
+    case 128: STEP_FP8(16, 1)
+    case 256: STEP_FP8(32, 1)
+    case 512: STEP_FP8(64, 1)
+    case 1024: STEP_FP8(64, 2)
+    default: STEP_FP8(64, 4)
   }
+#undef STEP_FP8
 #undef STEP
   MUON_CHECK_LAUNCH("muon_adamw");
   return MUON_OK;

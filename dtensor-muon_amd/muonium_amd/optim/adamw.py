@@ -197,6 +197,12 @@ class AdamWFp8(AdamW):
     The state is ``step``, ``exp_avg`` and ``exp_avg_sq_root``, the second moment's root, which spans half the
     binades that v does. A root that is too small for a code beside its block's largest has the least one
     where its mean has a code, so that no step is m / eps.
+    Codes are the nearest ones up to betas of 0.9375 (excluded) and 0.95, beyond which the moments would stay
+    where they are: they are rounded at random there, by the step and the value's place, so that a step
+    gives the same bits again and a moment follows on the average (a root by about 10 to 50% around
+    its value at 0.99 and 0.999). With the nearest codes a block's roots follow as its scale moves: beside
+    a largest value whose gradient never varies, small ones that do not vary either keep a root that
+    is too large, and are stepped too little.
     Parameters of fewer than 4096 values, or not a multiple of ``block_size`` (``MuonLP``'s rule), have
     fp32 moments as in :class:`AdamW`.
 

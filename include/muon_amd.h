@@ -391,7 +391,9 @@ int muon_expert_linear_backward_weight(const void* dy, int dtype, int64_t dy_str
  * (maximize: with -g), in fp32, p rounded once. Parameters and gradients are of one type and order of
  * values. block 0: exp_avg and exp_avg_sq are fp32 m and v, the scales unused. block a power of two from
  * 64 to 2048 that divides numel: they are float8_e4m3fn codes of m and of sqrt(v), value = float(code) *
- * scale of its block, scale = max(absmax, 1e-12) / 448, to nearest even; a root's code is the least one, 1, in
+ * scale of its block, scale = max(absmax, 1e-12) / 448. Codes are the nearest ones, to even, or, from beta1 =
+ * 0.9375 on or above beta2 = 0.95, where the nearest would keep moments where they are, one of the two around
+ * the value at random (by step and place: the same ones every time); a root's code is the least one, 1, in
  * place of 0 where the mean's is not 0. No two tensors may share memory. ws:
  * muon_adamw_workspace_bytes. `tensors` is host memory, read before the call returns. */
 typedef struct MuonAdamTensor {

@@ -114,3 +114,111 @@ def test_a_root_without_a_mean_may_fall_out():
         assert torch.equal(opt.state[p]["exp_avg_sq_root"].codes.view(torch.float8_e4m3fn).cpu().float(), least(cr, cm))
         m, root = (decoded(opt.state[p][name]) for name in ("exp_avg", "exp_avg_sq_root"))
     assert raised > 100 and fallen > 100
+
+
+def run_of(betas, size, steps, varying, seed=5):
+    """(root, its exact value, mean, its exact value) of the small values of a parameter whose gradients have
+    size(i) at step i, beside one of size 1 in every block, after so many steps; exact: in float64."""
+    n, block = 4096, 256
+    g = torch.Generator("cuda").manual_seed(seed)
+    p = torch.zeros(n, device="cuda", requires_grad=True)
+    opt = AdamWFp8([p], lr=1e-3, betas=betas, block_size=block)
+    p.grad = torch.zeros_like(p)
+    sizes = torch.ones(n, device="cuda")
+    inner = torch.arange(n, device="cuda") % block != 0
+    m, v = (torch.zeros(n, dtype=torch.float64, device="cuda") for _ in range(2))
+    for i in range(steps):
+        sizes.masked_fill_(inner, size(i))
+        torch.mul(torch.randn(n, generator=g, device="cuda") if varying else 1.0, sizes, out=p.grad)
+        opt.step()
+        d = p.grad.double()
+        m = m * betas[0] + d * (1 - betas[0])
+        v = v * betas[1] + d * d * (1 - betas[1])
+    held = [decoded(opt.state[p][name]).double()[inner.cpu()] for name in ("exp_avg_sq_root", "exp_avg")]
+    return held[0], v.sqrt()[inner].cpu(), held[1], m[inner].cpu()
+
+
+@pytest.mark.parametrize("varying", [True, False])
+@pytest.mark.parametrize("rising", [False, True])
+@pytest.mark.parametrize("beta2, steps", [(0.99, 2500), (0.999, 4000)])
+def test_roots_follow_gradients_whose_size_changes(beta2, steps, rising, varying):
+    """A hundred times smaller or larger gradients after 300 steps, beside others that stay. A code rounded at
+    random has the right mean, and a variance of at most step times move, where a step is 1/16 to 1/8 of a root
+    and moves it by (1 - b2) / 2 of it for each size of its relative change, 1 on the average: 6% of v at most
+    once it is steady, 3% of the root. Each of 4080 values is off by some ten percent, while it falls by
+    fifty: 4 deviations of the mean are 3%. (Rounded to nearest the roots were 32 to 100 times too large after a
+    fall, and half to a fifth of what they should be after a rise.) The mean, without varying gradients, is a
+    linear recursion: no bias."""
+    low, high = (0.5, 0.005) if rising else (0.005, 0.5)
+    root, root64, mean, mean64 = run_of((0.9, beta2), lambda i: high if i < 300 else low, steps, varying)
+    assert 0.97 <= (root.mean() / root64.mean()).item() <= 1.09
+    if not varying:
+        assert 0.97 <= (mean.mean() / mean64.mean()).item() <= 1.03
+
+
+@pytest.mark.parametrize("rising", [False, True])
+def test_roots_follow_varying_gradients_with_the_nearest_codes(rising):
+    """At beta2 = 0.95 the scale, which moves by 2.5% or more a step, moves the codes: within a code's step, 1/8."""
+    low, high = (0.5, 0.005) if rising else (0.005, 0.5)
+    root, root64, *_ = run_of((0.9, 0.95), lambda i: high if i < 300 else low, 1000, True)
+    assert 7 / 8 <= (root.mean() / root64.mean()).item() <= 9 / 8
+
+
+def test_a_mean_decays_at_any_beta1():
+    """Without further gradients, beside one of 1 that goes on. 0.3 for 30 steps leaves 0.14, which 512 steps bring to
+    the least code, 2^-9 / 448; from there on it is lost with a chance of 1 in 50 a step, and kept over 1058
+    with one of 5e-10. (The nearest codes are kept for good.)"""
+    *_, mean, mean64 = run_of((0.98, 0.95), lambda i: 0.3 if i < 30 else 0.0, 1600, False)
+    assert mean.abs().max() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_random_codes_are_the_neighbours_in_the_right_share(dtype):
+    """Each is one of the two codes around the quotient, up by its distance from the lower one: the mean of a
+    million differences, each within a step and at most half a step's deviation, is within 5 / 2048 steps of 0.
+    The same step of the same values gives the same bits."""
+    g = gen(3)
+    n, block = 1 << 20, 256
+    start, d = torch.randn(n, generator=g).to(dtype), torch.randn(n, generator=g).to(dtype)
+    states = []
+    for _ in range(2):
+        p = start.cuda().requires_grad_()
+        opt = AdamWFp8([p], block_size=block, lr=1e-3, betas=(0.9, 0.999))
+        p.grad = d.cuda()
+        opt.step()
+        states.append(opt.state[p])
+    x = d.float()
+    for name, value in (("exp_avg", x * (1 - 0.9)), ("exp_avg_sq_root", ((x * x) * (1 - 0.999)).double().sqrt().float())):
+        a, b = (s[name] for s in states)
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scale, b.scale)
+        nearest, scale = quantized(value, block)
+        assert torch.equal(a.scale.cpu(), scale)
+        y = (value.view(-1, block) / scale[:, None]).flatten().double()
+        got = a.codes.view(torch.float8_e4m3fn).cpu().double()
+        step = torch.exp2(torch.log2(y.abs().clamp(min=2.0**-6)).floor() - 3)
+        off = (got - y) / step
+        assert off.abs().max() <= 1.0
+        assert off.mean().abs() <= 5 / 2048 and (off * y.sign()).mean().abs() <= 5 / 2048
+        assert (got != nearest.double()).float().mean() > 0.1
+
+
+def test_captured_random_codes_are_those_of_the_steps():
+    g = gen(4)
+    values, grads = torch.randn(8192, generator=g), [torch.randn(8192, generator=g).cuda() for _ in range(5)]
+    both = [values.cuda().requires_grad_() for _ in range(2)]
+    opts = [AdamWFp8([p], betas=(0.9, 0.999)) for p in both]
+    for p, o in zip(both, opts):
+        p.grad = grads[0].clone()
+        o.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opts[1].step()
+    for d in grads[1:]:
+        for p in both:
+            p.grad.copy_(d)
+        opts[0].step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(*both)
+        for name in ("exp_avg", "exp_avg_sq_root"):
+            assert torch.equal(*(o.state[p][name].codes for p, o in zip(both, opts)))
