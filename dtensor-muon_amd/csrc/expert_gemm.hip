@@ -488,8 +488,13 @@ struct Source {
                (uint32_t)__builtin_amdgcn_readfirstlane((int)n), 0x00020000u};
     so = 0;
   }
-  // Nothing is left: loads write zeros.
-  MUON_DEVICE void close() { rs[2] = 0; }
+  // Nothing is left: loads write zeros. The compiler moved the bare insertion of the 0 onto one of the ways to
+  // here, and left the buffer unwritten on the other, where no tile is left: loads of a garbage buffer. What an
+  // asm returns stays in its place.
+  MUON_DEVICE void close() {
+    rs[2] = 0;
+    asm volatile("" : "+s"(rs));
+  }
   // To the next K-tile; long before the offset leaves 31 bits the buffer begins anew.
   MUON_DEVICE void advance() {
     so += KR ? BK * step : BK * 2;
