@@ -44,6 +44,10 @@ MUON_DEVICE void bounds(const GArgs& g, int e, int& start, int& n) {
   n = (e < g.E ? std::min(std::max(g.offsets[e + 1], start), R) : R) - start;
 }
 
+// Tiles of BY among n, up to 2^31 - 1 of them.
+template <int BY>
+MUON_DEVICE int tiles_in(int n) { return (int)(((unsigned)n + (BY - 1)) / BY); }
+
 // Workgroup L's tile of `total`: one contiguous range of tiles for each of the 8 XCDs (consecutive
 // workgroups are dealt round robin), so those that share panels share an L2. -1: none is left.
 MUON_DEVICE int xcd_range(int L, int total) {
@@ -70,7 +74,7 @@ MUON_DEVICE bool find_tile(const GArgs& g, int L, int& e, int& row0, int& left, 
   int mine = 0, start, n;
   for (int i = e0; i < e1; ++i) {
     bounds(g, i, start, n);
-    mine += (n + BM - 1) / BM;
+    mine += tiles_in<BM>(n);
   }
   int incl = mine;
 #pragma unroll
@@ -90,7 +94,7 @@ MUON_DEVICE bool find_tile(const GArgs& g, int L, int& e, int& row0, int& left, 
   e = std::min(src * per, g.E);
   for (;; ++e) {
     bounds(g, e, start, n);
-    const int tiles = (n + BM - 1) / BM;
+    const int tiles = tiles_in<BM>(n);
     if (t < first + tiles || e >= g.E) break;
     first += tiles;
   }
@@ -324,7 +328,7 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void expert_gemm_kernel(GArgs g) {
         for (int j = 0; j < FN; ++j) acc[i][j] = mfma16<DT>(fb[j], fa[i], acc[i][j]);
     }
   };
-  const int KT = (K + BK - 1) / BK;
+  const int KT = tiles_in<BK>(K);
   const bool wide_a = (KRA ? g.M : g.K) >= 8, wide_b = (KRB ? g.N : g.K) >= 8;
   // Pairs of whole K-tiles; the last loads repeat the last of them, so that as many are under way in every
   // turn. (Few tiles gain: 8 experts of 100 x 4001, 6000 rows 76 -> 50 us, 64 of 1408 x 2048, 1024 rows 98 -> 80.
@@ -585,7 +589,7 @@ struct Walk {
       const int lane = threadIdx.x & 63, per = (g.E + 64) / 64;
       const int e0 = lane * per, e1 = std::min(e0 + per, g.E + 1);
       int mine = 0;
-      for (int i = e0; i < e1; ++i) mine += (rows_of[i] + 255) / 256;
+      for (int i = e0; i < e1; ++i) mine += tiles_in<256>(rows_of[i]);
       int incl = mine;
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
@@ -596,7 +600,7 @@ struct Walk {
         int sum = incl - mine;
         for (int i = e0; i < e1; ++i) {
           first[i] = sum;
-          sum += (rows_of[i] + 255) / 256;
+          sum += tiles_in<256>(rows_of[i]);
         }
         if (e1 == g.E + 1 && e0 < e1) first[g.E + 1] = sum;
       }
@@ -650,7 +654,7 @@ struct Walk {
 
 // K-tiles go by twos, since two sets of b fragments take turns; one at least, of nothing, so that every
 // tile is written.
-MUON_DEVICE int k_pairs(int K) { return std::max(1, (K + 2 * BK - 1) / (2 * BK)); }
+MUON_DEVICE int k_pairs(int K) { return std::max(1, tiles_in<2 * BK>(K)); }
 
 template <int DT, int FORM>
 __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
@@ -684,7 +688,7 @@ __global__ __launch_bounds__(256, 1) void expert_gemm_pipe_kernel(GArgs g) {
         b.set(B + o.e * g.sb + o.tn * BN, g.ldb, o.K, g.N - o.tn * BN, o.K);
     }
     kt_next = 0;
-    kt_last = (o.K + BK - 1) / BK - 1;
+    kt_last = tiles_in<BK>(o.K) - 1;
     kt_all = 2 * k_pairs(o.K);
   };
   // to the next K-tile, of the next tile where this one has no more
@@ -1045,7 +1049,7 @@ __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
   };
   // Whole K-tiles: while one is multiplied the next two are under way. The last loads repeat the last K-tile, so
   // that as many are under way in every turn.
-  const int KT = (K + F_K - 1) / F_K;
+  const int KT = tiles_in<F_K>(K);
   const int whole = (KRA ? g.M >= V : true) && (KRB ? g.N >= V : true) ? K / F_K / 2 * 2 : 0;
   if (whole) {
     F32Source<KRA, V> sa;
