@@ -48,6 +48,11 @@ MUON_DEVICE void bounds(const GArgs& g, int e, int& start, int& n) {
 template <int BY>
 MUON_DEVICE int tiles_in(int n) { return (int)(((unsigned)n + (BY - 1)) / BY); }
 
+// Workgroups of a launch: an extent of a grid has to stay below 2^32 threads, so more than 2^22 of them go
+// in rows of so many. Those behind the last tile find none.
+constexpr int GRID_ROW = 1 << 22;
+MUON_DEVICE int workgroup() { return (int)(blockIdx.y * GRID_ROW + blockIdx.x); }
+
 // Workgroup L's tile of `total`: one contiguous range of tiles for each of the 8 XCDs (consecutive
 // workgroups are dealt round robin), so those that share panels share an L2. -1: none is left.
 MUON_DEVICE int xcd_range(int L, int total) {
@@ -287,13 +292,14 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void expert_gemm_kernel(GArgs g) {
   int e, tm, tn, row0 = 0, left = 0, K, M;
   if constexpr (FORM == WGT) {
     // an expert's tiles, which take as long as its rows, on all XCDs
-    const int per = g.tiles_m * g.tiles_n, L = blockIdx.x;
+    const int per = g.tiles_m * g.tiles_n, L = workgroup();
     e = L / per;
+    if (e >= g.E) return;
     tile_of(L - e * per, g.tiles_m, g.tiles_n, tm, tn);
     bounds(g, e, row0, K);
     M = std::min(g.M - tm * BM, BM);
   } else {
-    if (!find_tile<BM>(g, blockIdx.x, e, row0, left, tn)) return;
+    if (!find_tile<BM>(g, workgroup(), e, row0, left, tn)) return;
     M = std::min(left, BM);
     K = e < g.E ? g.K : 0;
     tm = 0;
@@ -855,7 +861,7 @@ template <int DT, bool ALIGNED>
 __global__ __launch_bounds__(256) void expert_rows_kernel(GArgs g) {
   __shared__ f32x4 part[4][2][64];
   int e, row0, left, tn;
-  if (!find_tile<16>(g, blockIdx.x, e, row0, left, tn)) return;
+  if (!find_tile<16>(g, workgroup(), e, row0, left, tn)) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, gq = lane >> 4;
   const int K = e < g.E ? g.K : 0, n0 = tn * R_N;
   // rows and columns behind the last ones repeat them, and are not stored
@@ -989,13 +995,14 @@ __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
   __shared__ __align__(16) float lds[2][2][F_B * (F_K + 4)];
   int e, tm, tn, row0 = 0, left = 0, K, M;
   if constexpr (FORM == WGT) {
-    const int per = g.tiles_m * g.tiles_n, L = blockIdx.x;
+    const int per = g.tiles_m * g.tiles_n, L = workgroup();
     e = L / per;
+    if (e >= g.E) return;
     tile_of(L - e * per, g.tiles_m, g.tiles_n, tm, tn);
     bounds(g, e, row0, K);
     M = std::min(g.M - tm * F_B, F_B);
   } else {
-    if (!find_tile<F_B>(g, blockIdx.x, e, row0, left, tn)) return;
+    if (!find_tile<F_B>(g, workgroup(), e, row0, left, tn)) return;
     M = std::min(left, F_B);
     K = e < g.E ? g.K : 0;
     tm = 0;
@@ -1128,22 +1135,31 @@ __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
 // The most tiles of bm rows that R rows of E experts, and what lies behind them, can make.
 int64_t most_tiles(int64_t R, int64_t E, int bm) { return R / bm + std::min(R, E + 1); }
 
+// Whether workgroups have numbers of 31 bits, the last row of the grid's among them: always, for tensors
+// that fit the card.
+bool fits(int64_t workgroups) {
+  if (workgroups <= INT32_MAX - GRID_ROW) return true;
+  muon_set_error("muon_expert_linear: too many tiles");
+  return false;
+}
+dim3 grid_of(int64_t workgroups) {
+  return workgroups <= GRID_ROW ? dim3((unsigned)workgroups)
+                                : dim3(GRID_ROW, (unsigned)((workgroups + GRID_ROW - 1) / GRID_ROW));
+}
+
 template <int DT, int FORM, int BM, int BN, int WM, int WN>
 int launch16(GArgs g, bool aligned, hipStream_t s) {
   g.tiles_m = (int)(FORM == WGT ? (g.M + BM - 1) / BM : most_tiles(g.R, g.E, BM));
   g.tiles_n = (g.N + BN - 1) / BN;
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * (FORM == WGT ? g.E : 1);
-  if (grid >= (1ll << 32) / (64 * WM * WN)) {  // below 2^32 threads
-    muon_set_error("muon_expert_linear: too many tiles");
-    return MUON_ERR_SHAPE;
-  }
+  if (!fits(grid)) return MUON_ERR_SHAPE;
   constexpr int LDS = 2 * (BM + BN) * BK * 2;
   auto run = [&](auto* kernel) {
     if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {
       muon_set_error("muon_expert_linear: %d bytes of LDS refused", LDS);
       return MUON_ERR_LAUNCH;
     }
-    kernel<<<(unsigned)grid, 64 * WM * WN, LDS, s>>>(g);
+    kernel<<<grid_of(grid), 64 * WM * WN, LDS, s>>>(g);
     MUON_CHECK_LAUNCH("muon_expert_linear");
     return MUON_OK;
   };
@@ -1155,12 +1171,9 @@ template <int DT>
 int launch_rows(GArgs g, bool aligned, hipStream_t s) {
   g.tiles_n = (g.N + R_N - 1) / R_N;
   const int64_t grid = most_tiles(g.R, g.E, 16) * g.tiles_n;
-  if (grid >= (1ll << 32) / 256) {  // below 2^32 threads
-    muon_set_error("muon_expert_linear: too many tiles");
-    return MUON_ERR_SHAPE;
-  }
-  if (aligned) expert_rows_kernel<DT, true><<<(unsigned)grid, 256, 0, s>>>(g);
-  else expert_rows_kernel<DT, false><<<(unsigned)grid, 256, 0, s>>>(g);
+  if (!fits(grid)) return MUON_ERR_SHAPE;
+  if (aligned) expert_rows_kernel<DT, true><<<grid_of(grid), 256, 0, s>>>(g);
+  else expert_rows_kernel<DT, false><<<grid_of(grid), 256, 0, s>>>(g);
   MUON_CHECK_LAUNCH("muon_expert_linear");
   return MUON_OK;
 }
@@ -1193,11 +1206,8 @@ int launch32(GArgs g, hipStream_t s) {
   g.tiles_m = (int)(FORM == WGT ? (g.M + 64 * S - 1) / (64 * S) : most_tiles(g.R, g.E, 64 * S));
   g.tiles_n = (g.N + 64 * S - 1) / (64 * S);
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * (FORM == WGT ? g.E : 1);
-  if (grid >= (1ll << 32) / 256) {  // below 2^32 threads
-    muon_set_error("muon_expert_linear: too many tiles");
-    return MUON_ERR_SHAPE;
-  }
-  expert_gemm_f32_kernel<FORM, S><<<(unsigned)grid, 256, 0, s>>>(g);
+  if (!fits(grid)) return MUON_ERR_SHAPE;
+  expert_gemm_f32_kernel<FORM, S><<<grid_of(grid), 256, 0, s>>>(g);
   MUON_CHECK_LAUNCH("muon_expert_linear");
   return MUON_OK;
 }

@@ -62,3 +62,9 @@ def run(width, dtype):
 
 def test_most_rows_of_direct_loads():
     run(8, torch.bfloat16)
+
+
+@pytest.mark.parametrize("width, dtype", [(7, torch.bfloat16), (3, torch.float32)])
+def test_most_rows_of_small_tiles(width, dtype):
+    """2^24 tiles of 128 rows: as many workgroups of 256 and 512 threads have 2^32 threads and more."""
+    run(width, dtype)
