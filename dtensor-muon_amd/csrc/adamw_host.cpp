@@ -1,6 +1,6 @@
-// The host's side of an AdamW step over many small tensors, as a Python module of
-// libmuon_amd_torch.so: what the optimizer's state holds for each parameter is looked up here and handed to
-// the operator muonium_amd::adamw_ at once.
+// The host's side of an AdamW step over many small tensors, as a Python module (libmuon_amd_python.so):
+// what the optimizer's state holds for each parameter is looked up here and handed to the operator
+// muonium_amd::adamw_ of libmuon_amd_torch.so at once.
 //
 // A step of 129 tensors of a few thousand values takes the GPU 15 us; walking the parameters in Python
 // took 435 us, of which the lookups of gradients, states and layouts were most.
@@ -130,8 +130,8 @@ PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 PyMethodDef methods[] = {{"adamw_step", (PyCFunction)(void (*)(void))step, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "libmuon_amd_torch", nullptr, -1, methods};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "libmuon_amd_python", nullptr, -1, methods};
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_libmuon_amd_torch() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_libmuon_amd_python() { return PyModule_Create(&module); }

@@ -19,6 +19,7 @@ from torch import Tensor
 from . import _lib
 
 _TORCH_LIB_PATH = os.path.join(os.path.dirname(_lib.library_path()), "libmuon_amd_torch.so")
+_PYTHON_LIB_PATH = os.path.join(os.path.dirname(_lib.library_path()), "libmuon_amd_python.so")
 
 
 def _load() -> None:
@@ -33,16 +34,15 @@ def _load() -> None:
 
 
 def _module():
-    """The library as a Python module; None where it was built without Python's headers."""
+    """The module that walks an optimizer's parameters; None where it was built without Python's headers."""
     import importlib.machinery
     import importlib.util
 
-    loader = importlib.machinery.ExtensionFileLoader("libmuon_amd_torch", _TORCH_LIB_PATH)
-    try:
-        return importlib.util.module_from_spec(
-            importlib.util.spec_from_loader("libmuon_amd_torch", loader))
-    except ImportError:
+    if not os.path.exists(_PYTHON_LIB_PATH):
         return None
+    loader = importlib.machinery.ExtensionFileLoader("libmuon_amd_python", _PYTHON_LIB_PATH)
+    return importlib.util.module_from_spec(
+        importlib.util.spec_from_loader("libmuon_amd_python", loader))
 
 
 _load()
