@@ -393,23 +393,30 @@ Tensor combine_forward(const Tensor& rows_, const Tensor& slots_, const optional
   return y;
 }
 
-// Gradients that are not asked for come back empty.
-Tensor2 combine_backward(const Tensor& dy_, const Tensor& rows_, const Tensor& slots_,
+// Gradients that are not asked for come back empty; the rows are needed for the gates' alone.
+Tensor2 combine_backward(const Tensor& dy_, const optional<Tensor>& rows_, const Tensor& slots_,
                          const Tensor& gates_, bool rows_wanted, bool gates_wanted) {
-  const at::DeviceGuard guard(rows_.device());
-  const Tensor rows = rows_of(rows_), slots = slots_of(slots_, rows_), dy = rows_of(dy_);
-  TORCH_CHECK(rows.size(0) == slots.numel() && dy.size(0) == slots.size(0) &&
-                  dy.size(1) == rows.size(1) && dy.scalar_type() == rows.scalar_type() &&
-                  dy.device() == rows.device(),
-              "muonium_amd: the gradient is not like its output");
-  const Tensor gates = plain(gates_, rows, at::kFloat, slots.numel(), "the gates");
-  Tensor drows = rows_wanted ? fresh(rows) : empty(rows, {0}, rows.scalar_type());
-  Tensor dgates = gates_wanted ? empty(rows, slots.sizes(), at::kFloat) : empty(rows, {0}, at::kFloat);
-  check(muon_combine_backward(ptr(dy), dy.stride(0), ptr(rows), rows.stride(0), dtype_code(rows),
-                              slots.size(0), slots.size(1), rows.size(1), ptr<int32_t>(slots),
-                              ptr<float>(gates), rows_wanted ? ptr(drows) : nullptr,
-                              gates_wanted ? ptr<float>(dgates) : nullptr, stream_of(rows)),
+  const at::DeviceGuard guard(dy_.device());
+  const Tensor dy = rows_of(dy_), slots = slots_of(slots_, dy_);
+  TORCH_CHECK(dy.size(0) == slots.size(0), "muonium_amd: the gradient is not like its output");
+  const Tensor gates = plain(gates_, dy, at::kFloat, slots.numel(), "the gates");
+  Tensor rows;
+  if (gates_wanted) {
+    TORCH_CHECK(rows_ && rows_->defined(), "muonium_amd: the gates' gradient takes the rows");
+    rows = rows_of(*rows_);
+    TORCH_CHECK(rows.size(0) == slots.numel() && dy.size(1) == rows.size(1) &&
+                    dy.scalar_type() == rows.scalar_type() && dy.device() == rows.device(),
+                "muonium_amd: the gradient is not like its output");
+  }
+  Tensor drows = empty(dy, {rows_wanted ? slots.numel() : 0, dy.size(1)}, dy.scalar_type());
+  Tensor dgates = gates_wanted ? empty(dy, slots.sizes(), at::kFloat) : empty(dy, {0}, at::kFloat);
+  check(muon_combine_backward(ptr(dy), dy.stride(0), gates_wanted ? ptr(rows) : nullptr,
+                              gates_wanted ? rows.stride(0) : 0, dtype_code(dy), slots.size(0),
+                              slots.size(1), dy.size(1), ptr<int32_t>(slots), ptr<float>(gates),
+                              rows_wanted ? ptr(drows) : nullptr,
+                              gates_wanted ? ptr<float>(dgates) : nullptr, stream_of(dy)),
         "muon_combine_backward");
+  if (!rows_wanted) drows = empty(dy, {0}, dy.scalar_type());
   return {drows, dgates};
 }
 
@@ -785,8 +792,8 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& rows, const Tensor& slots,
                                const optional<Tensor>& gates) {
     at::AutoDispatchBelowADInplaceOrView below;
-    // without gates the gradient needs the slots alone
-    ctx->save_for_backward({gates ? rows : Tensor(), slots, or_undefined(gates)});
+    // the rows are for the gates' gradient alone; without gates the slots do
+    ctx->save_for_backward({needs(gates) ? rows : Tensor(), slots, or_undefined(gates)});
     return {OP("combine", combine_forward).call(rows, slots, gates)};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -799,7 +806,7 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
       } else {
         const bool rows = ctx->needs_input_grad(0), gates = ctx->needs_input_grad(2);
         auto [drows, dgates] = OP("combine_backward", combine_backward)
-                                   .call(grads[0], s[0], s[1], s[2], rows, gates);
+                                   .call(grads[0], or_none(s[0]), s[1], s[2], rows, gates);
         if (rows) out[0] = drows;
         if (gates) out[2] = dgates;
       }
@@ -819,7 +826,8 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weight,
                                const Tensor& offsets) {
     at::AutoDispatchBelowADInplaceOrView below;
-    ctx->save_for_backward({rows, weight, offsets});
+    // each is for the other's gradient
+    ctx->save_for_backward({needs(weight) ? rows : Tensor(), needs(rows) ? weight : Tensor(), offsets});
     return {OP("expert_linear", linear_forward).call(rows, weight, offsets)};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -849,7 +857,7 @@ TORCH_LIBRARY_FRAGMENT(muonium_amd, m) {
   m.def("sort_by_expert(Tensor experts, int num_experts) -> (Tensor, Tensor)");
   m.def("dispatch(Tensor x, Tensor slots) -> Tensor");
   m.def("combine(Tensor rows, Tensor slots, Tensor? gates) -> Tensor");
-  m.def("combine_backward(Tensor dy, Tensor rows, Tensor slots, Tensor gates, bool rows_wanted, "
+  m.def("combine_backward(Tensor dy, Tensor? rows, Tensor slots, Tensor gates, bool rows_wanted, "
         "bool gates_wanted) -> (Tensor, Tensor)");
   m.def("expert_linear(Tensor rows, Tensor weight, Tensor offsets) -> Tensor");
   m.def("expert_linear_backward_rows(Tensor dy, Tensor weight, Tensor offsets) -> Tensor");

@@ -156,7 +156,7 @@ def _(rows, slots, gates):
 
 @_fake("combine_backward")
 def _(dy, rows, slots, gates, rows_wanted, gates_wanted):
-    return (_like(rows) if rows_wanted else rows.new_empty(0),
+    return (dy.new_empty((slots.size(0) * slots.size(1), dy.size(1)) if rows_wanted else 0),
             gates.new_empty(slots.shape if gates_wanted else 0))
 
 
