@@ -227,5 +227,12 @@ class AdamWFp8(AdamW):
         self.block_size = block_size
         super().__init__(params, lr, wd, betas, eps, maximize)
 
+    def __getstate__(self) -> dict:
+        # torch's holds the groups and the state alone
+        return {**super().__getstate__(), "block_size": self.block_size}
+
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__({"block_size": 256, **state})
+
     def _block(self, p: Tensor) -> int:
         return self.block_size if p.numel() >= 4096 and p.numel() % self.block_size == 0 else 0
