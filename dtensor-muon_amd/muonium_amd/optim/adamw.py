@@ -27,6 +27,17 @@ def _is_dense(p: Tensor) -> bool:
     return torch.ops.aten.is_non_overlapping_and_dense.default(p)
 
 
+def _capturing(p: Tensor) -> bool:
+    return (p.is_cuda and not torch.compiler.is_compiling()
+            and torch.cuda.is_current_stream_capturing())
+
+
+def _check_not_captured(p: Tensor, what: str) -> None:
+    """What a captured step makes is made anew by every replay: state has to be there before."""
+    if _capturing(p):
+        raise RuntimeError(f"AdamW: {what} while a graph is captured; take a step before")
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW with fp32 moments: per value, with t the parameter's step, ::
 
@@ -43,7 +54,7 @@ class AdamW(torch.optim.Optimizer):
 
     The state of a parameter is ``step`` (an fp32 scalar on its device), ``exp_avg`` and ``exp_avg_sq``
     (fp32, also for 16-bit parameters). A step can be captured in a HIP graph once its state
-    exists: it counts on in every replay, with the ``lr`` and the other numbers that it was captured
+    exists (it is refused before): it counts on in every replay, with the ``lr`` and the other numbers that it was captured
     with. Parameters that share memory are stepped one after the other."""
 
     _moments = ("exp_avg", "exp_avg_sq")
@@ -92,6 +103,7 @@ class AdamW(torch.optim.Optimizer):
     def _init_state(self, p: Tensor) -> dict:
         state = self.state[p]
         if len(state) == 0:
+            _check_not_captured(p, "a parameter has no state")
             block = self._block(p)
             state["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
             for name in self._moments if not block else AdamWFp8._quantized:
@@ -143,9 +155,12 @@ class AdamW(torch.optim.Optimizer):
                     call[where].append(t)
             else:
                 for where, name in ((2, "exp_avg"), (3, "exp_avg_sq")):
-                    state[name] = _dense_like(state[name], here)
-                    call[where].append(state[name])
+                    if (laid := _dense_like(state[name], here)) is not state[name]:
+                        _check_not_captured(p, "a moment is laid out unlike its parameter")
+                        state[name] = laid
+                    call[where].append(laid)
             if state["step"].device != p.device:
+                _check_not_captured(p, "a parameter's step is on another device")
                 state["step"] = state["step"].to(p.device)
             call[6].append(state["step"])
         return calls

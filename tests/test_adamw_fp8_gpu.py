@@ -222,3 +222,21 @@ def test_captured_random_codes_are_those_of_the_steps():
         assert torch.equal(*both)
         for name in ("exp_avg", "exp_avg_sq_root"):
             assert torch.equal(*(o.state[p][name].codes for p, o in zip(both, opts)))
+
+
+def test_a_first_step_is_not_captured():
+    """Its state would be zeros again in every replay. The optimizer is as it was, and steps on."""
+    made = [AdamWFp8([torch.ones(8192, device="cuda").requires_grad_()]) for _ in range(2)]
+    for opt in made:
+        p = opt.param_groups[0]["params"][0]
+        p.grad = torch.ones_like(p)
+    made[0].step()
+    p = made[1].param_groups[0]["params"][0]
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="no state while a graph is captured"):
+        with torch.cuda.graph(graph):
+            made[1].step()
+    torch.cuda.synchronize()
+    assert (p == 1).all() and not made[1].state[p]
+    made[1].step()
+    assert torch.equal(p, made[0].param_groups[0]["params"][0])
