@@ -77,7 +77,7 @@ def dispatch(x: Tensor, order: ExpertOrder) -> Tensor:
     _check_floats("rows", x)
     slots = _slots(order, x)
     _row_ops.check_device(x.device)
-    return _row_ops.dispatch(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), slots)
+    return _row_ops.dispatch(x if x.dim() == 2 else x.reshape(slots.shape[0], x.shape[-1]), slots)
 
 
 def combine(rows: Tensor, order: ExpertOrder, gates: Tensor | None = None) -> Tensor:

@@ -81,3 +81,17 @@ def test_the_gates_gradient_asks_for_the_rows():
     assert drows.shape == ROWS and dgates.shape == (0,)
     with pytest.raises(RuntimeError, match="takes the rows"):
         torch.ops.muonium_amd.combine_backward(dy, None, order.slots, p["gates"], False, True)
+
+
+@pytest.mark.parametrize("lead", [(), (21,), (3, 7), (0, 7), (3, 0)])
+def test_rows_of_no_columns(lead):
+    """Of any leading dimensions, with their gradients."""
+    order = sort_by_expert(torch.zeros(*lead, TOP, dtype=torch.int64, device="cuda"), EXPERTS)
+    x = torch.zeros(*lead, 0, device="cuda", requires_grad=True)
+    gates = torch.ones(*lead, TOP, device="cuda", requires_grad=True)
+    rows = dispatch(x, order)
+    assert rows.shape == (order.slots.numel(), 0)
+    y = combine(rows, order, gates)
+    assert y.shape == x.shape
+    y.sum().backward()
+    assert x.grad.shape == x.shape and torch.equal(gates.grad, torch.zeros_like(gates))
