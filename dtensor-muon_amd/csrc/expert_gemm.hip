@@ -1222,7 +1222,10 @@ int launch32(GArgs g, hipStream_t s) {
 //   bytes count, which more workgroups fetch faster (64 of 1408 x 2048, 8192 rows: 123 and 117, 114 and
 //   114; 16384 rows: 160 and 151, 176 and 182).
 // * WGT where there is one for every CU (4 experts of 2048 x 2048, 4000 rows 73 and 91), or where fewer
-//   of them are very long (2 of 2048 x 2048, 8000 rows: 122 and 98, 32000 rows: 279 and 349).
+//   of them are very long (2 of 2048 x 2048, 8000 rows: 122 and 98, 32000 rows: 279 and 349) and there are
+//   more tiles of 128 than CUs: one tile a CU is multiplied faster the smaller it is (2 of 64 x 64, 65536 rows: 540
+//   and 382; 1 of 512 x 512, 8192: 141 and 96; 8 of 512 x 512, 131072: 276 and 215; 1 of 2048 x 2048, 65536:
+//   1086 and 960; with 352 of them 2 of 1408 x 2048, 65536: 555 and 636).
 // * Else, and where rows are no whole 16-byte runs, tiles of 128.
 template <int DT, int FORM>
 int launch_typed(const GArgs& g, hipStream_t s) {
@@ -1233,7 +1236,8 @@ int launch_typed(const GArgs& g, hipStream_t s) {
   const int64_t wa = FORM == WGT ? g.M : g.K, wb = FORM == FWD ? g.K : g.N;
   const bool direct = aligned && g.lda >= wa && g.ldb >= wb && std::max({g.lda, g.ldb, (int64_t)g.N}) <= P_MOST;
   const int64_t area = FORM == WGT ? (int64_t)g.M * g.N * g.E : g.R * g.N, tile = 256 * 256;
-  const bool large = FORM == WGT ? area >= P_GROUPS * tile || g.R >= 8192 * (int64_t)g.E
+  const int64_t small = (int64_t)((g.M + 127) / 128) * ((g.N + 127) / 128) * g.E;
+  const bool large = FORM == WGT ? area >= P_GROUPS * tile || (small > P_GROUPS && g.R >= 8192 * (int64_t)g.E)
                                  : area >= 112 * tile && g.R >= 192 * (int64_t)g.E;
   return direct && large ? launch_pipe<DT, FORM>(g, s) : launch16<DT, FORM, 128, 128, 4, 2>(g, aligned, s);
 }
