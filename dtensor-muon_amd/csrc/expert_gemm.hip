@@ -34,7 +34,10 @@ struct GArgs {
   int64_t R;  // rows in all
   int E, N, K, M;  // FWD: N out, K in; ROWS: N in, K out; WGT: M out, N in
   int tiles_m, tiles_n;  // FWD, ROWS: the most row tiles there can be
+  int first;             // number of this launch's first workgroup
 };
+MUON_DEVICE int workgroup(const GArgs& g) { return g.first + (int)blockIdx.x; }
+
 
 // The bounds of expert e's rows, whatever the offsets hold: within 0 .. R, the end no less than the
 // start; the first expert's start at 0. e == E: the rows behind the last expert's.
@@ -47,11 +50,6 @@ MUON_DEVICE void bounds(const GArgs& g, int e, int& start, int& n) {
 // Tiles of BY among n, up to 2^31 - 1 of them.
 template <int BY>
 MUON_DEVICE int tiles_in(int n) { return (int)(((unsigned)n + (BY - 1)) / BY); }
-
-// Workgroups of a launch: an extent of a grid has to stay below 2^32 threads, so more than 2^22 of them go
-// in rows of so many. Those behind the last tile find none.
-constexpr int GRID_ROW = 1 << 22;
-MUON_DEVICE int workgroup() { return (int)(blockIdx.y * GRID_ROW + blockIdx.x); }
 
 // Workgroup L's tile of `total`: one contiguous range of tiles for each of the 8 XCDs (consecutive
 // workgroups are dealt round robin), so those that share panels share an L2. -1: none is left.
@@ -292,14 +290,13 @@ __global__ __launch_bounds__(64 * WM * WN, 4) void expert_gemm_kernel(GArgs g) {
   int e, tm, tn, row0 = 0, left = 0, K, M;
   if constexpr (FORM == WGT) {
     // an expert's tiles, which take as long as its rows, on all XCDs
-    const int per = g.tiles_m * g.tiles_n, L = workgroup();
+    const int per = g.tiles_m * g.tiles_n, L = workgroup(g);
     e = L / per;
-    if (e >= g.E) return;
     tile_of(L - e * per, g.tiles_m, g.tiles_n, tm, tn);
     bounds(g, e, row0, K);
     M = std::min(g.M - tm * BM, BM);
   } else {
-    if (!find_tile<BM>(g, workgroup(), e, row0, left, tn)) return;
+    if (!find_tile<BM>(g, workgroup(g), e, row0, left, tn)) return;
     M = std::min(left, BM);
     K = e < g.E ? g.K : 0;
     tm = 0;
@@ -861,7 +858,7 @@ template <int DT, bool ALIGNED>
 __global__ __launch_bounds__(256) void expert_rows_kernel(GArgs g) {
   __shared__ f32x4 part[4][2][64];
   int e, row0, left, tn;
-  if (!find_tile<16>(g, workgroup(), e, row0, left, tn)) return;
+  if (!find_tile<16>(g, workgroup(g), e, row0, left, tn)) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, gq = lane >> 4;
   const int K = e < g.E ? g.K : 0, n0 = tn * R_N;
   // rows and columns behind the last ones repeat them, and are not stored
@@ -995,14 +992,13 @@ __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
   __shared__ __align__(16) float lds[2][2][F_B * (F_K + 4)];
   int e, tm, tn, row0 = 0, left = 0, K, M;
   if constexpr (FORM == WGT) {
-    const int per = g.tiles_m * g.tiles_n, L = workgroup();
+    const int per = g.tiles_m * g.tiles_n, L = workgroup(g);
     e = L / per;
-    if (e >= g.E) return;
     tile_of(L - e * per, g.tiles_m, g.tiles_n, tm, tn);
     bounds(g, e, row0, K);
     M = std::min(g.M - tm * F_B, F_B);
   } else {
-    if (!find_tile<F_B>(g, workgroup(), e, row0, left, tn)) return;
+    if (!find_tile<F_B>(g, workgroup(g), e, row0, left, tn)) return;
     M = std::min(left, F_B);
     K = e < g.E ? g.K : 0;
     tm = 0;
@@ -1135,16 +1131,20 @@ __global__ __launch_bounds__(256, 2) void expert_gemm_f32_kernel(GArgs g) {
 // The most tiles of bm rows that R rows of E experts, and what lies behind them, can make.
 int64_t most_tiles(int64_t R, int64_t E, int bm) { return R / bm + std::min(R, E + 1); }
 
-// Whether workgroups have numbers of 31 bits, the last row of the grid's among them: always, for tensors
-// that fit the card.
-bool fits(int64_t workgroups) {
-  if (workgroups <= INT32_MAX - GRID_ROW) return true;
-  muon_set_error("muon_expert_linear: too many tiles");
-  return false;
-}
-dim3 grid_of(int64_t workgroups) {
-  return workgroups <= GRID_ROW ? dim3((unsigned)workgroups)
-                                : dim3(GRID_ROW, (unsigned)((workgroups + GRID_ROW - 1) / GRID_ROW));
+// So many workgroups, launch(g, n) of n of them at a time: an extent of a grid has to stay below 2^32 threads.
+template <typename Launch>
+int launch_all(GArgs g, int64_t workgroups, Launch launch) {
+  if (workgroups > INT32_MAX) {  // of no tensors that fit the card
+    muon_set_error("muon_expert_linear: too many tiles");
+    return MUON_ERR_SHAPE;
+  }
+  constexpr int64_t MOST = 1 << 22;
+  for (int64_t at = 0; at < workgroups; at += MOST) {
+    g.first = (int)at;
+    launch(g, (unsigned)std::min(workgroups - at, MOST));
+    MUON_CHECK_LAUNCH("muon_expert_linear");
+  }
+  return MUON_OK;
 }
 
 template <int DT, int FORM, int BM, int BN, int WM, int WN>
@@ -1152,16 +1152,13 @@ int launch16(GArgs g, bool aligned, hipStream_t s) {
   g.tiles_m = (int)(FORM == WGT ? (g.M + BM - 1) / BM : most_tiles(g.R, g.E, BM));
   g.tiles_n = (g.N + BN - 1) / BN;
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * (FORM == WGT ? g.E : 1);
-  if (!fits(grid)) return MUON_ERR_SHAPE;
   constexpr int LDS = 2 * (BM + BN) * BK * 2;
   auto run = [&](auto* kernel) {
     if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {
       muon_set_error("muon_expert_linear: %d bytes of LDS refused", LDS);
       return MUON_ERR_LAUNCH;
     }
-    kernel<<<grid_of(grid), 64 * WM * WN, LDS, s>>>(g);
-    MUON_CHECK_LAUNCH("muon_expert_linear");
-    return MUON_OK;
+    return launch_all(g, grid, [&](const GArgs& a, unsigned n) { kernel<<<n, 64 * WM * WN, LDS, s>>>(a); });
   };
   return aligned ? run(expert_gemm_kernel<DT, FORM, BM, BN, WM, WN, true>)
                  : run(expert_gemm_kernel<DT, FORM, BM, BN, WM, WN, false>);
@@ -1171,11 +1168,10 @@ template <int DT>
 int launch_rows(GArgs g, bool aligned, hipStream_t s) {
   g.tiles_n = (g.N + R_N - 1) / R_N;
   const int64_t grid = most_tiles(g.R, g.E, 16) * g.tiles_n;
-  if (!fits(grid)) return MUON_ERR_SHAPE;
-  if (aligned) expert_rows_kernel<DT, true><<<grid_of(grid), 256, 0, s>>>(g);
-  else expert_rows_kernel<DT, false><<<grid_of(grid), 256, 0, s>>>(g);
-  MUON_CHECK_LAUNCH("muon_expert_linear");
-  return MUON_OK;
+  return launch_all(g, grid, [&](const GArgs& a, unsigned n) {
+    if (aligned) expert_rows_kernel<DT, true><<<n, 256, 0, s>>>(a);
+    else expert_rows_kernel<DT, false><<<n, 256, 0, s>>>(a);
+  });
 }
 
 // What the direct loads and stores index by 32 bits: 256 rows of a panel, 64 of one along k, 128 of a result.
@@ -1206,10 +1202,7 @@ int launch32(GArgs g, hipStream_t s) {
   g.tiles_m = (int)(FORM == WGT ? (g.M + 64 * S - 1) / (64 * S) : most_tiles(g.R, g.E, 64 * S));
   g.tiles_n = (g.N + 64 * S - 1) / (64 * S);
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * (FORM == WGT ? g.E : 1);
-  if (!fits(grid)) return MUON_ERR_SHAPE;
-  expert_gemm_f32_kernel<FORM, S><<<grid_of(grid), 256, 0, s>>>(g);
-  MUON_CHECK_LAUNCH("muon_expert_linear");
-  return MUON_OK;
+  return launch_all(g, grid, [&](const GArgs& a, unsigned n) { expert_gemm_f32_kernel<FORM, S><<<n, 256, 0, s>>>(a); });
 }
 
 // Which kernel, all sides measured on 8 to 128 experts of 1024 x 1024 to 4096 x 4096 (us):
@@ -1282,7 +1275,7 @@ extern "C" int muon_expert_linear(const void* rows, int dtype, int64_t row_strid
     muon_set_error("muon_expert_linear: null pointer");
     return MUON_ERR_ARG;
   }
-  GArgs g{rows, weight, y, row_stride, in, out * in, offsets, nrows, (int)experts, (int)out, (int)in, 0, 0, 0};
+  GArgs g{rows, weight, y, row_stride, in, out * in, offsets, nrows, (int)experts, (int)out, (int)in, 0, 0, 0, 0};
   return launch<FWD>(g, dtype, (hipStream_t)stream);
 }
 
@@ -1296,7 +1289,7 @@ extern "C" int muon_expert_linear_backward_rows(const void* dy, int dtype, int64
     muon_set_error("muon_expert_linear_backward_rows: null pointer");
     return MUON_ERR_ARG;
   }
-  GArgs g{dy, weight, drows, dy_stride, in, out * in, offsets, nrows, (int)experts, (int)in, (int)out, 0, 0, 0};
+  GArgs g{dy, weight, drows, dy_stride, in, out * in, offsets, nrows, (int)experts, (int)in, (int)out, 0, 0, 0, 0};
   return launch<ROWS>(g, dtype, (hipStream_t)stream);
 }
 
@@ -1310,6 +1303,6 @@ extern "C" int muon_expert_linear_backward_weight(const void* dy, int dtype, int
     muon_set_error("muon_expert_linear_backward_weight: null pointer");
     return MUON_ERR_ARG;
   }
-  GArgs g{dy, rows, dweight, dy_stride, row_stride, 0, offsets, nrows, (int)experts, (int)in, 0, (int)out, 0, 0};
+  GArgs g{dy, rows, dweight, dy_stride, row_stride, 0, offsets, nrows, (int)experts, (int)in, 0, (int)out, 0, 0, 0};
   return launch<WGT>(g, dtype, (hipStream_t)stream);
 }
