@@ -22,7 +22,7 @@
 //
 // It moves bytes: 28 a value in fp32, 22 with 16-bit parameters, 10 with those and fp8 moments. 39.4
 // million fp32 values in 63 tensors take 231 us (4.8 TB/s), two bf16 tensors of 64000 x 4096 with fp8
-// moments 1000 to 1056 (5.0 to 5.2), where a copy runs at 4.9. 129 tensors of 128 and 4096 values: 6.6
+// moments 1040 to 1120 (4.7 to 5.0; 1300 to 1390 with codes at random), where a copy runs at 4.9. 129 tensors of 128 and 4096 values: 6.6
 // us after tables of 1.6 to 3.9 for 48 of them.
 #include <algorithm>
 #include <cmath>

@@ -910,10 +910,10 @@ __global__ __launch_bounds__(256) void expert_rows_kernel(GArgs g) {
 // lane holds four k in a row for four products, the other half of the wave the next four: in that order a KC
 // fragment of all four is one read. The sums of 256 k are added up apart from the products' own: a
 // sum that runs over all of k takes a rounding of its whole size at each. 4094 rows of 8 experts of
-// 1001 x 769: 80 to 86 us each, 73 to 79 TFLOP/s of 154 (8192 cubed): about 1090 tiles of 64, so that some
-// CUs have five of them and others four, whose edges hold a tenth of nothing. Two K-tiles are under way, in
-// counted loads; with one, behind conditions, 91, 94 and 84 us. More of these workgroups on a CU
-// help, wider tiles and K-tiles do not.
+// 1001 x 769: 72 to 76 us each among many passes, 83 to 87 TFLOP/s of 154 (8192 cubed): about 1090 tiles of
+// 64, so that some CUs have five of them and others four, whose edges hold a tenth of nothing. Two K-tiles
+// are under way, in counted loads (with one, behind conditions, all three took 255 us for 220 to 227). More
+// of these workgroups on a CU help, wider tiles and K-tiles do not.
 constexpr int F_K = 16, F_SUM = 256 / F_K;
 
 // A thread's V = 4 S values: KR: of row k; KC: of row r, V k in a row.
