@@ -13,7 +13,9 @@
 // scale, which its largest value moves, shifts the codes enough for the roots to follow. Beyond that they
 // stay (b2 = 0.99, gradients that fall from 0.5 to 0.005 beside others: roots 59 times too large), and
 // from b1 = 15/16 on a mean does: codes are rounded up or down at random then, by a number made from the
-// step and the value's place, with the chance that keeps the value on the average.
+// step and the value's place, with the chance that keeps the value on the average. The nearest codes of a mean
+// below 8 of the least codes stay too, at any b1: without a gradient it gives up half of one more a step, or a
+// row that is not met beside others in its block would be stepped for good (0.2 lr after 1000 steps).
 //
 // Two kinds of launches: a table of the tensors (pointers, first piece of work, and the two factors that
 // depend on t, whose counters it moves on), as many as a launch's arguments hold at a time; then one
@@ -130,12 +132,16 @@ MUON_DEVICE void store8(void* p, int64_t e, int left, const float (&x)[8]) {
   }
 }
 
-// The step of one value; m and v are the new moments, root = sqrt(v).
+// The step of one value; m and v are the new moments, root = sqrt(v). HELD, half of the least code: without a
+// gradient a mean below 8 codes, where 1/16 of it is less than that, gives it up beside its decay.
+template <bool HELD>
 MUON_DEVICE void step_value(const StepArgs& a, const Entry& t, float g, float& p, float& m, float& v,
-                            float& root) {
+                            float& root, float half = 0.0f) {
 #pragma clang fp contract(off)
   if (a.maximize) g = -g;
-  m = m * a.b1 + g * a.c1;
+  float more = g * a.c1;
+  if constexpr (HELD) more = g == 0.0f && fabsf(m) < 16.0f * half ? -__builtin_amdgcn_fmed3f(m, -half, half) : more;
+  m = m * a.b1 + more;
   v = v * a.b2 + (g * g) * a.c2;
   root = sqrtf(v);
   p = p * a.decay - t.size * (m / (root * t.scale + a.eps));
@@ -156,7 +162,7 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float root;
-      step_value(a, t, g[j], p[j], m[j], v[j], root);
+      step_value<false>(a, t, g[j], p[j], m[j], v[j], root);
     }
     store8<DT>(t.p, e, left, p);
     store8<MUON_DT_F32>(t.m, e, left, m);
@@ -273,7 +279,7 @@ __global__ __launch_bounds__(THREADS) void adamw_fp8_kernel(StepArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float v = root[q][j] * root[q][j];
-        step_value(a, t, g[j], p[j], m[q][j], v, root[q][j]);
+        step_value<!RANDOM>(a, t, g[j], p[j], m[q][j], v, root[q][j], ms * 0x1p-10f);
         mt = larger_bits(mt, m[q][j]);
         vt = larger_bits(vt, root[q][j]);
       }

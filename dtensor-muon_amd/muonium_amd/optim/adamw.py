@@ -211,7 +211,7 @@ class AdamWFp8(AdamW):
 
     The state is ``step``, ``exp_avg`` and ``exp_avg_sq_root``, the second moment's root, which spans half the
     binades that v does. A root that is too small for a code beside its block's largest has the least one
-    where its mean has a code, so that no step is m / eps.
+    where its mean has a code, so that no step is m / eps. Without a gradient, a mean decays to 0.
     Codes are the nearest ones up to betas of 0.9375 (excluded) and 0.95, beyond which the moments would stay
     where they are: they are rounded at random there, by the step and the value's place, so that a step
     gives the same bits again and a moment follows on the average (a root by about 10 to 50% around

@@ -394,7 +394,8 @@ int muon_expert_linear_backward_weight(const void* dy, int dtype, int64_t dy_str
  * scale of its block, scale = max(absmax, 1e-12) / 448. Codes are the nearest ones, to even, or, from beta1 =
  * 0.9375 on or above beta2 = 0.95, where the nearest would keep moments where they are, one of the two around
  * the value at random (by step and place: the same ones every time); a root's code is the least one, 1, in
- * place of 0 where the mean's is not 0. No two tensors may share memory. ws:
+ * place of 0 where the mean's is not 0, and with the nearest codes a mean below 8 of them whose gradient is 0
+ * gives up half of one beside its decay. No two tensors may share memory. ws:
  * muon_adamw_workspace_bytes. `tensors` is host memory, read before the call returns. */
 typedef struct MuonAdamTensor {
   void* param;

@@ -240,3 +240,28 @@ def test_a_first_step_is_not_captured():
     assert (p == 1).all() and not made[1].state[p]
     made[1].step()
     assert torch.equal(p, made[0].param_groups[0]["params"][0])
+
+
+@pytest.mark.parametrize("betas", [(0.9, 0.95), (0.93, 0.9), (0.9, 0.999), (0.95, 0.95)])
+def test_a_row_that_is_not_met_comes_to_rest(betas):
+    """Rows of 64 values, four to a block, of which one goes on: the others' means lose a code at least a step
+    without a gradient (at random one in ten or twenty steps: of 0.9^700 or 0.95^700 none is left), and are at 0
+    after at most 130 + 17 codes' steps of them. AdamW in 64 bits moves such a row by under 1e-20 lr then; a
+    mean that kept its last code moved it by 0.1 to 0.3 lr."""
+    n = 4096
+    g = torch.Generator("cuda").manual_seed(7)
+    p = torch.zeros(n, device="cuda", requires_grad=True)
+    opt = AdamWFp8([p], lr=1e-3, wd=0.0, betas=betas, block_size=256)
+    met = torch.arange(n, device="cuda") // 64 % 4 == 0
+    p.grad = torch.zeros_like(p)
+    for i in range(2000):
+        p.grad.normal_(generator=g)
+        if i >= 50:
+            p.grad.masked_fill_(~met, 0.0)
+        if i == 1000:
+            at_rest = p.detach().clone()
+        opt.step()
+    assert torch.equal(p.detach()[~met], at_rest[~met])
+    assert not torch.equal(p.detach()[met], at_rest[met])
+    codes = opt.state[p]["exp_avg"].codes.view(torch.float8_e4m3fn).float()
+    assert (codes[~met] == 0).all() and (codes[met] != 0).any()
