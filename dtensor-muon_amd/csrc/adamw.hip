@@ -24,8 +24,8 @@
 //
 // It moves bytes: 28 a value in fp32, 22 with 16-bit parameters, 10 with those and fp8 moments. 39.4
 // million fp32 values in 63 tensors take 231 us (4.8 TB/s), two bf16 tensors of 64000 x 4096 with fp8
-// moments 1040 to 1120 (4.7 to 5.0; 1300 to 1390 with codes at random), where a copy runs at 4.9. 129 tensors of 128 and 4096 values: 6.6
-// us after tables of 1.6 to 3.9 for 48 of them.
+// moments 1040 to 1120 (4.7 to 5.0; 1300 to 1390 with codes at random), where a copy runs at 4.9. 129 tensors
+// of 128 and 4096 values: 6.6 us after tables of 1.6 to 3.9 for 48 of them.
 #include <algorithm>
 #include <cmath>
 
@@ -80,8 +80,7 @@ struct StepArgs {
   const Entry* table;
   const int* pieces;  // first piece of each tensor, in order
   int n, runs;        // tensors; runs of THREADS * 8 values in a piece
-  float b1, c1, b2, c2, eps, decay;  // c = 1 - b
-  int maximize;
+  float b1, c1, b2, c2, eps, decay;  // c = 1 - b; c1 below 0 to maximize
 };
 
 constexpr int THREADS = 256;
@@ -132,16 +131,11 @@ MUON_DEVICE void store8(void* p, int64_t e, int left, const float (&x)[8]) {
   }
 }
 
-// The step of one value; m and v are the new moments, root = sqrt(v). HELD, half of the least code: without a
-// gradient a mean below 8 codes, where 1/16 of it is less than that, gives it up beside its decay.
-template <bool HELD>
+// The step of one value; m and v are the new moments, root = sqrt(v).
 MUON_DEVICE void step_value(const StepArgs& a, const Entry& t, float g, float& p, float& m, float& v,
-                            float& root, float half = 0.0f) {
+                            float& root) {
 #pragma clang fp contract(off)
-  if (a.maximize) g = -g;
-  float more = g * a.c1;
-  if constexpr (HELD) more = g == 0.0f && fabsf(m) < 16.0f * half ? -__builtin_amdgcn_fmed3f(m, -half, half) : more;
-  m = m * a.b1 + more;
+  m = m * a.b1 + g * a.c1;
   v = v * a.b2 + (g * g) * a.c2;
   root = sqrtf(v);
   p = p * a.decay - t.size * (m / (root * t.scale + a.eps));
@@ -162,7 +156,7 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float root;
-      step_value<false>(a, t, g[j], p[j], m[j], v[j], root);
+      step_value(a, t, g[j], p[j], m[j], v[j], root);
     }
     store8<DT>(t.p, e, left, p);
     store8<MUON_DT_F32>(t.m, e, left, m);
@@ -244,6 +238,18 @@ MUON_DEVICE uint32_t least_root(uint32_t v, uint32_t m) {
   constexpr uint32_t low = 0x7f7f7f7fu, top = 0x80808080u;  // a byte of 7 bits and low: top set if it is not 0
   return v | (((m & low) + low) & ~((v & low) + low) & top) >> 7;
 }
+// Without a gradient, means below 8 of the least code, whose decay by up to 1/16 is less than half a code, give up
+// half of one before it.
+MUON_DEVICE void rest8(const float (&g)[8], float scale, float (&m)[8]) {
+  float least = fabsf(g[0]);
+#pragma unroll
+  for (int j = 1; j < 8; ++j) least = fminf(least, fabsf(g[j]));
+  if (least != 0.0f) return;
+  const float half = scale * 0x1p-10f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (g[j] == 0.0f && fabsf(m[j]) < 16.0f * half) m[j] -= __builtin_amdgcn_fmed3f(m[j], -half, half);
+}
 // absmax / 448 of a block; bits are compared as integers, so that a NaN is the largest
 MUON_DEVICE float block_scale(uint32_t bits) {
   const float top = __uint_as_float(bits);
@@ -276,12 +282,13 @@ __global__ __launch_bounds__(THREADS) void adamw_fp8_kernel(StepArgs a) {
       __builtin_memcpy(&cv, (const uint8_t*)t.v + e, 8);
       decode8(cm, ms, m[q]);
       decode8(cv, vs, root[q]);
+      if constexpr (!RANDOM) rest8(g, ms, m[q]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float v = root[q][j] * root[q][j];
-        step_value<!RANDOM>(a, t, g[j], p[j], m[q][j], v, root[q][j], ms * 0x1p-10f);
+        step_value(a, t, g[j], p[j], m[q][j], v, root[q][j]);
         mt = larger_bits(mt, m[q][j]);
-        vt = larger_bits(vt, root[q][j]);
+        vt = std::max(vt, __float_as_uint(root[q][j]));  // at least 0, or a NaN of either sign
       }
       store8<DT>(t.p, e, 8, p);
     }
@@ -384,8 +391,9 @@ extern "C" int muon_adamw(int64_t ntensors, const MuonAdamTensor* tensors, int d
     MUON_CHECK_LAUNCH("muon_adamw: table");
   }
   if (!piece) return MUON_OK;
-  const StepArgs a{table, pieces, (int)ntensors, runs, (float)beta1, (float)(1.0 - beta1), (float)beta2,
-                   (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay), maximize};
+  const float c1 = (float)(1.0 - beta1);
+  const StepArgs a{table, pieces, (int)ntensors, runs, (float)beta1, maximize ? -c1 : c1, (float)beta2,
+                   (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay)};
   const bool random = beta1 >= 0.9375 || beta2 > 0.95;
   const unsigned grid = (unsigned)piece;
 #define STEP(KERNEL)                                                                       \

@@ -54,8 +54,8 @@ class AdamW(torch.optim.Optimizer):
 
     The state of a parameter is ``step`` (an fp32 scalar on its device), ``exp_avg`` and ``exp_avg_sq``
     (fp32, also for 16-bit parameters). A step can be captured in a HIP graph once its state
-    exists (it is refused before): it counts on in every replay, with the ``lr`` and the other numbers that it was captured
-    with. Parameters that share memory are stepped one after the other."""
+    exists (it is refused before): it counts on in every replay, with the ``lr`` and the other
+    numbers that it was captured with. Parameters that share memory are stepped one after the other."""
 
     _moments = ("exp_avg", "exp_avg_sq")
 
